@@ -1,0 +1,806 @@
+// The attention half of a trunk layer over a cache in pages.
+//
+// K and V lie in a pool of pages [n_pages][Hkv][page][hd] (the engine's cache
+// is one page of max_ctx tokens per row); sequence s has the pages table[s][0 ..
+// width), slot j of it in page j / page.  Its n new tokens of a call are the
+// packed rows starts[s] .. starts[s + 1] of q, and lens[s] is its length with
+// them, so token i has slot lens[s] - n + i.  Query heads h G .. h G + G - 1 share key
+// head h.  A page is a multiple of 16 tokens: 16 keys of one tile lie in one
+// page, one look into the table serves a tile, and a tile is loaded whole (its
+// slots past the length are memory of the pool).
+//
+// starts, lens and table are device memory that the host does not look at, so the
+// kernels hold them in range: starts to [0, T] and not falling, lens to [0,
+// width * page], and an entry outside the pool reads page 0 with its keys counted as
+// NaN, so that rows that see it come out as NaN.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace sk {
+namespace paged {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int TILE = 16;                          // keys of a tile
+
+struct Cache {
+  void* k; void* v;                               // [n_pages][Hkv][page][hd]
+  const int* table; int64_t stride; int width;    // [S][width] at rows of stride entries
+  const int* starts; const int* lens;             // [S + 1], [S]
+  int T, S, Hq, Hkv, G, n_pages, page;
+};
+
+// ------------------------------------------------------------ small helpers
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over 2, 4, 8 or 16 neighbouring lanes, in every one of them.
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f<0xb1>(v);                            // quad_perm [1,0,3,2]
+  if constexpr (N >= 4) v += dpp_f<0x4e>(v);      // quad_perm [2,3,0,1]
+  if constexpr (N >= 8) v += dpp_f<0x141>(v);     // row_half_mirror
+  if constexpr (N >= 16) v += dpp_f<0x140>(v);    // row_mirror
+  return v;
+}
+// v of lanes 16, 32 and 48 further, added or compared with this one's.
+__device__ __forceinline__ float swap16(float v) { return __shfl_xor(v, 16, 64); }
+__device__ __forceinline__ float swap32(float v) { return __shfl_xor(v, 32, 64); }
+
+__device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }   // to nearest even
+
+// N consecutive elements as loaded; get(i) widens one.
+template <typename T, int N>
+struct Piece {
+  uint32_t w[(N * sizeof(T) + 3) / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (N * sizeof(T) > 16) {
+#pragma unroll
+      for (int i = 0; i < N * (int)sizeof(T) / 16; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (N * sizeof(T) == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N * sizeof(T) == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else if constexpr (N * sizeof(T) == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (auto& x : w) x = 0;
+  }
+  // some element is infinite or NaN
+  __device__ __forceinline__ bool wild() const {
+    bool b = false;
+#pragma unroll
+    for (uint32_t x : w) {
+      if constexpr (sizeof(T) == 4) b |= (x & 0x7f800000u) == 0x7f800000u;
+      else b |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+    }
+    return b;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(to_bf16(a) | (uint32_t)to_bf16(b) << 16, to_bf16(c) | (uint32_t)to_bf16(d) << 16);
+}
+
+// First row and number of sequence s's new tokens.
+__device__ __forceinline__ void seq_rows(const Cache& c, int s, int& first, int& n) {
+  first = min(max(c.starts[s], 0), c.T);
+  n = min(max(c.starts[s + 1], first), c.T) - first;
+}
+__device__ __forceinline__ int seq_len(const Cache& c, int s) { return min(max(c.lens[s], 0), c.width * c.page); }
+
+// The sequence that row m belongs to (wave-uniform; S if none): the last one that starts at or before it.
+__device__ __forceinline__ int seq_of_row(const Cache& c, int m) {
+  int count = 0;
+  for (int s0 = 0; s0 < c.S; s0 += 64) {
+    const int s = s0 + (threadIdx.x & 63);
+    count += __popcll(__ballot(s < c.S && c.starts[min(s, c.S)] <= m));
+  }
+  if (count == 0) return c.S;
+  return m < c.starts[count] ? count - 1 : c.S;
+}
+
+// Tile x of all sequences' tiles of R (token, head of the group) rows: its
+// sequence and its number there; false past the last.
+__device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, int& seq, int& tile) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int s0 = 0; s0 < c.S; s0 += 64) {
+    int t = 0;
+    if (s0 + lane < c.S) {
+      int first, n;
+      seq_rows(c, s0 + lane, first, n);
+      t = (n * c.G + R - 1) / R;
+    }
+    int sum = t;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += o;
+    }
+    const uint64_t past = __ballot(base + sum > x);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      seq = s0 + l;
+      tile = x - base - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(t, l));
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// ------------------------------------------------------------ append
+// Token m: q and k of every head normalised over the head (RMSNorm with a gain,
+// if there are gains), then rotated: pair (i, i + hd / 2) by the angle position
+// * inv_freq[i]; q to its row, k and v to the token's slot, whose account of
+// attention weight starts at 0.  One workgroup per token, hd / 8 lanes per
+// head with four pairs each, so that every load and store is 16 bytes (8 of BF16).
+//
+// The angle is formed and brought into [-pi, pi] in 64 bits (in 32 a product
+// of 2^17 is off by 2^-7), then cos(r + e) = cos r - e sin r with r its nearest FP32
+// and e the rest; one lane per pair, shared through LDS.
+template <typename XT, typename KT, int HD>
+__global__ __launch_bounds__(256) void append_kernel(Cache c, const XT* qkv, const float* q_gain, const float* k_gain,
+                                                     const float* inv_freq, const int* positions, float eps,
+                                                     float* mass, XT* q_out) {
+  constexpr int LPH = HD / 8, NG = 256 / LPH, HALF = HD / 2;
+  __shared__ float2 cs[HALF];
+  const int m = blockIdx.x, tid = threadIdx.x, g = tid / LPH, i = (tid % LPH) * 4;
+  const int H = c.Hq + 2 * c.Hkv;
+  const XT* row = qkv + (size_t)m * H * HD + i;
+  Piece<XT, 4> a, b;
+  if (g < H) { a.load(row + (size_t)g * HD); b.load(row + (size_t)g * HD + HALF); }
+  if (tid < HALF) {
+    constexpr double TWO_PI = 6.283185307179586476925286766559;
+    const double t = (double)positions[m] * (double)inv_freq[tid];
+    const double w = t - rint(t / TWO_PI) * TWO_PI;
+    const float r = (float)w, e = (float)(w - (double)r), co = cosf(r), si = sinf(r);
+    cs[tid] = make_float2(fmaf(-e, si, co), fmaf(e, co, si));
+  }
+  const int s = seq_of_row(c, m);
+  if (s >= c.S) return;                           // behind the last sequence (the whole workgroup)
+  int first, n;
+  seq_rows(c, s, first, n);
+  const int slot = seq_len(c, s) - n + (m - first);
+  int at = -1;                                    // the slot's page, if it has one
+  if (slot >= 0 && m - first < n) at = c.table[s * c.stride + slot / c.page];
+  const bool live = at >= 0 && at < c.n_pages;
+  const size_t base = live ? (size_t)at * c.Hkv * c.page + slot % c.page : 0;   // in rows of hd, for head 0
+  __syncthreads();
+  float2 t4[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) t4[u] = cs[i + u];
+  for (int h = g; h < H; h += NG) {
+    if (h != g) { a.load(row + (size_t)h * HD); b.load(row + (size_t)h * HD + HALF); }
+    float y1[4], y2[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { y1[u] = a.get(u); y2[u] = b.get(u); }
+    if (h < c.Hq + c.Hkv) {
+      const float* gain = h < c.Hq ? q_gain : k_gain;
+      if (gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) ss = fmaf(y1[u], y1[u], fmaf(y2[u], y2[u], ss));
+        const float inv = 1.0f / sqrtf(group_sum<LPH>(ss) / (float)HD + eps);
+        const float4 g1 = *reinterpret_cast<const float4*>(gain + i), g2 = *reinterpret_cast<const float4*>(gain + i + HALF);
+        y1[0] = g1.x * (y1[0] * inv); y1[1] = g1.y * (y1[1] * inv); y1[2] = g1.z * (y1[2] * inv); y1[3] = g1.w * (y1[3] * inv);
+        y2[0] = g2.x * (y2[0] * inv); y2[1] = g2.y * (y2[1] * inv); y2[2] = g2.z * (y2[2] * inv); y2[3] = g2.w * (y2[3] * inv);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float p = y1[u], q = y2[u];
+        y1[u] = p * t4[u].x - q * t4[u].y;
+        y2[u] = q * t4[u].x + p * t4[u].y;
+      }
+    }
+    if (h < c.Hq) {
+      XT* d = q_out + ((size_t)m * c.Hq + h) * HD + i;
+      store4(d, y1[0], y1[1], y1[2], y1[3]);
+      store4(d + HALF, y2[0], y2[1], y2[2], y2[3]);
+    } else if (live) {
+      const bool isk = h < c.Hq + c.Hkv;
+      const size_t r = base + (size_t)(h - c.Hq - (isk ? 0 : c.Hkv)) * c.page;
+      KT* d = static_cast<KT*>(isk ? c.k : c.v) + r * HD + i;
+      store4(d, y1[0], y1[1], y1[2], y1[3]);
+      store4(d + HALF, y2[0], y2[1], y2[2], y2[3]);
+      if (isk && mass && i == 0) mass[r] = 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------ attention
+// Rows are (token, head of the group) pairs, token by token: row f of a sequence
+// is token f / G, head f % G, so any group size fills the matrix tiles.  Row
+// at slot p sees key j when j <= p and, with a window, j > p - window or j < sinks.
+//   s_j = scale q . k_j;  m = max s_j;  l = sum exp(s_j - m);  out = sum exp(s_j - m) v_j / l
+//   lse = m + ln l
+// in one pass with a running m (of the raw q . k_j, scale > 0), l and out; a key
+// range cut over workgroups leaves (out, m, l) per cut, joined by combine_kernel.
+// A row that sees nothing gives 0 and -infinity.
+struct AttendArgs {
+  Cache c;
+  const void* q; void* out; float* lse;           // [T][Hq][hd], [T][Hq] (may be null)
+  float scale2;                                   // scale * log2 e: exp(s - m) = 2^(scale2 (qk - max qk))
+  int window, sinks;                              // window 0: all keys
+  int cut;                                        // tiles of keys per cut; cuts of a row: blockIdx.z
+  float* part; float* ml;                         // [cuts][T * Hq][hd], [cuts][T * Hq][2]
+};
+
+// The tiles that the rows of slots p_lo .. p_hi walk: 0 .. n - 1, first those of the sinks, then the window's.
+struct Walk {
+  int n, sink, skip;
+  __device__ __forceinline__ int tile(int t) const { return t < sink ? t : t + skip; }
+};
+__device__ __forceinline__ Walk walk_of(int p_lo, int p_hi, int window, int sinks) {
+  Walk w;
+  const int lo = window > 0 && p_lo >= window ? (p_lo - window + 1) / TILE : 0;
+  w.sink = min(sinks / TILE + (sinks % TILE != 0), lo);
+  w.skip = lo - w.sink;
+  w.n = p_hi < 0 ? 0 : p_hi / TILE + 1 - w.skip;
+  return w;
+}
+__device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
+  return j <= p && (window == 0 || j > p - window || j < sinks);
+}
+
+// Offsets (in elements, for head 0 dims) of a run of tiles: lane i holds that of
+// the wave's i-th tile from a walk position on; one division and table entry per lane, for 64 tiles.
+struct TileOffsets {
+  uint32_t lo, hi;
+  uint64_t bad;                                   // lanes whose page is not in the pool
+  __device__ __forceinline__ void load(const Cache& c, const int* table, const Walk& w, int t0, int step, int end, int h,
+                                       int hd) {
+    const int t = min(t0 + (int)(threadIdx.x & 63) * step, end - 1);
+    const int g = w.tile(t), tpp = c.page / TILE, pg = g / tpp;
+    const int e = table[pg];
+    const bool ok = e >= 0 && e < c.n_pages;
+    const size_t off = (((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (size_t)(g - pg * tpp) * TILE) * hd;
+    lo = (uint32_t)off;
+    hi = (uint32_t)(off >> 32);
+    bad = __ballot(!ok);
+  }
+  __device__ __forceinline__ size_t at(int i) const {
+    return (size_t)(uint32_t)__builtin_amdgcn_readlane(lo, i) | (size_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32;
+  }
+};
+
+template <typename KT, int HD>
+struct Dims {
+  static constexpr int KW = (16 / (int)sizeof(KT)) < HD / 4 ? 16 / (int)sizeof(KT) : HD / 4;   // dims per K load
+  static constexpr int NK = HD / (4 * KW);                                                     // K loads per tile
+  static constexpr int NDT = HD / 16;                                                          // 16-dim output tiles
+  static constexpr int VW = (16 / (int)sizeof(KT)) < NDT ? 16 / (int)sizeof(KT) : NDT;         // dims per V load
+  static constexpr int NV = NDT / VW;                                                          // V loads per key row
+  static constexpr int LDO = HD + 4;                                                           // merge row stride
+};
+
+// The workgroup holds NT matrix tiles of 16 rows; its WK waves take key tiles in
+// turn, each with its own running maximum, and meet in LDS at the end.  No LDS and no barrier in the loop:
+//   S^T = K Q^T on the FP32 matrix cores: lane l holds row l % 16's products with
+//     keys 4 (l / 16) + v, v < 4; a row's maximum is 4 values and two exchanges;
+//   O^T += V^T P^T takes those values as they are: step v multiplies keys 4 q + v, q = 0 .. 3.
+// K and V come straight from the pages, 16 bytes per lane; K of the next tile loads under this one's softmax and V.
+template <typename QT, typename KT, int HD, int NT, int WK>
+__global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
+  using D = Dims<KT, HD>;
+  constexpr int KW = D::KW, NK = D::NK, NDT = D::NDT, VW = D::VW, NV = D::NV, LDO = D::LDO, R = NT * 16;
+  __shared__ __attribute__((aligned(16))) float po[WK * R * LDO];
+  __shared__ float pm[WK * R], pl[WK * R];
+  const Cache& c = a.c;
+  const int h = blockIdx.x, cut = blockIdx.z;
+  int seq, tile_no;
+  if (!find_tile(c, R, blockIdx.y, seq, tile_no)) return;
+  int first, n;
+  seq_rows(c, seq, first, n);
+  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
+  const int end = min(w.n, (cut + 1) * a.cut);
+  if (cut > 0 && cut * a.cut >= w.n) return;      // the first cut also answers for rows that see nothing
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, q4 = lane >> 4;
+  const int* table = c.table + seq * c.stride;
+  const KT* kp = static_cast<const KT*>(c.k);
+  const KT* vp = static_cast<const KT*>(c.v);
+
+  int qp[NT];                                     // the slot of this lane's rows (rows past the last repeat it)
+  float qf[NT][NK * KW];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int f = min(f0 + j * 16 + i16, rows - 1), tok = f / c.G;
+    qp[j] = p0 + tok;
+    const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
+#pragma unroll
+    for (int t = 0; t < NK; ++t) {
+      Piece<QT, KW> x;
+      x.load(qr + t * 4 * KW + KW * q4);
+#pragma unroll
+      for (int e = 0; e < KW; ++e) qf[j][t * KW + e] = x.get(e);
+    }
+  }
+  Piece<KT, KW> kf[NK];
+  Piece<KT, VW> vf[4][NV];
+  auto load_k = [&](size_t off) {
+    const KT* p = kp + off + i16 * HD + KW * q4;
+#pragma unroll
+    for (int t = 0; t < NK; ++t) kf[t].load(p + t * 4 * KW);
+  };
+  auto load_v = [&](size_t off) {
+    const KT* p = vp + off + 4 * q4 * HD + VW * i16;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int t = 0; t < NV; ++t) vf[v][t].load(p + v * HD + t * 16 * VW);
+  };
+  v4f o[NT][NDT];
+  float mr[NT], lr[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    mr[j] = -INFINITY;
+    lr[j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) o[j][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+
+  TileOffsets offs;
+  const int t_first = cut * a.cut + wave;
+  if (t_first < end) {
+    offs.load(c, table, w, t_first, WK, end, h, HD);
+    load_k(offs.at(0));
+  }
+  int i = 0;                                      // the tile's lane in offs
+  for (int t = t_first; t < end; t += WK) {
+    const size_t off = offs.at(i);
+    const bool bad = offs.bad >> i & 1;
+    load_v(off);
+    v4f s[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) s[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NK; ++u)
+#pragma unroll
+      for (int e = 0; e < KW; ++e) {
+        const float k = kf[u].get(e);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(k, qf[j][u * KW + e], s[j], 0, 0, 0);
+      }
+    if (++i == 64 && t + WK < end) {
+      i = 0;
+      offs.load(c, table, w, t + WK, WK, end, h, HD);
+    }
+    load_k(offs.at(min(i, 63)));                  // the last tile again after the last: a load without a branch
+    const int k0 = w.tile(t) * TILE;
+    const bool whole = !bad && k0 + TILE - 1 <= p_lo &&
+                       (a.window == 0 || k0 > p_hi - a.window || k0 + TILE <= a.sinks);   // every row sees every key
+    bool mixed = false;
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int key = k0 + 4 * q4 + v;
+          if (bad) s[j][v] = NAN;
+          if (!sees(qp[j], key, a.window, a.sinks)) s[j][v] = -INFINITY;
+        }
+      // V of keys that a row does not see must not reach it, not even times 0
+      bool odd = false;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          if (bad) vf[v][u].clear();
+          odd |= vf[v][u].wild();
+        }
+      mixed = __any(odd);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float mx = fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3]));
+      mx = fmaxf(mx, swap16(mx));
+      mx = fmaxf(mx, swap32(mx));
+      const float mn = fmaxf(mr[j], mx);
+      const float m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
+      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale2, -m2));
+        sum += s[j][v];
+      }
+      lr[j] = lr[j] * sc + sum;                   // this lane's keys; a row's four lanes add up at the end
+      mr[j] = mn;
+      if (__any(sc != 1.f)) {
+#pragma unroll
+        for (int u = 0; u < NDT; ++u) o[j][u] *= sc;
+      }
+    }
+    if (!mixed) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            const float x = vf[v][u].get(e);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              o[j][u * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[j][v], o[j][u * VW + e], 0, 0, 0);
+          }
+    } else {                                      // infinities or NaN beside a mask: key by key, where it is seen
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        for (int kq = 0; kq < 4; ++kq) {
+          const KT* vr = vp + off + (4 * kq + v) * HD;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const float p = __shfl(s[j][v], i16 + 16 * kq, 64);
+            if (!sees(qp[j], k0 + 4 * kq + v, a.window, a.sinks)) continue;
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+              for (int e = 0; e < VW; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  Piece<KT, 1> x;
+                  x.load(vr + 16 * VW * u + VW * (4 * q4 + r) + e);
+                  o[j][u * VW + e][r] = fmaf(p, x.get(0), o[j][u * VW + e][r]);
+                }
+          }
+        }
+    }
+  }
+  // the waves meet: their rows of O and (max, sum), then a weight for each
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float l = lr[j];
+    l += swap16(l);
+    l += swap32(l);
+    const int at = wave * R + j * 16 + i16;
+    if (q4 == 0) { pm[at] = mr[j]; pl[at] = l; }
+    float* row = po + at * LDO;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) row[16 * VW * u + VW * (4 * q4 + v) + e] = o[j][u * VW + e][v];
+  }
+  __syncthreads();
+  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
+  if (tid < R) {
+    float mx = -INFINITY, l = 0.f, f[WK];
+#pragma unroll
+    for (int u = 0; u < WK; ++u) mx = fmaxf(mx, pm[u * R + tid]);
+    const float m2 = mx == -INFINITY ? 0.f : mx * a.scale2;
+#pragma unroll
+    for (int u = 0; u < WK; ++u) {
+      f[u] = __builtin_amdgcn_exp2f(fmaf(pm[u * R + tid], a.scale2, -m2));
+      l = fmaf(f[u], pl[u * R + tid], l);
+    }
+    const int row = f0 + tid, tok = row / c.G;
+    const bool none = p0 + tok < 0;               // no key is seen
+#pragma unroll
+    for (int u = 0; u < WK; ++u) pm[u * R + tid] = alone ? none ? 0.f : f[u] / l : f[u];
+    if (row < rows) {
+      const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
+      if (!alone) {
+        float* d = a.ml + ((size_t)cut * c.T * c.Hq + at) * 2;
+        d[0] = mx;
+        d[1] = l;
+      } else if (a.lse) {
+        a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int NF = HD / 4;
+  for (int it = tid; it < R * NF; it += WK * 64) {
+    const int r = it / NF, d = (it - r * NF) * 4, row = f0 + r, tok = row / c.G;
+    if (row >= rows) break;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < WK; ++u) {
+      const float wt = pm[u * R + r];
+      const float4 x = *reinterpret_cast<const float4*>(po + (u * R + r) * LDO + d);
+      y.x = fmaf(wt, x.x, y.x); y.y = fmaf(wt, x.y, y.y); y.z = fmaf(wt, x.z, y.z); y.w = fmaf(wt, x.w, y.w);
+    }
+    const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
+    if (alone) store4(static_cast<QT*>(a.out) + at * HD + d, y.x, y.y, y.z, y.w);
+    else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + at) * HD + d) = y;
+  }
+}
+
+// Joins the cuts of rows that have several; one wave per row (token, query head).
+// R: the rows of a tile of the kernel before, whose walk says how many cuts there are.
+template <typename QT, int HD>
+__global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int R, int cuts) {
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= c.T * c.Hq) return;
+  const int m = at / c.Hq, g = (at - m * c.Hq) % c.G, seq = seq_of_row(c, m);
+  if (seq >= c.S) return;
+  int first, n;
+  seq_rows(c, seq, first, n);
+  if (m - first >= n) return;
+  const int p0 = seq_len(c, seq) - n, f0 = ((m - first) * c.G + g) / R * R;
+  const Walk w = walk_of(p0 + f0 / c.G, p0 + (min(f0 + R, n * c.G) - 1) / c.G, a.window, a.sinks);
+  if (w.n <= a.cut) return;                       // one cut: its workgroup wrote the answer
+  const int ns = min((w.n + a.cut - 1) / a.cut, cuts);
+  const size_t step = (size_t)c.T * c.Hq;
+  float mx = -INFINITY;
+  for (int s = lane; s < ns; s += 64) mx = fmaxf(mx, a.ml[(s * step + at) * 2]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+  const float m2 = mx == -INFINITY ? 0.f : mx * a.scale2;
+  constexpr int E = HD >= 64 ? HD / 64 : 1;       // dims per lane
+  float y[E] = {}, l = 0.f;
+  for (int s = 0; s < ns; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.ml + (s * step + at) * 2);
+    const float wt = __builtin_amdgcn_exp2f(fmaf(ml.x, a.scale2, -m2));
+    l = fmaf(wt, ml.y, l);
+    const float* p = a.part + (s * step + at) * HD;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = fmaf(wt, p[min(lane * E + e, HD - 1)], y[e]);
+  }
+  const bool none = p0 + (m - first) < 0;
+  if (lane * E < HD) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = none ? 0.f : y[e] / l;
+      QT* d = static_cast<QT*>(a.out) + (size_t)at * HD + lane * E + e;
+      if constexpr (sizeof(QT) == 4) *d = x;
+      else *d = to_bf16(x);
+    }
+  }
+  if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------ accounts of attention weight
+// mass[j] += sum over the rows of key head h that see j of exp(s_j - lse): with
+// the statistics known every weight is one exponential, and a workgroup that holds
+// its keys and walks the rows adds up without atomics, in one order.
+//   S = Q K^T: lane l holds rows 4 (l / 16) + v against key l % 16; the sum over rows stays in the lane.
+// A wave holds NK2 tiles of 16 keys in registers; four waves per workgroup.
+struct MassArgs {
+  Cache c;
+  const void* q; const float* lse; float* mass;   // [n_pages][Hkv][page]
+  float scale;
+  int window, sinks;
+};
+
+template <typename QT, typename KT, int HD, int NK2>
+__global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
+  using D = Dims<KT, HD>;
+  constexpr int KW = D::KW, NK = D::NK;
+  const Cache& c = a.c;
+  const int h = blockIdx.x, seq = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i16 = lane & 15, q4 = lane >> 4;
+  int first, n;
+  seq_rows(c, seq, first, n);
+  const int len = seq_len(c, seq), p0 = len - n;
+  const int k0 = (blockIdx.y * 4 + wave) * NK2 * TILE;
+  if (n == 0 || k0 >= len) return;
+  const int* table = c.table + seq * c.stride;
+  const KT* kp = static_cast<const KT*>(c.k);
+  float kf[NK2][NK * KW], sum[NK2];
+  size_t at[NK2];
+  bool bad[NK2];
+#pragma unroll
+  for (int j = 0; j < NK2; ++j) {
+    const int key0 = min(k0 + j * TILE, (len - 1) / TILE * TILE), e = table[key0 / c.page];
+    bad[j] = e < 0 || e >= c.n_pages;
+    at[j] = ((size_t)(bad[j] ? 0 : e) * c.Hkv + h) * c.page + key0 % c.page + i16;
+    sum[j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NK; ++t) {
+      Piece<KT, KW> x;
+      x.load(kp + at[j] * HD + t * 4 * KW + KW * q4);
+#pragma unroll
+      for (int e2 = 0; e2 < KW; ++e2) kf[j][t * KW + e2] = x.get(e2);
+    }
+  }
+  // the rows that can see a key of this wave
+  const int t_lo = max(0, k0 - p0);
+  int t_hi = n;
+  if (a.window > 0 && k0 >= a.sinks) t_hi = (int)min((int64_t)n, (int64_t)k0 + NK2 * TILE - 1 + a.window - p0);
+  for (int f0 = t_lo * c.G; f0 < t_hi * c.G; f0 += 16) {
+    const int f = min(f0 + i16, n * c.G - 1), tok = f / c.G;
+    const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
+    Piece<QT, KW> x[NK];
+#pragma unroll
+    for (int t = 0; t < NK; ++t) x[t].load(qr + t * 4 * KW + KW * q4);
+    float ls[4];
+    int p[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int fv = f0 + 4 * q4 + v, tv = min(fv, n * c.G - 1) / c.G;
+      p[v] = fv < n * c.G ? p0 + tv : -1;
+      ls[v] = a.lse[(size_t)(first + tv) * c.Hq + h * c.G + (min(fv, n * c.G - 1) - tv * c.G)];
+    }
+    v4f s[NK2];
+#pragma unroll
+    for (int j = 0; j < NK2; ++j) s[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < NK; ++t)
+#pragma unroll
+      for (int e = 0; e < KW; ++e) {
+        const float xq = x[t].get(e);
+#pragma unroll
+        for (int j = 0; j < NK2; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xq, kf[j][t * KW + e], s[j], 0, 0, 0);
+      }
+#pragma unroll
+    for (int j = 0; j < NK2; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale, -ls[v]) * LOG2E);
+        sum[j] += sees(p[v], k0 + j * TILE + i16, a.window, a.sinks) ? y : 0.f;
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < NK2; ++j) {
+    float y = sum[j];
+    y += swap16(y);
+    y += swap32(y);
+    if (q4 == 0 && k0 + j * TILE + i16 < len && !bad[j]) a.mass[at[j]] += y;
+  }
+}
+
+// ------------------------------------------------------------ eviction
+// Which slots of key head h of a sequence stay: n = min(len, keep) of them, the
+// first `sinks`, the last `recent`, and of the others those of most attention
+// weight, ties to the lowest slot.  A slot's rank is a 32-bit whole number that orders as the
+// weights do (NaN above all, a sure slot above that, none for slots past the length), so the
+// n-th largest is found bit by bit with one count each.
+//
+// One workgroup per (sequence, head); wave w owns a run of slots, lane by lane, NV per lane in registers
+// (NV 0: read again for each count).
+__device__ __forceinline__ uint32_t rank_of(float x) {
+  if (x != x) return 0xfffffffeu;
+  const uint32_t b = __float_as_uint(x + 0.f);    // -0 counts as 0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template <int NV>
+__global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass, int keep, int sinks, int recent,
+                                                      int* new_lens, int* kept) {
+  __shared__ int red[2][16], eq_of[16];
+  const int h = blockIdx.x, seq = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int len = seq_len(c, seq), n = min(len, keep);
+  const int per = NV > 0 ? NV : (len + 1023) / 1024;   // slots per lane
+  const int j0 = wave * per * 64 + lane;
+  const int* table = c.table + seq * c.stride;
+  int* out = kept + ((size_t)seq * c.Hkv + h) * keep;
+  if (tid == 0 && h == 0) new_lens[seq] = n;
+  for (int d = n + tid; d < keep; d += 1024) out[d] = -1;
+  if (n == 0) return;
+  auto rank_at = [&](int j) -> uint32_t {
+    if (j >= len) return 0;
+    if (j < sinks || j >= len - recent) return 0xffffffffu;
+    const int e = table[j / c.page];
+    return e < 0 || e >= c.n_pages ? 0xfffffffeu : rank_of(mass[((size_t)e * c.Hkv + h) * c.page + j % c.page]);
+  };
+  uint32_t r[NV > 0 ? NV : 1];
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r[i] = rank_at(j0 + i * 64);
+  }
+  auto at = [&](int i) -> uint32_t {
+    if constexpr (NV > 0) return r[i];
+    else return rank_at(j0 + i * 64);
+  };
+  // this wave's slots for which f holds
+  auto count = [&](auto f) {
+    int k = 0;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) k += f(r[i]);
+    } else {
+      for (int i = 0; i < per; ++i) k += f(at(i));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) k += __shfl_xor(k, d, 64);
+    return k;
+  };
+  uint32_t cut = 0;                               // the n-th largest rank, from its highest bit on
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t x = cut | 1u << bit;
+    const int k = count([&](uint32_t y) { return y >= x; });
+    if (lane == 0) red[bit & 1][wave] = k;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) all += red[bit & 1][u];
+    if (all >= n) cut = x;
+  }
+  const int more = count([&](uint32_t y) { return y > cut; }), same = count([&](uint32_t y) { return y == cut; });
+  __syncthreads();
+  if (lane == 0) { red[0][wave] = more; eq_of[wave] = same; }
+  __syncthreads();
+  int above = 0, pos = 0, ties = 0;               // slots above the cut in all; kept ones and ties before this wave
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    above += red[0][u];
+    if (u < wave) { pos += red[0][u]; ties += eq_of[u]; }
+  }
+  const int room = n - above;                     // ties that stay
+  auto put = [&](int i, uint32_t y) {
+    const uint64_t gt = __ballot(y > cut), eq = __ballot(y == cut), below = (1ull << lane) - 1;
+    const int gb = __popcll(gt & below), eb = __popcll(eq & below);
+    if (y > cut || (y == cut && ties + eb < room)) out[pos + gb + min(ties + eb, room)] = j0 + i * 64;
+    pos += __popcll(gt);
+    ties += __popcll(eq);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put(i, r[i]);
+  } else {
+    for (int i = 0; i < per; ++i) put(i, at(i));
+  }
+}
+
+// K, V and weight of the slots that stay, in their order, to the pages of `to`
+// [S][to_width]; a slot on a page outside the pool becomes NaN, one for such a
+// page is dropped.  Rows as 16-byte pieces, SLOTS slots of a head per workgroup.
+template <int PIECES, int SLOTS>
+__global__ __launch_bounds__(256) void move_kernel(Cache c, float* mass, const int* kept, int keep, const int* to,
+                                                   int64_t to_stride) {
+  constexpr int RPW = 256 / PIECES, U = SLOTS / RPW;   // rows at a time, times
+  static_assert(SLOTS % RPW == 0, "whole rows");
+  const int h = blockIdx.y, seq = blockIdx.z, piece = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES;
+  const int n = min(seq_len(c, seq), keep), d0 = blockIdx.x * SLOTS + r0;
+  if (blockIdx.x * SLOTS >= n) return;
+  const int* out = kept + ((size_t)seq * c.Hkv + h) * keep;
+  uint4 k[U], v[U];
+  float w[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int d = d0 + u * RPW, j = out[min(d, n - 1)], e = c.table[seq * c.stride + j / c.page];
+    const bool ok = e >= 0 && e < c.n_pages;
+    const size_t row = ((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + j % c.page;
+    k[u] = static_cast<const uint4*>(c.k)[row * PIECES + piece];
+    v[u] = static_cast<const uint4*>(c.v)[row * PIECES + piece];
+    w[u] = mass[row];
+    if (!ok) {
+      k[u] = v[u] = make_uint4(~0u, ~0u, ~0u, ~0u);
+      w[u] = NAN;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int d = d0 + u * RPW;
+    if (d >= n) break;
+    const int e = to[seq * to_stride + d / c.page];
+    if (e < 0 || e >= c.n_pages) continue;
+    const size_t row = ((size_t)e * c.Hkv + h) * c.page + d % c.page;
+    static_cast<uint4*>(c.k)[row * PIECES + piece] = k[u];
+    static_cast<uint4*>(c.v)[row * PIECES + piece] = v[u];
+    if (piece == 0) mass[row] = w[u];
+  }
+}
+
+}  // namespace paged
+}  // namespace sk

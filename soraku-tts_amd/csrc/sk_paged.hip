@@ -1,0 +1,255 @@
+// Operator API: the attention half of a trunk layer over a cache in pages
+// (append, attention, accounts of attention weight, eviction), on a caller
+// stream.  The layer's arithmetic is that of the reference's trunk
+// (modeling_qwen3.py:237-262); pages, window and eviction have no counterpart there.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "sk_error.h"
+#include "sk_paged.h"
+#include "soraku_mi355x.h"
+
+using namespace sk;
+using namespace sk::paged;
+
+namespace {
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// What every entry point asks of its sizes.
+int check_sizes(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages, int32_t width,
+                int64_t stride) {
+  SK_CHECK(T >= 0 && S > 0, SK_EINVAL, "T must not be negative and S must be positive");
+  SK_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 4096, SK_EINVAL,
+           "Hq must be a positive multiple of Hkv, at most 4096");
+  SK_CHECK(hd == 16 || hd == 32 || hd == 64 || hd == 128, SK_EINVAL, "hd must be a power of two in [16, 128]");
+  SK_CHECK(page > 0 && page % TILE == 0, SK_EINVAL, "page must be a positive multiple of %d", TILE);
+  SK_CHECK(n_pages > 0 && width > 0 && stride >= width, SK_EINVAL,
+           "n_pages and width must be positive, and the table's rows at least width entries apart");
+  SK_CHECK((int64_t)page * width <= INT32_MAX / 2, SK_EINVAL, "width * page must be at most 2^30 tokens");
+  SK_CHECK((int64_t)T * Hq <= INT32_MAX / 2, SK_EINVAL, "T * Hq must be at most 2^30");
+  return SK_OK;
+}
+int check_types(int32_t xdtype, int32_t kvdtype) {
+  SK_CHECK((xdtype == SK_F32 && (kvdtype == SK_F32 || kvdtype == SK_BF16)) || (xdtype == SK_BF16 && kvdtype == SK_BF16),
+           SK_EINVAL, "types must be float32 on either cache, or bfloat16 on a bfloat16 cache");
+  return SK_OK;
+}
+int check_window(float scale, int32_t window, int32_t sinks) {
+  SK_CHECK(scale > 0.f && isfinite(scale), SK_EINVAL, "scale must be positive and finite");
+  SK_CHECK(window >= 0 && sinks >= 0, SK_EINVAL, "window and sinks must not be negative");
+  return SK_OK;
+}
+
+Cache cache_of(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t page, int32_t n_pages, int32_t width,
+               int64_t stride, const int32_t* starts, const int32_t* lens, const int32_t* table, const void* k,
+               const void* v) {
+  return {const_cast<void*>(k), const_cast<void*>(v), table, stride, width, starts, lens, T, S, Hq, Hkv, Hq / Hkv,
+          n_pages, page};
+}
+
+template <int N> using Int = std::integral_constant<int, N>;
+template <typename F>
+void with_hd(int hd, F&& f) {
+  switch (hd) {
+    case 16: f(Int<16>{}); break;
+    case 32: f(Int<32>{}); break;
+    case 64: f(Int<64>{}); break;
+    default: f(Int<128>{}); break;
+  }
+}
+// f(a value of the activations' type, one of the cache's)
+template <typename F>
+void with_types(int32_t xdtype, int32_t kvdtype, F&& f) {
+  if (xdtype == SK_BF16) f(uint16_t{}, uint16_t{});
+  else if (kvdtype == SK_BF16) f(float{}, uint16_t{});
+  else f(float{}, float{});
+}
+
+// How an attention call is cut up: R rows per workgroup, `cut` tiles of keys
+// per cut.
+struct Plan {
+  int R, blocks, cut, cuts;
+};
+Plan plan_attention(int T, int S, int Hq, int Hkv, int page, int width, int window, int sinks) {
+  Plan p;
+  const int G = Hq / Hkv;
+  p.R = (int64_t)T * G > 16ll * S ? 32 : 16;
+  p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - 1)) / p.R);
+  int64_t tiles = (int64_t)page * width / TILE;   // what a row tile can walk at most
+  if (window > 0)
+    tiles = std::min(tiles, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
+  const int64_t base = (int64_t)p.blocks * Hkv;
+  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(base, 1), tiles / 16));
+  p.cut = (int)((tiles + cuts - 1) / cuts);
+  p.cuts = (int)((tiles + p.cut - 1) / p.cut);
+  return p;
+}
+int64_t workspace_of(const Plan& p, int T, int Hq, int hd) {
+  return p.cuts > 1 ? (int64_t)p.cuts * T * Hq * (hd + 2) * 4 : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sk_op_paged_append(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
+                       int32_t n_pages, int32_t width, int64_t table_stride, int32_t xdtype, int32_t kvdtype, float eps,
+                       const void* qkv, const float* q_gain, const float* k_gain, const float* inv_freq,
+                       const int32_t* positions, const int32_t* starts, const int32_t* lens, const int32_t* table,
+                       void* k_pages, void* v_pages, float* mass, void* q_out) {
+  if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, n_pages, width, table_stride)) return rc;
+  if (int rc = check_types(xdtype, kvdtype)) return rc;
+  SK_CHECK(eps >= 0.f && isfinite(eps), SK_EINVAL, "eps must be finite and not negative");
+  if (T == 0) return SK_OK;
+  SK_CHECK(qkv && inv_freq && positions && starts && lens && table && k_pages && v_pages && q_out, SK_EINVAL,
+           "NULL operand");
+  SK_CHECK(!q_gain == !k_gain, SK_EINVAL, "gains of q and k come together");
+  SK_CHECK(aligned16(qkv) && aligned16(q_gain) && aligned16(k_gain) && aligned16(k_pages) && aligned16(v_pages) &&
+               aligned16(q_out),
+           SK_EINVAL, "operands must be 16-byte aligned");
+  const Cache c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, v_pages);
+  with_hd(hd, [&](auto d) {
+    with_types(xdtype, kvdtype, [&](auto x, auto k) {
+      using X = decltype(x);
+      using K = decltype(k);
+      hipLaunchKernelGGL((append_kernel<X, K, decltype(d)::value>), dim3(T), dim3(256), 0, (hipStream_t)stream, c,
+                         (const X*)qkv, q_gain, k_gain, inv_freq, positions, eps, mass, (X*)q_out);
+    });
+  });
+  SK_HIP(hipGetLastError());
+  return SK_OK;
+}
+
+int sk_op_paged_attention_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
+                                    int32_t width, int32_t xdtype, int32_t kvdtype, int32_t window, int32_t sinks,
+                                    int64_t* bytes) {
+  if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, 1, width, width)) return rc;
+  if (int rc = check_types(xdtype, kvdtype)) return rc;
+  if (int rc = check_window(1.f, window, sinks)) return rc;
+  SK_CHECK(bytes, SK_EINVAL, "NULL operand");
+  *bytes = workspace_of(plan_attention(T, S, Hq, Hkv, page, width, window, sinks), T, Hq, hd);
+  return SK_OK;
+}
+
+int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
+                          int32_t n_pages, int32_t width, int64_t table_stride, int32_t xdtype, int32_t kvdtype,
+                          float scale, int32_t window, int32_t sinks, const void* q, const void* k_pages,
+                          const void* v_pages, const int32_t* table, const int32_t* starts, const int32_t* lens,
+                          void* out, float* lse, void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, n_pages, width, table_stride)) return rc;
+  if (int rc = check_types(xdtype, kvdtype)) return rc;
+  if (int rc = check_window(scale, window, sinks)) return rc;
+  if (T == 0) return SK_OK;
+  SK_CHECK(q && k_pages && v_pages && table && starts && lens && out, SK_EINVAL, "NULL operand");
+  SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace), SK_EINVAL,
+           "operands must be 16-byte aligned");
+  const Plan p = plan_attention(T, S, Hq, Hkv, page, width, window, sinks);
+  SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= workspace_of(p, T, Hq, hd)), SK_EINVAL,
+           "the workspace must hold %lld bytes", (long long)workspace_of(p, T, Hq, hd));
+  SK_CHECK(p.blocks <= 65535 && p.cuts <= 65535, SK_EINVAL, "too many rows for one call");
+  AttendArgs a;
+  a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, v_pages);
+  a.q = q; a.out = out; a.lse = lse;
+  a.scale2 = scale * LOG2E;
+  a.window = window; a.sinks = sinks;
+  a.cut = p.cut;
+  a.part = (float*)workspace;
+  a.ml = a.part ? a.part + (size_t)p.cuts * T * Hq * hd : nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  hipError_t err = hipSuccess;
+  with_hd(hd, [&](auto d) {
+    with_types(xdtype, kvdtype, [&](auto x, auto k) {
+      using X = decltype(x);
+      using K = decltype(k);
+      constexpr int HD = decltype(d)::value;
+      const dim3 grid(Hkv, p.blocks, p.cuts);
+      if (p.R == 32) hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 1, 4>), grid, dim3(256), 0, st, a);
+      err = hipGetLastError();
+      if (p.cuts == 1 || err != hipSuccess) return;
+      hipLaunchKernelGGL((combine_kernel<X, HD>), dim3((T * Hq + 3) / 4), dim3(256), 0, st, a, p.R, p.cuts);
+      err = hipGetLastError();
+    });
+  });
+  SK_HIP(err);
+  return SK_OK;
+}
+
+int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
+                               int32_t n_pages, int32_t width, int64_t table_stride, int32_t xdtype, int32_t kvdtype,
+                               float scale, int32_t window, int32_t sinks, const void* q, const float* lse,
+                               const void* k_pages, const int32_t* table, const int32_t* starts, const int32_t* lens,
+                               float* mass) {
+  if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, n_pages, width, table_stride)) return rc;
+  if (int rc = check_types(xdtype, kvdtype)) return rc;
+  if (int rc = check_window(scale, window, sinks)) return rc;
+  if (T == 0) return SK_OK;
+  SK_CHECK(q && lse && k_pages && table && starts && lens && mass, SK_EINVAL, "NULL operand");
+  SK_CHECK(aligned16(q) && aligned16(k_pages), SK_EINVAL, "operands must be 16-byte aligned");
+  SK_CHECK(S <= 65535, SK_EINVAL, "S must be at most 65535");
+  MassArgs a;
+  a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, nullptr);
+  a.q = q; a.lse = lse; a.mass = mass;
+  a.scale = scale; a.window = window; a.sinks = sinks;
+  constexpr int NK2 = 2;
+  const int64_t blocks = ((int64_t)page * width + 64 * NK2 - 1) / (64 * NK2);
+  SK_CHECK(blocks <= 65535, SK_EINVAL, "width * page must be at most %d tokens", 65535 * 64 * NK2);
+  with_hd(hd, [&](auto d) {
+    with_types(xdtype, kvdtype, [&](auto x, auto k) {
+      hipLaunchKernelGGL((mass_kernel<decltype(x), decltype(k), decltype(d)::value, NK2>), dim3(Hkv, (unsigned)blocks, S),
+                         dim3(256), 0, (hipStream_t)stream, a);
+    });
+  });
+  SK_HIP(hipGetLastError());
+  return SK_OK;
+}
+
+int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages, int32_t width,
+                      int64_t table_stride, int32_t kvdtype, int32_t keep, int32_t sinks, int32_t recent, void* k_pages,
+                      void* v_pages, float* mass, const int32_t* table, const int32_t* lens, const int32_t* to,
+                      int64_t to_stride, int32_t to_width, int32_t* new_lens, int32_t* kept) {
+  if (int rc = check_sizes(0, S, Hkv, Hkv, hd, page, n_pages, width, table_stride)) return rc;
+  if (int rc = check_types(SK_F32, kvdtype)) return rc;
+  SK_CHECK(keep > 0 && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= keep, SK_EINVAL,
+           "keep must be positive, sinks and recent not negative, and their sum at most keep");
+  SK_CHECK(to_width > 0 && to_stride >= to_width && (int64_t)to_width * page >= keep, SK_EINVAL,
+           "the new table must have pages for keep tokens");
+  SK_CHECK(S <= 65535 && Hkv <= 65535 && (int64_t)S * Hkv * keep <= INT32_MAX, SK_EINVAL,
+           "S must be at most 65535 and S * Hkv * keep at most 2^31");
+  SK_CHECK(k_pages && v_pages && mass && table && lens && to && new_lens && kept, SK_EINVAL, "NULL operand");
+  SK_CHECK(table != to, SK_EINVAL, "the new table must have pages of its own");
+  SK_CHECK(aligned16(k_pages) && aligned16(v_pages), SK_EINVAL, "operands must be 16-byte aligned");
+  const Cache c = cache_of(0, S, Hkv, Hkv, page, n_pages, width, table_stride, nullptr, lens, table, k_pages, v_pages);
+  const hipStream_t st = (hipStream_t)stream;
+  const int64_t cap = (int64_t)page * width;
+  auto choose = [&](auto nv) {
+    hipLaunchKernelGGL((choose_kernel<decltype(nv)::value>), dim3(Hkv, S), dim3(1024), 0, st, c, mass, keep, sinks,
+                       recent, new_lens, kept);
+  };
+  if (cap <= 4 * 1024) choose(Int<4>{});
+  else if (cap <= 16 * 1024) choose(Int<16>{});
+  else if (cap <= 32 * 1024) choose(Int<32>{});
+  else choose(Int<0>{});
+  SK_HIP(hipGetLastError());
+  const int pieces = hd * (kvdtype == SK_BF16 ? 2 : 4) / 16;
+  auto move = [&](auto np) {
+    constexpr int P = decltype(np)::value, SLOTS = 256 / P * 4;
+    hipLaunchKernelGGL((move_kernel<P, SLOTS>), dim3((keep + SLOTS - 1) / SLOTS, Hkv, S), dim3(256), 0, st, c, mass,
+                       (const int*)kept, keep, to, to_stride);
+  };
+  switch (pieces) {
+    case 2: move(Int<2>{}); break;
+    case 4: move(Int<4>{}); break;
+    case 8: move(Int<8>{}); break;
+    case 16: move(Int<16>{}); break;
+    default: move(Int<32>{}); break;
+  }
+  SK_HIP(hipGetLastError());
+  return SK_OK;
+}
+
+}  // extern "C"

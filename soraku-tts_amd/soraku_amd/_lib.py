@@ -47,6 +47,7 @@ _P = C.c_void_p
 _I = C.c_int32
 _F = C.c_float
 _D = C.c_double
+_L = C.c_int64
 _PI64 = C.POINTER(C.c_int64)
 _PI32 = C.POINTER(C.c_int32)
 _PF = C.POINTER(C.c_float)
@@ -88,6 +89,11 @@ PROTOTYPES = {
     "sk_op_prefix_add": (_I, [_P, _I, _I, _I, _F, _P, _P, _P, _P]),
     "sk_op_sampling_prep": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P]),
     "sk_op_sample": (_I, [_P, _I, _I, _P, _F, _I, _I, _I, _I, _I, _F, _I, _F, _D, _P]),
+    "sk_op_paged_append": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, *[_P] * 12]),
+    "sk_op_paged_attention_workspace": (_I, [*[_I] * 11, _PI64]),
+    "sk_op_paged_attention": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 9, _L]),
+    "sk_op_paged_attention_mass": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 7]),
+    "sk_op_paged_evict": (_I, [_P, *[_I] * 6, _L, *[_I] * 4, *[_P] * 6, _L, _I, _P, _P]),
 }
 
 

@@ -9,6 +9,7 @@ as the native path does (model.py:582-584), not -1e30 (tilelang_kernels.py:31).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 from . import _lib
 from ._lib import check, lib
@@ -139,4 +140,165 @@ def sample(V: int, bos_id: int, eos_id: int, pad_id: int):
                                  int(bool(mask_eos_q0)), bos_id, eos_id, pad_id, float(temperature),
                                  int(top_k or 0), float(top_p or 0.0), float(u), _ptr(out)))
         return out
+    return kernel
+
+
+# ---- attention over a cache in pages (no counterpart in the reference) ----
+# Pools k_pages / v_pages [n_pages, Hkv, page, hd] (float32 or bfloat16), table
+# [S, width] int32 (any row stride, so a slice of a wider one will do), starts
+# [S + 1] and lens [S] int32, all on the HIP device: sequence s's new tokens are
+# the packed rows starts[s]:starts[s + 1] and lens[s] its length with them.
+# include/soraku_mi355x.h holds the whole contract.
+
+def _need(t, name, dtype, dev, *shape):
+    if t.dtype is not dtype or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {dev}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
+    return t.data_ptr()
+
+
+def _table(t, name, dev, S):
+    import torch
+
+    if t.dtype is not torch.int32 or t.device != dev or t.dim() != 2 or t.shape[0] != S or (
+            t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor [{S}, pages] on {dev} with its rows contiguous")
+    if S > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}'s rows overlap")
+    return t.data_ptr(), max(t.stride(0), t.shape[1]) if S > 1 else t.shape[1], t.shape[1]
+
+
+def _pool(k_pages, v_pages, Hkv, page, hd):
+    if k_pages.dim() != 4:
+        raise ValueError("pages must be [n_pages, Hkv, page, hd]")
+    if not k_pages.is_cuda:
+        raise ValueError("operands must live on the HIP device")
+    dev, n = k_pages.device, k_pages.shape[0]
+    kp = _need(k_pages, "k_pages", k_pages.dtype, dev, n, Hkv, page, hd)
+    vp = None if v_pages is None else _need(v_pages, "v_pages", k_pages.dtype, dev, n, Hkv, page, hd)
+    return dev, n, kp, vp, _wdtype(k_pages)
+
+
+class _On:
+    """The device of the operands as the current one, where it is another."""
+
+    def __init__(self, dev):
+        import torch
+
+        self._guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(*sizes) -> int:
+    n = C.c_int64()
+    check(lib().sk_op_paged_attention_workspace(*sizes, C.byref(n)))
+    return n.value
+
+
+def paged_append(Hq: int, Hkv: int, hd: int, page: int, eps: float):
+    """New tokens into the cache: per-head RMSNorm of q and k (gains ``[hd]``, or
+    both None for none), rotation by ``positions * inv_freq``, k and v to
+    their slots; returns q ``[T, Hq, hd]`` of qkv's dtype (``out``, if given).
+    ``mass`` (accounts, ``[n_pages, Hkv, page]`` float32) is set to 0 at the new slots."""
+    def kernel(qkv, q_gain, k_gain, inv_freq, positions, starts, lens, table, k_pages, v_pages, mass=None, out=None):
+        import torch
+
+        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
+        T, S, i32, f32 = qkv.shape[0], lens.shape[0], torch.int32, torch.float32
+        tp, stride, width = _table(table, "table", dev, S)
+        if out is None:
+            out = torch.empty(T, Hq, hd, device=dev, dtype=qkv.dtype)
+        gains = [None if g is None else _need(g, "gain", f32, dev, hd) for g in (q_gain, k_gain)]
+        with _On(dev):
+            check(lib().sk_op_paged_append(
+                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, _wdtype(qkv), kd, eps,
+                _need(qkv, "qkv", qkv.dtype, dev, T, (Hq + 2 * Hkv) * hd), *gains,
+                _need(inv_freq, "inv_freq", f32, dev, hd // 2), _need(positions, "positions", i32, dev, T),
+                _need(starts, "starts", i32, dev, S + 1), _need(lens, "lens", i32, dev, S), tp, kp, vp,
+                None if mass is None else _need(mass, "mass", f32, dev, n, Hkv, page),
+                _need(out, "out", qkv.dtype, dev, T, Hq, hd)))
+        return out
+    return kernel
+
+
+def paged_attention(Hq: int, Hkv: int, hd: int, page: int, scale: float | None = None, window: int = 0,
+                    sinks: int = 0):
+    """out ``[T, Hq, hd]`` = softmax(scale q k^T) v of the new tokens over their
+    sequences' slots, causal; with a ``window`` only the last ``window`` slots and the
+    first ``sinks``.  ``scale`` defaults to hd ** -0.5.  ``lse`` ``[T, Hq]`` float32,
+    if given, receives the softmax's logarithms.  Tokens that see nothing give 0 and -inf."""
+    scale = hd ** -0.5 if scale is None else float(scale)
+
+    def kernel(q, k_pages, v_pages, table, starts, lens, out=None, lse=None):
+        import torch
+
+        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
+        T, S, xd = q.shape[0], lens.shape[0], _wdtype(q)
+        tp, stride, width = _table(table, "table", dev, S)
+        if out is None:
+            out = torch.empty(T, Hq, hd, device=dev, dtype=q.dtype)
+        with _On(dev):
+            size = _attention_workspace(T, S, Hq, Hkv, hd, page, width, xd, kd, window, sinks)
+            ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+            check(lib().sk_op_paged_attention(
+                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,
+                sinks, _need(q, "q", q.dtype, dev, T, Hq, hd), kp, vp, tp, _need(starts, "starts", torch.int32, dev, S + 1),
+                _need(lens, "lens", torch.int32, dev, S), _need(out, "out", q.dtype, dev, T, Hq, hd),
+                None if lse is None else _need(lse, "lse", torch.float32, dev, T, Hq),
+                ws.data_ptr() if size else None, size))
+        return out
+    return kernel
+
+
+def paged_attention_mass(Hq: int, Hkv: int, hd: int, page: int, scale: float | None = None, window: int = 0,
+                         sinks: int = 0):
+    """Adds the weight every slot got in the ``paged_attention`` call of the same
+    arguments (its ``q`` and ``lse``) to ``mass`` ``[n_pages, Hkv, page]`` float32, summed over
+    tokens and the query heads that share a key head; returns ``mass``."""
+    scale = hd ** -0.5 if scale is None else float(scale)
+
+    def kernel(q, lse, k_pages, table, starts, lens, mass):
+        import torch
+
+        dev, n, kp, _, kd = _pool(k_pages, None, Hkv, page, hd)
+        T, S, f32 = q.shape[0], lens.shape[0], torch.float32
+        tp, stride, width = _table(table, "table", dev, S)
+        with _On(dev):
+            check(lib().sk_op_paged_attention_mass(
+                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, _wdtype(q), kd, scale,
+                window, sinks, _need(q, "q", q.dtype, dev, T, Hq, hd), _need(lse, "lse", f32, dev, T, Hq), kp, tp,
+                _need(starts, "starts", torch.int32, dev, S + 1), _need(lens, "lens", torch.int32, dev, S),
+                _need(mass, "mass", f32, dev, n, Hkv, page)))
+        return mass
+    return kernel
+
+
+def paged_evict(Hkv: int, hd: int, page: int, keep: int, sinks: int = 0, recent: int = 0):
+    """Cuts caches back to ``keep`` slots per key head: the first ``sinks``, the last
+    ``recent``, and of the others those of the largest accounts (ties to the lowest slot) move in
+    order, with their accounts, to the pages of ``to`` ``[S, pages]``, none of which may be in ``table``.
+    Returns the new lengths ``[S]`` and the old slots ``[S, Hkv, keep]`` (-1 past the length), int32."""
+    def kernel(k_pages, v_pages, mass, table, lens, to):
+        import torch
+
+        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
+        S = lens.shape[0]
+        tp, stride, width = _table(table, "table", dev, S)
+        dp, to_stride, to_width = _table(to, "to", dev, S)
+        new_lens = torch.empty(S, device=dev, dtype=torch.int32)
+        kept = torch.empty(S, Hkv, keep, device=dev, dtype=torch.int32)
+        with _On(dev):
+            check(lib().sk_op_paged_evict(
+                torch.cuda.current_stream(dev).cuda_stream, S, Hkv, hd, page, n, width, stride, kd, keep, sinks, recent, kp, vp,
+                _need(mass, "mass", torch.float32, dev, n, Hkv, page), tp, _need(lens, "lens", torch.int32, dev, S), dp,
+                to_stride, to_width, new_lens.data_ptr(), kept.data_ptr()))
+        return new_lens, kept
     return kernel

@@ -1,0 +1,247 @@
+"""The paged-cache operators without a GPU: what their entry points refuse
+(before any HIP call), what they launch, and the 64-bit oracle of their GPU tests against
+a second form."""
+
+import ctypes as C
+import math
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+from conftest import ROOT
+
+P = 4096          # an aligned address that nothing reads
+
+
+@pytest.fixture(scope="module")
+def L():
+    from soraku_amd import _lib
+
+    return _lib.load()
+
+
+APPEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, eps=1e-6,
+              qkv=P, q_gain=P, k_gain=P, inv_freq=P, positions=P, starts=P, lens=P, table=P, k=P, v=P, mass=None, out=P)
+ATTEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
+              window=0, sinks=0, q=P, k=P, v=P, table=P, starts=P, lens=P, out=P, lse=None, ws=None, ws_bytes=0)
+MASS = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
+            window=0, sinks=0, q=P, lse=P, k=P, table=P, starts=P, lens=P, mass=P)
+EVICT = dict(stream=None, S=2, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, kd=1, keep=32, sinks=4, recent=8,
+             k=P, v=P, mass=P, table=P, lens=P, to=2 * P, to_stride=2, to_width=2, new_lens=P, kept=P)
+ENTRY = {"append": ("sk_op_paged_append", APPEND), "attention": ("sk_op_paged_attention", ATTEND),
+         "mass": ("sk_op_paged_attention_mass", MASS), "evict": ("sk_op_paged_evict", EVICT)}
+
+SIZES = [("S", 0), ("Hkv", 0), ("Hkv", -8), ("hd", 48), ("hd", 256), ("hd", 0), ("page", 0), ("page", 24), ("page", -16),
+         ("n_pages", 0), ("width", 0), ("stride", 3), ("width", 2 ** 27), ("kd", 2)]
+ROWS = [("T", -1), ("T", 2 ** 27), ("Hq", 12), ("Hq", 0), ("Hq", 8192), ("xd", 2), ("xd", 3)]
+WINDOW = [("scale", 0.0), ("scale", -1.0), ("scale", math.inf), ("scale", math.nan), ("window", -1), ("sinks", -1)]
+BAD = {
+    "append": [*ROWS, ("eps", -1.0), ("eps", math.nan), ("q_gain", None), ("k_gain", None), ("qkv", P + 4), ("v", P + 8),
+               ("out", P + 2), ("q_gain", P + 4)] + [(n, None) for n in ("qkv", "inv_freq", "positions", "starts", "lens",
+                                                                         "table", "k", "v", "out")],
+    "attention": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("out", P + 8), ("ws", P + 4)] + [
+        (n, None) for n in ("q", "k", "v", "table", "starts", "lens", "out")],
+    "mass": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2)] + [(n, None) for n in ("q", "lse", "k", "table", "starts", "lens",
+                                                                              "mass")],
+    "evict": [("keep", 0), ("keep", -5), ("sinks", -1), ("recent", -1), ("sinks", 25), ("sinks", 2 ** 31 - 1), ("keep", 33),
+              ("to_width", 0), ("to_stride", 1), ("to", P), ("k", P + 4), ("v", P + 4)] + [
+                  (n, None) for n in ("k", "v", "mass", "table", "lens", "to", "new_lens", "kept")],
+}
+
+
+@pytest.mark.parametrize("entry,field,value", [(e, *b) for e in BAD for b in SIZES + BAD[e]])
+def test_refusals(L, entry, field, value):
+    from soraku_amd._lib import SK_EINVAL
+
+    name, good = ENTRY[entry]
+    args = dict(good)
+    assert field in args
+    args[field] = value
+    if field == "width":
+        args["stride"] = value
+    assert getattr(L, name)(*args.values()) == SK_EINVAL
+    assert L.sk_last_error().decode()
+
+
+@pytest.mark.parametrize("entry", ["append", "attention", "mass"])
+def test_bf16_activations_need_a_bf16_cache(L, entry):
+    name, good = ENTRY[entry]
+    assert getattr(L, name)(*dict(good, xd=1, kd=0).values()) == -1
+    assert "bfloat16" in L.sk_last_error().decode()
+
+
+def test_attention_asks_for_its_workspace(L):
+    from soraku_amd._lib import SK_EINVAL, SK_OK
+
+    n = C.c_int64(-1)
+    sizes = (2, 2, 16, 8, 128, 16, 4096, 0, 1, 0, 0)
+    assert L.sk_op_paged_attention_workspace(*sizes, C.byref(n)) == SK_OK and n.value > 0
+    args = dict(ATTEND, T=2, width=4096, stride=4096, ws=P, ws_bytes=n.value - 1)
+    assert L.sk_op_paged_attention(*args.values()) == SK_EINVAL
+    assert str(n.value) in L.sk_last_error().decode()
+    assert L.sk_op_paged_attention_workspace(*sizes, None) == SK_EINVAL
+    assert L.sk_op_paged_attention_workspace(2, 0, *sizes[2:], C.byref(n)) == SK_EINVAL
+
+
+def test_python_refusals():
+    """Wrong devices, shapes and types raise before the library is called."""
+    from soraku_amd import ops
+
+    k = torch.zeros(4, 2, 16, 16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="HIP device"):
+        ops.paged_attention(4, 2, 16, 16)(torch.zeros(1, 4, 16), k, k, i[:, None], i, i)
+    with pytest.raises(ValueError, match="pages must be"):
+        ops.paged_evict(2, 16, 16, 4)(k[0], k[0], k, i[:, None], i, i[:, None])
+    cpu = torch.device("cpu")
+    for bad in (torch.zeros(2, 3), torch.zeros(3, 2).t(), torch.zeros(2, 3, dtype=torch.float64)[:, :2]):
+        with pytest.raises(ValueError, match="must be a contiguous"):
+            ops._need(bad, "x", torch.float32, cpu, 2, 2)
+    for bad in (i, i[:, None].long(), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32).t(),
+                torch.zeros(1, 3, dtype=torch.int32).expand(2, 3)):
+        with pytest.raises(ValueError):
+            ops._table(bad, "table", cpu, 2)
+    wide = torch.zeros(2, 7, dtype=torch.int32)
+    assert ops._table(wide[:, :3], "table", cpu, 2)[1:] == (7, 3)
+    assert ops._table(wide[:1, :3], "table", cpu, 1)[1:] == (3, 3)
+
+
+# ------------------------------------------------------------------ launches (stand-in HIP runtime)
+
+SCRIPT = '''
+import json
+import test_paged_cpu as t
+cases = json.load(open(sys.argv[3]))
+out = []
+for entry, change in cases:
+    name, good = t.ENTRY[entry]
+    args = dict(good, **change)
+    if entry == "attention":
+        n = C.c_int64()
+        _lib.check(L.sk_op_paged_attention_workspace(*[args[k] for k in ("T", "S", "Hq", "Hkv", "hd", "page", "width", "xd",
+                                                                         "kd", "window", "sinks")], C.byref(n)))
+        args.update(ws=t.P if n.value else None, ws_bytes=n.value)
+    calls()
+    rc = getattr(L, name)(*args.values())
+    cs = calls()
+    out.append([rc, [c[0] for c in cs], kernels(cs), args.get("ws_bytes", 0)])
+    stub.stub_fail(b"hipLaunchKernel", 0)
+    out[-1].append(getattr(L, name)(*args.values()))
+    stub.stub_fail(b"", -1)
+    calls()
+print(json.dumps(out))
+'''
+
+
+@pytest.fixture(scope="module")
+def launches(tmp_path_factory):
+    tmp = tmp_path_factory.mktemp("stub")
+    so = tmp / "stub.so"
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    os.path.join(ROOT, "tests", "hip_host_stub.cpp"), "-o", str(so)], check=True)
+
+    def run(cases):
+        import json
+
+        (tmp / "s.py").write_text(SCRIPT)
+        (tmp / "c.json").write_text(json.dumps(cases))
+        env = dict(os.environ, PYTHONPATH=os.path.join(ROOT, "tests"))
+        r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "host_engine.py"), str(so), str(tmp / "s.py"),
+                            str(tmp / "c.json")], capture_output=True, text=True, env=env)
+        assert r.returncode == 0, r.stderr
+        return json.loads(r.stdout.strip().splitlines()[-1])
+    return run
+
+
+def test_launches(launches):
+    """Nothing but kernels is asked of the device, a launch that fails is an
+    error, and no tokens means no launch."""
+    from soraku_amd._lib import SK_EHIP, SK_OK
+
+    cases = [[e, c] for e in ENTRY for c in ({}, {"kd": 0}, {"hd": 16, "stride": 9})]
+    cases += [["attention", {"T": 1, "S": 1, "width": 4096, "stride": 4096}]]
+    for (entry, _), (rc, calls, kern, ws, failed) in zip(cases, launches(cases)):
+        assert rc == SK_OK and set(calls) == {"hipLaunchKernel"} and failed == SK_EHIP
+        assert len(kern) == (2 if entry == "evict" or ws else 1)
+        for _, grid in kern:
+            assert all(0 < g <= (2 ** 31 - 1 if i == 0 else 65535) for i, g in enumerate(grid))
+    for entry in ("append", "attention", "mass"):
+        (rc, calls, *_), = launches([[entry, {"T": 0}]])
+        assert rc == SK_OK and calls == []
+
+
+def test_attention_plans_cover_rows_and_keys(launches):
+    """Every row tile has a workgroup whatever way T rows fall on S sequences,
+    and the cuts reach the table's end."""
+    rng = np.random.default_rng(1)
+    cases = []
+    for _ in range(60):
+        hkv = int(rng.choice([1, 2, 3, 8]))
+        cases.append(["attention", dict(T=int(rng.integers(1, 400)), S=int(rng.integers(1, 40)), Hkv=hkv,
+                                        Hq=hkv * int(rng.integers(1, 9)), width=int(rng.integers(1, 300)), stride=300,
+                                        page=16 * int(rng.integers(1, 20)), window=int(rng.choice([0, 1, 700])),
+                                        sinks=int(rng.choice([0, 5])))])
+    for (_, c), (rc, _, kern, ws, _) in zip(cases, launches(cases)):
+        assert rc == 0
+        (name, grid) = kern[0]
+        R, G = rows_of(name), c["Hq"] // c["Hkv"]
+        assert grid[0] == c["Hkv"]
+        for _ in range(20):                          # rows of the sequences, some with none
+            cuts = np.sort(rng.integers(0, c["T"] + 1, c["S"] - 1))
+            n = np.diff(np.concatenate(([0], cuts, [c["T"]])))
+            assert sum(-(-int(x) * G // R) for x in n) <= grid[1]
+        assert ws == (grid[2] * c["T"] * c["Hq"] * (128 + 2) * 4 if grid[2] > 1 else 0)
+
+
+def rows_of(kernel):
+    """Rows of a workgroup, by the kernel's name and template arguments."""
+    import re
+
+    args = [int(x) for x in re.findall(r"Li(\d+)E", kernel)]
+    assert "attend_rows_kernel" in kernel, kernel
+    return 16 * args[1]
+
+
+# ------------------------------------------------------------------ the oracle
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3, 2), (20, 0)])
+def test_oracle_attention_and_mass(window, sinks):
+    u = ref.Setup([(3, 20), (0, 5), (6, 6), (2, 1)], 4, 2, 16, 16, seed=1)
+    out, lse, _, _ = ref.attention(u, None, window, sinks)
+    acc, _ = ref.mass(u, lse, None, window, sinks)
+    grown = acc - u.mass.double().numpy()
+    for s, (n, length) in enumerate(u.seqs):
+        if n == 0:
+            continue
+        pool = lambda x: x[torch.from_numpy(u.table[s]).long()].double().transpose(0, 1).flatten(1, 2)[:, :length]  # noqa: E731
+        k, v = (pool(x).repeat_interleave(u.G, 0) for x in (u.k, u.v))
+        q = u.q[u.starts[s]: u.starts[s + 1]].double().transpose(0, 1)
+        p, j = torch.arange(length - n, length)[:, None], torch.arange(length)
+        see = (j <= p) & ((j > p - window) | (j < sinks) if window else True)
+        x = (q @ k.transpose(1, 2) / 4.0).masked_fill(~see, -math.inf)
+        w = torch.softmax(x, -1).nan_to_num(0.0)
+        want = (w @ v).transpose(0, 1)
+        assert torch.allclose(torch.from_numpy(out[u.starts[s]: u.starts[s + 1]]), want)
+        got = torch.from_numpy(grown)[torch.from_numpy(u.table[s]).long()].transpose(0, 1).flatten(1, 2)[:, :length]
+        assert torch.allclose(got, w.sum(1).view(u.Hkv, u.G, -1).sum(1), atol=1e-12)
+
+
+def test_oracle_evict_and_append():
+    u = ref.Setup([(1, 9), (1, 30)], 2, 1, 16, 16, seed=2)
+    u.mass = torch.zeros_like(u.mass)
+    u.mass[u.table[1, 0], 0, 5] = 2.0
+    u.mass[u.table[1, 1], 0, 3] = float("nan")
+    lens, kept = ref.evict(u, 10, 2, 3)
+    assert lens.tolist() == [9, 10] and kept[0, 0].tolist() == [*range(9), -1]
+    assert kept[1, 0].tolist() == [0, 1, 2, 3, 4, 5, 19, 27, 28, 29]
+    q, k, v, mass = ref.append(u, None, None, np.ones(8, np.float32), np.array([0, 1]), 0.0)
+    x = u.qkv.double().numpy().reshape(2, 4, 16)
+    assert np.allclose(q[0], x[0, :2]) and np.allclose(k[u.table[0, 0], 0, 8], x[0, 2])
+    z = (x[1, 0, :8] + 1j * x[1, 0, 8:]) * np.exp(1j)
+    assert np.allclose(q[1, 0], np.concatenate((z.real, z.imag))) and np.allclose(v[u.table[1, 1], 0, 13], x[1, 3])
+    assert mass[u.table[1, 1], 0, 13] == 0.0
