@@ -20,6 +20,8 @@
 
 #include <type_traits>
 
+#include "sk_lds.h"
+
 namespace sk {
 namespace paged {
 
@@ -49,9 +51,18 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (N >= 16) v += dpp_f<0x140>(v);    // row_mirror
   return v;
 }
-// v of lanes 16, 32 and 48 further, added or compared with this one's.
-__device__ __forceinline__ float swap16(float v) { return __shfl_xor(v, 16, 64); }
-__device__ __forceinline__ float swap32(float v) { return __shfl_xor(v, 32, 64); }
+// Over lanes l, l ^ 16, l ^ 32 and l ^ 48 (the four that share a row or key of a
+// matrix tile), in every one of them: two exchanges in registers.
+template <typename F>
+__device__ __forceinline__ float fold4(float v, F f) {
+  const int x = __float_as_int(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const int y = __float_as_int(f(__int_as_float(a[0]), __int_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return f(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float sum4(float v) { return fold4(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float max4(float v) { return fold4(v, [](float a, float b) { return fmaxf(a, b); }); }
 
 __device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }   // to nearest even
 
@@ -86,13 +97,15 @@ struct Piece {
 #pragma unroll
     for (auto& x : w) x = 0;
   }
-  // some element is infinite or NaN
-  __device__ __forceinline__ bool wild() const {
+  // infinities and NaN to 0; whether there were any
+  __device__ __forceinline__ bool tame() {
     bool b = false;
 #pragma unroll
-    for (uint32_t x : w) {
-      if constexpr (sizeof(T) == 4) b |= (x & 0x7f800000u) == 0x7f800000u;
-      else b |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+    for (uint32_t& x : w) {
+      const bool hi = (x & 0x7f800000u) == 0x7f800000u, lo = sizeof(T) == 2 && (x & 0x7f80u) == 0x7f80u;
+      b |= hi || lo;
+      if (hi) x = sizeof(T) == 4 ? 0u : x & 0xffffu;
+      if (lo) x &= 0xffff0000u;
     }
     return b;
   }
@@ -264,6 +277,10 @@ __device__ __forceinline__ Walk walk_of(int p_lo, int p_hi, int window, int sink
 __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
   return j <= p && (window == 0 || j > p - window || j < sinks);
 }
+// whether every row of slots p_lo .. p_hi sees every key j0 .. j1
+__device__ __forceinline__ bool all_see(int j0, int j1, int p_lo, int p_hi, int window, int sinks) {
+  return j1 <= p_lo && (window == 0 || j0 > p_hi - window || j1 < sinks);
+}
 
 // Offsets (in elements, for head 0 dims) of a run of tiles: lane i holds that of
 // the wave's i-th tile from a walk position on; one division and table entry per lane, for 64 tiles.
@@ -296,6 +313,62 @@ struct Dims {
   static constexpr int LDO = HD + 4;                                                           // merge row stride
 };
 
+// V of a key that a row does not see must not reach it, but a matrix product
+// takes 0 times infinity or NaN for NaN.  So where a tile is seen by some rows only, the
+// loops take such elements of V as 0, and this adds them afterwards, element by element, to the
+// rows that do see them, in the output (or the cut's part) already stored: rare, and slow.
+// Rows f_lo .. f_hi of the sequence by one wave; tiles begin .. end for which tamed(t); stat(f):
+// the row's maximum (times scale2) and the factor of its sums.
+template <typename QT, typename KT, int HD, typename Tamed, typename Stat>
+__device__ __forceinline__ void add_wild(const AttendArgs& a, int h, const int* table, int first, int p0, int f_lo,
+                                         int f_hi, const Walk& w, int begin, int end, float* part, Tamed tamed,
+                                         Stat stat) {
+  constexpr int E = HD >= 64 ? HD / 64 : 1;
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, d = min(lane, HD / E - 1) * E;
+  const bool live = lane * E < HD;
+  for (int t = begin; t < end; ++t) {
+    const int k0 = w.tile(t) * TILE, e = table[k0 / c.page];
+    if (!tamed(t) || e < 0 || e >= c.n_pages) continue;
+    for (int key = k0; key < k0 + TILE; ++key) {
+      const size_t at = (((size_t)e * c.Hkv + h) * c.page + key % c.page) * HD + d;
+      Piece<KT, E> v;
+      v.load(static_cast<const KT*>(c.v) + at);
+      Piece<KT, E> x = v;
+      const bool odd = x.tame() && live;
+      if (!__any(odd)) continue;
+      Piece<KT, E> k;
+      k.load(static_cast<const KT*>(c.k) + at);
+      for (int f = f_lo; f < f_hi; ++f) {
+        const int tok = f / c.G;
+        if (!sees(p0 + tok, key, a.window, a.sinks)) continue;
+        const size_t row = (size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G);
+        Piece<QT, E> q;
+        q.load(static_cast<const QT*>(a.q) + row * HD + d);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) s = live ? fmaf(q.get(i), k.get(i), s) : 0.f;
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) s += __shfl_xor(s, i, 64);
+        const float2 st = stat(f);
+        const float p = __builtin_amdgcn_exp2f(fmaf(s, a.scale2, -st.x)) * st.y;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (odd && x.get(i) != v.get(i)) {      // the elements that were taken as 0
+            if (part) {
+              part[row * HD + d + i] += p * v.get(i);
+            } else if constexpr (sizeof(QT) == 4) {
+              static_cast<QT*>(a.out)[row * HD + d + i] += p * v.get(i);
+            } else {
+              QT* y = static_cast<QT*>(a.out) + row * HD + d + i;
+              *y = to_bf16(__uint_as_float((uint32_t)*y << 16) + p * v.get(i));
+            }
+          }
+      }
+    }
+  }
+}
+
 // The workgroup holds NT matrix tiles of 16 rows; its WK waves take key tiles in
 // turn, each with its own running maximum, and meet in LDS at the end.  No LDS and no barrier in the loop:
 //   S^T = K Q^T on the FP32 matrix cores: lane l holds row l % 16's products with
@@ -303,11 +376,12 @@ struct Dims {
 //   O^T += V^T P^T takes those values as they are: step v multiplies keys 4 q + v, q = 0 .. 3.
 // K and V come straight from the pages, 16 bytes per lane; K of the next tile loads under this one's softmax and V.
 template <typename QT, typename KT, int HD, int NT, int WK>
-__global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
+__global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_rows_kernel(AttendArgs a) {
   using D = Dims<KT, HD>;
   constexpr int KW = D::KW, NK = D::NK, NDT = D::NDT, VW = D::VW, NV = D::NV, LDO = D::LDO, R = NT * 16;
   __shared__ __attribute__((aligned(16))) float po[WK * R * LDO];
   __shared__ float pm[WK * R], pl[WK * R];
+  __shared__ float2 stats[R];
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   int seq, tile_no;
@@ -366,6 +440,7 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
 
   TileOffsets offs;
   const int t_first = cut * a.cut + wave;
+  bool wild = false;                              // infinities or NaN in V beside a mask
   if (t_first < end) {
     offs.load(c, table, w, t_first, WK, end, h, HD);
     load_k(offs.at(0));
@@ -392,9 +467,7 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
     }
     load_k(offs.at(min(i, 63)));                  // the last tile again after the last: a load without a branch
     const int k0 = w.tile(t) * TILE;
-    const bool whole = !bad && k0 + TILE - 1 <= p_lo &&
-                       (a.window == 0 || k0 > p_hi - a.window || k0 + TILE <= a.sinks);   // every row sees every key
-    bool mixed = false;
+    const bool whole = !bad && all_see(k0, k0 + TILE - 1, p_lo, p_hi, a.window, a.sinks);
     if (!whole) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
@@ -404,22 +477,17 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
           if (bad) s[j][v] = NAN;
           if (!sees(qp[j], key, a.window, a.sinks)) s[j][v] = -INFINITY;
         }
-      // V of keys that a row does not see must not reach it, not even times 0
       bool odd = false;
 #pragma unroll
       for (int v = 0; v < 4; ++v)
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-          if (bad) vf[v][u].clear();
-          odd |= vf[v][u].wild();
-        }
-      mixed = __any(odd);
+        for (int u = 0; u < NV; ++u) odd |= vf[v][u].tame();
+      if (__any(odd)) wild = true;
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float mx = fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3]));
-      mx = fmaxf(mx, swap16(mx));
-      mx = fmaxf(mx, swap32(mx));
+      mx = max4(mx);
       const float mn = fmaxf(mr[j], mx);
       const float m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
       const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
@@ -436,47 +504,22 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
         for (int u = 0; u < NDT; ++u) o[j][u] *= sc;
       }
     }
-    if (!mixed) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
+      for (int u = 0; u < NV; ++u)
 #pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            const float x = vf[v][u].get(e);
+        for (int e = 0; e < VW; ++e) {
+          const float x = vf[v][u].get(e);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-              o[j][u * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[j][v], o[j][u * VW + e], 0, 0, 0);
-          }
-    } else {                                      // infinities or NaN beside a mask: key by key, where it is seen
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        for (int kq = 0; kq < 4; ++kq) {
-          const KT* vr = vp + off + (4 * kq + v) * HD;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const float p = __shfl(s[j][v], i16 + 16 * kq, 64);
-            if (!sees(qp[j], k0 + 4 * kq + v, a.window, a.sinks)) continue;
-#pragma unroll
-            for (int u = 0; u < NV; ++u)
-#pragma unroll
-              for (int e = 0; e < VW; ++e)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  Piece<KT, 1> x;
-                  x.load(vr + 16 * VW * u + VW * (4 * q4 + r) + e);
-                  o[j][u * VW + e][r] = fmaf(p, x.get(0), o[j][u * VW + e][r]);
-                }
-          }
+          for (int j = 0; j < NT; ++j)
+            o[j][u * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[j][v], o[j][u * VW + e], 0, 0, 0);
         }
-    }
   }
   // the waves meet: their rows of O and (max, sum), then a weight for each
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    float l = lr[j];
-    l += swap16(l);
-    l += swap32(l);
+    const float l = sum4(lr[j]);
     const int at = wave * R + j * 16 + i16;
     if (q4 == 0) { pm[at] = mr[j]; pl[at] = l; }
     float* row = po + at * LDO;
@@ -503,6 +546,7 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
     const bool none = p0 + tok < 0;               // no key is seen
 #pragma unroll
     for (int u = 0; u < WK; ++u) pm[u * R + tid] = alone ? none ? 0.f : f[u] / l : f[u];
+    stats[tid] = make_float2(m2, alone ? 1.f / l : 1.f);
     if (row < rows) {
       const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
       if (!alone) {
@@ -529,6 +573,299 @@ __global__ __launch_bounds__(WK * 64) void attend_rows_kernel(AttendArgs a) {
     const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
     if (alone) store4(static_cast<QT*>(a.out) + at * HD + d, y.x, y.y, y.z, y.w);
     else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + at) * HD + d) = y;
+  }
+  if (__syncthreads_or(wild) && wave == 0)
+    add_wild<QT, KT, HD>(a, h, table, first, p0, f0, min(f0 + R, rows), w, cut * a.cut, end,
+                         alone ? nullptr : a.part + (size_t)cut * c.T * c.Hq * HD,
+                         [&](int t) { const int k0 = w.tile(t) * TILE;
+                                      return !all_see(k0, k0 + TILE - 1, p_lo, p_hi, a.window, a.sinks); },
+                         [&](int f) { return stats[f - f0]; });
+}
+
+// ------------------------------------------------------------ many rows, BF16 cache
+// The same sums for chunks, on the BF16 matrix cores.  A workgroup's 4 waves own
+// 16 RT rows each and share tiles of 64 keys in LDS (two stages, loaded ahead straight from the pages).
+//   S^T = K Q^T: K as 16 x 32 fragments, whole in LDS, Q in registers; lane l holds row l % 16 against keys
+//     4 (l / 16) + v of each 16;
+//   O^T += V^T P^T: those values are P's fragment for a set of 32 keys as they are: element e of
+//     lane group g is key 4 g + e of the first 16 or (e >= 4) of the second.  V lies in LDS
+//     row by row; the transposing LDS read gives a lane 4 keys of one dim.
+// FP32 activations: Q and P as three BF16 parts of 8 bits that add up to the FP32 value
+// exactly, three products each, so results are those of FP32 products (NP = 3).  BF16
+// activations: P rounds to BF16 once (2^-9 of a weight on average, under the output's own rounding).
+constexpr int KEYS = 64;                          // keys of a step
+
+template <int HD>
+struct TileLds {
+  static constexpr int K = KEYS * HD * 2, STAGE = 2 * K;   // bytes
+  // 16-byte piece of V row `key` that holds piece x: rows that the transposing read takes together
+  // lie in different banks
+  static __device__ __forceinline__ int swizzle(int key) { return HD == 128 ? 2 * (key & 7) : HD == 64 ? 2 * (key >> 1 & 3) : 2 * (key >> 2 & 1); }
+};
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+// Eight FP32 values as NP BF16 fragments: cut to 8 bits, what is left cut again; the
+// third takes the rest exactly.  NP = 1 rounds to nearest.
+template <int NP>
+__device__ __forceinline__ void parts8(const float* x, bf8* out) {
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[0][i] = (__bf16)x[i];
+  } else {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      uint4 w;
+      uint32_t* u = &w.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = __builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302);
+      out[p] = __builtin_bit_cast(bf8, w);
+      if (p + 1 < NP) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+      }
+    }
+  }
+}
+
+template <typename QT, int HD, int RT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_tiles_kernel(AttendArgs a) {
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, NDT = HD / 16, R = 64 * RT;
+  constexpr int GROUP = TILE * HD * 2;            // bytes of 16 keys
+  using L = TileLds<HD>;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * L::STAGE];
+  const Cache& c = a.c;
+  const int h = blockIdx.x, cut = blockIdx.z;
+  int seq, tile_no;
+  // the last tiles of a sequence walk furthest: they start first
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;
+  int first, n;
+  seq_rows(c, seq, first, n);
+  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
+  const int begin = cut * a.cut, end = min(w.n, begin + a.cut);
+  if (cut > 0 && begin >= w.n) return;            // the first cut also answers for rows that see nothing
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, q4 = lane >> 4;
+  const int* table = c.table + seq * c.stride;
+
+  int qp[RT];                                     // the slot of this lane's rows (rows past the last repeat it)
+  bf8 qf[RT][NP][KS];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const int f = min(f0 + (wave * RT + j) * 16 + i16, rows - 1), tok = f / c.G;
+    qp[j] = p0 + tok;
+    const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      Piece<QT, 8> x;
+      x.load(qr + k * 32 + q4 * 8);
+      if constexpr (NP == 1) {
+        qf[j][0][k] = __builtin_bit_cast(bf8, x);
+      } else {
+        float y[8];
+        bf8 part[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x.get(e);
+        parts8<NP>(y, part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) qf[j][p][k] = part[p];
+      }
+    }
+  }
+
+  // wave u loads the u-th 16 keys of a step: K as fragments, V as rows, KS loads
+  // of 1 KB each; V's 8 rows further are swizzled alike
+  const unsigned koff = (i16 * HD + q4 * 8) * 2;
+  constexpr int NVO = HD == 128 ? 2 : 1;
+  unsigned voff[NVO];
+#pragma unroll
+  for (int k = 0; k < NVO; ++k) {
+    const int piece = k * 64 + lane, key = piece / (HD / 8), x = piece % (HD / 8);
+    voff[k] = (key * HD + (x ^ L::swizzle(key)) * 8) * 2;
+  }
+  unsigned vread[NDT];                            // this lane's bytes of 16 dims of V's first 16 keys
+#pragma unroll
+  for (int t = 0; t < NDT; ++t) {
+    const int key = 4 * q4 + (i16 >> 2), x = 2 * t + ((i16 & 3) >> 1);
+    vread[t] = L::K + key * HD * 2 + (x ^ L::swizzle(key)) * 16 + (i16 & 1) * 8;
+  }
+  TileOffsets offs;
+  int at = 0;                                     // the next step's first lane in offs
+  // loads the step whose first tile is t; gives which of its four tiles have no page
+  auto prefetch = [&](int t) -> int {
+    if (at == 64) at = 0;
+    if (at == 0) offs.load(c, table, w, t, 1, end, h, HD);
+    const size_t off = offs.at(at + wave) * 2;
+    const int none = offs.bad >> at & 15;
+    at += 4;
+    const char* st = lds + ((t - begin) / 4 % 2) * L::STAGE + wave * GROUP;
+    const char* kb = static_cast<const char*>(c.k) + off;
+    const char* vb = static_cast<const char*>(c.v) + off;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) lds_load16(kb + k * 64, koff, st + k * 1024);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) lds_load16(vb + k / NVO * NVO * 1024, voff[k % NVO], st + L::K + k * 1024);
+    return none;
+  };
+  v4f o[RT][NDT];
+  float mr[RT], lr[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    mr[j] = -INFINITY;
+    lr[j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) o[j][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  int bad_next = begin < end ? prefetch(begin) : 0;
+  bool wild = false;                              // infinities or NaN in V beside a mask
+  for (int t = begin; t < end; t += 4) {
+    stage_sync<0>();                              // this step is in, and every wave is done with the other stage
+    const int bad = bad_next;
+    if (t + 4 < end) bad_next = prefetch(t + 4);
+    char* st = lds + ((t - begin) / 4 % 2) * L::STAGE;
+    const int k_first = w.tile(t) * TILE, k_last = w.tile(min(t + 3, end - 1)) * TILE + TILE - 1;
+    const bool whole = !bad && t + 4 <= end && all_see(k_first, k_last, p_lo, p_hi, a.window, a.sinks);
+    if (!whole) {                                 // each wave tames the V that it loaded
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        auto* x = reinterpret_cast<Piece<uint16_t, 8>*>(st + L::K + wave * GROUP + k * 1024 + lane * 16);
+        Piece<uint16_t, 8> y = *x;
+        odd |= y.tame();
+        *x = y;
+      }
+      wild |= __syncthreads_or(odd);
+    }
+    v4f s[RT][4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+#pragma unroll
+      for (int j = 0; j < RT; ++j) s[j][g] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const bf8 kf = *reinterpret_cast<const bf8*>(st + (g * KS + k) * 1024 + lane * 16);
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) s[j][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[j][p][k], s[j][g], 0, 0, 0);
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int k0 = w.tile(min(t + g, end - 1)) * TILE;
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (bad >> g & 1) s[j][g][v] = NAN;
+            if (t + g >= end || !sees(qp[j], k0 + 4 * q4 + v, a.window, a.sinks)) s[j][g][v] = -INFINITY;
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      float mx = s[j][0][0];
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][g][v]);
+      mx = max4(mx);
+      const float mn = fmaxf(mr[j], mx);
+      const float m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
+      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          s[j][g][v] = __builtin_amdgcn_exp2f(fmaf(s[j][g][v], a.scale2, -m2));
+          sum += s[j][g][v];
+        }
+      lr[j] = lr[j] * sc + sum;                   // this lane's keys; a row's four lanes add up at the end
+      mr[j] = mn;
+      if (__any(sc != 1.f)) {
+#pragma unroll
+        for (int u = 0; u < NDT; ++u) o[j][u] *= sc;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {                 // sets of 32 keys
+      bf8 pf[RT][NP];
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = s[j][2 * g + e / 4][e % 4];
+        parts8<NP>(y, pf[j]);
+      }
+#pragma unroll
+      for (int u = 0; u < NDT; ++u) {
+        typedef __attribute__((address_space(3))) s4 lds4;
+        const char* vr = st + vread[u] + 2 * g * GROUP;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vr);
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vr + GROUP));
+        const bf8 vf = __builtin_bit_cast(bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) o[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[j][p], o[j][u], 0, 0, 0);
+      }
+    }
+  }
+  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const int f = f0 + (wave * RT + j) * 16 + i16, tok = f / c.G;
+    const float l = lr[j] = sum4(lr[j]);
+    if (f >= rows) continue;
+    const size_t row = (size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G);
+    const bool none = qp[j] < 0;                  // no key is seen
+    const float y = alone ? none ? 0.f : 1.f / l : 1.f;
+    if (q4 == 0) {
+      if (!alone) {
+        float* d = a.ml + ((size_t)cut * c.T * c.Hq + row) * 2;
+        d[0] = mr[j];
+        d[1] = l;
+      } else if (a.lse) {
+        a.lse[row] = none ? -INFINITY : ((mr[j] == -INFINITY ? 0.f : mr[j] * a.scale2) + log2f(l)) * LN2;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NDT; ++u) {
+      const int d = 16 * u + 4 * q4;
+      if (alone) store4(static_cast<QT*>(a.out) + row * HD + d, y * o[j][u][0], y * o[j][u][1], y * o[j][u][2], y * o[j][u][3]);
+      else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + row) * HD + d) =
+          make_float4(o[j][u][0], o[j][u][1], o[j][u][2], o[j][u][3]);
+    }
+  }  if (wild) {
+    __threadfence_block();                        // the stores above, by other lanes
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      const int f_lo = f0 + (wave * RT + j) * 16;
+      add_wild<QT, uint16_t, HD>(
+          a, h, table, first, p0, f_lo, min(f_lo + 16, rows), w, begin, end,
+          alone ? nullptr : a.part + (size_t)cut * c.T * c.Hq * HD,
+          [&](int t) {
+            const int t0 = begin + (t - begin) / 4 * 4, t3 = min(t0 + 3, end - 1);
+            bool none = t0 + 4 > end;             // as the loop above judged the step
+            for (int u = t0; u <= t3; ++u) {
+              const int e = table[w.tile(u) * TILE / c.page];
+              none |= e < 0 || e >= c.n_pages;
+            }
+            return none || !all_see(w.tile(t0) * TILE, w.tile(t3) * TILE + TILE - 1, p_lo, p_hi, a.window, a.sinks);
+          },
+          [&](int f) {
+            const float m = __shfl(mr[j], f - f_lo, 64);
+            return make_float2(m == -INFINITY ? 0.f : m * a.scale2, alone ? 1.f / __shfl(lr[j], f - f_lo, 64) : 1.f);
+          });
+    }
   }
 }
 
@@ -661,9 +998,7 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   }
 #pragma unroll
   for (int j = 0; j < NK2; ++j) {
-    float y = sum[j];
-    y += swap16(y);
-    y += swap32(y);
+    const float y = sum4(sum[j]);
     if (q4 == 0 && k0 + j * TILE + i16 < len && !bad[j]) a.mass[at[j]] += y;
   }
 }

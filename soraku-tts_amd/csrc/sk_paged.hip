@@ -69,22 +69,25 @@ void with_types(int32_t xdtype, int32_t kvdtype, F&& f) {
   else f(float{}, float{});
 }
 
-// How an attention call is cut up: R rows per workgroup, `cut` tiles of keys
-// per cut.
+// How an attention call is cut up: R rows per workgroup (of 64-key steps on the
+// BF16 matrix cores: `tiles`), `cut` tiles of keys per cut.
 struct Plan {
+  bool tiles;
   int R, blocks, cut, cuts;
 };
-Plan plan_attention(int T, int S, int Hq, int Hkv, int page, int width, int window, int sinks) {
+Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page, int width, int window, int sinks) {
   Plan p;
   const int G = Hq / Hkv;
-  p.R = (int64_t)T * G > 16ll * S ? 32 : 16;
+  const int64_t rows = (int64_t)T * G / S;        // of a sequence, on average
+  p.tiles = kvdtype == SK_BF16 && hd >= 32 && rows > 32;
+  p.R = p.tiles ? 128 : rows > 16 ? 32 : 16;
   p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - 1)) / p.R);
   int64_t tiles = (int64_t)page * width / TILE;   // what a row tile can walk at most
   if (window > 0)
     tiles = std::min(tiles, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
   const int64_t base = (int64_t)p.blocks * Hkv;
   const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(base, 1), tiles / 16));
-  p.cut = (int)((tiles + cuts - 1) / cuts);
+  p.cut = (int)((tiles + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
   p.cuts = (int)((tiles + p.cut - 1) / p.cut);
   return p;
 }
@@ -131,7 +134,7 @@ int sk_op_paged_attention_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hk
   if (int rc = check_types(xdtype, kvdtype)) return rc;
   if (int rc = check_window(1.f, window, sinks)) return rc;
   SK_CHECK(bytes, SK_EINVAL, "NULL operand");
-  *bytes = workspace_of(plan_attention(T, S, Hq, Hkv, page, width, window, sinks), T, Hq, hd);
+  *bytes = workspace_of(plan_attention(T, S, Hq, Hkv, hd, kvdtype, page, width, window, sinks), T, Hq, hd);
   return SK_OK;
 }
 
@@ -147,7 +150,7 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   SK_CHECK(q && k_pages && v_pages && table && starts && lens && out, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace), SK_EINVAL,
            "operands must be 16-byte aligned");
-  const Plan p = plan_attention(T, S, Hq, Hkv, page, width, window, sinks);
+  const Plan p = plan_attention(T, S, Hq, Hkv, hd, kvdtype, page, width, window, sinks);
   SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= workspace_of(p, T, Hq, hd)), SK_EINVAL,
            "the workspace must hold %lld bytes", (long long)workspace_of(p, T, Hq, hd));
   SK_CHECK(p.blocks <= 65535 && p.cuts <= 65535, SK_EINVAL, "too many rows for one call");
@@ -167,7 +170,11 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
       using K = decltype(k);
       constexpr int HD = decltype(d)::value;
       const dim3 grid(Hkv, p.blocks, p.cuts);
-      if (p.R == 32) hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
+      if constexpr (HD >= 32 && sizeof(K) == 2) {
+        if (p.tiles) hipLaunchKernelGGL((attend_tiles_kernel<X, HD, 2>), grid, dim3(256), 0, st, a);
+      }
+      if (p.tiles) ;
+      else if (p.R == 32) hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
       else hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 1, 4>), grid, dim3(256), 0, st, a);
       err = hipGetLastError();
       if (p.cuts == 1 || err != hipSuccess) return;

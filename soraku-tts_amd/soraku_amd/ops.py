@@ -149,54 +149,75 @@ def sample(V: int, bos_id: int, eos_id: int, pad_id: int):
 # [S + 1] and lens [S] int32, all on the HIP device: sequence s's new tokens are
 # the packed rows starts[s]:starts[s + 1] and lens[s] its length with them.
 # include/soraku_mi355x.h holds the whole contract.
+#
+# A single-token call runs for 4 to 25 us on the GPU, so the host's part is kept
+# short: one pass of cheap checks, the raw stream handle, no Stream or pointer
+# objects.
 
-def _need(t, name, dtype, dev, *shape):
-    if t.dtype is not dtype or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {dev}, got {t.dtype} "
+class _Torch:
+    """What the paged operators use of torch, looked up once."""
+
+    def __init__(self):
+        import torch
+
+        self.f32, self.bf16, self.i32, self.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
+        self.empty, self.on = torch.empty, torch.cuda.device
+        self.stream, self.device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+        self.codes = {torch.float32: _lib.SK_F32, torch.bfloat16: _lib.SK_BF16}
+        self.lib = lib()
+
+
+@functools.lru_cache(maxsize=None)
+def _torch() -> _Torch:
+    return _Torch()
+
+
+def _need(t, name, dtype, at, shape):
+    """t's address; t must be contiguous, of that type and shape, on device number ``at``."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != at or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on HIP device {at}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
     return t.data_ptr()
 
 
-def _table(t, name, dev, S):
-    import torch
+def _table(t, name, dtype, at, S):
+    """(address, row stride, entries per row) of a page table."""
+    if t.dtype is not dtype or t.get_device() != at or t.dim() != 2 or t.shape[0] != S:
+        raise ValueError(f"{name} must be an int32 tensor [{S}, pages] on HIP device {at}")
+    width, (stride, step) = t.shape[1], t.stride()
+    if (width > 1 and step != 1) or (S > 1 and stride < width):
+        raise ValueError(f"{name}'s rows must be contiguous and apart")
+    return t.data_ptr(), stride if S > 1 else width, width
 
-    if t.dtype is not torch.int32 or t.device != dev or t.dim() != 2 or t.shape[0] != S or (
-            t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be an int32 tensor [{S}, pages] on {dev} with its rows contiguous")
-    if S > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}'s rows overlap")
-    return t.data_ptr(), max(t.stride(0), t.shape[1]) if S > 1 else t.shape[1], t.shape[1]
 
-
-def _pool(k_pages, v_pages, Hkv, page, hd):
-    if k_pages.dim() != 4:
-        raise ValueError("pages must be [n_pages, Hkv, page, hd]")
+def _pool(k_pages, v_pages, Hkv, page, hd, codes):
+    """(device number, pages, addresses of K and V, type code)."""
     if not k_pages.is_cuda:
         raise ValueError("operands must live on the HIP device")
-    dev, n = k_pages.device, k_pages.shape[0]
-    kp = _need(k_pages, "k_pages", k_pages.dtype, dev, n, Hkv, page, hd)
-    vp = None if v_pages is None else _need(v_pages, "v_pages", k_pages.dtype, dev, n, Hkv, page, hd)
-    return dev, n, kp, vp, _wdtype(k_pages)
+    if k_pages.dim() != 4 or k_pages.dtype not in codes:
+        raise ValueError("pages must be [n_pages, Hkv, page, hd], float32 or bfloat16")
+    dt, at, n = k_pages.dtype, k_pages.get_device(), k_pages.shape[0]
+    shape = (n, Hkv, page, hd)
+    kp = _need(k_pages, "k_pages", dt, at, shape)
+    return at, n, kp, None if v_pages is None else _need(v_pages, "v_pages", dt, at, shape), codes[dt]
 
 
-class _On:
-    """The device of the operands as the current one, where it is another."""
-
-    def __init__(self, dev):
-        import torch
-
-        self._guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _code(t, codes):
+    if t.dtype not in codes:
+        raise ValueError(f"dtype {t.dtype} not supported (float32 or bfloat16)")
+    return codes[t.dtype]
 
 
-@functools.lru_cache(maxsize=256)
+def _call(T, fn, at, *args):
+    """fn(stream, *args) on device ``at`` and its current stream."""
+    if at == T.device():
+        check(fn(T.stream(at), *args))
+    else:
+        with T.on(at):
+            check(fn(T.stream(at), *args))
+
+
+@functools.lru_cache(maxsize=1024)
 def _attention_workspace(*sizes) -> int:
     n = C.c_int64()
     check(lib().sk_op_paged_attention_workspace(*sizes, C.byref(n)))
@@ -209,22 +230,21 @@ def paged_append(Hq: int, Hkv: int, hd: int, page: int, eps: float):
     their slots; returns q ``[T, Hq, hd]`` of qkv's dtype (``out``, if given).
     ``mass`` (accounts, ``[n_pages, Hkv, page]`` float32) is set to 0 at the new slots."""
     def kernel(qkv, q_gain, k_gain, inv_freq, positions, starts, lens, table, k_pages, v_pages, mass=None, out=None):
-        import torch
-
-        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
-        T, S, i32, f32 = qkv.shape[0], lens.shape[0], torch.int32, torch.float32
-        tp, stride, width = _table(table, "table", dev, S)
+        T = _torch()
+        f32, i32 = T.f32, T.i32
+        at, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd, T.codes)
+        xd, dt, rows, S = _code(qkv, T.codes), qkv.dtype, qkv.shape[0], lens.shape[0]
+        tp, stride, width = _table(table, "table", i32, at, S)
         if out is None:
-            out = torch.empty(T, Hq, hd, device=dev, dtype=qkv.dtype)
-        gains = [None if g is None else _need(g, "gain", f32, dev, hd) for g in (q_gain, k_gain)]
-        with _On(dev):
-            check(lib().sk_op_paged_append(
-                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, _wdtype(qkv), kd, eps,
-                _need(qkv, "qkv", qkv.dtype, dev, T, (Hq + 2 * Hkv) * hd), *gains,
-                _need(inv_freq, "inv_freq", f32, dev, hd // 2), _need(positions, "positions", i32, dev, T),
-                _need(starts, "starts", i32, dev, S + 1), _need(lens, "lens", i32, dev, S), tp, kp, vp,
-                None if mass is None else _need(mass, "mass", f32, dev, n, Hkv, page),
-                _need(out, "out", qkv.dtype, dev, T, Hq, hd)))
+            out = T.empty(rows, Hq, hd, device=k_pages.device, dtype=dt)
+        _call(T, T.lib.sk_op_paged_append, at, rows, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, eps,
+              _need(qkv, "qkv", dt, at, (rows, (Hq + 2 * Hkv) * hd)),
+              None if q_gain is None else _need(q_gain, "q_gain", f32, at, (hd,)),
+              None if k_gain is None else _need(k_gain, "k_gain", f32, at, (hd,)),
+              _need(inv_freq, "inv_freq", f32, at, (hd // 2,)), _need(positions, "positions", i32, at, (rows,)),
+              _need(starts, "starts", i32, at, (S + 1,)), _need(lens, "lens", i32, at, (S,)), tp, kp, vp,
+              None if mass is None else _need(mass, "mass", f32, at, (n, Hkv, page)),
+              _need(out, "out", dt, at, (rows, Hq, hd)))
         return out
     return kernel
 
@@ -238,22 +258,20 @@ def paged_attention(Hq: int, Hkv: int, hd: int, page: int, scale: float | None =
     scale = hd ** -0.5 if scale is None else float(scale)
 
     def kernel(q, k_pages, v_pages, table, starts, lens, out=None, lse=None):
-        import torch
-
-        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
-        T, S, xd = q.shape[0], lens.shape[0], _wdtype(q)
-        tp, stride, width = _table(table, "table", dev, S)
+        T = _torch()
+        i32 = T.i32
+        at, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd, T.codes)
+        xd, dt, rows, S = _code(q, T.codes), q.dtype, q.shape[0], lens.shape[0]
+        tp, stride, width = _table(table, "table", i32, at, S)
+        shape = (rows, Hq, hd)
         if out is None:
-            out = torch.empty(T, Hq, hd, device=dev, dtype=q.dtype)
-        with _On(dev):
-            size = _attention_workspace(T, S, Hq, Hkv, hd, page, width, xd, kd, window, sinks)
-            ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
-            check(lib().sk_op_paged_attention(
-                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,
-                sinks, _need(q, "q", q.dtype, dev, T, Hq, hd), kp, vp, tp, _need(starts, "starts", torch.int32, dev, S + 1),
-                _need(lens, "lens", torch.int32, dev, S), _need(out, "out", q.dtype, dev, T, Hq, hd),
-                None if lse is None else _need(lse, "lse", torch.float32, dev, T, Hq),
-                ws.data_ptr() if size else None, size))
+            out = T.empty(shape, device=k_pages.device, dtype=dt)
+        size = _attention_workspace(rows, S, Hq, Hkv, hd, page, width, xd, kd, window, sinks)
+        ws = T.empty(size, device=k_pages.device, dtype=T.u8) if size else None
+        _call(T, T.lib.sk_op_paged_attention, at, rows, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,
+              sinks, _need(q, "q", dt, at, shape), kp, vp, tp, _need(starts, "starts", i32, at, (S + 1,)),
+              _need(lens, "lens", i32, at, (S,)), _need(out, "out", dt, at, shape),
+              None if lse is None else _need(lse, "lse", T.f32, at, (rows, Hq)), ws.data_ptr() if size else None, size)
         return out
     return kernel
 
@@ -266,17 +284,15 @@ def paged_attention_mass(Hq: int, Hkv: int, hd: int, page: int, scale: float | N
     scale = hd ** -0.5 if scale is None else float(scale)
 
     def kernel(q, lse, k_pages, table, starts, lens, mass):
-        import torch
-
-        dev, n, kp, _, kd = _pool(k_pages, None, Hkv, page, hd)
-        T, S, f32 = q.shape[0], lens.shape[0], torch.float32
-        tp, stride, width = _table(table, "table", dev, S)
-        with _On(dev):
-            check(lib().sk_op_paged_attention_mass(
-                torch.cuda.current_stream(dev).cuda_stream, T, S, Hq, Hkv, hd, page, n, width, stride, _wdtype(q), kd, scale,
-                window, sinks, _need(q, "q", q.dtype, dev, T, Hq, hd), _need(lse, "lse", f32, dev, T, Hq), kp, tp,
-                _need(starts, "starts", torch.int32, dev, S + 1), _need(lens, "lens", torch.int32, dev, S),
-                _need(mass, "mass", f32, dev, n, Hkv, page)))
+        T = _torch()
+        f32, i32 = T.f32, T.i32
+        at, n, kp, _, kd = _pool(k_pages, None, Hkv, page, hd, T.codes)
+        xd, rows, S = _code(q, T.codes), q.shape[0], lens.shape[0]
+        tp, stride, width = _table(table, "table", i32, at, S)
+        _call(T, T.lib.sk_op_paged_attention_mass, at, rows, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,
+              sinks, _need(q, "q", q.dtype, at, (rows, Hq, hd)), _need(lse, "lse", f32, at, (rows, Hq)), kp, tp,
+              _need(starts, "starts", i32, at, (S + 1,)), _need(lens, "lens", i32, at, (S,)),
+              _need(mass, "mass", f32, at, (n, Hkv, page)))
         return mass
     return kernel
 
@@ -287,18 +303,16 @@ def paged_evict(Hkv: int, hd: int, page: int, keep: int, sinks: int = 0, recent:
     order, with their accounts, to the pages of ``to`` ``[S, pages]``, none of which may be in ``table``.
     Returns the new lengths ``[S]`` and the old slots ``[S, Hkv, keep]`` (-1 past the length), int32."""
     def kernel(k_pages, v_pages, mass, table, lens, to):
-        import torch
-
-        dev, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd)
-        S = lens.shape[0]
-        tp, stride, width = _table(table, "table", dev, S)
-        dp, to_stride, to_width = _table(to, "to", dev, S)
-        new_lens = torch.empty(S, device=dev, dtype=torch.int32)
-        kept = torch.empty(S, Hkv, keep, device=dev, dtype=torch.int32)
-        with _On(dev):
-            check(lib().sk_op_paged_evict(
-                torch.cuda.current_stream(dev).cuda_stream, S, Hkv, hd, page, n, width, stride, kd, keep, sinks, recent, kp, vp,
-                _need(mass, "mass", torch.float32, dev, n, Hkv, page), tp, _need(lens, "lens", torch.int32, dev, S), dp,
-                to_stride, to_width, new_lens.data_ptr(), kept.data_ptr()))
+        T = _torch()
+        i32 = T.i32
+        at, n, kp, vp, kd = _pool(k_pages, v_pages, Hkv, page, hd, T.codes)
+        S, dev = lens.shape[0], k_pages.device
+        tp, stride, width = _table(table, "table", i32, at, S)
+        dp, to_stride, to_width = _table(to, "to", i32, at, S)
+        new_lens = T.empty(S, device=dev, dtype=i32)
+        kept = T.empty((S, Hkv, keep), device=dev, dtype=i32)
+        _call(T, T.lib.sk_op_paged_evict, at, S, Hkv, hd, page, n, width, stride, kd, keep, sinks, recent, kp, vp,
+              _need(mass, "mass", T.f32, at, (n, Hkv, page)), tp, _need(lens, "lens", i32, at, (S,)), dp, to_stride,
+              to_width, new_lens.data_ptr(), kept.data_ptr())
         return new_lens, kept
     return kernel

@@ -96,19 +96,24 @@ def test_python_refusals():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="HIP device"):
         ops.paged_attention(4, 2, 16, 16)(torch.zeros(1, 4, 16), k, k, i[:, None], i, i)
-    with pytest.raises(ValueError, match="pages must be"):
+    with pytest.raises(ValueError, match="HIP device"):
         ops.paged_evict(2, 16, 16, 4)(k[0], k[0], k, i[:, None], i, i[:, None])
-    cpu = torch.device("cpu")
-    for bad in (torch.zeros(2, 3), torch.zeros(3, 2).t(), torch.zeros(2, 3, dtype=torch.float64)[:, :2]):
+    i32, cpu = torch.int32, -1                       # a CPU tensor's device number
+    for bad in (torch.zeros(2, 3), torch.zeros(3, 2).t(), torch.zeros(2, 3, dtype=torch.float64)[:, :2],
+                torch.zeros(2, 3)[:, :2]):
         with pytest.raises(ValueError, match="must be a contiguous"):
-            ops._need(bad, "x", torch.float32, cpu, 2, 2)
-    for bad in (i, i[:, None].long(), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32).t(),
-                torch.zeros(1, 3, dtype=torch.int32).expand(2, 3)):
+            ops._need(bad, "x", torch.float32, cpu, (2, 2))
+    with pytest.raises(ValueError, match="HIP device 0"):
+        ops._need(torch.zeros(2, 2), "x", torch.float32, 0, (2, 2))
+    for bad in (i, i[:, None].long(), torch.zeros(3, 2, dtype=i32), torch.zeros(3, 2, dtype=i32).t(),
+                torch.zeros(1, 3, dtype=i32).expand(2, 3)):
         with pytest.raises(ValueError):
-            ops._table(bad, "table", cpu, 2)
-    wide = torch.zeros(2, 7, dtype=torch.int32)
-    assert ops._table(wide[:, :3], "table", cpu, 2)[1:] == (7, 3)
-    assert ops._table(wide[:1, :3], "table", cpu, 1)[1:] == (3, 3)
+            ops._table(bad, "table", i32, cpu, 2)
+    wide = torch.zeros(2, 7, dtype=i32)
+    assert ops._table(wide[:, :3], "table", i32, cpu, 2)[1:] == (7, 3)
+    assert ops._table(wide[:1, :3], "table", i32, cpu, 1)[1:] == (3, 3)
+    with pytest.raises(ValueError, match="not supported"):
+        ops._code(torch.zeros(1, dtype=torch.float16), {torch.float32: 0})
 
 
 # ------------------------------------------------------------------ launches (stand-in HIP runtime)
@@ -203,8 +208,8 @@ def rows_of(kernel):
     import re
 
     args = [int(x) for x in re.findall(r"Li(\d+)E", kernel)]
-    assert "attend_rows_kernel" in kernel, kernel
-    return 16 * args[1]
+    assert "attend_rows_kernel" in kernel or "attend_tiles_kernel" in kernel, kernel
+    return (64 if "tiles" in kernel else 16) * args[1]
 
 
 # ------------------------------------------------------------------ the oracle
