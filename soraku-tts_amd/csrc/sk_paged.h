@@ -35,6 +35,7 @@ struct Cache {
   const int* table; int64_t stride; int width;    // [S][width] at rows of stride entries
   const int* starts; const int* lens;             // [S + 1], [S]
   int T, S, Hq, Hkv, G, n_pages, page;
+  uint32_t page_mul; int page_shift;              // j / page = j * page_mul >> page_shift for 0 <= j < 2^31
 };
 
 // ------------------------------------------------------------ small helpers
@@ -121,6 +122,9 @@ __device__ __forceinline__ void seq_rows(const Cache& c, int s, int& first, int&
   first = min(max(c.starts[s], 0), c.T);
   n = min(max(c.starts[s + 1], first), c.T) - first;
 }
+__device__ __forceinline__ int page_of(const Cache& c, int j) {
+  return (int)(__umulhi((uint32_t)j, c.page_mul) >> (c.page_shift - 32));
+}
 __device__ __forceinline__ int seq_len(const Cache& c, int s) { return min(max(c.lens[s], 0), c.width * c.page); }
 
 // The sequence that row m belongs to (wave-uniform; S if none): the last one that starts at or before it.
@@ -198,9 +202,10 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, const XT* qkv, con
   seq_rows(c, s, first, n);
   const int slot = seq_len(c, s) - n + (m - first);
   int at = -1;                                    // the slot's page, if it has one
-  if (slot >= 0 && m - first < n) at = c.table[s * c.stride + slot / c.page];
+  const int pg = page_of(c, max(slot, 0));
+  if (slot >= 0 && m - first < n) at = c.table[s * c.stride + pg];
   const bool live = at >= 0 && at < c.n_pages;
-  const size_t base = live ? (size_t)at * c.Hkv * c.page + slot % c.page : 0;   // in rows of hd, for head 0
+  const size_t base = live ? (size_t)at * c.Hkv * c.page + (slot - pg * c.page) : 0;   // in rows of hd, for head 0
   __syncthreads();
   float2 t4[4];
 #pragma unroll
@@ -290,10 +295,10 @@ struct TileOffsets {
   __device__ __forceinline__ void load(const Cache& c, const int* table, const Walk& w, int t0, int step, int end, int h,
                                        int hd) {
     const int t = min(t0 + (int)(threadIdx.x & 63) * step, end - 1);
-    const int g = w.tile(t), tpp = c.page / TILE, pg = g / tpp;
+    const int j = w.tile(t) * TILE, pg = page_of(c, j);
     const int e = table[pg];
     const bool ok = e >= 0 && e < c.n_pages;
-    const size_t off = (((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (size_t)(g - pg * tpp) * TILE) * hd;
+    const size_t off = (((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (j - pg * c.page)) * hd;
     lo = (uint32_t)off;
     hi = (uint32_t)(off >> 32);
     bad = __ballot(!ok);
@@ -1003,6 +1008,136 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   }
 }
 
+// BF16 cache, on the BF16 matrix cores: wave u of the workgroup's 4 holds 64 keys (group
+// u % KG) as fragments in registers and takes every RG-th (RG = 4 / KG) tile of 16 rows.  Rows
+// come through LDS, 16 RG at a time, FP32 ones cut into their three BF16 parts there
+// once for all waves, the next ones loading meanwhile; one barrier per stage.
+template <typename QT, int HD, int KG>
+__global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, RG = 4 / KG, SR = 16 * RG, NF = (RG * KS + 3) / 4;
+  __shared__ __attribute__((aligned(1024))) char frag[2][RG * KS * NP * 1024];
+  __shared__ __attribute__((aligned(16))) float lse[2][SR];
+  __shared__ __attribute__((aligned(16))) int slot[2][SR];
+  __shared__ float meet[RG > 1 ? (RG - 1) * KG * 64 : 1];
+  const Cache& c = a.c;
+  const int h = blockIdx.x, seq = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, q4 = lane >> 4, kg = wave % KG, rg = wave / KG;
+  int first, n;
+  seq_rows(c, seq, first, n);
+  const int len = seq_len(c, seq), p0 = len - n, rows = n * c.G;
+  const int b0 = blockIdx.y * KG * KEYS, k0 = b0 + kg * KEYS;   // first keys of the workgroup, of the wave
+  if (n == 0 || b0 >= len) return;
+  const int* table = c.table + seq * c.stride;
+  // this lane's account: key k0 + lane
+  const int key = min(k0 + lane, len - 1), pg = page_of(c, key), page = table[pg];
+  const bool live = k0 + lane < len && page >= 0 && page < c.n_pages;
+  float* account = a.mass + ((size_t)(live ? page : 0) * c.Hkv + h) * c.page + (key - pg * c.page);
+  const float before = live ? *account : 0.f;
+  bf8 kf[4][KS];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = min(k0 + j * TILE, (len - 1) / TILE * TILE), g = page_of(c, t), e = table[g];
+    const uint16_t* kr = static_cast<const uint16_t*>(c.k) +
+                         (((size_t)(e >= 0 && e < c.n_pages ? e : 0) * c.Hkv + h) * c.page + (t - g * c.page) + i16) * HD + q4 * 8;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) kf[j][k] = *reinterpret_cast<const bf8*>(kr + k * 32);
+  }
+  // the rows that can see a key of this workgroup
+  const int f_lo = max(0, b0 - p0) * c.G;
+  int t_hi = n;
+  if (a.window > 0 && b0 >= a.sinks) t_hi = (int)max((int64_t)0, min((int64_t)n, (int64_t)b0 + KG * KEYS - 1 + a.window - p0));
+  const int f_hi = t_hi * c.G;
+
+  Piece<QT, 8> next[NF];
+  float lse_next = 0.f;
+  int slot_next = -1;
+  auto load = [&](int f0) {                       // rows f0 .. f0 + SR - 1
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      const int u = wave + 4 * i, f = min(f0 + u / KS * 16 + i16, rows - 1), tok = f / c.G;   // fragment u: row tile, 32 dims
+      if (u < RG * KS)
+        next[i].load(static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD +
+                     u % KS * 32 + q4 * 8);
+    }
+    if (tid < SR) {
+      const int f = f0 + tid, tok = min(f, rows - 1) / c.G;
+      slot_next = f < f_hi ? p0 + tok : -1;       // -1: sees nothing
+      lse_next = a.lse[(size_t)(first + tok) * c.Hq + h * c.G + (min(f, rows - 1) - tok * c.G)];
+    }
+  };
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (f_lo < f_hi) load(f_lo);
+  int b = 0;
+  for (int f0 = f_lo; f0 < f_hi; f0 += SR, b ^= 1) {
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      const int u = wave + 4 * i;
+      if (u >= RG * KS) break;
+      char* d = frag[b] + u * NP * 1024 + lane * 16;
+      if constexpr (NP == 1) {
+        *reinterpret_cast<Piece<QT, 8>*>(d) = next[i];
+      } else {
+        float y[8];
+        bf8 part[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = next[i].get(e);
+        parts8<NP>(y, part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf8*>(d + p * 1024) = part[p];
+      }
+    }
+    if (tid < SR) {
+      lse[b][tid] = lse_next;
+      slot[b][tid] = slot_next;
+    }
+    __syncthreads();
+    if (f0 + SR < f_hi) load(f0 + SR);
+    v4f s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p) {
+        const bf8 qf = *reinterpret_cast<const bf8*>(frag[b] + ((rg * KS + k) * NP + p) * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf, kf[j][k], s[j], 0, 0, 0);
+      }
+    const float4 l4 = *reinterpret_cast<const float4*>(&lse[b][rg * 16 + 4 * q4]);
+    const int4 p4 = *reinterpret_cast<const int4*>(&slot[b][rg * 16 + 4 * q4]);
+    const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+    const int ps[4] = {p4.x, p4.y, p4.z, p4.w};
+    const int p_lo = slot[b][rg * 16], p_hi = slot[b][rg * 16 + 15];
+    const bool whole = __builtin_amdgcn_readfirstlane(p_hi >= 0 && all_see(k0, k0 + KEYS - 1, p_lo, p_hi, a.window, a.sinks));
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sum[j] += __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale, -ls[v]) * LOG2E);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale, -ls[v]) * LOG2E);
+          sum[j] += sees(ps[v], k0 + j * TILE + i16, a.window, a.sinks) ? y : 0.f;
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = sum4(sum[j]);
+  float y = q4 == 0 ? sum[0] : q4 == 1 ? sum[1] : q4 == 2 ? sum[2] : sum[3];   // key k0 + lane
+  if constexpr (RG > 1) {
+    if (rg > 0) meet[(wave - KG) * 64 + lane] = y;
+    __syncthreads();
+    if (rg > 0) return;
+#pragma unroll
+    for (int r = 0; r < RG - 1; ++r) y += meet[(r * KG + kg) * 64 + lane];
+  }
+  if (live) *account = before + y;
+}
+
 // ------------------------------------------------------------ eviction
 // Which slots of key head h of a sequence stay: n = min(len, keep) of them, the
 // first `sinks`, the last `recent`, and of the others those of most attention
@@ -1010,8 +1145,10 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
 // weights do (NaN above all, a sure slot above that, none for slots past the length), so the
 // n-th largest is found bit by bit with one count each.
 //
-// One workgroup per (sequence, head); wave w owns a run of slots, lane by lane, NV per lane in registers
-// (NV 0: read again for each count).
+// One workgroup per (sequence, head).  Wave w owns a run of slots, lane by lane, up to
+// NV per lane, whose ranks stay in registers (NV 0: longer, read again for each count).
+// The search takes two bits at a time, three counts by ballot; it ends early where a
+// bound has exactly n ranks at or above it.
 __device__ __forceinline__ uint32_t rank_of(float x) {
   if (x != x) return 0xfffffffeu;
   const uint32_t b = __float_as_uint(x + 0.f);    // -0 counts as 0
@@ -1021,11 +1158,11 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
 template <int NV>
 __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass, int keep, int sinks, int recent,
                                                       int* new_lens, int* kept) {
-  __shared__ int red[2][16], eq_of[16];
+  __shared__ int red[2][3][16], eq_of[16];
   const int h = blockIdx.x, seq = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = seq_len(c, seq), n = min(len, keep);
-  const int per = NV > 0 ? NV : (len + 1023) / 1024;   // slots per lane
+  const int per = (len + 1023) / 1024;            // slots per lane
   const int j0 = wave * per * 64 + lane;
   const int* table = c.table + seq * c.stride;
   int* out = kept + ((size_t)seq * c.Hkv + h) * keep;
@@ -1033,68 +1170,79 @@ __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass
   for (int d = n + tid; d < keep; d += 1024) out[d] = -1;
   if (n == 0) return;
   auto rank_at = [&](int j) -> uint32_t {
-    if (j >= len) return 0;
-    if (j < sinks || j >= len - recent) return 0xffffffffu;
-    const int e = table[j / c.page];
-    return e < 0 || e >= c.n_pages ? 0xfffffffeu : rank_of(mass[((size_t)e * c.Hkv + h) * c.page + j % c.page]);
+    const int jc = min(j, len - 1), pg = page_of(c, jc), e = table[pg];
+    const bool ok = e >= 0 && e < c.n_pages;
+    const float x = mass[((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (jc - pg * c.page)];
+    return j >= len ? 0u : j < sinks || j >= len - recent ? 0xffffffffu : ok ? rank_of(x) : 0xfffffffeu;
   };
+  constexpr int LOADS = 8;                        // under way at a time (more spill)
   uint32_t r[NV > 0 ? NV : 1];
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) r[i] = rank_at(j0 + i * 64);
+    for (int i = 0; i < NV; ++i) {
+      if (i % LOADS == 0) asm volatile("" ::: "memory");
+      r[i] = i < per ? rank_at(j0 + i * 64) : 0u;
+    }
   }
-  auto at = [&](int i) -> uint32_t {
-    if constexpr (NV > 0) return r[i];
-    else return rank_at(j0 + i * 64);
-  };
-  // this wave's slots for which f holds
-  auto count = [&](auto f) {
-    int k = 0;
+  // f(rank, i) for this lane's slots
+  auto each = [&](auto f) {
     if constexpr (NV > 0) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) k += f(r[i]);
+      for (int i = 0; i < NV; ++i)
+        if (i < per) f(r[i], i);
     } else {
-      for (int i = 0; i < per; ++i) k += f(at(i));
+      for (int i = 0; i < per; ++i) f(rank_at(j0 + i * 64), i);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) k += __shfl_xor(k, d, 64);
-    return k;
   };
-  uint32_t cut = 0;                               // the n-th largest rank, from its highest bit on
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t x = cut | 1u << bit;
-    const int k = count([&](uint32_t y) { return y >= x; });
-    if (lane == 0) red[bit & 1][wave] = k;
+  uint32_t cut = 0;                               // the n-th largest rank, from its highest bits on
+  bool exact = false;                             // n ranks are above it
+  for (int bit = 30; bit >= 0 && !exact; bit -= 2) {
+    const uint32_t x = 1u << bit;
+    int k1 = 0, k2 = 0, k3 = 0;
+    each([&](uint32_t y, int) {
+      k1 += __popcll(__ballot(y >= cut + x));
+      k2 += __popcll(__ballot(y >= cut + 2 * x));
+      k3 += __popcll(__ballot(y >= cut + 3 * x));
+    });
+    int(*rd)[16] = red[bit >> 1 & 1];
+    if (lane == 0) { rd[0][wave] = k1; rd[1][wave] = k2; rd[2][wave] = k3; }
     __syncthreads();
-    int all = 0;
+    int all[3];
 #pragma unroll
-    for (int u = 0; u < 16; ++u) all += red[bit & 1][u];
-    if (all >= n) cut = x;
+    for (int u = 0; u < 3; ++u) {
+      int v = rd[u][lane & 15];
+      v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);
+      v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);
+      v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+      v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
+      all[u] = __builtin_amdgcn_readfirstlane(v);
+    }
+    const int at = all[2] >= n ? 3 : all[1] >= n ? 2 : all[0] >= n ? 1 : 0;
+    cut += at * x;
+    if (at > 0 && all[at - 1] == n) {
+      --cut;
+      exact = true;
+    }
   }
-  const int more = count([&](uint32_t y) { return y > cut; }), same = count([&](uint32_t y) { return y == cut; });
+  int more = 0, same = 0;
+  each([&](uint32_t y, int) { more += __popcll(__ballot(y > cut)); same += __popcll(__ballot(y == cut)); });
   __syncthreads();
-  if (lane == 0) { red[0][wave] = more; eq_of[wave] = same; }
+  if (lane == 0) { red[0][0][wave] = more; eq_of[wave] = same; }
   __syncthreads();
-  int above = 0, pos = 0, ties = 0;               // slots above the cut in all; kept ones and ties before this wave
+  int above = 0, pos = 0, ties = 0;               // slots above the cut in all; above it and on it before this wave
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
-    above += red[0][u];
-    if (u < wave) { pos += red[0][u]; ties += eq_of[u]; }
+    above += red[0][0][u];
+    if (u < wave) { pos += red[0][0][u]; ties += eq_of[u]; }
   }
-  const int room = n - above;                     // ties that stay
-  auto put = [&](int i, uint32_t y) {
+  const int room = n - above;                     // of those on it, the first ones stay
+  each([&](uint32_t y, int i) {
     const uint64_t gt = __ballot(y > cut), eq = __ballot(y == cut), below = (1ull << lane) - 1;
-    const int gb = __popcll(gt & below), eb = __popcll(eq & below);
-    if (y > cut || (y == cut && ties + eb < room)) out[pos + gb + min(ties + eb, room)] = j0 + i * 64;
+    const int gb = __popcll(gt & below), eb = ties + __popcll(eq & below);
+    if (y > cut || (y == cut && eb < room)) out[pos + gb + min(eb, room)] = j0 + i * 64;
     pos += __popcll(gt);
     ties += __popcll(eq);
-  };
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) put(i, r[i]);
-  } else {
-    for (int i = 0; i < per; ++i) put(i, at(i));
-  }
+  });
 }
 
 // K, V and weight of the slots that stay, in their order, to the pages of `to`
@@ -1113,9 +1261,9 @@ __global__ __launch_bounds__(256) void move_kernel(Cache c, float* mass, const i
   float w[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int d = d0 + u * RPW, j = out[min(d, n - 1)], e = c.table[seq * c.stride + j / c.page];
+    const int d = d0 + u * RPW, j = out[min(d, n - 1)], pg = page_of(c, j), e = c.table[seq * c.stride + pg];
     const bool ok = e >= 0 && e < c.n_pages;
-    const size_t row = ((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + j % c.page;
+    const size_t row = ((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (j - pg * c.page);
     k[u] = static_cast<const uint4*>(c.k)[row * PIECES + piece];
     v[u] = static_cast<const uint4*>(c.v)[row * PIECES + piece];
     w[u] = mass[row];
@@ -1128,9 +1276,9 @@ __global__ __launch_bounds__(256) void move_kernel(Cache c, float* mass, const i
   for (int u = 0; u < U; ++u) {
     const int d = d0 + u * RPW;
     if (d >= n) break;
-    const int e = to[seq * to_stride + d / c.page];
+    const int pg = page_of(c, d), e = to[seq * to_stride + pg];
     if (e < 0 || e >= c.n_pages) continue;
-    const size_t row = ((size_t)e * c.Hkv + h) * c.page + d % c.page;
+    const size_t row = ((size_t)e * c.Hkv + h) * c.page + (d - pg * c.page);
     static_cast<uint4*>(c.k)[row * PIECES + piece] = k[u];
     static_cast<uint4*>(c.v)[row * PIECES + piece] = v[u];
     if (piece == 0) mass[row] = w[u];

@@ -47,8 +47,11 @@ int check_window(float scale, int32_t window, int32_t sinks) {
 Cache cache_of(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t page, int32_t n_pages, int32_t width,
                int64_t stride, const int32_t* starts, const int32_t* lens, const int32_t* table, const void* k,
                const void* v) {
+  int bits = 4;                                   // 2^bits >= page
+  while ((int64_t)1 << bits < page) ++bits;
+  const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + bits)) + page - 1) / page);
   return {const_cast<void*>(k), const_cast<void*>(v), table, stride, width, starts, lens, T, S, Hq, Hkv, Hq / Hkv,
-          n_pages, page};
+          n_pages, page, mul, 31 + bits};
 }
 
 template <int N> using Int = std::integral_constant<int, N>;
@@ -202,13 +205,25 @@ int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, i
   a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, nullptr);
   a.q = q; a.lse = lse; a.mass = mass;
   a.scale = scale; a.window = window; a.sinks = sinks;
+  // keys per workgroup: matrix tiles of BF16 with 4 (few rows) or 2 waves' keys of 64, or FP32 products
+  const bool tiles = kvdtype == SK_BF16 && hd >= 32, few = (int64_t)T * a.c.G <= 16ll * S;
   constexpr int NK2 = 2;
-  const int64_t blocks = ((int64_t)page * width + 64 * NK2 - 1) / (64 * NK2);
-  SK_CHECK(blocks <= 65535, SK_EINVAL, "width * page must be at most %d tokens", 65535 * 64 * NK2);
+  const int keys = tiles ? (few ? 4 : 2) * KEYS : 4 * NK2 * TILE;
+  const int64_t blocks = ((int64_t)page * width + keys - 1) / keys;
+  SK_CHECK(blocks <= 65535, SK_EINVAL, "width * page must be at most %d tokens", 65535 * keys);
+  const dim3 grid(Hkv, (unsigned)blocks, S);
   with_hd(hd, [&](auto d) {
     with_types(xdtype, kvdtype, [&](auto x, auto k) {
-      hipLaunchKernelGGL((mass_kernel<decltype(x), decltype(k), decltype(d)::value, NK2>), dim3(Hkv, (unsigned)blocks, S),
-                         dim3(256), 0, (hipStream_t)stream, a);
+      using X = decltype(x);
+      using K = decltype(k);
+      constexpr int HD = decltype(d)::value;
+      const hipStream_t st = (hipStream_t)stream;
+      if constexpr (HD >= 32 && sizeof(K) == 2) {
+        if (few) hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 4>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 2>), grid, dim3(256), 0, st, a);
+      } else {
+        hipLaunchKernelGGL((mass_kernel<X, K, HD, NK2>), grid, dim3(256), 0, st, a);
+      }
     });
   });
   SK_HIP(hipGetLastError());
@@ -237,9 +252,9 @@ int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t 
     hipLaunchKernelGGL((choose_kernel<decltype(nv)::value>), dim3(Hkv, S), dim3(1024), 0, st, c, mass, keep, sinks,
                        recent, new_lens, kept);
   };
-  if (cap <= 4 * 1024) choose(Int<4>{});
-  else if (cap <= 16 * 1024) choose(Int<16>{});
+  if (cap <= 8 * 1024) choose(Int<8>{});
   else if (cap <= 32 * 1024) choose(Int<32>{});
+  else if (cap <= 64 * 1024) choose(Int<64>{});
   else choose(Int<0>{});
   SK_HIP(hipGetLastError());
   const int pieces = hd * (kvdtype == SK_BF16 ? 2 : 4) / 16;
