@@ -302,12 +302,16 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
 /* Adds the attention weight that every slot got from the new tokens, exp(scale q k
  * - lse) summed over tokens and the group's heads, to its account in mass [n_pages][Hkv][page].  q, lse,
  * scale, window, sinks as in the attention call.  The order of sums is fixed; two sequences of
- * one call must not share a page that both see. */
+ * one call must not share a page that both see.  Workspace as for attention. */
+int sk_op_paged_attention_mass_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd,
+                                         int32_t page, int32_t width, int32_t xdtype, int32_t kvdtype,
+                                         int64_t* bytes);
 int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd,
                                int32_t page, int32_t n_pages, int32_t width, int64_t table_stride,
                                int32_t xdtype, int32_t kvdtype, float scale, int32_t window, int32_t sinks,
                                const void* q, const float* lse, const void* k_pages, const int32_t* table,
-                               const int32_t* starts, const int32_t* lens, float* mass);
+                               const int32_t* starts, const int32_t* lens, float* mass, void* workspace,
+                               int64_t workspace_bytes);
 /* Cuts caches back to n = min(lens[s], keep) slots: of every key head the first
  * `sinks`, the last `recent` and, of the others, those with the largest accounts (ties to
  * the lowest slot, NaN above all) move in their order, with their accounts, to slots 0 .. n - 1 of the

@@ -62,6 +62,14 @@ __device__ __forceinline__ float fold4(float v, F f) {
   const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
   return f(__int_as_float(b[0]), __int_as_float(b[1]));
 }
+template <typename F>
+__device__ __forceinline__ float fold2(float v, F f) {   // lanes l and l ^ 32
+  const int x = __float_as_int(v);
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(__int_as_float(a[0]), __int_as_float(a[1]));
+}
+__device__ __forceinline__ float sum2(float v) { return fold2(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float max2(float v) { return fold2(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float sum4(float v) { return fold4(v, [](float a, float b) { return a + b; }); }
 __device__ __forceinline__ float max4(float v) { return fold4(v, [](float a, float b) { return fmaxf(a, b); }); }
 
@@ -263,8 +271,9 @@ struct AttendArgs {
   float scale2;                                   // scale * log2 e: exp(s - m) = 2^(scale2 (qk - max qk))
   int window, sinks;                              // window 0: all keys
   int cut;                                        // tiles of keys per cut; cuts of a row: blockIdx.z
-  float* part; float* ml;                         // [cuts][T * Hq][hd], [cuts][T * Hq][2]
+  float* part; float* ml;                         // [cuts][T * Hq][hd], [cuts][T * Hq][2]: sums of V, (maximum times scale2, sum)
 };
+constexpr float LOWEST = -3e38f;                  // a maximum of nothing: finite, so that -infinity less it is -infinity
 
 // The tiles that the rows of slots p_lo .. p_hi walk: 0 .. n - 1, first those of the sinks, then the window's.
 struct Walk {
@@ -541,7 +550,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     float mx = -INFINITY, l = 0.f, f[WK];
 #pragma unroll
     for (int u = 0; u < WK; ++u) mx = fmaxf(mx, pm[u * R + tid]);
-    const float m2 = mx == -INFINITY ? 0.f : mx * a.scale2;
+    const float m2 = mx == -INFINITY ? LOWEST : mx * a.scale2;
 #pragma unroll
     for (int u = 0; u < WK; ++u) {
       f[u] = __builtin_amdgcn_exp2f(fmaf(pm[u * R + tid], a.scale2, -m2));
@@ -556,7 +565,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
       if (!alone) {
         float* d = a.ml + ((size_t)cut * c.T * c.Hq + at) * 2;
-        d[0] = mx;
+        d[0] = m2;
         d[1] = l;
       } else if (a.lse) {
         a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
@@ -588,13 +597,14 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 }
 
 // ------------------------------------------------------------ many rows, BF16 cache
-// The same sums for chunks, on the BF16 matrix cores.  A workgroup's 4 waves own
-// 16 RT rows each and share tiles of 64 keys in LDS (two stages, loaded ahead straight from the pages).
-//   S^T = K Q^T: K as 16 x 32 fragments, whole in LDS, Q in registers; lane l holds row l % 16 against keys
-//     4 (l / 16) + v of each 16;
-//   O^T += V^T P^T: those values are P's fragment for a set of 32 keys as they are: element e of
-//     lane group g is key 4 g + e of the first 16 or (e >= 4) of the second.  V lies in LDS
-//     row by row; the transposing LDS read gives a lane 4 keys of one dim.
+// The same sums for chunks, on the BF16 matrix cores (32 x 32 x 16: half the
+// instructions of 16 x 16 x 32 for the same products, and VALU work beside them runs under
+// them).  A workgroup's 4 waves own 32 rows each and share steps of 64 keys in LDS, two
+// slots each for K and V, loaded ahead straight from the pages.
+//   S^T = K Q^T: K in fragments, Q in registers; lane l holds row l % 32's products with keys
+//     8 i + 4 (l / 32) + r (i, r < 4) of each 32;
+//   O^T += V^T P^T: eight of those values are P's fragment for 16 keys as they are.  V
+//     lies in LDS row by row; the transposing LDS read gives a lane 4 keys of one dim.
 // FP32 activations: Q and P as three BF16 parts of 8 bits that add up to the FP32 value
 // exactly, three products each, so results are those of FP32 products (NP = 3).  BF16
 // activations: P rounds to BF16 once (2^-9 of a weight on average, under the output's own rounding).
@@ -602,12 +612,13 @@ constexpr int KEYS = 64;                          // keys of a step
 
 template <int HD>
 struct TileLds {
-  static constexpr int K = KEYS * HD * 2, STAGE = 2 * K;   // bytes
-  // 16-byte piece of V row `key` that holds piece x: rows that the transposing read takes together
-  // lie in different banks
-  static __device__ __forceinline__ int swizzle(int key) { return HD == 128 ? 2 * (key & 7) : HD == 64 ? 2 * (key >> 1 & 3) : 2 * (key >> 2 & 1); }
+  static constexpr int K = KEYS * HD * 2;         // bytes of a slot
+  // V row `key` holds its 32 bytes number x at x ^ turn(key): rows that the
+  // transposing read takes together lie in different banks
+  static __device__ __forceinline__ int turn(int key) { return HD == 128 ? key & 7 : HD == 64 ? key >> 1 & 3 : key >> 2 & 1; }
 };
 
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -637,12 +648,12 @@ __device__ __forceinline__ void parts8(const float* x, bf8* out) {
   }
 }
 
-template <typename QT, int HD, int RT>
+template <typename QT, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_tiles_kernel(AttendArgs a) {
-  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, NDT = HD / 16, R = 64 * RT;
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, R = 128;
   constexpr int GROUP = TILE * HD * 2;            // bytes of 16 keys
   using L = TileLds<HD>;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * L::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * L::K];   // two slots of K, two of V
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   int seq, tile_no;
@@ -656,22 +667,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int begin = cut * a.cut, end = min(w.n, begin + a.cut);
   if (cut > 0 && begin >= w.n) return;            // the first cut also answers for rows that see nothing
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane & 15, q4 = lane >> 4;
+  const int i16 = lane & 15, q4 = lane >> 4, i32 = lane & 31, half = lane >> 5;
   const int* table = c.table + seq * c.stride;
 
-  int qp[RT];                                     // the slot of this lane's rows (rows past the last repeat it)
-  bf8 qf[RT][NP][KS];
-#pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const int f = min(f0 + (wave * RT + j) * 16 + i16, rows - 1), tok = f / c.G;
-    qp[j] = p0 + tok;
+  int qp;                                         // the slot of this lane's row (rows past the last repeat it)
+  bf8 qf[NP][2 * KS];
+  {
+    const int f = min(f0 + wave * 32 + i32, rows - 1), tok = f / c.G;
+    qp = p0 + tok;
     const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
+    for (int k = 0; k < 2 * KS; ++k) {
       Piece<QT, 8> x;
-      x.load(qr + k * 32 + q4 * 8);
+      x.load(qr + k * 16 + half * 8);
       if constexpr (NP == 1) {
-        qf[j][0][k] = __builtin_bit_cast(bf8, x);
+        qf[0][k] = __builtin_bit_cast(bf8, x);
       } else {
         float y[8];
         bf8 part[NP];
@@ -679,198 +689,293 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int e = 0; e < 8; ++e) y[e] = x.get(e);
         parts8<NP>(y, part);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) qf[j][p][k] = part[p];
+        for (int p = 0; p < NP; ++p) qf[p][k] = part[p];
       }
     }
   }
 
-  // wave u loads the u-th 16 keys of a step: K as fragments, V as rows, KS loads
-  // of 1 KB each; V's 8 rows further are swizzled alike
+  // wave u loads the u-th 16 keys of a step: K as blocks of 16 keys x 32 dims (16 bytes per
+  // lane, keys first), V as rows, KS loads of 1 KB each (with 128 dims 4 rows, every other
+  // load turned by 4 more)
   const unsigned koff = (i16 * HD + q4 * 8) * 2;
-  constexpr int NVO = HD == 128 ? 2 : 1;
-  unsigned voff[NVO];
-#pragma unroll
-  for (int k = 0; k < NVO; ++k) {
-    const int piece = k * 64 + lane, key = piece / (HD / 8), x = piece % (HD / 8);
-    voff[k] = (key * HD + (x ^ L::swizzle(key)) * 8) * 2;
-  }
-  unsigned vread[NDT];                            // this lane's bytes of 16 dims of V's first 16 keys
-#pragma unroll
-  for (int t = 0; t < NDT; ++t) {
-    const int key = 4 * q4 + (i16 >> 2), x = 2 * t + ((i16 & 3) >> 1);
-    vread[t] = L::K + key * HD * 2 + (x ^ L::swizzle(key)) * 16 + (i16 & 1) * 8;
-  }
+  const int vrow = lane / (HD / 8);
+  const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn(vrow)) * 8) * 2;
+  // this lane's bytes of K's fragment for a 32 x 16 block, and of 32 dims (the u-th) of V: vbase + (64 u ^ vturn)
+  const unsigned kbase = (i32 >> 4) * KS * 1024 + (half * 16 + i16) * 16;
+  const int vkey = 4 * half + (i16 >> 2);
+  const unsigned vbase = vkey * HD * 2 + (i16 & 3) * 8, vturn = ((q4 & 1) ^ L::turn(vkey)) * 32;
+  // AHEAD: K runs a step ahead of V, and while the weights of one step form, the matrix
+  // cores have the next one's scores to work on (registers for both scores: not
+  // beside the three parts of 128 dims)
+  constexpr bool AHEAD = NP * HD <= 256;
   TileOffsets offs;
   int at = 0;                                     // the next step's first lane in offs
-  // loads the step whose first tile is t; gives which of its four tiles have no page
-  auto prefetch = [&](int t) -> int {
+  size_t v_off = 0;                               // where V of the step after lies
+  auto place = [&](int t) -> int {                // the step whose first tile is t; gives which of its tiles have no page
     if (at == 64) at = 0;
     if (at == 0) offs.load(c, table, w, t, 1, end, h, HD);
-    const size_t off = offs.at(at + wave) * 2;
+    v_off = offs.at(at + wave) * 2;
     const int none = offs.bad >> at & 15;
     at += 4;
-    const char* st = lds + ((t - begin) / 4 % 2) * L::STAGE + wave * GROUP;
-    const char* kb = static_cast<const char*>(c.k) + off;
-    const char* vb = static_cast<const char*>(c.v) + off;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) lds_load16(kb + k * 64, koff, st + k * 1024);
-#pragma unroll
-    for (int k = 0; k < KS; ++k) lds_load16(vb + k / NVO * NVO * 1024, voff[k % NVO], st + L::K + k * 1024);
     return none;
   };
-  v4f o[RT][NDT];
-  float mr[RT], lr[RT];
+  auto load_k = [&](int t) {
+    const char* st = lds + ((t - begin) / 4 % 2) * L::K + wave * GROUP;
+    const char* kb = static_cast<const char*>(c.k) + v_off;
 #pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    mr[j] = -INFINITY;
-    lr[j] = 0.f;
+    for (int k = 0; k < KS; ++k) lds_load16(kb + k * 64, koff, st + k * 1024);
+  };
+  auto load_v = [&](int t, size_t off) {
+    const char* st = lds + 2 * L::K + ((t - begin) / 4 % 2) * L::K + wave * GROUP;
+    const char* vb = static_cast<const char*>(c.v) + off;
 #pragma unroll
-    for (int t = 0; t < NDT; ++t) o[j][t] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
-  int bad_next = begin < end ? prefetch(begin) : 0;
+    for (int k = 0; k < KS; ++k) lds_load16(vb + k * 1024, HD == 128 && k % 2 ? voff ^ 128 : voff, st + k * 1024);
+  };
+  v16f o[KS], s[2];
+  float m2 = LOWEST, lr = 0.f;                    // the maximum that sums refer to (times scale2), the sum
+#pragma unroll
+  for (int u = 0; u < KS; ++u)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[u][v] = 0.f;
+  // scores against 32 keys (i / KP) of a step, KU times 16 dims at a time: the fragments, the products
+  constexpr int KU = AHEAD ? KS : KS / 2, KP = 2 * KS / KU;
+  auto read_k = [&](int t, int i, bf8 (&kf)[KU]) {
+    const char* st = lds + ((t - begin) / 4 % 2) * L::K + kbase + i / KP * 2 * GROUP;
+#pragma unroll
+    for (int k = 0; k < KU; ++k) kf[k] = *reinterpret_cast<const bf8*>(st + (i % KP * KU + k) * 512);
+  };
+  auto scores = [&](int i, const bf8 (&kf)[KU], v16f (&x)[2]) {
+    if (i % KP == 0) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[i / KP][v] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < KU; ++k)
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+        x[i / KP] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k], qf[p][i % KP * KU + k], x[i / KP], 0, 0, 0);
+  };
+  // V of 16 keys (q / VP): VU times 32 dims at a time
+  constexpr int VU = AHEAD ? KS : KS / 2, VP = KS / VU;
+  auto read_v = [&](const char* vst, int q, bf8 (&vf)[VU]) {
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      typedef __attribute__((address_space(3))) s4 lds4;
+      const char* vr = vst + (vbase + ((q % VP * VU + u) * 64 ^ vturn)) + q / VP * GROUP;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vr);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vr + GROUP / 2));
+      vf[u] = __builtin_bit_cast(bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
   bool wild = false;                              // infinities or NaN in V beside a mask
-  for (int t = begin; t < end; t += 4) {
-    stage_sync<0>();                              // this step is in, and every wave is done with the other stage
-    const int bad = bad_next;
-    if (t + 4 < end) bad_next = prefetch(t + 4);
-    char* st = lds + ((t - begin) / 4 % 2) * L::STAGE;
+  int bad = 0, bad1 = 0;                          // tiles without a page of this step, the next
+  // the step at t: V of it and K (of the next one with AHEAD, whose scores of this one are in s) are loaded
+  auto step = [&](int t, auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    int bad2 = 0;
+    stage_sync<0>();                              // they are in, and every wave is done with the slots loaded next
+    bf8 kf[2][KU];
+    if constexpr (!AHEAD) {
+      if (t + 4 < end) {
+        bad2 = place(t + 4);
+        load_k(t + 4);
+        load_v(t + 4, v_off);
+      }
+      read_k(t, 0, kf[0]);
+#pragma unroll
+      for (int i = 0; i < 2 * KP; ++i) {
+        if (i + 1 < 2 * KP) read_k(t, i + 1, kf[(i + 1) % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        scores(i, kf[i % 2], s);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (MORE) {
+      load_v(t + 4, v_off);
+      if (t + 8 < end) {
+        bad2 = place(t + 8);
+        load_k(t + 8);
+      }
+      read_k(t + 4, 0, kf[0]);
+    }
+    char* vst = lds + 2 * L::K + ((t - begin) / 4 % 2) * L::K;
     const int k_first = w.tile(t) * TILE, k_last = w.tile(min(t + 3, end - 1)) * TILE + TILE - 1;
-    const bool whole = !bad && t + 4 <= end && all_see(k_first, k_last, p_lo, p_hi, a.window, a.sinks);
-    if (!whole) {                                 // each wave tames the V that it loaded
-      bool odd = false;
+    if (bad || t + 4 > end || !all_see(k_first, k_last, p_lo, p_hi, a.window, a.sinks)) {
+      bool odd = false;                           // each wave tames the V that it loaded
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        auto* x = reinterpret_cast<Piece<uint16_t, 8>*>(st + L::K + wave * GROUP + k * 1024 + lane * 16);
+        auto* x = reinterpret_cast<Piece<uint16_t, 8>*>(vst + wave * GROUP + k * 1024 + lane * 16);
         Piece<uint16_t, 8> y = *x;
         odd |= y.tame();
         *x = y;
       }
-      wild |= __syncthreads_or(odd);
-    }
-    v4f s[RT][4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-#pragma unroll
-      for (int j = 0; j < RT; ++j) s[j][g] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const bf8 kf = *reinterpret_cast<const bf8*>(st + (g * KS + k) * 1024 + lane * 16);
-#pragma unroll
-        for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) s[j][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[j][p][k], s[j][g], 0, 0, 0);
-      }
-    }
-    if (!whole) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int k0 = w.tile(min(t + g, end - 1)) * TILE;
+        const int k0 = w.tile(min(t + g, end - 1)) * TILE + 4 * half;
 #pragma unroll
-        for (int j = 0; j < RT; ++j)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            if (bad >> g & 1) s[j][g][v] = NAN;
-            if (t + g >= end || !sees(qp[j], k0 + 4 * q4 + v, a.window, a.sinks)) s[j][g][v] = -INFINITY;
-          }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      float mx = s[j][0][0];
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][g][v]);
-      mx = max4(mx);
-      const float mn = fmaxf(mr[j], mx);
-      const float m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
-      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
-      float sum = 0.f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          s[j][g][v] = __builtin_amdgcn_exp2f(fmaf(s[j][g][v], a.scale2, -m2));
-          sum += s[j][g][v];
+        for (int v = 0; v < 8; ++v) {
+          if (bad >> g & 1) s[g / 2][g % 2 * 8 + v] = NAN;
+          if (t + g >= end || !sees(qp, k0 + v / 4 * 8 + v % 4, a.window, a.sinks)) s[g / 2][g % 2 * 8 + v] = -INFINITY;
         }
-      lr[j] = lr[j] * sc + sum;                   // this lane's keys; a row's four lanes add up at the end
-      mr[j] = mn;
-      if (__any(sc != 1.f)) {
-#pragma unroll
-        for (int u = 0; u < NDT; ++u) o[j][u] *= sc;
       }
+      wild |= __builtin_amdgcn_readfirstlane(__syncthreads_or(odd)) != 0;
     }
+    // a row's sums refer to a maximum of earlier steps until one is past it by 2^8: weights are
+    // at most that, and O is rarely rescaled
+    float sc = s[0][0];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {                 // sets of 32 keys
-      bf8 pf[RT][NP];
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        float y[8];
+      for (int v = 0; v < 16; ++v) sc = fmaxf(sc, s[g][v]);
+    sc = max2(sc);
+    sc *= a.scale2;
+    const bool grown = __any(sc > m2 + 8.f);
+    if (grown) {
+      const float x = fmaxf(m2, sc);
+      sc = m2 == x ? 1.f : __builtin_amdgcn_exp2f(m2 - x);
+      lr *= sc;
+      m2 = x;
+    }
+    // the matrix cores' part of a step goes first where two waves of a SIMD are apart (2,047
+    // tokens over 16,384, BF16: 287 -> 262 us; no change with three parts)
+    if constexpr (AHEAD) __builtin_amdgcn_s_setprio(1);
+    v16f s2[2];
+    bf8 pf[4][NP], vf[2][VU];                     // weights of the four sets of 16 keys
+    auto weights = [&](int g) {
+      float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = s[j][2 * g + e / 4][e % 4];
-        parts8<NP>(y, pf[j]);
+      for (int e = 0; e < 8; ++e) {
+        y[e] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][g % 2 * 8 + e], a.scale2, -m2));
+        lr += y[e];                               // this lane's keys; a row's two lanes add up at the end
       }
+      parts8<NP>(y, pf[g]);
+      // formed here, under the products beside it
 #pragma unroll
-      for (int u = 0; u < NDT; ++u) {
-        typedef __attribute__((address_space(3))) s4 lds4;
-        const char* vr = st + vread[u] + 2 * g * GROUP;
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vr);
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vr + GROUP));
-        const bf8 vf = __builtin_bit_cast(bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int p = 0; p < NP; ++p) asm volatile("" : "+v"(pf[g][p]));
+      asm volatile("" : "+v"(lr));
+    };
+    auto values = [&](int q) {
+#pragma unroll
+      for (int u = 0; u < VU; ++u)
 #pragma unroll
         for (int p = NP - 1; p >= 0; --p)
+          o[q % VP * VU + u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[q % 2][u], pf[q / VP][p], o[q % VP * VU + u], 0, 0, 0);
+    };
+    auto rescale = [&]() {
+      if (!grown) return;
 #pragma unroll
-          for (int j = 0; j < RT; ++j) o[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[j][p], o[j][u], 0, 0, 0);
+      for (int u = 0; u < KS; ++u) o[u] *= sc;
+    };
+    // sets of products with the LDS reads of the next ahead of each and the weights spread under them
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {               // 0, 1: scores of the next step's first 32 keys; 2 - 5: values; 6, 7: the other scores
+        constexpr int NEXT_K[8] = {1, -1, -1, -1, -1, 2, 3, -1}, NEXT_V[8] = {-1, 0, 1, 2, 3, -1, -1, -1};
+        if constexpr (MORE) {
+          if (NEXT_K[i] >= 0) read_k(t + 4, NEXT_K[i], kf[NEXT_K[i] % 2]);
+        }
+        if (NEXT_V[i] >= 0) read_v(vst, NEXT_V[i], vf[NEXT_V[i] % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MORE) {
+          if (i < 2) scores(i, kf[i % 2], s2);
+          if (i > 5) scores(i - 4, kf[i % 2], s2);
+        }
+        if (i == 2) rescale();
+        if (i >= 2 && i < 6) values(i - 2);
+        if (i < 4) weights(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i <= 4 * VP; ++i) {
+        if (i < 4 * VP) read_v(vst, i, vf[i % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 1) rescale();
+        if (i > 0) values(i - 1);
+        if (i % VP == 0 && i < 4 * VP) weights(i / VP);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if constexpr (MORE) {
+      s[0] = s2[0];
+      s[1] = s2[1];
+    }
+    if constexpr (AHEAD) __builtin_amdgcn_s_setprio(0);
+    bad = AHEAD ? bad1 : bad2;
+    bad1 = bad2;
+  };
+  if (begin < end) {
+    bad = place(begin);
+    load_k(begin);
+    load_v(begin, v_off);
   }
-  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
+  if constexpr (!AHEAD) {
+    for (int t = begin; t < end; t += 4) step(t, std::false_type{});
+  } else if (begin < end) {
+    if (begin + 4 < end) bad1 = place(begin + 4);
+    stage_sync<0>();
+    if (begin + 4 < end) load_k(begin + 4);
 #pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const int f = f0 + (wave * RT + j) * 16 + i16, tok = f / c.G;
-    const float l = lr[j] = sum4(lr[j]);
-    if (f >= rows) continue;
+    for (int i = 0; i < 4; ++i) {
+      bf8 kf[KU];
+      read_k(begin, i, kf);
+      scores(i, kf, s);
+    }
+    int t = begin;
+    for (; t + 4 < end; t += 4) step(t, std::true_type{});
+    step(t, std::false_type{});
+  }
+
+  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
+  const int f = f0 + wave * 32 + i32, tok = f / c.G;
+  const float l = sum2(lr);
+  if (f < rows) {
     const size_t row = (size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G);
-    const bool none = qp[j] < 0;                  // no key is seen
+    const bool none = qp < 0;                     // no key is seen
     const float y = alone ? none ? 0.f : 1.f / l : 1.f;
-    if (q4 == 0) {
+    if (half == 0) {
       if (!alone) {
         float* d = a.ml + ((size_t)cut * c.T * c.Hq + row) * 2;
-        d[0] = mr[j];
+        d[0] = m2;
         d[1] = l;
       } else if (a.lse) {
-        a.lse[row] = none ? -INFINITY : ((mr[j] == -INFINITY ? 0.f : mr[j] * a.scale2) + log2f(l)) * LN2;
+        a.lse[row] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
       }
     }
 #pragma unroll
-    for (int u = 0; u < NDT; ++u) {
-      const int d = 16 * u + 4 * q4;
-      if (alone) store4(static_cast<QT*>(a.out) + row * HD + d, y * o[j][u][0], y * o[j][u][1], y * o[j][u][2], y * o[j][u][3]);
-      else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + row) * HD + d) =
-          make_float4(o[j][u][0], o[j][u][1], o[j][u][2], o[j][u][3]);
-    }
-  }  if (wild) {
-    __threadfence_block();                        // the stores above, by other lanes
+    for (int u = 0; u < KS; ++u)
 #pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      const int f_lo = f0 + (wave * RT + j) * 16;
-      add_wild<QT, uint16_t, HD>(
-          a, h, table, first, p0, f_lo, min(f_lo + 16, rows), w, begin, end,
-          alone ? nullptr : a.part + (size_t)cut * c.T * c.Hq * HD,
-          [&](int t) {
-            const int t0 = begin + (t - begin) / 4 * 4, t3 = min(t0 + 3, end - 1);
-            bool none = t0 + 4 > end;             // as the loop above judged the step
-            for (int u = t0; u <= t3; ++u) {
-              const int e = table[w.tile(u) * TILE / c.page];
-              none |= e < 0 || e >= c.n_pages;
-            }
-            return none || !all_see(w.tile(t0) * TILE, w.tile(t3) * TILE + TILE - 1, p_lo, p_hi, a.window, a.sinks);
-          },
-          [&](int f) {
-            const float m = __shfl(mr[j], f - f_lo, 64);
-            return make_float2(m == -INFINITY ? 0.f : m * a.scale2, alone ? 1.f / __shfl(lr[j], f - f_lo, 64) : 1.f);
-          });
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * u + 8 * i + 4 * half;
+        if (alone) store4(static_cast<QT*>(a.out) + row * HD + d, y * o[u][4 * i], y * o[u][4 * i + 1], y * o[u][4 * i + 2], y * o[u][4 * i + 3]);
+        else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + row) * HD + d) =
+            make_float4(o[u][4 * i], o[u][4 * i + 1], o[u][4 * i + 2], o[u][4 * i + 3]);
+      }
+  }
+  if (wild) {
+    __threadfence_block();                        // the stores above, by other lanes
+    int seq2, tile2, first2, n2;                  // found again: few registers are held for this through the loop
+    find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq2, tile2);
+    seq_rows(c, seq2, first2, n2);
+    const int q0 = seq_len(c, seq2) - n2, f_lo = tile2 * R + wave * 32, f_hi = min(tile2 * R + R, n2 * c.G);
+    const int q_lo = q0 + tile2 * R / c.G, q_hi = q0 + (f_hi - 1) / c.G;
+    const Walk v = walk_of(q_lo, q_hi, a.window, a.sinks);
+    const int b2 = blockIdx.z * a.cut, e2 = min(v.n, b2 + a.cut);
+    const int* tab = c.table + seq2 * c.stride;
+    add_wild<QT, uint16_t, HD>(
+        a, h, tab, first2, q0, f_lo, min(f_lo + 32, f_hi), v, b2, e2,
+        v.n <= a.cut ? nullptr : a.part + (size_t)blockIdx.z * c.T * c.Hq * HD,
+        [&](int t) {
+          const int t0 = b2 + (t - b2) / 4 * 4, t3 = min(t0 + 3, e2 - 1);
+          bool none = t0 + 4 > e2;                // as the loop above judged the step
+          for (int u = t0; u <= t3; ++u) {
+            const int e = tab[page_of(c, v.tile(u) * TILE)];
+            none |= e < 0 || e >= c.n_pages;
+          }
+          return none || !all_see(v.tile(t0) * TILE, v.tile(t3) * TILE + TILE - 1, q_lo, q_hi, a.window, a.sinks);
+        },
+        [&](int g) {
+          return make_float2(__shfl(m2, g - f_lo, 64), v.n <= a.cut ? 1.f / __shfl(l, g - f_lo, 64) : 1.f);
+        });
   }
 }
 
@@ -891,16 +996,15 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int R, int c
   if (w.n <= a.cut) return;                       // one cut: its workgroup wrote the answer
   const int ns = min((w.n + a.cut - 1) / a.cut, cuts);
   const size_t step = (size_t)c.T * c.Hq;
-  float mx = -INFINITY;
-  for (int s = lane; s < ns; s += 64) mx = fmaxf(mx, a.ml[(s * step + at) * 2]);
+  float m2 = LOWEST;
+  for (int s = lane; s < ns; s += 64) m2 = fmaxf(m2, a.ml[(s * step + at) * 2]);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-  const float m2 = mx == -INFINITY ? 0.f : mx * a.scale2;
+  for (int d = 1; d < 64; d *= 2) m2 = fmaxf(m2, __shfl_xor(m2, d, 64));
   constexpr int E = HD >= 64 ? HD / 64 : 1;       // dims per lane
   float y[E] = {}, l = 0.f;
   for (int s = 0; s < ns; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(a.ml + (s * step + at) * 2);
-    const float wt = __builtin_amdgcn_exp2f(fmaf(ml.x, a.scale2, -m2));
+    const float wt = __builtin_amdgcn_exp2f(ml.x - m2);
     l = fmaf(wt, ml.y, l);
     const float* p = a.part + (s * step + at) * HD;
 #pragma unroll
@@ -930,7 +1034,17 @@ struct MassArgs {
   const void* q; const float* lse; float* mass;   // [n_pages][Hkv][page]
   float scale;
   int window, sinks;
+  int cut, cuts;                                  // rows per cut, cuts of a sequence's rows
+  float* part;                                    // [S][cuts][Hkv][width * page] of sequences with several
 };
+// The rows (token, head of the group) of a sequence that can see one of `keys` slots from k0 on.
+__device__ __forceinline__ void mass_rows(const MassArgs& a, int n, int p0, int k0, int keys, int& f_lo, int& f_hi) {
+  const int G = a.c.G;
+  f_lo = min(max(0, k0 - p0), n) * G;
+  f_hi = n * G;
+  if (a.window > 0 && k0 >= a.sinks)
+    f_hi = (int)max((int64_t)0, min((int64_t)n, (int64_t)k0 + keys - 1 + a.window - p0)) * G;
+}
 
 template <typename QT, typename KT, int HD, int NK2>
 __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
@@ -1008,134 +1122,192 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   }
 }
 
-// BF16 cache, on the BF16 matrix cores: wave u of the workgroup's 4 holds 64 keys (group
-// u % KG) as fragments in registers and takes every RG-th (RG = 4 / KG) tile of 16 rows.  Rows
-// come through LDS, 16 RG at a time, FP32 ones cut into their three BF16 parts there
-// once for all waves, the next ones loading meanwhile; one barrier per stage.
-template <typename QT, int HD, int KG>
+// BF16 cache, on the BF16 matrix cores.  Each wave holds 64 keys as fragments in registers, and the
+// workgroup's 256 keys meet the rows in LDS, N at a time: FP32 ones are cut into
+// their three BF16 parts there, once for all waves, the next ones loading meanwhile in registers; two slots, one
+// barrier per stage.
+//   N = 32 (many rows): S = Q K^T by 32 x 32 x 16; lane l holds rows 8 i + 4 (l / 32) + r (i, r < 4) against key l % 32.
+//   N = 16 (few rows, where the bytes of K decide: 64 bytes of 16 keys per load): 16 x 16 x 32; rows
+//     4 (l / 16) + r against key l % 16.
+// Many rows on few keys are cut over workgroups, whose sums mass_join_kernel adds in order.
+template <typename QT, int HD, int N>
 __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
-  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, RG = 4 / KG, SR = 16 * RG, NF = (RG * KS + 3) / 4;
-  __shared__ __attribute__((aligned(1024))) char frag[2][RG * KS * NP * 1024];
-  __shared__ __attribute__((aligned(16))) float lse[2][SR];
-  __shared__ __attribute__((aligned(16))) int slot[2][SR];
-  __shared__ float meet[RG > 1 ? (RG - 1) * KG * 64 : 1];
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KD = 512 / N, KS = HD / KD;   // dims of a fragment, fragments of a row tile
+  constexpr int NJ = 64 / N, NV = N * N / 64, NF = (KS + 3) / 4;            // key tiles of a wave, values per lane, fragments per wave
+  using acc = std::conditional_t<N == 32, v16f, v4f>;
+  __shared__ __attribute__((aligned(1024))) char frag[2][KS * NP * 1024];
+  __shared__ __attribute__((aligned(16))) float lse[2][N];
+  __shared__ __attribute__((aligned(16))) int slot[2][N];
   const Cache& c = a.c;
-  const int h = blockIdx.x, seq = blockIdx.z;
+  const int h = blockIdx.x, seq = blockIdx.z / a.cuts, cut = blockIdx.z - seq * a.cuts;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane & 15, q4 = lane >> 4, kg = wave % KG, rg = wave / KG;
+  const int in = lane % N, part = lane / N;       // row or key of a fragment, its piece of 8 dims
   int first, n;
   seq_rows(c, seq, first, n);
   const int len = seq_len(c, seq), p0 = len - n, rows = n * c.G;
-  const int b0 = blockIdx.y * KG * KEYS, k0 = b0 + kg * KEYS;   // first keys of the workgroup, of the wave
+  const int b0 = blockIdx.y * 4 * KEYS, k0 = b0 + wave * KEYS;   // first keys of the workgroup, of the wave
   if (n == 0 || b0 >= len) return;
+  int f_lo, f_end;
+  mass_rows(a, n, p0, b0, 4 * KEYS, f_lo, f_end);
+  const bool alone = f_end - f_lo <= a.cut;       // one cut: added to the accounts here
+  f_lo += cut * a.cut;
+  if (f_lo >= f_end) return;
+  const int f_hi = min(f_end, f_lo + a.cut);
   const int* table = c.table + seq * c.stride;
   // this lane's account: key k0 + lane
   const int key = min(k0 + lane, len - 1), pg = page_of(c, key), page = table[pg];
   const bool live = k0 + lane < len && page >= 0 && page < c.n_pages;
-  float* account = a.mass + ((size_t)(live ? page : 0) * c.Hkv + h) * c.page + (key - pg * c.page);
-  const float before = live ? *account : 0.f;
-  bf8 kf[4][KS];
+  float* account = alone ? a.mass + ((size_t)(live ? page : 0) * c.Hkv + h) * c.page + (key - pg * c.page)
+                         : a.part + (((size_t)seq * a.cuts + cut) * c.Hkv + h) * ((size_t)c.width * c.page) + key;
+  const float before = alone && live ? *account : 0.f;
+  bf8 kf[NJ][KS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int t = min(k0 + j * TILE, (len - 1) / TILE * TILE), g = page_of(c, t), e = table[g];
+  for (int j = 0; j < NJ; ++j) {                  // lanes past the length read its last 16 keys
+    const int t = min((k0 + j * N + in) / TILE * TILE, (len - 1) / TILE * TILE), g = page_of(c, t), e = table[g];
     const uint16_t* kr = static_cast<const uint16_t*>(c.k) +
-                         (((size_t)(e >= 0 && e < c.n_pages ? e : 0) * c.Hkv + h) * c.page + (t - g * c.page) + i16) * HD + q4 * 8;
+                         (((size_t)(e >= 0 && e < c.n_pages ? e : 0) * c.Hkv + h) * c.page + (t - g * c.page) + in % TILE) * HD +
+                         part * 8;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) kf[j][k] = *reinterpret_cast<const bf8*>(kr + k * 32);
+    for (int k = 0; k < KS; ++k) kf[j][k] = *reinterpret_cast<const bf8*>(kr + k * KD);
   }
-  // the rows that can see a key of this workgroup
-  const int f_lo = max(0, b0 - p0) * c.G;
-  int t_hi = n;
-  if (a.window > 0 && b0 >= a.sinks) t_hi = (int)max((int64_t)0, min((int64_t)n, (int64_t)b0 + KG * KEYS - 1 + a.window - p0));
-  const int f_hi = t_hi * c.G;
 
+  // this lane's rows by (token, head), carried along: a stage is N / G tokens and N % G heads further
+  const int dt = N / c.G, dg = N - dt * c.G;
+  struct Row {
+    int f, tok, g;
+  };
+  auto row_at = [&](int f) { const int tok = f / c.G; return Row{f, tok, f - tok * c.G}; };
+  auto advance = [&](Row& r) {
+    r.f += N;
+    r.tok += dt;
+    r.g += dg;
+    if (r.g >= c.G) { r.g -= c.G; ++r.tok; }
+  };
+  auto place = [&](const Row& r) -> size_t {      // rows past the last read the first
+    return r.f < rows ? (size_t)(first + r.tok) * c.Hq + h * c.G + r.g : (size_t)first * c.Hq + h * c.G;
+  };
+  Row mine = row_at(f_lo + in);                   // threads of the first row's N lanes also bring lse and slot
   Piece<QT, 8> next[NF];
   float lse_next = 0.f;
   int slot_next = -1;
-  auto load = [&](int f0) {                       // rows f0 .. f0 + SR - 1
+  auto load = [&]() {
+    const size_t at = place(mine);
+    const QT* q = static_cast<const QT*>(a.q) + at * HD + part * 8;
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      const int u = wave + 4 * i, f = min(f0 + u / KS * 16 + i16, rows - 1), tok = f / c.G;   // fragment u: row tile, 32 dims
-      if (u < RG * KS)
-        next[i].load(static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD +
-                     u % KS * 32 + q4 * 8);
+    for (int i = 0; i < NF; ++i) next[i].load(q + min(wave * NF + i, KS - 1) * KD);
+    if (tid < N) {
+      slot_next = mine.f < f_hi ? p0 + mine.tok : -1;   // -1: sees nothing
+      lse_next = a.lse[at];
     }
-    if (tid < SR) {
-      const int f = f0 + tid, tok = min(f, rows - 1) / c.G;
-      slot_next = f < f_hi ? p0 + tok : -1;       // -1: sees nothing
-      lse_next = a.lse[(size_t)(first + tok) * c.Hq + h * c.G + (min(f, rows - 1) - tok * c.G)];
-    }
+    advance(mine);
   };
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (f_lo < f_hi) load(f_lo);
+  float sum[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) sum[j] = 0.f;
+  load();
   int b = 0;
-  for (int f0 = f_lo; f0 < f_hi; f0 += SR, b ^= 1) {
+  for (int f0 = f_lo; f0 < f_hi; f0 += N, b ^= 1) {
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
-      const int u = wave + 4 * i;
-      if (u >= RG * KS) break;
-      char* d = frag[b] + u * NP * 1024 + lane * 16;
+      if (wave * NF + i >= KS) break;
+      char* d = frag[b] + (wave * NF + i) * NP * 1024 + lane * 16;
       if constexpr (NP == 1) {
         *reinterpret_cast<Piece<QT, 8>*>(d) = next[i];
       } else {
         float y[8];
-        bf8 part[NP];
+        bf8 parts[NP];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = next[i].get(e);
-        parts8<NP>(y, part);
+        parts8<NP>(y, parts);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf8*>(d + p * 1024) = part[p];
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf8*>(d + p * 1024) = parts[p];
       }
     }
-    if (tid < SR) {
+    if (tid < N) {
       lse[b][tid] = lse_next;
       slot[b][tid] = slot_next;
     }
-    __syncthreads();
-    if (f0 + SR < f_hi) load(f0 + SR);
-    v4f s[4];
+    __syncthreads();                              // also: every wave is done with this slot's stage before last
+    if (f0 + N < f_hi) load();
+    acc s[NJ];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+      for (int v = 0; v < NV; ++v) s[j][v] = 0.f;
+    constexpr int ALL = KS * NP, C = ALL % 4 == 0 ? 4 : ALL % 3 == 0 ? 3 : ALL % 2 == 0 ? 2 : 1;   // fragments read ahead of the products
+    static_assert(ALL % C == 0, "whole sets of fragments");
+    bf8 qf[2][C];
+    auto read = [&](int i) {
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p) {
-        const bf8 qf = *reinterpret_cast<const bf8*>(frag[b] + ((rg * KS + k) * NP + p) * 1024 + lane * 16);
+      for (int u = 0; u < C; ++u) qf[i % 2][u] = *reinterpret_cast<const bf8*>(frag[b] + (i * C + u) * 1024 + lane * 16);
+    };
+    read(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf, kf[j][k], s[j], 0, 0, 0);
-      }
-    const float4 l4 = *reinterpret_cast<const float4*>(&lse[b][rg * 16 + 4 * q4]);
-    const int4 p4 = *reinterpret_cast<const int4*>(&slot[b][rg * 16 + 4 * q4]);
-    const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
-    const int ps[4] = {p4.x, p4.y, p4.z, p4.w};
-    const int p_lo = slot[b][rg * 16], p_hi = slot[b][rg * 16 + 15];
-    const bool whole = __builtin_amdgcn_readfirstlane(p_hi >= 0 && all_see(k0, k0 + KEYS - 1, p_lo, p_hi, a.window, a.sinks));
-    if (whole) {
+    for (int i = 0; i < ALL / C; ++i) {
+      if (i + 1 < ALL / C) read(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int u = 0; u < C; ++u)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum[j] += __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale, -ls[v]) * LOG2E);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float y = __builtin_amdgcn_exp2f(fmaf(s[j][v], a.scale, -ls[v]) * LOG2E);
-          sum[j] += sees(ps[v], k0 + j * TILE + i16, a.window, a.sinks) ? y : 0.f;
+        for (int j = 0; j < NJ; ++j) {
+          const bf8 kk = kf[j][(i * C + u) / NP];
+          if constexpr (N == 32) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
+          else s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
         }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const int p_lo = slot[b][0], p_hi = slot[b][N - 1];
+    const bool whole = __builtin_amdgcn_readfirstlane(p_hi >= 0 && all_see(k0, k0 + KEYS - 1, p_lo, p_hi, a.window, a.sinks));
+#pragma unroll
+    for (int i = 0; i < NV / 4; ++i) {
+      const int r0 = 8 * i + 4 * part;
+      const float4 l4 = *reinterpret_cast<const float4*>(&lse[b][r0]);
+      const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[j] += __builtin_amdgcn_exp2f(fmaf(s[j][4 * i + r], a.scale, -ls[r]) * LOG2E);
+      } else {
+        const int4 p4 = *reinterpret_cast<const int4*>(&slot[b][r0]);
+        const int ps[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[j][4 * i + r], a.scale, -ls[r]) * LOG2E);
+            sum[j] += sees(ps[r], k0 + j * N + in, a.window, a.sinks) ? y : 0.f;
+          }
+      }
     }
   }
+  float y = 0.f;                                  // key k0 + lane
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sum[j] = sum4(sum[j]);
-  float y = q4 == 0 ? sum[0] : q4 == 1 ? sum[1] : q4 == 2 ? sum[2] : sum[3];   // key k0 + lane
-  if constexpr (RG > 1) {
-    if (rg > 0) meet[(wave - KG) * 64 + lane] = y;
-    __syncthreads();
-    if (rg > 0) return;
-#pragma unroll
-    for (int r = 0; r < RG - 1; ++r) y += meet[(r * KG + kg) * 64 + lane];
+  for (int j = 0; j < NJ; ++j) {
+    const float t = N == 32 ? sum2(sum[j]) : sum4(sum[j]);
+    y = part == j ? t : y;
   }
   if (live) *account = before + y;
+}
+
+// Adds the cuts' sums of keys whose rows took several; one thread per key.
+__global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int keys) {
+  const Cache& c = a.c;
+  const int h = blockIdx.x, seq = blockIdx.z, key = blockIdx.y * 256 + threadIdx.x;
+  int first, n, f_lo, f_hi;
+  seq_rows(c, seq, first, n);
+  const int len = seq_len(c, seq);
+  if (n == 0 || key >= len) return;
+  mass_rows(a, n, len - n, key / keys * keys, keys, f_lo, f_hi);
+  if (f_hi - f_lo <= a.cut) return;
+  const int pg = page_of(c, key), page = c.table[seq * c.stride + pg];
+  if (page < 0 || page >= c.n_pages) return;
+  const size_t step = (size_t)c.Hkv * c.width * c.page;
+  const float* p = a.part + (size_t)seq * a.cuts * step + (size_t)h * c.width * c.page + key;
+  const int cuts = min((f_hi - f_lo + a.cut - 1) / a.cut, a.cuts);
+  float y = 0.f;
+  for (int i = 0; i < cuts; ++i) y += p[i * step];
+  a.mass[((size_t)page * c.Hkv + h) * c.page + (key - pg * c.page)] += y;
 }
 
 // ------------------------------------------------------------ eviction

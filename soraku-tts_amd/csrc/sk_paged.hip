@@ -94,6 +94,30 @@ Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page
   p.cuts = (int)((tiles + p.cut - 1) / p.cut);
   return p;
 }
+
+// Keys per workgroup of a call for accounts, and its rows per cut.
+struct MassPlan {
+  bool tiles, few;
+  int keys, cut, cuts;
+  int64_t blocks;
+};
+constexpr int NK2 = 2;                            // key tiles per wave of mass_kernel
+MassPlan plan_mass(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page, int width) {
+  MassPlan p;
+  const int64_t rows = (int64_t)T * (Hq / Hkv);
+  p.tiles = kvdtype == SK_BF16 && hd >= 32;
+  p.few = rows <= 16ll * S;
+  p.keys = p.tiles ? 4 * KEYS : 4 * NK2 * TILE;
+  p.blocks = ((int64_t)page * width + p.keys - 1) / p.keys;
+  const int64_t base = p.blocks * Hkv * S;
+  const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(1536 / base, rows / 256)) : 1;
+  p.cut = (int)std::max<int64_t>(32, ((rows + cuts - 1) / cuts + 31) / 32 * 32);
+  p.cuts = (int)std::max<int64_t>(1, (rows + p.cut - 1) / p.cut);
+  return p;
+}
+int64_t workspace_of(const MassPlan& p, int S, int Hkv, int page, int width) {
+  return p.cuts > 1 ? (int64_t)p.cuts * S * Hkv * page * width * 4 : 0;
+}
 int64_t workspace_of(const Plan& p, int T, int Hq, int hd) {
   return p.cuts > 1 ? (int64_t)p.cuts * T * Hq * (hd + 2) * 4 : 0;
 }
@@ -174,7 +198,7 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
       constexpr int HD = decltype(d)::value;
       const dim3 grid(Hkv, p.blocks, p.cuts);
       if constexpr (HD >= 32 && sizeof(K) == 2) {
-        if (p.tiles) hipLaunchKernelGGL((attend_tiles_kernel<X, HD, 2>), grid, dim3(256), 0, st, a);
+        if (p.tiles) hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
       }
       if (p.tiles) ;
       else if (p.R == 32) hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
@@ -189,44 +213,60 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   return SK_OK;
 }
 
+int sk_op_paged_attention_mass_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
+                                         int32_t width, int32_t xdtype, int32_t kvdtype, int64_t* bytes) {
+  if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, 1, width, width)) return rc;
+  if (int rc = check_types(xdtype, kvdtype)) return rc;
+  SK_CHECK(bytes, SK_EINVAL, "NULL operand");
+  *bytes = workspace_of(plan_mass(T, S, Hq, Hkv, hd, kvdtype, page, width), S, Hkv, page, width);
+  return SK_OK;
+}
+
 int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
                                int32_t n_pages, int32_t width, int64_t table_stride, int32_t xdtype, int32_t kvdtype,
                                float scale, int32_t window, int32_t sinks, const void* q, const float* lse,
                                const void* k_pages, const int32_t* table, const int32_t* starts, const int32_t* lens,
-                               float* mass) {
+                               float* mass, void* workspace, int64_t workspace_bytes) {
   if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, n_pages, width, table_stride)) return rc;
   if (int rc = check_types(xdtype, kvdtype)) return rc;
   if (int rc = check_window(scale, window, sinks)) return rc;
   if (T == 0) return SK_OK;
   SK_CHECK(q && lse && k_pages && table && starts && lens && mass, SK_EINVAL, "NULL operand");
-  SK_CHECK(aligned16(q) && aligned16(k_pages), SK_EINVAL, "operands must be 16-byte aligned");
-  SK_CHECK(S <= 65535, SK_EINVAL, "S must be at most 65535");
+  SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(workspace), SK_EINVAL, "operands must be 16-byte aligned");
+  const MassPlan p = plan_mass(T, S, Hq, Hkv, hd, kvdtype, page, width);
+  const int64_t need = workspace_of(p, S, Hkv, page, width);
+  SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= need), SK_EINVAL, "the workspace must hold %lld bytes",
+           (long long)need);
+  SK_CHECK(p.blocks <= 65535 && (int64_t)S * p.cuts <= 65535, SK_EINVAL, "too many keys or sequences for one call");
   MassArgs a;
   a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, nullptr);
   a.q = q; a.lse = lse; a.mass = mass;
   a.scale = scale; a.window = window; a.sinks = sinks;
-  // keys per workgroup: matrix tiles of BF16 with 4 (few rows) or 2 waves' keys of 64, or FP32 products
-  const bool tiles = kvdtype == SK_BF16 && hd >= 32, few = (int64_t)T * a.c.G <= 16ll * S;
-  constexpr int NK2 = 2;
-  const int keys = tiles ? (few ? 4 : 2) * KEYS : 4 * NK2 * TILE;
-  const int64_t blocks = ((int64_t)page * width + keys - 1) / keys;
-  SK_CHECK(blocks <= 65535, SK_EINVAL, "width * page must be at most %d tokens", 65535 * keys);
-  const dim3 grid(Hkv, (unsigned)blocks, S);
+  a.cut = p.cut; a.cuts = p.cuts;
+  a.part = (float*)workspace;
+  const hipStream_t st = (hipStream_t)stream;
+  hipError_t err = hipSuccess;
   with_hd(hd, [&](auto d) {
     with_types(xdtype, kvdtype, [&](auto x, auto k) {
       using X = decltype(x);
       using K = decltype(k);
       constexpr int HD = decltype(d)::value;
-      const hipStream_t st = (hipStream_t)stream;
+      const dim3 grid(Hkv, (unsigned)p.blocks, S * p.cuts);
       if constexpr (HD >= 32 && sizeof(K) == 2) {
-        if (few) hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 4>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 2>), grid, dim3(256), 0, st, a);
+        if (p.few) hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 16>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 32>), grid, dim3(256), 0, st, a);
       } else {
         hipLaunchKernelGGL((mass_kernel<X, K, HD, NK2>), grid, dim3(256), 0, st, a);
       }
+      err = hipGetLastError();
     });
   });
-  SK_HIP(hipGetLastError());
+  SK_HIP(err);
+  if (p.cuts > 1) {
+    hipLaunchKernelGGL(mass_join_kernel, dim3(Hkv, (unsigned)(((int64_t)page * width + 255) / 256), S), dim3(256), 0, st, a,
+                       p.keys);
+    SK_HIP(hipGetLastError());
+  }
   return SK_OK;
 }
 

@@ -92,7 +92,8 @@ PROTOTYPES = {
     "sk_op_paged_append": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, *[_P] * 12]),
     "sk_op_paged_attention_workspace": (_I, [*[_I] * 11, _PI64]),
     "sk_op_paged_attention": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 9, _L]),
-    "sk_op_paged_attention_mass": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 7]),
+    "sk_op_paged_attention_mass_workspace": (_I, [*[_I] * 9, _PI64]),
+    "sk_op_paged_attention_mass": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 8, _L]),
     "sk_op_paged_evict": (_I, [_P, *[_I] * 6, _L, *[_I] * 4, *[_P] * 6, _L, _I, _P, _P]),
 }
 

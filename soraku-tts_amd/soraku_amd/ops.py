@@ -224,6 +224,13 @@ def _attention_workspace(*sizes) -> int:
     return n.value
 
 
+@functools.lru_cache(maxsize=1024)
+def _mass_workspace(*sizes) -> int:
+    n = C.c_int64()
+    check(lib().sk_op_paged_attention_mass_workspace(*sizes, C.byref(n)))
+    return n.value
+
+
 def paged_append(Hq: int, Hkv: int, hd: int, page: int, eps: float):
     """New tokens into the cache: per-head RMSNorm of q and k (gains ``[hd]``, or
     both None for none), rotation by ``positions * inv_freq``, k and v to
@@ -289,10 +296,12 @@ def paged_attention_mass(Hq: int, Hkv: int, hd: int, page: int, scale: float | N
         at, n, kp, _, kd = _pool(k_pages, None, Hkv, page, hd, T.codes)
         xd, rows, S = _code(q, T.codes), q.shape[0], lens.shape[0]
         tp, stride, width = _table(table, "table", i32, at, S)
+        size = _mass_workspace(rows, S, Hq, Hkv, hd, page, width, xd, kd)
+        ws = T.empty(size, device=k_pages.device, dtype=T.u8) if size else None
         _call(T, T.lib.sk_op_paged_attention_mass, at, rows, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,
               sinks, _need(q, "q", q.dtype, at, (rows, Hq, hd)), _need(lse, "lse", f32, at, (rows, Hq)), kp, tp,
               _need(starts, "starts", i32, at, (S + 1,)), _need(lens, "lens", i32, at, (S,)),
-              _need(mass, "mass", f32, at, (n, Hkv, page)))
+              _need(mass, "mass", f32, at, (n, Hkv, page)), ws.data_ptr() if size else None, size)
         return mass
     return kernel
 

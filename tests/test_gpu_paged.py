@@ -322,6 +322,21 @@ def test_mass(ops, hip_device, seqs, types):
         assert (np.abs(got.double().cpu().numpy() - want) <= rel * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+def test_mass_many_rows(ops, hip_device, window, sinks, types):
+    """Chunks whose rows are cut over workgroups and joined, beside short ones."""
+    xd, kd = TYPES[types]
+    u = Setup([(300, 300), (140, 333), (1, 200), (129, 129)], 12, 4, 64, 32, xd, kd, pad=2, seed=45)
+    d = u.on(hip_device)
+    _, lse = attend(ops, u, d, None, window, sinks)
+    got = ops.paged_attention_mass(12, 4, 64, 32, None, window, sinks)(d["q"], lse, d["k"], d["table"], d["starts"],
+                                                                       d["lens"], d["mass"])
+    want, terms = ref.mass(u, lse.cpu().numpy(), None, window, sinks)
+    rel = (2.0 * (64 + 8) * (1.0 + 60.0) + 8.0 + terms) * 2.0 ** -24
+    assert (np.abs(got.double().cpu().numpy() - want) <= rel * np.abs(want)).all()
+
+
 def test_mass_unseen_slots_do_not_matter(ops, hip_device):
     u = Setup([(9, 40), (1, 21)], 4, 2, 64, 16, F32, BF16, width=5, seed=50)
     for s, (_, length) in enumerate(u.seqs):

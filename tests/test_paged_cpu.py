@@ -30,7 +30,7 @@ APPEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, w
 ATTEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
               window=0, sinks=0, q=P, k=P, v=P, table=P, starts=P, lens=P, out=P, lse=None, ws=None, ws_bytes=0)
 MASS = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
-            window=0, sinks=0, q=P, lse=P, k=P, table=P, starts=P, lens=P, mass=P)
+            window=0, sinks=0, q=P, lse=P, k=P, table=P, starts=P, lens=P, mass=P, ws=None, ws_bytes=0)
 EVICT = dict(stream=None, S=2, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, kd=1, keep=32, sinks=4, recent=8,
              k=P, v=P, mass=P, table=P, lens=P, to=2 * P, to_stride=2, to_width=2, new_lens=P, kept=P)
 ENTRY = {"append": ("sk_op_paged_append", APPEND), "attention": ("sk_op_paged_attention", ATTEND),
@@ -46,7 +46,7 @@ BAD = {
                                                                          "table", "k", "v", "out")],
     "attention": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("out", P + 8), ("ws", P + 4)] + [
         (n, None) for n in ("q", "k", "v", "table", "starts", "lens", "out")],
-    "mass": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2)] + [(n, None) for n in ("q", "lse", "k", "table", "starts", "lens",
+    "mass": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("ws", P + 8)] + [(n, None) for n in ("q", "lse", "k", "table", "starts", "lens",
                                                                               "mass")],
     "evict": [("keep", 0), ("keep", -5), ("sinks", -1), ("recent", -1), ("sinks", 25), ("sinks", 2 ** 31 - 1), ("keep", 33),
               ("to_width", 0), ("to_stride", 1), ("to", P), ("k", P + 4), ("v", P + 4)] + [
@@ -86,6 +86,19 @@ def test_attention_asks_for_its_workspace(L):
     assert str(n.value) in L.sk_last_error().decode()
     assert L.sk_op_paged_attention_workspace(*sizes, None) == SK_EINVAL
     assert L.sk_op_paged_attention_workspace(2, 0, *sizes[2:], C.byref(n)) == SK_EINVAL
+
+
+def test_mass_asks_for_its_workspace(L):
+    from soraku_amd._lib import SK_EINVAL, SK_OK
+
+    n = C.c_int64(-1)
+    sizes = (2000, 1, 16, 8, 128, 16, 150, 0, 1)
+    assert L.sk_op_paged_attention_mass_workspace(*sizes, C.byref(n)) == SK_OK and n.value > 0
+    args = dict(MASS, T=2000, S=1, width=150, stride=150, ws=P, ws_bytes=n.value - 1)
+    assert L.sk_op_paged_attention_mass(*args.values()) == SK_EINVAL
+    assert str(n.value) in L.sk_last_error().decode()
+    assert L.sk_op_paged_attention_mass_workspace(*sizes, None) == SK_EINVAL
+    assert L.sk_op_paged_attention_mass_workspace(2, 0, *sizes[2:], C.byref(n)) == SK_EINVAL
 
 
 def test_python_refusals():
@@ -131,6 +144,11 @@ for entry, change in cases:
         _lib.check(L.sk_op_paged_attention_workspace(*[args[k] for k in ("T", "S", "Hq", "Hkv", "hd", "page", "width", "xd",
                                                                          "kd", "window", "sinks")], C.byref(n)))
         args.update(ws=t.P if n.value else None, ws_bytes=n.value)
+    if entry == "mass":
+        n = C.c_int64()
+        _lib.check(L.sk_op_paged_attention_mass_workspace(*[args[k] for k in ("T", "S", "Hq", "Hkv", "hd", "page", "width", "xd",
+                                                                              "kd")], C.byref(n)))
+        args.update(ws=t.P if n.value else None, ws_bytes=n.value)
     calls()
     rc = getattr(L, name)(*args.values())
     cs = calls()
@@ -169,7 +187,7 @@ def test_launches(launches):
     from soraku_amd._lib import SK_EHIP, SK_OK
 
     cases = [[e, c] for e in ENTRY for c in ({}, {"kd": 0}, {"hd": 16, "stride": 9})]
-    cases += [["attention", {"T": 1, "S": 1, "width": 4096, "stride": 4096}]]
+    cases += [["attention", {"T": 1, "S": 1, "width": 4096, "stride": 4096}], ["mass", {"T": 3000, "S": 1}]]
     for (entry, _), (rc, calls, kern, ws, failed) in zip(cases, launches(cases)):
         assert rc == SK_OK and set(calls) == {"hipLaunchKernel"} and failed == SK_EHIP
         assert len(kern) == (2 if entry == "evict" or ws else 1)
@@ -209,7 +227,7 @@ def rows_of(kernel):
 
     args = [int(x) for x in re.findall(r"Li(\d+)E", kernel)]
     assert "attend_rows_kernel" in kernel or "attend_tiles_kernel" in kernel, kernel
-    return (64 if "tiles" in kernel else 16) * args[1]
+    return 128 if "tiles" in kernel else 16 * args[1]
 
 
 # ------------------------------------------------------------------ the oracle
