@@ -272,6 +272,7 @@ struct AttendArgs {
   int window, sinks;                              // window 0: all keys
   int cut;                                        // tiles of keys per cut; cuts of a row: blockIdx.z
   float* part; float* ml;                         // [cuts][T * Hq][hd], [cuts][T * Hq][2]: sums of V, (maximum times scale2, sum)
+  int* count;                                     // [T * Hq]: a row's cuts to join (0: none), negative if it sees nothing
 };
 constexpr float LOWEST = -3e38f;                  // a maximum of nothing: finite, so that -infinity less it is -infinity
 
@@ -296,14 +297,20 @@ __device__ __forceinline__ bool all_see(int j0, int j1, int p_lo, int p_hi, int 
   return j1 <= p_lo && (window == 0 || j0 > p_hi - window || j1 < sinks);
 }
 
+__device__ __forceinline__ int cuts_of(const AttendArgs& a, const Walk& w, bool none) {
+  const int ns = w.n <= a.cut ? 0 : (w.n + a.cut - 1) / a.cut;
+  return none ? -ns : ns;
+}
+
 // Offsets (in elements, for head 0 dims) of a run of tiles: lane i holds that of
 // the wave's i-th tile from a walk position on; one division and table entry per lane, for 64 tiles.
 struct TileOffsets {
   uint32_t lo, hi;
   uint64_t bad;                                   // lanes whose page is not in the pool
+  // tiles t0, t0 + step ..; as pairs: t0, t0 + 1, t0 + step, t0 + step + 1 ..
   __device__ __forceinline__ void load(const Cache& c, const int* table, const Walk& w, int t0, int step, int end, int h,
-                                       int hd) {
-    const int t = min(t0 + (int)(threadIdx.x & 63) * step, end - 1);
+                                       int hd, bool pairs = false) {
+    const int l = threadIdx.x & 63, t = min(t0 + (pairs ? (l >> 1) * step + (l & 1) : l * step), end - 1);
     const int j = w.tile(t) * TILE, pg = page_of(c, j);
     const int e = table[pg];
     const bool ok = e >= 0 && e < c.n_pages;
@@ -381,6 +388,69 @@ __device__ __forceinline__ void add_wild(const AttendArgs& a, int h, const int* 
       }
     }
   }
+}
+
+// The end of a workgroup whose WK waves shared R rows' keys: each wave's sums of V are in po [WK][R][HD
+// + 4], maxima (of the raw products) and sums in pm, pl [WK][R].  Joins them, stores rows (or the cut's part)
+// and adds what V's infinities and NaN left out.
+template <typename QT, typename KT, int HD, int R, int WK>
+__device__ __forceinline__ void meet_rows(const AttendArgs& a, const float* po, float* pm, const float* pl, float2* stats,
+                                          bool wild, int h, int cut, const int* table, int first, int p0, int f0, int rows,
+                                          int p_lo, int p_hi, const Walk& w, int end) {
+  constexpr int LDO = HD + 4;
+  const Cache& c = a.c;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
+  if (tid < R) {
+    float mx = -INFINITY, l = 0.f, f[WK];
+#pragma unroll
+    for (int u = 0; u < WK; ++u) mx = fmaxf(mx, pm[u * R + tid]);
+    const float m2 = mx == -INFINITY ? LOWEST : mx * a.scale2;
+#pragma unroll
+    for (int u = 0; u < WK; ++u) {
+      f[u] = __builtin_amdgcn_exp2f(fmaf(pm[u * R + tid], a.scale2, -m2));
+      l = fmaf(f[u], pl[u * R + tid], l);
+    }
+    const int row = f0 + tid, tok = row / c.G;
+    const bool none = p0 + tok < 0;               // no key is seen
+#pragma unroll
+    for (int u = 0; u < WK; ++u) pm[u * R + tid] = alone ? none ? 0.f : f[u] / l : f[u];
+    stats[tid] = make_float2(m2, alone ? 1.f / l : 1.f);
+    if (row < rows) {
+      const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
+      if (cut == 0 && a.count) a.count[at] = cuts_of(a, w, none);
+      if (!alone) {
+        float* d = a.ml + ((size_t)cut * c.T * c.Hq + at) * 2;
+        d[0] = m2;
+        d[1] = l;
+      } else if (a.lse) {
+        a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int NF = HD / 4;
+  for (int it = tid; it < R * NF; it += WK * 64) {
+    const int r = it / NF, d = (it - r * NF) * 4, row = f0 + r, tok = row / c.G;
+    if (row >= rows) break;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < WK; ++u) {
+      const float wt = pm[u * R + r];
+      const float4 x = *reinterpret_cast<const float4*>(po + (u * R + r) * LDO + d);
+      y.x = fmaf(wt, x.x, y.x); y.y = fmaf(wt, x.y, y.y); y.z = fmaf(wt, x.z, y.z); y.w = fmaf(wt, x.w, y.w);
+    }
+    const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
+    if (alone) store4(static_cast<QT*>(a.out) + at * HD + d, y.x, y.y, y.z, y.w);
+    else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + at) * HD + d) = y;
+  }
+  if (__syncthreads_or(wild) && tid < 64)
+    add_wild<QT, KT, HD>(a, h, table, first, p0, f0, min(f0 + R, rows), w, cut * a.cut, end,
+                         alone ? nullptr : a.part + (size_t)cut * c.T * c.Hq * HD,
+                         [&](int t) { const int k0 = w.tile(t) * TILE;
+                                      return !all_see(k0, k0 + TILE - 1, p_lo, p_hi, a.window, a.sinks); },
+                         [&](int f) { return stats[f - f0]; });
 }
 
 // The workgroup holds NT matrix tiles of 16 rows; its WK waves take key tiles in
@@ -544,56 +614,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int e = 0; e < VW; ++e) row[16 * VW * u + VW * (4 * q4 + v) + e] = o[j][u * VW + e][v];
   }
-  __syncthreads();
-  const bool alone = w.n <= a.cut;                // no other cut: the answer itself
-  if (tid < R) {
-    float mx = -INFINITY, l = 0.f, f[WK];
-#pragma unroll
-    for (int u = 0; u < WK; ++u) mx = fmaxf(mx, pm[u * R + tid]);
-    const float m2 = mx == -INFINITY ? LOWEST : mx * a.scale2;
-#pragma unroll
-    for (int u = 0; u < WK; ++u) {
-      f[u] = __builtin_amdgcn_exp2f(fmaf(pm[u * R + tid], a.scale2, -m2));
-      l = fmaf(f[u], pl[u * R + tid], l);
-    }
-    const int row = f0 + tid, tok = row / c.G;
-    const bool none = p0 + tok < 0;               // no key is seen
-#pragma unroll
-    for (int u = 0; u < WK; ++u) pm[u * R + tid] = alone ? none ? 0.f : f[u] / l : f[u];
-    stats[tid] = make_float2(m2, alone ? 1.f / l : 1.f);
-    if (row < rows) {
-      const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
-      if (!alone) {
-        float* d = a.ml + ((size_t)cut * c.T * c.Hq + at) * 2;
-        d[0] = m2;
-        d[1] = l;
-      } else if (a.lse) {
-        a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
-      }
-    }
-  }
-  __syncthreads();
-  constexpr int NF = HD / 4;
-  for (int it = tid; it < R * NF; it += WK * 64) {
-    const int r = it / NF, d = (it - r * NF) * 4, row = f0 + r, tok = row / c.G;
-    if (row >= rows) break;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < WK; ++u) {
-      const float wt = pm[u * R + r];
-      const float4 x = *reinterpret_cast<const float4*>(po + (u * R + r) * LDO + d);
-      y.x = fmaf(wt, x.x, y.x); y.y = fmaf(wt, x.y, y.y); y.z = fmaf(wt, x.z, y.z); y.w = fmaf(wt, x.w, y.w);
-    }
-    const size_t at = (size_t)(first + tok) * c.Hq + h * c.G + (row - tok * c.G);
-    if (alone) store4(static_cast<QT*>(a.out) + at * HD + d, y.x, y.y, y.z, y.w);
-    else *reinterpret_cast<float4*>(a.part + ((size_t)cut * c.T * c.Hq + at) * HD + d) = y;
-  }
-  if (__syncthreads_or(wild) && wave == 0)
-    add_wild<QT, KT, HD>(a, h, table, first, p0, f0, min(f0 + R, rows), w, cut * a.cut, end,
-                         alone ? nullptr : a.part + (size_t)cut * c.T * c.Hq * HD,
-                         [&](int t) { const int k0 = w.tile(t) * TILE;
-                                      return !all_see(k0, k0 + TILE - 1, p_lo, p_hi, a.window, a.sinks); },
-                         [&](int f) { return stats[f - f0]; });
+  meet_rows<QT, KT, HD, R, WK>(a, po, pm, pl, stats, wild, h, cut, table, first, p0, f0, rows, p_lo, p_hi, w, end);
 }
 
 // ------------------------------------------------------------ many rows, BF16 cache
@@ -933,6 +954,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const bool none = qp < 0;                     // no key is seen
     const float y = alone ? none ? 0.f : 1.f / l : 1.f;
     if (half == 0) {
+      if (cut == 0 && a.count) a.count[row] = cuts_of(a, w, none);
       if (!alone) {
         float* d = a.ml + ((size_t)cut * c.T * c.Hq + row) * 2;
         d[0] = m2;
@@ -979,47 +1001,266 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
-// Joins the cuts of rows that have several; one wave per row (token, query head).
-// R: the rows of a tile of the kernel before, whose walk says how many cuts there are.
-template <typename QT, int HD>
-__global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int R, int cuts) {
+// ------------------------------------------------------------ few rows, BF16 cache
+// Single tokens and short chunks, where the bytes of K and V decide.  As in the row kernel a
+// workgroup's WK waves share NT tiles of 16 rows and take keys in turn, 32 at a
+// time, with no barrier in the loop, but on the BF16 matrix cores (16 x 16 x 32, parts as above): FP32 products
+// take 1,024 cycles of a SIMD per 4 KB of the cache, these 96 or 192.  K goes from the pages to registers as fragments, V to
+// two slots of LDS of the wave's own, both a step ahead.
+template <typename QT, int HD, int NT, int WK>
+__global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_few_kernel(AttendArgs a) {
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, NDT = HD / 16, R = NT * 16, LDO = HD + 4;
+  constexpr int GROUP = TILE * HD * 2;            // bytes of 16 keys
+  using L = TileLds<HD>;
+  constexpr int SLOTS = WK * 4 * GROUP, MEET = WK * R * LDO * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[SLOTS > MEET ? SLOTS : MEET];
+  __shared__ float pm[WK * R], pl[WK * R];
+  __shared__ float2 stats[R];
   const Cache& c = a.c;
-  const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (at >= c.T * c.Hq) return;
-  const int m = at / c.Hq, g = (at - m * c.Hq) % c.G, seq = seq_of_row(c, m);
-  if (seq >= c.S) return;
+  const int h = blockIdx.x, cut = blockIdx.z;
+  int seq, tile_no;
+  if (!find_tile(c, R, blockIdx.y, seq, tile_no)) return;
   int first, n;
   seq_rows(c, seq, first, n);
-  if (m - first >= n) return;
-  const int p0 = seq_len(c, seq) - n, f0 = ((m - first) * c.G + g) / R * R;
-  const Walk w = walk_of(p0 + f0 / c.G, p0 + (min(f0 + R, n * c.G) - 1) / c.G, a.window, a.sinks);
-  if (w.n <= a.cut) return;                       // one cut: its workgroup wrote the answer
-  const int ns = min((w.n + a.cut - 1) / a.cut, cuts);
-  const size_t step = (size_t)c.T * c.Hq;
-  float m2 = LOWEST;
-  for (int s = lane; s < ns; s += 64) m2 = fmaxf(m2, a.ml[(s * step + at) * 2]);
+  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
+  const int end = min(w.n, (cut + 1) * a.cut);
+  if (cut > 0 && cut * a.cut >= w.n) return;      // the first cut also answers for rows that see nothing
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, q4 = lane >> 4;
+  const int* table = c.table + seq * c.stride;
+
+  const int t_first = cut * a.cut + 2 * wave;     // the wave's tiles: two of every 2 WK
+  TileOffsets offs;
+  if (t_first < end) offs.load(c, table, w, t_first, 2 * WK, end, h, HD, true);
+  const unsigned koff = i16 * HD + q4 * 8;        // elements
+  const int vrow = lane / (HD / 8);
+  const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn(vrow)) * 8) * 2;
+  const int vkey = 4 * q4 + (i16 >> 2);
+  const unsigned vbase = vkey * HD * 2 + (i16 & 3) * 8, vturn = L::turn(vkey) * 32;
+  char* vlds = lds + wave * 4 * GROUP;
+  auto load = [&](int i, int slot, bf8 (&kf)[2][KS]) {   // tiles i, i + 1 of offs
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) m2 = fmaxf(m2, __shfl_xor(m2, d, 64));
-  constexpr int E = HD >= 64 ? HD / 64 : 1;       // dims per lane
-  float y[E] = {}, l = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.ml + (s * step + at) * 2);
-    const float wt = __builtin_amdgcn_exp2f(ml.x - m2);
-    l = fmaf(wt, ml.y, l);
-    const float* p = a.part + (s * step + at) * HD;
+    for (int g = 0; g < 2; ++g) {
+      const size_t off = offs.at(i + g);
+      const char* vb = static_cast<const char*>(c.v) + off * 2;
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = fmaf(wt, p[min(lane * E + e, HD - 1)], y[e]);
-  }
-  const bool none = p0 + (m - first) < 0;
-  if (lane * E < HD) {
+      for (int k = 0; k < KS; ++k)
+        lds_load16(vb + k * 1024, HD == 128 && k % 2 ? voff ^ 128 : voff, vlds + (2 * slot + g) * GROUP + k * 1024);
+      const uint16_t* kr = static_cast<const uint16_t*>(c.k) + off + koff;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float x = none ? 0.f : y[e] / l;
-      QT* d = static_cast<QT*>(a.out) + (size_t)at * HD + lane * E + e;
-      if constexpr (sizeof(QT) == 4) *d = x;
-      else *d = to_bf16(x);
+      for (int k = 0; k < KS; ++k) kf[g][k] = *reinterpret_cast<const bf8*>(kr + k * 32);
+    }
+  };
+  int qp[NT];                                     // the slot of this lane's rows (rows past the last repeat it)
+  bf8 qf[NT][NP][KS];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int f = min(f0 + j * 16 + i16, rows - 1), tok = f / c.G;
+    qp[j] = p0 + tok;
+    const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      Piece<QT, 8> x;
+      x.load(qr + k * 32 + q4 * 8);
+      if constexpr (NP == 1) {
+        qf[j][0][k] = __builtin_bit_cast(bf8, x);
+      } else {
+        float y[8];
+        bf8 part[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x.get(e);
+        parts8<NP>(y, part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) qf[j][p][k] = part[p];
+      }
     }
   }
+  v4f o[NT][NDT];
+  float mr[NT], lr[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    mr[j] = -INFINITY;
+    lr[j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) o[j][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  bool wild = false;                              // infinities or NaN in V beside a mask
+  int i = 0;                                      // the step's first lane in offs
+  // the step of tiles t and t + 1: kf and slot hold it; the next goes to the others
+  auto step = [&](int t, int slot, bf8 (&kf)[2][KS], bf8 (&other)[2][KS]) {
+    const int bad = offs.bad >> i & 3;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < 2; ++g)                   // here, not behind the next step's loads, which the compiler counts too
+#pragma unroll
+      for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(kf[g][k]));
+    i += 2;
+    if (t + 2 * WK < end) {
+      if (i == 64) {
+        i = 0;
+        offs.load(c, table, w, t + 2 * WK, 2 * WK, end, h, HD, true);
+      }
+      load(i, slot ^ 1, other);
+    }
+    v4f s[NT][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[j][g] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) s[j][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[g][k], qf[j][p][k], s[j][g], 0, 0, 0);
+    char* vst = vlds + 2 * slot * GROUP;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int k0 = w.tile(min(t + g, end - 1)) * TILE;
+      if (!(bad >> g & 1) && t + g < end && all_see(k0, k0 + TILE - 1, p_lo, p_hi, a.window, a.sinks)) continue;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          if (bad >> g & 1) s[j][g][v] = NAN;
+          if (t + g >= end || !sees(qp[j], k0 + 4 * q4 + v, a.window, a.sinks)) s[j][g][v] = -INFINITY;
+        }
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        auto* x = reinterpret_cast<Piece<uint16_t, 8>*>(vst + g * GROUP + k * 1024 + lane * 16);
+        Piece<uint16_t, 8> y = *x;
+        odd |= y.tame();
+        *x = y;
+      }
+      __builtin_amdgcn_wave_barrier();            // this wave's own LDS, read below by other lanes of it
+      if (__any(odd)) wild = true;
+    }
+    bf8 pf[NT][NP];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float mx = s[j][0][0];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][g][v]);
+      const float mn = fmaxf(mr[j], max4(mx)), m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
+      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
+      float y[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = __builtin_amdgcn_exp2f(fmaf(s[j][e / 4][e % 4], a.scale2, -m2));
+        sum += y[e];
+      }
+      parts8<NP>(y, pf[j]);
+      lr[j] = lr[j] * sc + sum;                   // this lane's keys; a row's four lanes add up at the end
+      mr[j] = mn;
+      if (__any(sc != 1.f)) {
+#pragma unroll
+        for (int u = 0; u < NDT; ++u) o[j][u] *= sc;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NDT; ++u) {
+      typedef __attribute__((address_space(3))) s4 lds4;
+      const char* vr = vst + (vbase + (u * 32 ^ vturn));
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vr);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vr + GROUP));
+      const bf8 vf = __builtin_bit_cast(bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[j][p], o[j][u], 0, 0, 0);
+    }
+    // the next step's loads into this slot come after these reads
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  bf8 ka[2][KS], kb[2][KS];
+  if (t_first < end) load(0, 0, ka);
+  for (int t = t_first; t < end; t += 4 * WK) {
+    step(t, 0, ka, kb);
+    if (t + 2 * WK < end) step(t + 2 * WK, 1, kb, ka);
+  }
+  // the waves meet: their rows of O and (max, sum)
+  __syncthreads();                                // V's slots become rows of O
+  float* po = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const float l = sum4(lr[j]);
+    const int at = wave * R + j * 16 + i16;
+    if (q4 == 0) { pm[at] = mr[j]; pl[at] = l; }
+#pragma unroll
+    for (int u = 0; u < NDT; ++u)
+      *reinterpret_cast<float4*>(po + at * LDO + 16 * u + 4 * q4) = make_float4(o[j][u][0], o[j][u][1], o[j][u][2], o[j][u][3]);
+  }
+  meet_rows<QT, uint16_t, HD, R, WK>(a, po, pm, pl, stats, wild, h, cut, table, first, p0, f0, rows, p_lo, p_hi, w, end);
+}
+
+// Joins the cuts of rows that have several (at most 64); WPR waves per row (token, query head),
+// half a wave per cut and 16 bytes per lane, the parts of a wave's cuts loading together.
+// What the kernel before left in `count` spares the way to the row's sequence (2,047
+// tokens: 25 -> 13 us).
+template <typename QT, int HD, int WPR>
+__global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int cuts) {
+  constexpr int NL = HD / 4, PER = 64 / NL < 2 ? 1 : 2, U = 4;   // lanes of a part, cuts of a wave at a time, loads under way
+  __shared__ float4 meet[WPR > 1 ? WPR * NL : 1];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = wave % WPR;
+  const int at = blockIdx.x * (4 / WPR) + wave / WPR;
+  if (at >= c.T * c.Hq) return;                   // WPR 4: one row per workgroup, so all of it
+  const size_t step = (size_t)c.T * c.Hq;
+  const int m = at / c.Hq, count = a.count[at], from = c.starts[0], to = c.starts[c.S];
+  const float2 own = *reinterpret_cast<const float2*>(a.ml + (min(lane, cuts - 1) * step + at) * 2);
+  if (m < from || m >= to || count == 0) return;  // no sequence's row, or one whose only cut's workgroup wrote the answer
+  const bool none = count < 0;
+  const int ns = min(none ? -count : count, cuts);
+  const float2 ml = lane < ns ? own : make_float2(LOWEST, 0.f);
+  float m2 = ml.x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) m2 = fmaxf(m2, __shfl_xor(m2, d, 64));
+  const float wt = __builtin_amdgcn_exp2f(ml.x - m2);   // of cut number `lane`
+  float l = lane < ns ? wt * ml.y : 0.f;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d, 64);
+  const int half = lane / NL, dim = lane % NL;    // lanes past PER parts (short heads) repeat the last one's work
+  const int mine = min(half, PER - 1);
+  const float* p = a.part + (size_t)at * HD + dim * 4;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = sub * PER * U; s0 < ns; s0 += WPR * PER * U) {
+    float4 x[U];
+    float f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * PER + mine;
+      x[u] = *reinterpret_cast<const float4*>(p + min(s, ns - 1) * step * HD);
+      f[u] = __shfl(wt, min(s, ns - 1), 64);
+      if (s >= ns) { f[u] = 0.f; x[u] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      y.x = fmaf(f[u], x[u].x, y.x); y.y = fmaf(f[u], x[u].y, y.y); y.z = fmaf(f[u], x[u].z, y.z); y.w = fmaf(f[u], x[u].w, y.w);
+    }
+  }
+  if constexpr (PER == 2) {
+    const float4 z = make_float4(__shfl_xor(y.x, NL, 64), __shfl_xor(y.y, NL, 64), __shfl_xor(y.z, NL, 64), __shfl_xor(y.w, NL, 64));
+    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+  }
+  if constexpr (WPR > 1) {
+    if (half == 0) meet[sub * NL + dim] = y;
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int u = 1; u < WPR; ++u) {
+      const float4 z = meet[u * NL + dim];
+      y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+    }
+  }
+  const float r = none ? 0.f : 1.f / l;
+  if (half == 0) store4(static_cast<QT*>(a.out) + (size_t)at * HD + dim * 4, none ? 0.f : r * y.x, none ? 0.f : r * y.y, none ? 0.f : r * y.z, none ? 0.f : r * y.w);
   if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * LN2;
 }
 
@@ -1317,20 +1558,25 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int keys) {
 // weights do (NaN above all, a sure slot above that, none for slots past the length), so the
 // n-th largest is found bit by bit with one count each.
 //
-// One workgroup per (sequence, head).  Wave w owns a run of slots, lane by lane, up to
-// NV per lane, whose ranks stay in registers (NV 0: longer, read again for each count).
-// The search takes two bits at a time, three counts by ballot; it ends early where a
-// bound has exactly n ranks at or above it.
+// One workgroup per (sequence, head).  Wave w owns a run of slots, lane by lane; a lane's first NV
+// ranks stay in registers, the next NLDS in LDS, what is past those is read again for each
+// look (61,440 slots: 54 us, 94 read again).
+// A histogram of the ranks' upper 12 bits leaves the few in the cut's bin; those go to a
+// list in LDS (where they fit), and two bits at a time, three counts by ballot, give the cut; it
+// ends early where a bound has exactly n ranks at or above it.
 __device__ __forceinline__ uint32_t rank_of(float x) {
   if (x != x) return 0xfffffffeu;
   const uint32_t b = __float_as_uint(x + 0.f);    // -0 counts as 0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <int NV>
+template <int NV, int NLDS>
 __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass, int keep, int sinks, int recent,
                                                       int* new_lens, int* kept) {
-  __shared__ int red[2][3][16], eq_of[16];
+  constexpr int BINS = 4096;
+  __shared__ uint32_t list[BINS];                 // bins, then the ranks of one
+  __shared__ uint32_t rest[NLDS > 0 ? NLDS * 1024 : 1];
+  __shared__ int red[2][3][16], eq_of[16], found[4];
   const int h = blockIdx.x, seq = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = seq_len(c, seq), n = min(len, keep);
@@ -1341,37 +1587,118 @@ __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass
   if (tid == 0 && h == 0) new_lens[seq] = n;
   for (int d = n + tid; d < keep; d += 1024) out[d] = -1;
   if (n == 0) return;
-  auto rank_at = [&](int j) -> uint32_t {
-    const int jc = min(j, len - 1), pg = page_of(c, jc), e = table[pg];
-    const bool ok = e >= 0 && e < c.n_pages;
-    const float x = mass[((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (jc - pg * c.page)];
-    return j >= len ? 0u : j < sinks || j >= len - recent ? 0xffffffffu : ok ? rank_of(x) : 0xfffffffeu;
+  auto rank_at = [&](float x, int j) -> uint32_t {
+    return j >= len ? 0u : j < sinks || j >= len - recent ? 0xffffffffu : rank_of(x);
   };
-  constexpr int LOADS = 8;                        // under way at a time (more spill)
-  uint32_t r[NV > 0 ? NV : 1];
-  if constexpr (NV > 0) {
+  auto page_at = [&](int j) { return table[page_of(c, min(j, len - 1))]; };
+  auto mass_at = [&](int j, int e) -> float {     // NaN where there is no page
+    const bool ok = e >= 0 && e < c.n_pages;
+    const int jc = min(j, len - 1);
+    const float x = mass[((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (jc - page_of(c, jc) * c.page)];
+    return ok ? x : NAN;
+  };
+  constexpr int SET = 8;                          // slots of a lane whose table entries, then accounts, load together
+  auto load = [&](int i0, uint32_t (&x)[SET]) {
+    int e[SET];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i % LOADS == 0) asm volatile("" ::: "memory");
-      r[i] = i < per ? rank_at(j0 + i * 64) : 0u;
-    }
+    for (int i = 0; i < SET; ++i) e[i] = page_at(j0 + (i0 + i) * 64);
+    float m[SET];
+#pragma unroll
+    for (int i = 0; i < SET; ++i) m[i] = mass_at(j0 + (i0 + i) * 64, e[i]);
+#pragma unroll
+    for (int i = 0; i < SET; ++i) x[i] = i0 + i < per ? rank_at(m[i], j0 + (i0 + i) * 64) : 0u;
+  };
+  uint32_t r[NV / SET][SET];
+#pragma unroll
+  for (int i0 = 0; i0 < NV; i0 += SET) {
+    asm volatile("" ::: "memory");                // one set under way at a time (more spill)
+    if (i0 < per) load(i0, r[i0 / SET]);
+  }
+  for (int i0 = NV; i0 < min(per, NV + NLDS); i0 += SET) {
+    uint32_t x[SET];
+    load(i0, x);
+#pragma unroll
+    for (int i = 0; i < SET; ++i) rest[(i0 - NV + i) * 1024 + tid] = x[i];
   }
   // f(rank, i) for this lane's slots
   auto each = [&](auto f) {
-    if constexpr (NV > 0) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i < per) f(r[i], i);
-    } else {
-      for (int i = 0; i < per; ++i) f(rank_at(j0 + i * 64), i);
+    for (int i = 0; i < NV; ++i)
+      if (i < per) f(r[i / SET][i % SET], i);
+    for (int i0 = NV; i0 < per; i0 += SET) {
+      uint32_t x[SET];
+      if (i0 < NV + NLDS) {
+#pragma unroll
+        for (int i = 0; i < SET; ++i) x[i] = rest[(i0 - NV + i) * 1024 + tid];
+      } else {
+        load(i0, x);
+      }
+#pragma unroll
+      for (int i = 0; i < SET; ++i)
+        if (i0 + i < per) f(x[i], i0 + i);
     }
   };
-  uint32_t cut = 0;                               // the n-th largest rank, from its highest bits on
-  bool exact = false;                             // n ranks are above it
-  for (int bit = 30; bit >= 0 && !exact; bit -= 2) {
+  // the bin of the n-th largest rank, from the top: rank >> 20, turned round
+  for (int i = tid; i < BINS; i += 1024) list[i] = 0;
+  __syncthreads();
+  each([&](uint32_t y, int) {
+    const int bin = BINS - 1 - (int)(y >> 20), one = __builtin_amdgcn_readfirstlane(bin);
+    if (__all(bin == one)) {                      // sure ones and ties: 64 at once
+      if (lane == 0) atomicAdd(&list[one], 64u);
+    } else {
+      atomicAdd(&list[bin], 1u);
+    }
+  });
+  __syncthreads();
+  int own[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum += own[i] = (int)list[4 * tid + i];
+  int upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) eq_of[wave] = upto;
+  __syncthreads();
+  for (int u = 0; u < wave; ++u) upto += eq_of[u];
+  int before = upto - sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (before < n && n <= before + own[i]) { found[0] = 4 * tid + i; found[1] = before; found[2] = own[i]; found[3] = 0; }
+    before += own[i];
+  }
+  __syncthreads();
+  // ranks >= cut + 2^20: hi; in the bin: inside
+  uint32_t cut = (uint32_t)(BINS - 1 - found[0]) << 20;
+  const int hi = found[1], inside = found[2];
+  bool exact = hi + inside == n;                  // n ranks are above the cut
+  if (exact) --cut;                               // not 0: the live ranks are above it, and at least n
+  const bool listed = inside <= BINS;
+  if (!exact && listed) {                         // any order: they are only counted
+    each([&](uint32_t y, int) {
+      const bool in = y - cut < 1u << 20;
+      const uint64_t who = __ballot(in);
+      if (!who) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&found[3], __popcll(who));
+      at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
+      if (in) list[at] = y;
+    });
+    __syncthreads();
+  }
+  const uint32_t base = cut;
+  auto in_bin = [&](auto f) {                     // f(rank) for whole waves, 0 in the place of others
+    if (listed) {
+      for (int i = wave * 64; i < inside; i += 1024) f(i + lane < inside ? list[i + lane] : 0u);
+    } else {
+      each([&](uint32_t y, int) { f(y - base < 1u << 20 ? y : 0u); });
+    }
+  };
+  for (int bit = 18; bit >= 0 && !exact; bit -= 2) {
     const uint32_t x = 1u << bit;
     int k1 = 0, k2 = 0, k3 = 0;
-    each([&](uint32_t y, int) {
+    in_bin([&](uint32_t y) {
       k1 += __popcll(__ballot(y >= cut + x));
       k2 += __popcll(__ballot(y >= cut + 2 * x));
       k3 += __popcll(__ballot(y >= cut + 3 * x));
@@ -1387,7 +1714,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass
       v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);
       v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
       v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
-      all[u] = __builtin_amdgcn_readfirstlane(v);
+      all[u] = hi + __builtin_amdgcn_readfirstlane(v);
     }
     const int at = all[2] >= n ? 3 : all[1] >= n ? 2 : all[0] >= n ? 1 : 0;
     cut += at * x;
@@ -1410,6 +1737,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass
   const int room = n - above;                     // of those on it, the first ones stay
   each([&](uint32_t y, int i) {
     const uint64_t gt = __ballot(y > cut), eq = __ballot(y == cut), below = (1ull << lane) - 1;
+    if (!(gt | eq)) return;
     const int gb = __popcll(gt & below), eb = ties + __popcll(eq & below);
     if (y > cut || (y == cut && eb < room)) out[pos + gb + min(eb, room)] = j0 + i * 64;
     pos += __popcll(gt);

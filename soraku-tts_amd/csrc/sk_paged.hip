@@ -78,18 +78,19 @@ struct Plan {
   bool tiles;
   int R, blocks, cut, cuts;
 };
-Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page, int width, int window, int sinks) {
+Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdtype, int page, int width, int window, int sinks) {
   Plan p;
   const int G = Hq / Hkv;
   const int64_t rows = (int64_t)T * G / S;        // of a sequence, on average
   p.tiles = kvdtype == SK_BF16 && hd >= 32 && rows > 32;
-  p.R = p.tiles ? 128 : rows > 16 ? 32 : 16;
+  // 32 rows where the registers hold them: not as three parts of 128 dims
+  p.R = p.tiles ? 128 : rows > 16 && (xdtype == kvdtype || hd < 128) ? 32 : 16;
   p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - 1)) / p.R);
   int64_t tiles = (int64_t)page * width / TILE;   // what a row tile can walk at most
   if (window > 0)
     tiles = std::min(tiles, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
   const int64_t base = (int64_t)p.blocks * Hkv;
-  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(base, 1), tiles / 16));
+  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(base, 1), tiles / (kvdtype == SK_BF16 ? 8 : 4), 64}));
   p.cut = (int)((tiles + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
   p.cuts = (int)((tiles + p.cut - 1) / p.cut);
   return p;
@@ -110,7 +111,7 @@ MassPlan plan_mass(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page,
   p.keys = p.tiles ? 4 * KEYS : 4 * NK2 * TILE;
   p.blocks = ((int64_t)page * width + p.keys - 1) / p.keys;
   const int64_t base = p.blocks * Hkv * S;
-  const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(1536 / base, rows / 256)) : 1;
+  const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(3072 / base, rows / 256)) : 1;
   p.cut = (int)std::max<int64_t>(32, ((rows + cuts - 1) / cuts + 31) / 32 * 32);
   p.cuts = (int)std::max<int64_t>(1, (rows + p.cut - 1) / p.cut);
   return p;
@@ -119,7 +120,7 @@ int64_t workspace_of(const MassPlan& p, int S, int Hkv, int page, int width) {
   return p.cuts > 1 ? (int64_t)p.cuts * S * Hkv * page * width * 4 : 0;
 }
 int64_t workspace_of(const Plan& p, int T, int Hq, int hd) {
-  return p.cuts > 1 ? (int64_t)p.cuts * T * Hq * (hd + 2) * 4 : 0;
+  return p.cuts > 1 ? ((int64_t)p.cuts * (hd + 2) + 1) * T * Hq * 4 : 0;
 }
 
 }  // namespace
@@ -161,7 +162,7 @@ int sk_op_paged_attention_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hk
   if (int rc = check_types(xdtype, kvdtype)) return rc;
   if (int rc = check_window(1.f, window, sinks)) return rc;
   SK_CHECK(bytes, SK_EINVAL, "NULL operand");
-  *bytes = workspace_of(plan_attention(T, S, Hq, Hkv, hd, kvdtype, page, width, window, sinks), T, Hq, hd);
+  *bytes = workspace_of(plan_attention(T, S, Hq, Hkv, hd, xdtype, kvdtype, page, width, window, sinks), T, Hq, hd);
   return SK_OK;
 }
 
@@ -177,7 +178,7 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   SK_CHECK(q && k_pages && v_pages && table && starts && lens && out, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace), SK_EINVAL,
            "operands must be 16-byte aligned");
-  const Plan p = plan_attention(T, S, Hq, Hkv, hd, kvdtype, page, width, window, sinks);
+  const Plan p = plan_attention(T, S, Hq, Hkv, hd, xdtype, kvdtype, page, width, window, sinks);
   SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= workspace_of(p, T, Hq, hd)), SK_EINVAL,
            "the workspace must hold %lld bytes", (long long)workspace_of(p, T, Hq, hd));
   SK_CHECK(p.blocks <= 65535 && p.cuts <= 65535, SK_EINVAL, "too many rows for one call");
@@ -187,8 +188,10 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   a.scale2 = scale * LOG2E;
   a.window = window; a.sinks = sinks;
   a.cut = p.cut;
-  a.part = (float*)workspace;
-  a.ml = a.part ? a.part + (size_t)p.cuts * T * Hq * hd : nullptr;
+  const bool cut = p.cuts > 1;
+  a.part = cut ? (float*)workspace : nullptr;
+  a.ml = cut ? a.part + (size_t)p.cuts * T * Hq * hd : nullptr;
+  a.count = cut ? (int*)(a.ml + (size_t)p.cuts * T * Hq * 2) : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   hipError_t err = hipSuccess;
   with_hd(hd, [&](auto d) {
@@ -199,13 +202,19 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
       const dim3 grid(Hkv, p.blocks, p.cuts);
       if constexpr (HD >= 32 && sizeof(K) == 2) {
         if (p.tiles) hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
+        else if constexpr (sizeof(X) * HD <= 256)
+          if (p.R == 32) hipLaunchKernelGGL((attend_few_kernel<X, HD, 2, 4>), grid, dim3(256), 0, st, a);
+        if (p.R == 16) hipLaunchKernelGGL((attend_few_kernel<X, HD, 1, 4>), grid, dim3(256), 0, st, a);
+      } else if (p.R == 32) {
+        hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
+      } else {
+        hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 1, 4>), grid, dim3(256), 0, st, a);
       }
-      if (p.tiles) ;
-      else if (p.R == 32) hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 1, 4>), grid, dim3(256), 0, st, a);
       err = hipGetLastError();
       if (p.cuts == 1 || err != hipSuccess) return;
-      hipLaunchKernelGGL((combine_kernel<X, HD>), dim3((T * Hq + 3) / 4), dim3(256), 0, st, a, p.R, p.cuts);
+      // 4 waves per row where there are few rows with many cuts to go through
+      if (p.cuts > 16) hipLaunchKernelGGL((combine_kernel<X, HD, 4>), dim3(T * Hq), dim3(256), 0, st, a, p.cuts);
+      else hipLaunchKernelGGL((combine_kernel<X, HD, 1>), dim3((T * Hq + 3) / 4), dim3(256), 0, st, a, p.cuts);
       err = hipGetLastError();
     });
   });
@@ -287,15 +296,14 @@ int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t 
   SK_CHECK(aligned16(k_pages) && aligned16(v_pages), SK_EINVAL, "operands must be 16-byte aligned");
   const Cache c = cache_of(0, S, Hkv, Hkv, page, n_pages, width, table_stride, nullptr, lens, table, k_pages, v_pages);
   const hipStream_t st = (hipStream_t)stream;
-  const int64_t cap = (int64_t)page * width;
-  auto choose = [&](auto nv) {
-    hipLaunchKernelGGL((choose_kernel<decltype(nv)::value>), dim3(Hkv, S), dim3(1024), 0, st, c, mass, keep, sinks,
-                       recent, new_lens, kept);
+  auto choose = [&](auto nv, auto nlds) {
+    hipLaunchKernelGGL((choose_kernel<decltype(nv)::value, decltype(nlds)::value>), dim3(Hkv, S), dim3(1024), 0, st, c,
+                       mass, keep, sinks, recent, new_lens, kept);
   };
-  if (cap <= 8 * 1024) choose(Int<8>{});
-  else if (cap <= 32 * 1024) choose(Int<32>{});
-  else if (cap <= 64 * 1024) choose(Int<64>{});
-  else choose(Int<0>{});
+  const int64_t cap = (int64_t)page * width;
+  if (cap <= 8 * 1024) choose(Int<8>{}, Int<0>{});
+  else if (cap <= 32 * 1024) choose(Int<32>{}, Int<0>{});
+  else choose(Int<32>{}, Int<32>{});
   SK_HIP(hipGetLastError());
   const int pieces = hd * (kvdtype == SK_BF16 ? 2 : 4) / 16;
   auto move = [&](auto np) {

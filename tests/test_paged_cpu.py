@@ -218,7 +218,7 @@ def test_attention_plans_cover_rows_and_keys(launches):
             cuts = np.sort(rng.integers(0, c["T"] + 1, c["S"] - 1))
             n = np.diff(np.concatenate(([0], cuts, [c["T"]])))
             assert sum(-(-int(x) * G // R) for x in n) <= grid[1]
-        assert ws == (grid[2] * c["T"] * c["Hq"] * (128 + 2) * 4 if grid[2] > 1 else 0)
+        assert ws == ((grid[2] * (128 + 2) + 1) * c["T"] * c["Hq"] * 4 if grid[2] > 1 else 0)
 
 
 def rows_of(kernel):
@@ -226,8 +226,8 @@ def rows_of(kernel):
     import re
 
     args = [int(x) for x in re.findall(r"Li(\d+)E", kernel)]
-    assert "attend_rows_kernel" in kernel or "attend_tiles_kernel" in kernel, kernel
-    return 128 if "tiles" in kernel else 16 * args[1]
+    assert "attend_" in kernel, kernel
+    return 128 if "attend_tiles_kernel" in kernel else 16 * args[1]
 
 
 # ------------------------------------------------------------------ the oracle
