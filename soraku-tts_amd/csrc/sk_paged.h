@@ -469,7 +469,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   int seq, tile_no;
-  if (!find_tile(c, R, blockIdx.y, seq, tile_no)) return;
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;   // the longest walks first
   int first, n;
   seq_rows(c, seq, first, n);
   const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
@@ -1005,11 +1005,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // Single tokens and short chunks, where the bytes of K and V decide.  As in the row kernel a
 // workgroup's WK waves share NT tiles of 16 rows and take keys in turn, 32 at a
 // time, with no barrier in the loop, but on the BF16 matrix cores (16 x 16 x 32, parts as above): FP32 products
-// take 1,024 cycles of a SIMD per 4 KB of the cache, these 96 or 192.  K goes from the pages to registers as fragments, V to
+// take 1,024 cycles of a SIMD per 4 KB of the cache, these 64 to 192 (with BF16 activations P keeps 16
+// bits, two parts: it costs nothing here).  K goes from the pages to registers as fragments, V to
 // two slots of LDS of the wave's own, both a step ahead.
 template <typename QT, int HD, int NT, int WK>
 __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_few_kernel(AttendArgs a) {
-  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, NDT = HD / 16, R = NT * 16, LDO = HD + 4;
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, PP = NP == 3 ? 3 : 2;   // parts of Q, of P
+  constexpr int KS = HD / 32, NDT = HD / 16, R = NT * 16, LDO = HD + 4;
   constexpr int GROUP = TILE * HD * 2;            // bytes of 16 keys
   using L = TileLds<HD>;
   constexpr int SLOTS = WK * 4 * GROUP, MEET = WK * R * LDO * 4;
@@ -1019,7 +1021,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   int seq, tile_no;
-  if (!find_tile(c, R, blockIdx.y, seq, tile_no)) return;
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;   // the longest walks first
   int first, n;
   seq_rows(c, seq, first, n);
   const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
@@ -1140,7 +1142,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       __builtin_amdgcn_wave_barrier();            // this wave's own LDS, read below by other lanes of it
       if (__any(odd)) wild = true;
     }
-    bf8 pf[NT][NP];
+    bf8 pf[NT][PP];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float mx = s[j][0][0];
@@ -1156,7 +1158,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         y[e] = __builtin_amdgcn_exp2f(fmaf(s[j][e / 4][e % 4], a.scale2, -m2));
         sum += y[e];
       }
-      parts8<NP>(y, pf[j]);
+      parts8<PP>(y, pf[j]);
       lr[j] = lr[j] * sc + sum;                   // this lane's keys; a row's four lanes add up at the end
       mr[j] = mn;
       if (__any(sc != 1.f)) {
@@ -1172,7 +1174,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vr + GROUP));
       const bf8 vf = __builtin_bit_cast(bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p)
+      for (int p = PP - 1; p >= 0; --p)
 #pragma unroll
         for (int j = 0; j < NT; ++j) o[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[j][p], o[j][u], 0, 0, 0);
     }

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <numeric>
 
 #include "sk_error.h"
 #include "sk_paged.h"
@@ -73,26 +74,36 @@ void with_types(int32_t xdtype, int32_t kvdtype, F&& f) {
 }
 
 // How an attention call is cut up: R rows per workgroup (of 64-key steps on the
-// BF16 matrix cores: `tiles`), `cut` tiles of keys per cut.
+// BF16 matrix cores: `tiles`; else WK waves that share the keys), `cut` tiles of keys per cut.
 struct Plan {
   bool tiles;
-  int R, blocks, cut, cuts;
+  int R, WK, blocks, cut, cuts;
 };
-Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdtype, int page, int width, int window, int sinks) {
+Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdtype, int page, int width, int window,
+                    int sinks) {
   Plan p;
   const int G = Hq / Hkv;
   const int64_t rows = (int64_t)T * G / S;        // of a sequence, on average
-  p.tiles = kvdtype == SK_BF16 && hd >= 32 && rows > 32;
+  const bool bf16 = kvdtype == SK_BF16 && hd >= 32;
+  p.tiles = bf16 && rows > 32;
   // 32 rows where the registers hold them: not as three parts of 128 dims
   p.R = p.tiles ? 128 : rows > 16 && (xdtype == kvdtype || hd < 128) ? 32 : 16;
-  p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - 1)) / p.R);
-  int64_t tiles = (int64_t)page * width / TILE;   // what a row tile can walk at most
+  // tiles of n G rows: at most R - gcd(G, R) of a sequence's last one are empty
+  p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - std::gcd(G, p.R))) / p.R);
+  int64_t most = (int64_t)page * width / TILE;    // tiles that a row tile can walk
   if (window > 0)
-    tiles = std::min(tiles, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
-  const int64_t base = (int64_t)p.blocks * Hkv;
-  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(base, 1), tiles / (kvdtype == SK_BF16 ? 8 : 4), 64}));
-  p.cut = (int)((tiles + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
-  p.cuts = (int)((tiles + p.cut - 1) / p.cut);
+    most = std::min(most, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
+  const int64_t base = std::max<int64_t>((int64_t)p.blocks * Hkv, 1);
+  // A CU draws some 40 GB/s, so keys are cut until every CU has a workgroup (two of the
+  // tile kernel's), down to one round of a workgroup's waves: a pair of FP32 rows over 481 tokens takes 17 us uncut, 8
+  // waves or not, 7 + 4 in 8 cuts.  Past that a cut only adds its parts and a launch (32 BF16 rows of up to
+  // 657: 17 us uncut, 18 + 4 in two).  8 waves where each still has 8 tiles (a pair over 61,441:
+  // 74 us in 32 cuts by 4 waves, 66 in 16 by 8).
+  const int64_t round = p.tiles || !bf16 ? 4 : 8;
+  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>({(p.tiles ? 512 : 256) / base, most / round, 64}));
+  p.cut = (int)((most + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
+  p.cuts = (int)((most + p.cut - 1) / p.cut);
+  p.WK = !p.tiles && base * p.cuts <= 256 && p.cut >= 64 ? 8 : 4;
   return p;
 }
 
@@ -200,15 +211,25 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
       using K = decltype(k);
       constexpr int HD = decltype(d)::value;
       const dim3 grid(Hkv, p.blocks, p.cuts);
-      if constexpr (HD >= 32 && sizeof(K) == 2) {
-        if (p.tiles) hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
-        else if constexpr (sizeof(X) * HD <= 256)
-          if (p.R == 32) hipLaunchKernelGGL((attend_few_kernel<X, HD, 2, 4>), grid, dim3(256), 0, st, a);
-        if (p.R == 16) hipLaunchKernelGGL((attend_few_kernel<X, HD, 1, 4>), grid, dim3(256), 0, st, a);
+      // the kernels that share keys, with 16 NT rows and WK waves
+      auto share = [&](auto nt, auto wk) {
+        constexpr int NT = decltype(nt)::value, WK = decltype(wk)::value;
+        if constexpr (HD >= 32 && sizeof(K) == 2) {
+          if constexpr (NT == 1 || sizeof(X) * HD <= 256)
+            hipLaunchKernelGGL((attend_few_kernel<X, HD, NT, WK>), grid, dim3(64 * WK), 0, st, a);
+        } else {
+          hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, NT, WK>), grid, dim3(64 * WK), 0, st, a);
+        }
+      };
+      if (p.tiles) {
+        if constexpr (HD >= 32 && sizeof(K) == 2)
+          hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
       } else if (p.R == 32) {
-        hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 2, 4>), grid, dim3(256), 0, st, a);
+        if (p.WK == 8) share(Int<2>{}, Int<8>{});
+        else share(Int<2>{}, Int<4>{});
       } else {
-        hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, 1, 4>), grid, dim3(256), 0, st, a);
+        if (p.WK == 8) share(Int<1>{}, Int<8>{});
+        else share(Int<1>{}, Int<4>{});
       }
       err = hipGetLastError();
       if (p.cuts == 1 || err != hipSuccess) return;

@@ -161,8 +161,8 @@ class _Torch:
         import torch
 
         self.f32, self.bf16, self.i32, self.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
-        self.empty, self.on = torch.empty, torch.cuda.device
-        self.stream, self.device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+        self.empty, self.empty_like, self.on = torch.empty, torch.empty_like, torch.cuda.device
+        self.stream, self.device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self.codes = {torch.float32: _lib.SK_F32, torch.bfloat16: _lib.SK_BF16}
         self.lib = lib()
 
@@ -272,7 +272,7 @@ def paged_attention(Hq: int, Hkv: int, hd: int, page: int, scale: float | None =
         tp, stride, width = _table(table, "table", i32, at, S)
         shape = (rows, Hq, hd)
         if out is None:
-            out = T.empty(shape, device=k_pages.device, dtype=dt)
+            out = T.empty_like(q)
         size = _attention_workspace(rows, S, Hq, Hkv, hd, page, width, xd, kd, window, sinks)
         ws = T.empty(size, device=k_pages.device, dtype=T.u8) if size else None
         _call(T, T.lib.sk_op_paged_attention, at, rows, S, Hq, Hkv, hd, page, n, width, stride, xd, kd, scale, window,

@@ -45,11 +45,11 @@ class Setup:
 
     def keys(self, pool, s, h, n):
         """Slots 0 .. n of one head in 64 bits (NaN where the page is none)."""
-        out = np.full((n, *pool.shape[3:]), np.nan)
-        for j in range(n):
-            e = int(self.table[s, j // self.page])
-            if 0 <= e < self.n_pages:
-                out[j] = pool[e, h, j % self.page].double().numpy()
+        j = np.arange(n)
+        e = self.table[s, j // self.page]
+        ok = (e >= 0) & (e < self.n_pages)
+        out = pool[torch.from_numpy(np.where(ok, e, 0)).long(), h, torch.from_numpy(j % self.page)].double().numpy()
+        out[~ok] = np.nan
         return out
 
     def on(self, dev):

@@ -106,16 +106,33 @@ def test_attention_large_groups_and_many_rows(ops, hip_device, seqs, types):
 
 
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("seqs,hq,hkv,hd,page", [
+    ([(1, 8300), (1, 1100)] + [(1, 3 + i) for i in range(30)], 8, 8, 32, 64),   # workgroups of 8 waves, no cuts, long walks
+    ([(1, 5000), (1, 3)], 4, 2, 64, 16),                                        # more than 16 cuts of a token's keys
+    ([(130, 5000)], 64, 64, 32, 128),                                           # long walks of a chunk's tiles
+    ([(12, 600), (5, 70)], 6, 2, 64, 16),                                       # 32 rows per workgroup
+])
+def test_attention_long_walks(ops, hip_device, seqs, hq, hkv, hd, page, types):
+    xd, kd = TYPES[types]
+    u = Setup(seqs, hq, hkv, hd, page, xd, kd, seed=8)
+    d = u.on(hip_device)
+    check_attention(u, *attend(ops, u, d))
+    if len(seqs) > 1:
+        check_attention(u, *attend(ops, u, d, None, 2100, 40), None, 2100, 40)
+
+
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("hd", [16, 64, 128])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
 def test_attention_unseen_slots_do_not_matter(ops, hip_device, what, hd, types):
     """Slots past a length, before a window and of later tokens of the same
     chunk hold NaN or infinities: rows that do not see them are what they are without them."""
     xd, kd = TYPES[types]
-    for seqs, window, sinks in (([(9, 40), (1, 21), (150, 150)], 0, 0), ([(9, 90), (1, 130), (140, 200)], 30, 5)):
-        u = Setup(seqs, 4, 2, hd, 16, xd, kd, width=14, seed=9)
+    for seqs, window, sinks, width in (([(9, 40), (1, 21), (150, 150)], 0, 0, 14), ([(9, 90), (1, 130), (140, 200)], 30, 5, 14),
+                                       ([(3, 900), (1, 700)], 0, 0, 60), ([(60, 1200), (40, 900)], 0, 0, 80)):
+        u = Setup(seqs, 4, 2, hd, 16, xd, kd, width=width, seed=9)
         for s, (n, length) in enumerate(seqs):
-            for j in range(14 * 16):
+            for j in range(width * 16):
                 e = u.table[s, j // 16]
                 first = length - n
                 if j >= length or (window and sinks <= j <= first - window):
@@ -130,7 +147,7 @@ def test_attention_unseen_slots_do_not_matter(ops, hip_device, what, hd, types):
         got, used = out.double().cpu().numpy(), int(u.starts[-1])
         fin = np.isfinite(want[:used])
         assert fin.any() and not fin.all()
-        tol = ref.attention_bound(u, want, weight, np.where(np.isfinite(size), size, 0), 300, xd == BF16)[:used]
+        tol = ref.attention_bound(u, want, weight, np.where(np.isfinite(size), size, 0), 16 * width, xd == BF16)[:used]
         assert (np.isfinite(got[:used]) == fin).all(), np.argwhere(np.isfinite(got[:used]) != fin)[:5]
         assert (np.abs(got[:used] - want[:used])[fin] <= tol[fin]).all()
 
