@@ -1365,18 +1365,19 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   }
 }
 
-// BF16 cache, on the BF16 matrix cores.  Each wave holds 64 keys as fragments in registers, and the
-// workgroup's 256 keys meet the rows in LDS, N at a time: FP32 ones are cut into
+// On the BF16 matrix cores.  Each wave holds 64 keys as fragments in registers (32 of an FP32 cache,
+// in three parts), and the workgroup's keys meet the rows in LDS, N at a time: FP32 ones are cut into
 // their three BF16 parts there, once for all waves, the next ones loading meanwhile in registers; two slots, one
-// barrier per stage.
+// barrier per stage.  Parts of both sides: the six products down to 2^-16 of the largest; what is
+// left out is under 2^-21 of a product, always towards 0.
 //   N = 32 (many rows): S = Q K^T by 32 x 32 x 16; lane l holds rows 8 i + 4 (l / 32) + r (i, r < 4) against key l % 32.
 //   N = 16 (few rows, where the bytes of K decide: 64 bytes of 16 keys per load): 16 x 16 x 32; rows
 //     4 (l / 16) + r against key l % 16.
 // Many rows on few keys are cut over workgroups, whose sums mass_join_kernel adds in order.
-template <typename QT, int HD, int N>
+template <typename QT, typename KT, int HD, int N>
 __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
   constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KD = 512 / N, KS = HD / KD;   // dims of a fragment, fragments of a row tile
-  constexpr int NJ = 64 / N, NV = N * N / 64, NF = (KS + 3) / 4;            // key tiles of a wave, values per lane, fragments per wave
+  constexpr int KP = sizeof(KT) == 4 ? 3 : 1, NJ = (KP == 1 ? 64 : 32) / N, KEYS = NJ * N, NV = N * N / 64, NF = (KS + 3) / 4;            // key tiles of a wave, values per lane, fragments per wave
   using acc = std::conditional_t<N == 32, v16f, v4f>;
   __shared__ __attribute__((aligned(1024))) char frag[2][KS * NP * 1024];
   __shared__ __attribute__((aligned(16))) float lse[2][N];
@@ -1399,19 +1400,32 @@ __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
   const int* table = c.table + seq * c.stride;
   // this lane's account: key k0 + lane
   const int key = min(k0 + lane, len - 1), pg = page_of(c, key), page = table[pg];
-  const bool live = k0 + lane < len && page >= 0 && page < c.n_pages;
+  const bool live = lane < KEYS && k0 + lane < len && page >= 0 && page < c.n_pages;
   float* account = alone ? a.mass + ((size_t)(live ? page : 0) * c.Hkv + h) * c.page + (key - pg * c.page)
                          : a.part + (((size_t)seq * a.cuts + cut) * c.Hkv + h) * ((size_t)c.width * c.page) + key;
   const float before = alone && live ? *account : 0.f;
-  bf8 kf[NJ][KS];
+  bf8 kf[NJ][KP][KS];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {                  // lanes past the length read its last 16 keys
     const int t = min((k0 + j * N + in) / TILE * TILE, (len - 1) / TILE * TILE), g = page_of(c, t), e = table[g];
-    const uint16_t* kr = static_cast<const uint16_t*>(c.k) +
-                         (((size_t)(e >= 0 && e < c.n_pages ? e : 0) * c.Hkv + h) * c.page + (t - g * c.page) + in % TILE) * HD +
-                         part * 8;
+    const KT* kr = static_cast<const KT*>(c.k) +
+                   (((size_t)(e >= 0 && e < c.n_pages ? e : 0) * c.Hkv + h) * c.page + (t - g * c.page) + in % TILE) * HD + part * 8;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) kf[j][k] = *reinterpret_cast<const bf8*>(kr + k * KD);
+    for (int k = 0; k < KS; ++k) {
+      if constexpr (KP == 1) {
+        kf[j][0][k] = *reinterpret_cast<const bf8*>(kr + k * KD);
+      } else {
+        Piece<KT, 8> x;
+        float y[8];
+        bf8 parts[KP];
+        x.load(kr + k * KD);
+#pragma unroll
+        for (int e2 = 0; e2 < 8; ++e2) y[e2] = x.get(e2);
+        parts8<KP>(y, parts);
+#pragma unroll
+        for (int p = 0; p < KP; ++p) kf[j][p][k] = parts[p];
+      }
+    }
   }
 
   // this lane's rows by (token, head), carried along: a stage is N / G tokens and N % G heads further
@@ -1492,11 +1506,14 @@ __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
 #pragma unroll
       for (int u = 0; u < C; ++u)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const bf8 kk = kf[j][(i * C + u) / NP];
-          if constexpr (N == 32) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
-          else s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
-        }
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int p = KP - 1; p >= 0; --p) {
+            if (p + (i * C + u) % NP >= 3) continue;
+            const bf8 kk = kf[j][p][(i * C + u) / NP];
+            if constexpr (N == 32) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
+            else s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[i % 2][u], kk, s[j], 0, 0, 0);
+          }
       __builtin_amdgcn_sched_barrier(0);
     }
     const int p_lo = slot[b][0], p_hi = slot[b][N - 1];

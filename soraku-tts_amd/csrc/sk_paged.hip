@@ -117,9 +117,9 @@ constexpr int NK2 = 2;                            // key tiles per wave of mass_
 MassPlan plan_mass(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page, int width) {
   MassPlan p;
   const int64_t rows = (int64_t)T * (Hq / Hkv);
-  p.tiles = kvdtype == SK_BF16 && hd >= 32;
   p.few = rows <= 16ll * S;
-  p.keys = p.tiles ? 4 * KEYS : 4 * NK2 * TILE;
+  p.tiles = hd >= 32 && (kvdtype == SK_BF16 || !p.few);   // few FP32 rows: FP32 products are enough beside K's bytes
+  p.keys = !p.tiles ? 4 * NK2 * TILE : kvdtype == SK_BF16 ? 4 * 64 : 4 * 32;
   p.blocks = ((int64_t)page * width + p.keys - 1) / p.keys;
   const int64_t base = p.blocks * Hkv * S;
   const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(3072 / base, rows / 256)) : 1;
@@ -282,9 +282,13 @@ int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, i
       using K = decltype(k);
       constexpr int HD = decltype(d)::value;
       const dim3 grid(Hkv, (unsigned)p.blocks, S * p.cuts);
-      if constexpr (HD >= 32 && sizeof(K) == 2) {
-        if (p.few) hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 16>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((mass_tiles_kernel<X, HD, 32>), grid, dim3(256), 0, st, a);
+      if constexpr (HD >= 32) {
+        if (p.tiles && !p.few)
+          hipLaunchKernelGGL((mass_tiles_kernel<X, K, HD, 32>), grid, dim3(256), 0, st, a);
+        else if constexpr (sizeof(K) == 2)
+          hipLaunchKernelGGL((mass_tiles_kernel<X, K, HD, 16>), grid, dim3(256), 0, st, a);
+        else
+          hipLaunchKernelGGL((mass_kernel<X, K, HD, NK2>), grid, dim3(256), 0, st, a);
       } else {
         hipLaunchKernelGGL((mass_kernel<X, K, HD, NK2>), grid, dim3(256), 0, st, a);
       }
