@@ -252,45 +252,53 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * operator at a time; no counterpart in the reference, whose caches are one
  * tensor per row.
  *
- * K and V lie in pools [n_pages][Hkv][page][hd] (page a multiple of 16; an
- * engine's cache, sk_kv_ptr, is such a pool with one page of max_ctx tokens per
- * row where max_ctx is one).  Sequence s (of S) has the pages table[s][0 .. width),
- * rows of the table table_stride entries apart; slot j of it lies in page
- * table[s][j / page].  Its new tokens of a call are the packed rows starts[s] ..
- * starts[s + 1] of T, and lens[s] is its length with them: token i of n has slot lens[s] -
- * n + i.  Sequences without new tokens and lengths of 0 are fine; rows past starts[S] are
- * padding and left alone.  table, starts and lens are device int32.
+ * K and V lie in pools [n_pages][Hkv][page][hd], page a multiple of 16 (an
+ * engine's cache, sk_kv_ptr, is such a pool where max_ctx is a multiple of 16:
+ * one page of max_ctx tokens per row).  Sequence s of S has the pages
+ * table[s][0 .. width), rows of the table table_stride entries apart; slot j of
+ * it lies in page table[s][j / page].  Its new tokens of a call are the packed
+ * rows starts[s] .. starts[s + 1] of T, and lens[s] is its length with them:
+ * token i of n has slot lens[s] - n + i.  Sequences without new tokens and
+ * lengths of 0 are fine; rows from starts[S] on are padding and left alone.
+ * table, starts and lens are device int32.
  *
- * The host does not look at device memory, so the kernels hold what they
- * find there in range: lens to [0, width * page], starts to [0, T].  A table entry
- * outside [0, n_pages) is no page: append drops what would go there, attention's rows
- * that see a key there become NaN, accounts there are not kept, eviction moves
- * NaN from it.  Entries of pages that no row sees may be anything.
+ * The host does not look at device memory, so the kernels hold what they find
+ * there in range: lens to [0, width * page], starts to [0, T].  A table entry
+ * outside [0, n_pages) is no page: append drops what would go there, tokens
+ * that see a key there come out of attention as NaN, accounts there are not
+ * kept, eviction moves NaN from it and nothing to it.  Entries of pages that no
+ * token sees may be anything.
  *
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
- * SK_BF16 / SK_BF16; sums and softmax in FP32.  hd: 16, 32, 64 or 128.  Hq: a
- * multiple of Hkv; query heads h G .. h G + G - 1 share key head h.  T may be 0.
- * No call allocates, waits or copies to the host, and each may be captured. */
+ * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
+ * exact.  hd: 16, 32, 64 or 128.  Hq: a multiple of Hkv, at most 4096; query
+ * heads h G .. h G + G - 1 share key head h.  T may be 0; width * page and T * Hq
+ * are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and workspaces are
+ * 16-byte aligned.  No call allocates, waits or copies to the host, and each may
+ * be captured into a graph. */
 
-/* New tokens into the cache: qkv [T][(Hq + 2 Hkv) hd] as projected; q and k
- * normalised per head (RMSNorm, gains [hd], or both NULL for none), rotated
- * by positions[T] * inv_freq[hd / 2] (pairs i and i + hd / 2; the angle in 64 bits); q to q_out [T][Hq][hd]
- * of xdtype, k and v to their slots.  mass (may be NULL): accounts of attention weight
- * [n_pages][Hkv][page], set to 0 at those slots.  Positions go their own way from slots:
- * a cache that was cut back keeps counting. */
+/* New tokens into the cache: qkv [T][(Hq + 2 Hkv) hd] as projected.  q and k are
+ * normalised per head (RMSNorm with gains [hd]; both NULL: not) and rotated by
+ * positions[T] * inv_freq[hd / 2] (pairs i and i + hd / 2; the angle in 64 bits,
+ * so far positions are exact); q goes to q_out [T][Hq][hd] of xdtype, k and v to
+ * their slots.  mass (may be NULL): accounts of attention weight
+ * [n_pages][Hkv][page], set to 0 at those slots.  Positions go their own way from
+ * slots: a cache that was cut back keeps counting. */
 int sk_op_paged_append(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
                        int32_t n_pages, int32_t width, int64_t table_stride, int32_t xdtype, int32_t kvdtype,
                        float eps, const void* qkv, const float* q_gain, const float* k_gain,
                        const float* inv_freq, const int32_t* positions, const int32_t* starts,
                        const int32_t* lens, const int32_t* table, void* k_pages, void* v_pages, float* mass,
                        void* q_out);
-/* Attention of the new tokens over their sequences' slots: out = softmax(scale
- * q k^T) v [T][Hq][hd] of xdtype, lse (may be NULL) [T][Hq] the natural logarithm of the
- * softmax's sum.  The token at slot p sees slot j when j <= p and, with a window > 0, also j > p
- * - window or j < sinks.  A token that sees nothing (slot below 0) gives 0 and -infinity.  Keys that a
- * token does not see do not reach it, whatever they hold.  The workspace holds the
- * bytes that _workspace gives for the same arguments (none: 0, and it may be NULL) and
- * belongs to the call until it has run. */
+/* Attention of the new tokens over their sequences' slots: out = softmax(scale q
+ * k^T) v [T][Hq][hd] of xdtype, lse (may be NULL) [T][Hq] the natural logarithm of
+ * the softmax's sum.  The token at slot p sees slot j when j <= p and, with a
+ * window > 0, also j > p - window or j < sinks.  A token that sees nothing (slot
+ * below 0) gives 0 and -infinity.  What a token does not see does not reach it,
+ * whatever it holds; what it sees should be finite (infinities there may come out
+ * as NaN).  The workspace holds the bytes that _workspace gives for the same
+ * arguments (where that is 0 it may be NULL) and belongs to the call until it has
+ * run. */
 int sk_op_paged_attention_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page,
                                     int32_t width, int32_t xdtype, int32_t kvdtype, int32_t window,
                                     int32_t sinks, int64_t* bytes);
@@ -300,9 +308,11 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
                           const void* v_pages, const int32_t* table, const int32_t* starts, const int32_t* lens,
                           void* out, float* lse, void* workspace, int64_t workspace_bytes);
 /* Adds the attention weight that every slot got from the new tokens, exp(scale q k
- * - lse) summed over tokens and the group's heads, to its account in mass [n_pages][Hkv][page].  q, lse,
- * scale, window, sinks as in the attention call.  The order of sums is fixed; two sequences of
- * one call must not share a page that both see.  Workspace as for attention. */
+ * - lse) summed over tokens and the group's heads, to its account in mass
+ * [n_pages][Hkv][page].  q, lse, scale, window and sinks as in the attention call.
+ * The order of sums is fixed.  Two sequences of one call that both have new tokens
+ * must not share a page: each would add to accounts that the other adds to.
+ * Workspace as for attention. */
 int sk_op_paged_attention_mass_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd,
                                          int32_t page, int32_t width, int32_t xdtype, int32_t kvdtype,
                                          int64_t* bytes);
@@ -313,11 +323,12 @@ int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, i
                                const int32_t* starts, const int32_t* lens, float* mass, void* workspace,
                                int64_t workspace_bytes);
 /* Cuts caches back to n = min(lens[s], keep) slots: of every key head the first
- * `sinks`, the last `recent` and, of the others, those with the largest accounts (ties to
- * the lowest slot, NaN above all) move in their order, with their accounts, to slots 0 .. n - 1 of the
- * pages `to` [S][to_width] (rows to_stride apart).  Those pages must be no pages of `table`: old
- * pages may be shared with other sequences, as a prompt's are, and are only read.  new_lens [S], and
- * kept [S][Hkv][keep] the old slots, -1 past n. */
+ * `sinks`, the last `recent` and, of the others, those with the largest accounts
+ * (ties to the lowest slot, NaN above all) move in their order, with their
+ * accounts, to slots 0 .. n - 1 of the pages `to` [S][to_width] (rows to_stride
+ * apart).  A page of `to` appears there once and not in `table`: old pages, which
+ * other sequences may share as they share a prompt, are only read.  new_lens [S],
+ * and kept [S][Hkv][keep] the old slots, -1 past n. */
 int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages,
                       int32_t width, int64_t table_stride, int32_t kvdtype, int32_t keep, int32_t sinks,
                       int32_t recent, void* k_pages, void* v_pages, float* mass, const int32_t* table,

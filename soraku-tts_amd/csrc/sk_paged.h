@@ -1368,8 +1368,8 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
 // On the BF16 matrix cores.  Each wave holds 64 keys as fragments in registers (32 of an FP32 cache,
 // in three parts), and the workgroup's keys meet the rows in LDS, N at a time: FP32 ones are cut into
 // their three BF16 parts there, once for all waves, the next ones loading meanwhile in registers; two slots, one
-// barrier per stage.  Parts of both sides: the six products down to 2^-16 of the largest; what is
-// left out is under 2^-21 of a product, always towards 0.
+// barrier per stage.  Parts of both sides: the six products of the
+// largest parts; what is left out is 2^-20 of a product at most, 2^-23 on average, towards 0.
 //   N = 32 (many rows): S = Q K^T by 32 x 32 x 16; lane l holds rows 8 i + 4 (l / 32) + r (i, r < 4) against key l % 32.
 //   N = 16 (few rows, where the bytes of K decide: 64 bytes of 16 keys per load): 16 x 16 x 32; rows
 //     4 (l / 16) + r against key l % 16.

@@ -40,7 +40,7 @@ int check_types(int32_t xdtype, int32_t kvdtype) {
   return SK_OK;
 }
 int check_window(float scale, int32_t window, int32_t sinks) {
-  SK_CHECK(scale > 0.f && isfinite(scale), SK_EINVAL, "scale must be positive and finite");
+  SK_CHECK(scale > 0.f && scale <= 1e30f, SK_EINVAL, "scale must be positive and at most 1e30");
   SK_CHECK(window >= 0 && sinks >= 0, SK_EINVAL, "window and sinks must not be negative");
   return SK_OK;
 }

@@ -39,7 +39,7 @@ ENTRY = {"append": ("sk_op_paged_append", APPEND), "attention": ("sk_op_paged_at
 SIZES = [("S", 0), ("Hkv", 0), ("Hkv", -8), ("hd", 48), ("hd", 256), ("hd", 0), ("page", 0), ("page", 24), ("page", -16),
          ("n_pages", 0), ("width", 0), ("stride", 3), ("width", 2 ** 27), ("kd", 2)]
 ROWS = [("T", -1), ("T", 2 ** 27), ("Hq", 12), ("Hq", 0), ("Hq", 8192), ("xd", 2), ("xd", 3)]
-WINDOW = [("scale", 0.0), ("scale", -1.0), ("scale", math.inf), ("scale", math.nan), ("window", -1), ("sinks", -1)]
+WINDOW = [("scale", 0.0), ("scale", -1.0), ("scale", math.inf), ("scale", 3e38), ("scale", math.nan), ("window", -1), ("sinks", -1)]
 BAD = {
     "append": [*ROWS, ("eps", -1.0), ("eps", math.nan), ("q_gain", None), ("k_gain", None), ("qkv", P + 4), ("v", P + 8),
                ("out", P + 2), ("q_gain", P + 4)] + [(n, None) for n in ("qkv", "inv_freq", "positions", "starts", "lens",
