@@ -146,29 +146,39 @@ __device__ __forceinline__ int seq_of_row(const Cache& c, int m) {
   return m < c.starts[count] ? count - 1 : c.S;
 }
 
-// Tile x of all sequences' tiles of R (token, head of the group) rows: its
-// sequence and its number there; false past the last.
-__device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, int& seq, int& tile) {
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);    // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);    // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);    // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// Tile x of all sequences' tiles of R (token, head of the group) rows: its sequence, its number
+// there, and the sequence's first row, new tokens and length; false past the last.
+// Every lane brings one sequence's numbers, in one trip to memory.
+struct TileAt {
+  int seq, tile, first, n, len;
+};
+__device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, TileAt& at) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int s0 = 0; s0 < c.S; s0 += 64) {
-    int t = 0;
-    if (s0 + lane < c.S) {
-      int first, n;
-      seq_rows(c, s0 + lane, first, n);
-      t = (n * c.G + R - 1) / R;
-    }
-    int sum = t;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int o = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += o;
-    }
+    const int s = min(s0 + lane, c.S - 1);
+    int first, n;
+    seq_rows(c, s, first, n);
+    const int len = seq_len(c, s), t = s0 + lane < c.S ? (n * c.G + R - 1) / R : 0, sum = wave_scan(t);
     const uint64_t past = __ballot(base + sum > x);
     if (past) {
       const int l = __builtin_ctzll(past);
-      seq = s0 + l;
-      tile = x - base - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(t, l));
+      at.seq = s0 + l;
+      at.tile = x - base - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(t, l));
+      at.first = __builtin_amdgcn_readlane(first, l);
+      at.n = __builtin_amdgcn_readlane(n, l);
+      at.len = __builtin_amdgcn_readlane(len, l);
       return true;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -468,11 +478,9 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   __shared__ float2 stats[R];
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
-  int seq, tile_no;
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;   // the longest walks first
-  int first, n;
-  seq_rows(c, seq, first, n);
-  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  TileAt tile;
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;   // the longest walks first
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int end = min(w.n, (cut + 1) * a.cut);
@@ -677,12 +685,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __attribute__((aligned(1024))) char lds[4 * L::K];   // two slots of K, two of V
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
-  int seq, tile_no;
+  TileAt tile;
   // the last tiles of a sequence walk furthest: they start first
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;
-  int first, n;
-  seq_rows(c, seq, first, n);
-  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int begin = cut * a.cut, end = min(w.n, begin + a.cut);
@@ -932,9 +938,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if constexpr (!AHEAD) {
     for (int t = begin; t < end; t += 4) step(t, std::false_type{});
   } else if (begin < end) {
-    if (begin + 4 < end) bad1 = place(begin + 4);
+    if (begin + 4 < end) {
+      bad1 = place(begin + 4);
+      load_k(begin + 4);
+    }
     stage_sync<0>();
-    if (begin + 4 < end) load_k(begin + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       bf8 kf[KU];
@@ -975,16 +983,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   if (wild) {
     __threadfence_block();                        // the stores above, by other lanes
-    int seq2, tile2, first2, n2;                  // found again: few registers are held for this through the loop
-    find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq2, tile2);
-    seq_rows(c, seq2, first2, n2);
-    const int q0 = seq_len(c, seq2) - n2, f_lo = tile2 * R + wave * 32, f_hi = min(tile2 * R + R, n2 * c.G);
-    const int q_lo = q0 + tile2 * R / c.G, q_hi = q0 + (f_hi - 1) / c.G;
+    TileAt again;                                 // few registers are held for this through the loop
+    find_tile(c, R, gridDim.y - 1 - blockIdx.y, again);
+    const int q0 = again.len - again.n, t2 = again.tile * R, f_lo = t2 + wave * 32, f_hi = min(t2 + R, again.n * c.G);
+    const int q_lo = q0 + t2 / c.G, q_hi = q0 + (f_hi - 1) / c.G;
     const Walk v = walk_of(q_lo, q_hi, a.window, a.sinks);
     const int b2 = blockIdx.z * a.cut, e2 = min(v.n, b2 + a.cut);
-    const int* tab = c.table + seq2 * c.stride;
+    const int* tab = c.table + again.seq * c.stride;
     add_wild<QT, uint16_t, HD>(
-        a, h, tab, first2, q0, f_lo, min(f_lo + 32, f_hi), v, b2, e2,
+        a, h, tab, again.first, q0, f_lo, min(f_lo + 32, f_hi), v, b2, e2,
         v.n <= a.cut ? nullptr : a.part + (size_t)blockIdx.z * c.T * c.Hq * HD,
         [&](int t) {
           const int t0 = b2 + (t - b2) / 4 * 4, t3 = min(t0 + 3, e2 - 1);
@@ -1020,11 +1027,9 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   __shared__ float2 stats[R];
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
-  int seq, tile_no;
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, seq, tile_no)) return;   // the longest walks first
-  int first, n;
-  seq_rows(c, seq, first, n);
-  const int p0 = seq_len(c, seq) - n, rows = n * c.G, f0 = tile_no * R;
+  TileAt tile;
+  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;   // the longest walks first
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int end = min(w.n, (cut + 1) * a.cut);

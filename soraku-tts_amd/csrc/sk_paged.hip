@@ -85,22 +85,30 @@ Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdty
   const int G = Hq / Hkv;
   const int64_t rows = (int64_t)T * G / S;        // of a sequence, on average
   const bool bf16 = kvdtype == SK_BF16 && hd >= 32;
-  p.tiles = bf16 && rows > 32;
-  // 32 rows where the registers hold them: not as three parts of 128 dims
-  p.R = p.tiles ? 128 : rows > 16 && (xdtype == kvdtype || hd < 128) ? 32 : 16;
   // tiles of n G rows: at most R - gcd(G, R) of a sequence's last one are empty
-  p.blocks = (int)(((int64_t)T * G + (int64_t)std::min(S, T) * (p.R - std::gcd(G, p.R))) / p.R);
+  auto blocks = [&](int R) { return ((int64_t)T * G + (int64_t)std::min(S, T) * (R - std::gcd(G, R))) / R; };
+  const int64_t keys = window > 0 ? std::min((int64_t)page * width, (int64_t)window + sinks) : (int64_t)page * width;
+  // Up to 1,024 keys, and where tiles of 16 rows still fit on the GPU at once, those start and end sooner
+  // (FP32 on BF16, 16 heads on 8: a prompt of 33 tokens 8 us against 12, of 200 10 against 17 + 4; eight
+  // of 200, past that bound: 22 by tiles of 128 rows).
+  const bool small = keys <= 1024 && blocks(16) * Hkv <= 512;
+  p.tiles = bf16 && rows > 32 && !small;
+  // 32 rows where the registers hold them (not as three parts of 128 dims) and every CU has a workgroup
+  p.R = p.tiles ? 128 : rows > 16 && (xdtype == kvdtype || hd < 128) && blocks(32) * Hkv >= 256 ? 32 : 16;
+  p.blocks = (int)blocks(p.R);
   int64_t most = (int64_t)page * width / TILE;    // tiles that a row tile can walk
   if (window > 0)
     most = std::min(most, ((int64_t)window + p.R / G + 2) / TILE + 2 + ((int64_t)sinks + TILE - 1) / TILE);
   const int64_t base = std::max<int64_t>((int64_t)p.blocks * Hkv, 1);
-  // A CU draws some 40 GB/s, so keys are cut until every CU has a workgroup (two of the
-  // tile kernel's), down to one round of a workgroup's waves: a pair of FP32 rows over 481 tokens takes 17 us uncut, 8
-  // waves or not, 7 + 4 in 8 cuts.  Past that a cut only adds its parts and a launch (32 BF16 rows of up to
-  // 657: 17 us uncut, 18 + 4 in two).  8 waves where each still has 8 tiles (a pair over 61,441:
-  // 74 us in 32 cuts by 4 waves, 66 in 16 by 8).
+  // A CU draws some 40 GB/s, so keys are cut until every CU has a workgroup (two of the tile kernel's), down to
+  // one round of a workgroup's waves: a pair of FP32 rows over 481 tokens takes 17 us uncut, with 8 waves or
+  // not, 7 + 4 in 8 cuts.  Past that a cut only adds its parts and a launch (32 BF16 rows of up to 657: 17 us
+  // uncut, 18 + 4 in two), and below six rounds it saves less than the launch (FP32 on BF16, 128 tokens: 9 us
+  // uncut, 16 + 4 in two).  8 waves where each still has 8 tiles (a pair over 61,441: 74 us in 32 cuts by 4
+  // waves, 66 in 16 by 8).
   const int64_t round = p.tiles || !bf16 ? 4 : 8;
-  const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>({(p.tiles ? 512 : 256) / base, most / round, 64}));
+  const int64_t most_cuts = std::min<int64_t>({(p.tiles ? 512 : 256) / base, most / round, 64});
+  const int64_t cuts = most < 6 * round ? 1 : std::max<int64_t>(1, most_cuts);
   p.cut = (int)((most + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
   p.cuts = (int)((most + p.cut - 1) / p.cut);
   p.WK = !p.tiles && base * p.cuts <= 256 && p.cut >= 64 ? 8 : 4;
