@@ -1326,11 +1326,9 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
       for (int e2 = 0; e2 < KW; ++e2) kf[j][t * KW + e2] = x.get(e2);
     }
   }
-  // the rows that can see a key of this wave
-  const int t_lo = max(0, k0 - p0);
-  int t_hi = n;
-  if (a.window > 0 && k0 >= a.sinks) t_hi = (int)min((int64_t)n, (int64_t)k0 + NK2 * TILE - 1 + a.window - p0);
-  for (int f0 = t_lo * c.G; f0 < t_hi * c.G; f0 += 16) {
+  int f_lo, f_hi;
+  mass_rows(a, n, p0, k0, NK2 * TILE, f_lo, f_hi);
+  for (int f0 = f_lo; f0 < f_hi; f0 += 16) {
     const int f = min(f0 + i16, n * c.G - 1), tok = f / c.G;
     const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
     Piece<QT, KW> x[NK];

@@ -354,6 +354,31 @@ def test_mass_many_rows(ops, hip_device, window, sinks, types):
     assert (np.abs(got.double().cpu().numpy() - want) <= rel * np.abs(want)).all()
 
 
+def test_mass_window_at_the_end_of_millions(ops, hip_device):
+    """A window far from most keys, under a group whose rows times slots pass 2^31: keys
+    that no row sees are left at once and unchanged."""
+    g = torch.Generator().manual_seed(51)
+    H, page, width, window = 384, 16, 65535 * 8, 40
+    q = torch.randn(1, H, 16, generator=g, dtype=torch.float64).float()
+    k = torch.randn(5, 1, page, 16, generator=g, dtype=torch.float64).float()
+    lse = torch.rand(1, H, generator=g) + 1.0
+    table = torch.full((1, width), -1, dtype=torch.int32)
+    table[0, -4:] = torch.tensor([3, 0, 4, 1])
+    mass = torch.full((5, 1, page), 2.0)
+    i32 = dict(dtype=torch.int32, device=hip_device)
+    got = ops.paged_attention_mass(H, 1, 16, page, None, window)(
+        q.to(hip_device), lse.to(hip_device), k.to(hip_device), table.to(hip_device), torch.tensor([0, 1], **i32),
+        torch.tensor([width * page], **i32), mass.to(hip_device)).cpu().double()
+    keys = k[[3, 0, 4, 1], 0].reshape(64, 16).double()
+    add = torch.exp(0.25 * q[0].double() @ keys.T - lse[0].double()[:, None]).sum(0)
+    add[: 64 - window] = 0.0
+    want = mass.double()
+    want[[3, 0, 4, 1], 0] += add.reshape(4, 16)
+    # 384 sums in one lane's order, and exponents below 32 off by 24 steps
+    assert torch.allclose(got, want, rtol=(384 + 2 * 24 * 32) * 2.0 ** -24, atol=0.0)
+    assert torch.equal(got[2], mass[2].double())
+
+
 def test_mass_unseen_slots_do_not_matter(ops, hip_device):
     u = Setup([(9, 40), (1, 21)], 4, 2, 64, 16, F32, BF16, width=5, seed=50)
     for s, (_, length) in enumerate(u.seqs):
