@@ -272,9 +272,9 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
  * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
  * exact.  hd: 16, 32, 64 or 128.  Hq: a multiple of Hkv, at most 4096; query
- * heads h G .. h G + G - 1 share key head h.  T may be 0; width * page and T * Hq
- * are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and workspaces are
- * 16-byte aligned.  No call allocates, waits or copies to the host, and each may
+ * heads h G .. h G + G - 1 share key head h.  T may be 0 and is below 2^24; width *
+ * page and T * Hq are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and
+ * workspaces are 16-byte aligned; outputs overlap no operand.  No call allocates, waits or copies to the host, and each may
  * be captured into a graph. */
 
 /* New tokens into the cache: qkv [T][(Hq + 2 Hkv) hd] as projected.  q and k are

@@ -23,7 +23,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // What every entry point asks of its sizes.
 int check_sizes(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages, int32_t width,
                 int64_t stride) {
-  SK_CHECK(T >= 0 && S > 0, SK_EINVAL, "T must not be negative and S must be positive");
+  SK_CHECK(T >= 0 && T < 1 << 24 && S > 0, SK_EINVAL, "T must be in [0, 2^24) and S positive");
   SK_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 4096, SK_EINVAL,
            "Hq must be a positive multiple of Hkv, at most 4096");
   SK_CHECK(hd == 16 || hd == 32 || hd == 64 || hd == 128, SK_EINVAL, "hd must be a power of two in [16, 128]");
@@ -130,7 +130,7 @@ MassPlan plan_mass(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page,
   p.keys = !p.tiles ? 4 * NK2 * TILE : kvdtype == SK_BF16 ? 4 * 64 : 4 * 32;
   p.blocks = ((int64_t)page * width + p.keys - 1) / p.keys;
   const int64_t base = p.blocks * Hkv * S;
-  const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(3072 / base, rows / 256)) : 1;
+  const int64_t cuts = p.tiles && !p.few ? std::max<int64_t>(1, std::min<int64_t>(12 * 256 / base, rows / 256)) : 1;
   p.cut = (int)std::max<int64_t>(32, ((rows + cuts - 1) / cuts + 31) / 32 * 32);
   p.cuts = (int)std::max<int64_t>(1, (rows + p.cut - 1) / p.cut);
   return p;
@@ -158,6 +158,7 @@ int sk_op_paged_append(void* stream, int32_t T, int32_t S, int32_t Hq, int32_t H
   SK_CHECK(qkv && inv_freq && positions && starts && lens && table && k_pages && v_pages && q_out, SK_EINVAL,
            "NULL operand");
   SK_CHECK(!q_gain == !k_gain, SK_EINVAL, "gains of q and k come together");
+  SK_CHECK(q_out != qkv, SK_EINVAL, "q_out must not be qkv");
   SK_CHECK(aligned16(qkv) && aligned16(q_gain) && aligned16(k_gain) && aligned16(k_pages) && aligned16(v_pages) &&
                aligned16(q_out),
            SK_EINVAL, "operands must be 16-byte aligned");
@@ -197,6 +198,7 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   SK_CHECK(q && k_pages && v_pages && table && starts && lens && out, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace), SK_EINVAL,
            "operands must be 16-byte aligned");
+  SK_CHECK(out != q, SK_EINVAL, "out must not be q");
   const Plan p = plan_attention(T, S, Hq, Hkv, hd, xdtype, kvdtype, page, width, window, sinks);
   SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= workspace_of(p, T, Hq, hd)), SK_EINVAL,
            "the workspace must hold %lld bytes", (long long)workspace_of(p, T, Hq, hd));
@@ -326,6 +328,7 @@ int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t 
            "S must be at most 65535 and S * Hkv * keep at most 2^31");
   SK_CHECK(k_pages && v_pages && mass && table && lens && to && new_lens && kept, SK_EINVAL, "NULL operand");
   SK_CHECK(table != to, SK_EINVAL, "the new table must have pages of its own");
+  SK_CHECK(lens != new_lens, SK_EINVAL, "new_lens must not be lens");
   SK_CHECK(aligned16(k_pages) && aligned16(v_pages), SK_EINVAL, "operands must be 16-byte aligned");
   const Cache c = cache_of(0, S, Hkv, Hkv, page, n_pages, width, table_stride, nullptr, lens, table, k_pages, v_pages);
   const hipStream_t st = (hipStream_t)stream;

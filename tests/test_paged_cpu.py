@@ -26,30 +26,30 @@ def L():
 
 
 APPEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, eps=1e-6,
-              qkv=P, q_gain=P, k_gain=P, inv_freq=P, positions=P, starts=P, lens=P, table=P, k=P, v=P, mass=None, out=P)
+              qkv=P, q_gain=P, k_gain=P, inv_freq=P, positions=P, starts=P, lens=P, table=P, k=P, v=P, mass=None, out=2 * P)
 ATTEND = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
-              window=0, sinks=0, q=P, k=P, v=P, table=P, starts=P, lens=P, out=P, lse=None, ws=None, ws_bytes=0)
+              window=0, sinks=0, q=P, k=P, v=P, table=P, starts=P, lens=P, out=2 * P, lse=None, ws=None, ws_bytes=0)
 MASS = dict(stream=None, T=3, S=2, Hq=16, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, xd=0, kd=1, scale=0.1,
             window=0, sinks=0, q=P, lse=P, k=P, table=P, starts=P, lens=P, mass=P, ws=None, ws_bytes=0)
 EVICT = dict(stream=None, S=2, Hkv=8, hd=128, page=16, n_pages=9, width=4, stride=4, kd=1, keep=32, sinks=4, recent=8,
-             k=P, v=P, mass=P, table=P, lens=P, to=2 * P, to_stride=2, to_width=2, new_lens=P, kept=P)
+             k=P, v=P, mass=P, table=P, lens=P, to=2 * P, to_stride=2, to_width=2, new_lens=2 * P, kept=P)
 ENTRY = {"append": ("sk_op_paged_append", APPEND), "attention": ("sk_op_paged_attention", ATTEND),
          "mass": ("sk_op_paged_attention_mass", MASS), "evict": ("sk_op_paged_evict", EVICT)}
 
 SIZES = [("S", 0), ("Hkv", 0), ("Hkv", -8), ("hd", 48), ("hd", 256), ("hd", 0), ("page", 0), ("page", 24), ("page", -16),
          ("n_pages", 0), ("width", 0), ("stride", 3), ("width", 2 ** 27), ("kd", 2)]
-ROWS = [("T", -1), ("T", 2 ** 27), ("Hq", 12), ("Hq", 0), ("Hq", 8192), ("xd", 2), ("xd", 3)]
+ROWS = [("T", -1), ("T", 2 ** 24), ("T", 2 ** 27), ("Hq", 12), ("Hq", 0), ("Hq", 8192), ("xd", 2), ("xd", 3)]
 WINDOW = [("scale", 0.0), ("scale", -1.0), ("scale", math.inf), ("scale", 3e38), ("scale", math.nan), ("window", -1), ("sinks", -1)]
 BAD = {
     "append": [*ROWS, ("eps", -1.0), ("eps", math.nan), ("q_gain", None), ("k_gain", None), ("qkv", P + 4), ("v", P + 8),
-               ("out", P + 2), ("q_gain", P + 4)] + [(n, None) for n in ("qkv", "inv_freq", "positions", "starts", "lens",
+               ("out", P), ("out", P + 2), ("q_gain", P + 4)] + [(n, None) for n in ("qkv", "inv_freq", "positions", "starts", "lens",
                                                                          "table", "k", "v", "out")],
-    "attention": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("out", P + 8), ("ws", P + 4)] + [
+    "attention": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("out", P), ("out", P + 8), ("ws", P + 4)] + [
         (n, None) for n in ("q", "k", "v", "table", "starts", "lens", "out")],
     "mass": [*ROWS, *WINDOW, ("q", P + 4), ("k", P + 2), ("ws", P + 8)] + [(n, None) for n in ("q", "lse", "k", "table", "starts", "lens",
                                                                               "mass")],
     "evict": [("keep", 0), ("keep", -5), ("sinks", -1), ("recent", -1), ("sinks", 25), ("sinks", 2 ** 31 - 1), ("keep", 33),
-              ("to_width", 0), ("to_stride", 1), ("to", P), ("k", P + 4), ("v", P + 4)] + [
+              ("to_width", 0), ("to_stride", 1), ("to", P), ("new_lens", P), ("k", P + 4), ("v", P + 4)] + [
                   (n, None) for n in ("k", "v", "mass", "table", "lens", "to", "new_lens", "kept")],
 }
 
