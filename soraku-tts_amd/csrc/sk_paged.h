@@ -642,9 +642,10 @@ constexpr int KEYS = 64;                          // keys of a step
 template <int HD>
 struct TileLds {
   static constexpr int K = KEYS * HD * 2;         // bytes of a slot
-  // V row `key` holds its 32 bytes number x at x ^ turn(key): rows that the
-  // transposing read takes together lie in different banks
-  static __device__ __forceinline__ int turn(int key) { return HD == 128 ? key & 7 : HD == 64 ? key >> 1 & 3 : key >> 2 & 1; }
+  // V row `key` holds its 32 bytes number x at x ^ turn(key), so that what half a wave's
+  // transposing read takes, 4 keys x 64 bytes for 32 dims or 8 x 32 for 16 (turn16), lies in different banks
+  static __device__ __forceinline__ int turn(int key) { return HD == 128 ? 2 * (key & 3) : HD == 64 ? key & 2 : 0; }
+  static __device__ __forceinline__ int turn16(int key) { return HD == 128 ? key & 7 : HD == 64 ? key >> 1 & 3 : key >> 2 & 1; }
 };
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -722,8 +723,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 
   // wave u loads the u-th 16 keys of a step: K as blocks of 16 keys x 32 dims (16 bytes per
-  // lane, keys first), V as rows, KS loads of 1 KB each (with 128 dims 4 rows, every other
-  // load turned by 4 more)
+  // lane, keys first), V as rows, KS loads of 1 KB each
   const unsigned koff = (i16 * HD + q4 * 8) * 2;
   const int vrow = lane / (HD / 8);
   const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn(vrow)) * 8) * 2;
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const char* st = lds + 2 * L::K + ((t - begin) / 4 % 2) * L::K + wave * GROUP;
     const char* vb = static_cast<const char*>(c.v) + off;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) lds_load16(vb + k * 1024, HD == 128 && k % 2 ? voff ^ 128 : voff, st + k * 1024);
+    for (int k = 0; k < KS; ++k) lds_load16(vb + k * 1024, voff, st + k * 1024);
   };
   v16f o[KS], s[2];
   float m2 = LOWEST, lr = 0.f;                    // the maximum that sums refer to (times scale2), the sum
@@ -1043,9 +1043,9 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if (t_first < end) offs.load(c, table, w, t_first, 2 * WK, end, h, HD, true);
   const unsigned koff = i16 * HD + q4 * 8;        // elements
   const int vrow = lane / (HD / 8);
-  const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn(vrow)) * 8) * 2;
+  const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn16(vrow)) * 8) * 2;
   const int vkey = 4 * q4 + (i16 >> 2);
-  const unsigned vbase = vkey * HD * 2 + (i16 & 3) * 8, vturn = L::turn(vkey) * 32;
+  const unsigned vbase = vkey * HD * 2 + (i16 & 3) * 8, vturn = L::turn16(vkey) * 32;
   char* vlds = lds + wave * 4 * GROUP;
   auto load = [&](int i, int slot, bf8 (&kf)[2][KS]) {   // tiles i, i + 1 of offs
 #pragma unroll
