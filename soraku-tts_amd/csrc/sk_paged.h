@@ -196,6 +196,10 @@ __device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, TileAt& 
 // The angle is formed and brought into [-pi, pi] in 64 bits (in 32 a product
 // of 2^17 is off by 2^-7), then cos(r + e) = cos r - e sin r with r its nearest FP32
 // and e the rest; one lane per pair, shared through LDS.
+//
+// Bound by bytes: 5,760 tokens of 16 + 2 x 8 heads of 128, FP32 into BF16 with accounts, 165 MB in
+// 28.8 us (5.7 TB/s, part of it from the last-level cache).  32 tokens take 3.8 us, three trips to
+// memory (starts, the table, the store) beside the angle.
 template <typename XT, typename KT, int HD>
 __global__ __launch_bounds__(256) void append_kernel(Cache c, const XT* qkv, const float* q_gain, const float* k_gain,
                                                      const float* inv_freq, const int* positions, float eps,
@@ -469,6 +473,10 @@ __device__ __forceinline__ void meet_rows(const AttendArgs& a, const float* po, 
 //     keys 4 (l / 16) + v, v < 4; a row's maximum is 4 values and two exchanges;
 //   O^T += V^T P^T takes those values as they are: step v multiplies keys 4 q + v, q = 0 .. 3.
 // K and V come straight from the pages, 16 bytes per lane; K of the next tile loads under this one's softmax and V.
+// Two rows of 240 and 481 tokens, FP32, 8 cuts: 6.7 us, latency.  Prompts of 194 and 387: 27 us (28 TFLOP/s,
+// matrix cores 37% busy): what a CU draws of K and V, and the ends of uneven walks.  2,047 tokens over 8,000:
+// 980 us, 119 TFLOP/s of the 151 that a large FP32 product reaches here.  Products of BF16 parts, three of K, Q, P
+// and V each, took 870 us there, but 88 for 69 with a prompt of 1,000 tokens and 125 for 93 with a window.
 template <typename QT, typename KT, int HD, int NT, int WK>
 __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_rows_kernel(AttendArgs a) {
   using D = Dims<KT, HD>;
@@ -637,6 +645,12 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // FP32 activations: Q and P as three BF16 parts of 8 bits that add up to the FP32 value
 // exactly, three products each, so results are those of FP32 products (NP = 3).  BF16
 // activations: P rounds to BF16 once (2^-9 of a weight on average, under the output's own rounding).
+//
+// 2,047 BF16 tokens over 16,384, 16 heads on 8 of 128: 265 us, 972 TFLOP/s (a large BF16 product reaches
+// 1,225 here).  The matrix cores are busy 59% of the time and the VALU (exponentials, maxima) 56%: two waves of a
+// SIMD hide only so much of one under the other.  LDS does not bound it (no bank conflicts); 16 x 16 x 32 took 310.
+// 4,500 FP32 tokens with a window of 1,024: 168 us, 740 TFLOP/s of the three-part products, matrix cores 52%
+// busy: no registers are left to run a step's scores ahead.
 constexpr int KEYS = 64;                          // keys of a step
 
 template <int HD>
@@ -1015,6 +1029,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // take 1,024 cycles of a SIMD per 4 KB of the cache, these 64 to 192 (with BF16 activations P keeps 16
 // bits, two parts: it costs nothing here).  K goes from the pages to registers as fragments, V to
 // two slots of LDS of the wave's own, both a step ahead.
+// 32 rows of 328 to 657 tokens, FP32 on BF16: 16.8 us for 65 MB, one workgroup per CU at what it draws (12.7 at
+// a large copy's rate); two rows of 30,720 and 61,441 in 16 cuts: 66 us, 5.7 TB/s.
 template <typename QT, int HD, int NT, int WK>
 __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_few_kernel(AttendArgs a) {
   constexpr int NP = sizeof(QT) == 4 ? 3 : 1, PP = NP == 3 ? 3 : 2;   // parts of Q, of P
@@ -1276,7 +1292,8 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int cuts) {
 // the statistics known every weight is one exponential, and a workgroup that holds
 // its keys and walks the rows adds up without atomics, in one order.
 //   S = Q K^T: lane l holds rows 4 (l / 16) + v against key l % 16; the sum over rows stays in the lane.
-// A wave holds NK2 tiles of 16 keys in registers; four waves per workgroup.
+// A wave holds NK2 tiles of 16 keys in registers; four waves per workgroup.  On the FP32 matrix cores: for single
+// tokens over FP32 caches, where the bytes of K decide, and for heads of 16.
 struct MassArgs {
   Cache c;
   const void* q; const float* lse; float* mass;   // [n_pages][Hkv][page]
@@ -1377,6 +1394,10 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
 //   N = 16 (few rows, where the bytes of K decide: 64 bytes of 16 keys per load): 16 x 16 x 32; rows
 //     4 (l / 16) + r against key l % 16.
 // Many rows on few keys are cut over workgroups, whose sums mass_join_kernel adds in order.
+//
+// 32 rows of 2,400 to 4,800 tokens, FP32 on BF16: 52 us, 244 MB at 4.7 TB/s.  Prompts of 900 and 1,800 over
+// 1,800 and 3,600: 90 + 5 us, 830 TFLOP/s of the three-part products, matrix cores 48% busy beside one exponential
+// per weight and the parts (three waves per SIMD spill: 109; cuts for fewer than twelve workgroups per CU: 132 to 140).
 template <typename QT, typename KT, int HD, int N>
 __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
   constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KD = 512 / N, KS = HD / KD;   // dims of a fragment, fragments of a row tile
@@ -1585,7 +1606,8 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int keys) {
 // look (61,440 slots: 54 us, 94 read again).
 // A histogram of the ranks' upper 12 bits leaves the few in the cut's bin; those go to a
 // list in LDS (where they fit), and two bits at a time, three counts by ballot, give the cut; it
-// ends early where a bound has exactly n ranks at or above it.
+// ends early where a bound has exactly n ranks at or above it.  256 heads of up to 4,800 slots: 14 us;
+// 16 of up to 61,440: 55, one workgroup's latencies (table, accounts, histogram, places) on 16 of 256 CUs.
 __device__ __forceinline__ uint32_t rank_of(float x) {
   if (x != x) return 0xfffffffeu;
   const uint32_t b = __float_as_uint(x + 0.f);    // -0 counts as 0
@@ -1770,6 +1792,8 @@ __global__ __launch_bounds__(1024) void choose_kernel(Cache c, const float* mass
 // K, V and weight of the slots that stay, in their order, to the pages of `to`
 // [S][to_width]; a slot on a page outside the pool becomes NaN, one for such a
 // page is dropped.  Rows as 16-byte pieces, SLOTS slots of a head per workgroup.
+// Bound by bytes: 629 MB of BF16 rows (2,400 slots of 32 x 8 heads) in 134 us, 4.7 TB/s of the 5.1 that a large
+// copy reaches here; 252 MB of FP32 in 58, 4.3.
 template <int PIECES, int SLOTS>
 __global__ __launch_bounds__(256) void move_kernel(Cache c, float* mass, const int* kept, int keep, const int* to,
                                                    int64_t to_stride) {
