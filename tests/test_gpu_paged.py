@@ -524,6 +524,86 @@ def test_run_of_all(ops, hip_device, types):
         step([1] * S, lens, to, window=0 if i else 20, sinks=0 if i else 4)
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("new", [1, 180])
+def test_run_captured(ops, hip_device, types, new):
+    """Append, attention, accounts and the lengths' step in one graph, and eviction in another,
+    replayed on new contents with eager runs of the same between: equal bit for bit."""
+    xd, kd = TYPES[types]
+    hq, hkv, hd, page, S, keep = 8, 2, 128, 64, 2, 300
+    u = Setup([(new, 700)] * S, hq, hkv, hd, page, xd, kd, width=22, spare=S * 5, seed=80)
+    inv = torch.from_numpy((1e6 ** (-np.arange(0, hd, 2) / hd)).astype(np.float32)).to(hip_device)
+    to = torch.from_numpy(u.free[: S * 5].reshape(S, 5).copy()).to(hip_device)
+    app, att = ops.paged_append(hq, hkv, hd, page, 1e-6), ops.paged_attention(hq, hkv, hd, page)
+    acc, evi = ops.paged_attention_mass(hq, hkv, hd, page), ops.paged_evict(hkv, hd, page, keep, 4, 16)
+
+    def state():
+        d = u.on(hip_device)
+        d["pos"] = torch.arange(u.T, dtype=torch.int32, device=hip_device) % new + 700 - new
+        d["lse"] = torch.zeros(u.T, hq, device=hip_device)
+        return d
+
+    def step(d):
+        q = app(d["qkv"], None, None, inv, d["pos"], d["starts"], d["lens"], d["table"], d["k"], d["v"], mass=d["mass"])
+        out = att(q, d["k"], d["v"], d["table"], d["starts"], d["lens"], lse=d["lse"])
+        acc(q, d["lse"], d["k"], d["table"], d["starts"], d["lens"], d["mass"])
+        d["lens"].add_(new)
+        d["pos"].add_(new)
+        return q, out
+
+    def cut(d):
+        return evi(d["k"], d["v"], d["mass"], d["table"], d["lens"], to)
+
+    a, b = state(), state()
+    for f in (step, cut):                           # on a state of their own: kernels loaded before they are captured
+        f(state())
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for f in (step, cut):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(f(b))
+        graphs.append(g)
+    g = torch.Generator().manual_seed(81)
+    for _ in range(3):
+        x = torch.randn(u.T, (hq + 2 * hkv) * hd, generator=g).to(xd).to(hip_device)
+        for d in (a, b):
+            d["qkv"].copy_(x)
+        graphs[0].replay()
+        want = step(a)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, outs[0]))
+        graphs[1].replay()
+        want = cut(a)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, outs[1]))
+        assert all(torch.equal(a[n], b[n]) for n in ("k", "v", "mass", "lens", "lse"))
+        assert want[0].tolist() == [keep] * S
+
+
+def test_calls_on_two_streams_at_once(ops, hip_device):
+    """Calls with workspaces of their own, interleaved on two streams."""
+    runs = []
+    for seed, (xd, kd) in enumerate(TYPES.values()):
+        u = Setup([(1, 2900), (40, 1300)], 16, 8, 128, 64, xd, kd, seed=90 + seed)
+        d = u.on(hip_device)
+        out, lse = attend(ops, u, d)
+        mass = ops.paged_attention_mass(16, 8, 128, 64)(d["q"], lse, d["k"], d["table"], d["starts"], d["lens"],
+                                                        d["mass"].clone())
+        runs.append((u, d, out, lse, mass))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(12):
+        u, d, _, lse, _ = runs[i % 3]
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((*attend(ops, u, d), ops.paged_attention_mass(16, 8, 128, 64)(
+                d["q"], lse, d["k"], d["table"], d["starts"], d["lens"], d["mass"].clone())))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert all(torch.equal(p, q) for p, q in zip(x, runs[i % 3][2:]))
+
+
 def test_trunk_layers_from_operators(ops, hip_device):
     """The tiny trunk driven through the operator API on a paged cache gives the
     hidden state of the engine's prefill, prompt in chunks included."""
