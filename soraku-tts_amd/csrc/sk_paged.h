@@ -473,8 +473,8 @@ __device__ __forceinline__ void meet_rows(const AttendArgs& a, const float* po, 
 //     keys 4 (l / 16) + v, v < 4; a row's maximum is 4 values and two exchanges;
 //   O^T += V^T P^T takes those values as they are: step v multiplies keys 4 q + v, q = 0 .. 3.
 // K and V come straight from the pages, 16 bytes per lane; K of the next tile loads under this one's softmax and V.
-// Two rows of 240 and 481 tokens, FP32, 8 cuts: 6.7 us, latency.  Prompts of 194 and 387: 27 us (28 TFLOP/s,
-// matrix cores 37% busy): what a CU draws of K and V, and the ends of uneven walks.  2,047 tokens over 8,000:
+// Two rows of 240 and 481 tokens, FP32, 8 cuts: 6.7 us, latency.  Prompts of 194 and 387: 22 us (34 TFLOP/s):
+// what a CU draws of K and V, and the ends of uneven walks.  2,047 tokens over 8,000:
 // 980 us, 119 TFLOP/s of the 151 that a large FP32 product reaches here.  Products of BF16 parts, three of K, Q, P
 // and V each, took 870 us there, but 88 for 69 with a prompt of 1,000 tokens and 125 for 93 with a window.
 template <typename QT, typename KT, int HD, int NT, int WK>

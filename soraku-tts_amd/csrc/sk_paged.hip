@@ -93,8 +93,11 @@ Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdty
   // of 200, past that bound: 22 by tiles of 128 rows).
   const bool small = keys <= 1024 && blocks(16) * Hkv <= 512;
   p.tiles = bf16 && rows > 32 && !small;
-  // 32 rows where the registers hold them (not as three parts of 128 dims) and every CU has a workgroup
-  p.R = p.tiles ? 128 : rows > 16 && (xdtype == kvdtype || hd < 128) && blocks(32) * Hkv >= 256 ? 32 : 16;
+  // 32 rows where the registers hold them (not as three parts of 128 dims) and every CU has a workgroup, two on
+  // the FP32 matrix cores, whose long walks then even out (prompts of 194 and 387: 22 us, 28 by tiles of 32 on 304
+  // workgroups; of 2,047: 189 by 32 on 1,024, 199 by 16; 30 x 16 BF16 tokens of up to 2,000: 36 by 32, 43 by 16)
+  const bool pairs = rows > 16 && (xdtype == kvdtype || hd < 128) && blocks(32) * Hkv >= (bf16 ? 256 : 512);
+  p.R = p.tiles ? 128 : pairs ? 32 : 16;
   p.blocks = (int)blocks(p.R);
   int64_t most = (int64_t)page * width / TILE;    // tiles that a row tile can walk
   if (window > 0)
