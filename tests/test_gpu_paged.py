@@ -525,6 +525,38 @@ def test_run_of_all(ops, hip_device, types):
 
 
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n", [1, 30])
+def test_more_sequences_than_lanes(ops, hip_device, n, types):
+    """150 sequences, some without new tokens and some empty, ends and starts of 64 among them."""
+    xd, kd = TYPES[types]
+    rng = np.random.default_rng(95)
+    seqs = [(0, 0) if s % 17 == 3 else (0, 20) if s % 13 == 5 else (k := int(rng.integers(1, 2 * n + 1)),
+                                                                   k + int(rng.integers(0, 50))) for s in range(150)]
+    for s in (62, 63, 64, 65, 127, 128, 149):
+        seqs[s] = (n, n + 7) if s % 2 else (0, 9)
+    u = Setup(seqs, 8, 2, 32, 16, xd, kd, pad=3, seed=96)
+    d = u.on(hip_device)
+    out, lse = attend(ops, u, d)
+    check_attention(u, out, lse)
+    mass = ops.paged_attention_mass(8, 2, 32, 16)(d["q"], lse, d["k"], d["table"], d["starts"], d["lens"], d["mass"].clone())
+    want, terms = ref.mass(u, lse.cpu().numpy())
+    size = 32 ** 0.5 * float(u.k.abs().max()) * float(u.q.abs().max())
+    rel = (2.0 * (32 + 8) * (1.0 + size) + 8.0 + terms) * 2.0 ** -24
+    assert (np.abs(mass.double().cpu().numpy() - want) <= rel * np.abs(want)).all()
+    inv = (1e6 ** (-np.arange(0, 32, 2) / 32)).astype(np.float32)
+    pos = rng.integers(0, 2 ** 21, u.T).astype(np.int32)
+    want = ref.append(u, None, None, inv, pos, 1e-6)
+    q = ops.paged_append(8, 2, 32, 16, 1e-6)(d["qkv"], None, None, torch.from_numpy(inv).to(hip_device),
+                                             torch.from_numpy(pos).to(hip_device), d["starts"], d["lens"], d["table"],
+                                             d["k"], d["v"], mass=d["mass"])
+    used = int(u.starts[-1])
+    fine = (32 / 2 + 16) * 2.0 ** -24 * 2 * float(u.qkv.abs().max())
+    for got, w, t in ((q[:used], want[0][:used], xd), (d["k"], want[1], kd), (d["v"], want[2], kd)):
+        assert (np.abs(got.double().cpu().numpy() - w) <= fine + HALF_STEP[t] * np.abs(w)).all()
+    assert np.array_equal(d["mass"].cpu().numpy(), want[3])
+
+
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("new", [1, 180])
 def test_run_captured(ops, hip_device, types, new):
     """Append, attention, accounts and the lengths' step in one graph, and eviction in another,
