@@ -114,7 +114,7 @@ Plan plan_attention(int T, int S, int Hq, int Hkv, int hd, int xdtype, int kvdty
   const int64_t cuts = most < 6 * round ? 1 : std::max<int64_t>(1, most_cuts);
   p.cut = (int)((most + cuts - 1) / cuts + 3) / 4 * 4;   // whole steps of 64 keys
   p.cuts = (int)((most + p.cut - 1) / p.cut);
-  p.WK = !p.tiles && base * p.cuts <= 256 && p.cut >= 64 ? 8 : 4;
+  p.WK = p.R == 16 && base * p.cuts <= 256 && p.cut >= 64 ? 8 : 4;
   return p;
 }
 
@@ -238,8 +238,7 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
         if constexpr (HD >= 32 && sizeof(K) == 2)
           hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
       } else if (p.R == 32) {
-        if (p.WK == 8) share(Int<2>{}, Int<8>{});
-        else share(Int<2>{}, Int<4>{});
+        share(Int<2>{}, Int<4>{});
       } else {
         if (p.WK == 8) share(Int<1>{}, Int<8>{});
         else share(Int<1>{}, Int<4>{});

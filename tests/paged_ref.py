@@ -8,6 +8,13 @@ import torch
 
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}   # of a rounding, relative
 
+# (new tokens, length) of the sequences, heads of 64 with a key head each and width of the table at pages of 16, and the attention kernel
+# that takes them by type: with many heads a few short sequences reach the kernels of many rows
+MANY_HEADS = [
+    ([(150, 150), (40, 200), (9, 90)], 64, 13, {"f32": ("rows", 2), "f32_on_bf16": ("tiles", 0), "bf16": ("tiles", 0)}),
+    ([(20, 90), (17, 300), (31, 31), (2, 40)], 64, 19, {"f32": ("rows", 1), "f32_on_bf16": ("few", 2), "bf16": ("few", 2)}),
+]
+
 
 class Setup:
     """Random pools, a table of pages in random order and packed new tokens.

@@ -122,6 +122,27 @@ def test_attention_long_walks(ops, hip_device, seqs, hq, hkv, hd, page, types):
 
 
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("case", [0, 1])
+def test_attention_many_heads(ops, hip_device, case, hd, types):
+    """Row tiles of 32 and 128, with windows, pages that are none and slots that no row sees."""
+    seqs, heads, width, _ = ref.MANY_HEADS[case]
+    xd, kd = TYPES[types]
+    u = Setup(seqs, heads, heads, hd, 16, xd, kd, width=width, pad=1, seed=7)
+    d = u.on(hip_device)
+    for window, sinks in ((0, 0), (30, 5), (1, 0), (100, 40)):
+        check_attention(u, *attend(ops, u, d, None, window, sinks), None, window, sinks)
+    u.table[0, 2], u.table[1, 1], u.table[2, -1] = -1, u.n_pages, 2 ** 31 - 1
+    for pool in (u.k, u.v):                         # slots past the lengths, and before the second's window
+        for s, (_, length) in enumerate(seqs):
+            for j in [*range(length, width * 16), *((37,) if s == 1 else ())]:
+                if 0 <= u.table[s, j // 16] < u.n_pages:
+                    pool[u.table[s, j // 16], :, j % 16] = float("inf") if j % 2 else float("nan")
+    d = u.on(hip_device)
+    check_attention(u, *attend(ops, u, d, None, 50, 16), None, 50, 16)
+
+
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("hd", [16, 64, 128])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
 def test_attention_unseen_slots_do_not_matter(ops, hip_device, what, hd, types):

@@ -221,6 +221,23 @@ def test_attention_plans_cover_rows_and_keys(launches):
         assert ws == ((grid[2] * (128 + 2) + 1) * c["T"] * c["Hq"] * 4 if grid[2] > 1 else 0)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 5)])
+def test_attention_kernels_of_many_heads(launches, window, sinks):
+    """The GPU tests' shapes reach the kernels that they are there for."""
+    import re
+
+    types = {"f32": (0, 0), "f32_on_bf16": (0, 1), "bf16": (1, 1)}
+    cases, want = [], []
+    for seqs, heads, width, kernels in ref.MANY_HEADS:
+        for t, (xd, kd) in types.items():
+            cases.append(["attention", dict(T=sum(n for n, _ in seqs), S=len(seqs), Hq=heads, Hkv=heads, hd=64, page=16,
+                                            width=width, stride=width, xd=xd, kd=kd, window=window, sinks=sinks)])
+            want.append(kernels[t])
+    for (name, nt), (rc, _, kern, _, _) in zip(want, launches(cases)):
+        assert rc == 0 and f"attend_{name}_kernel" in kern[0][0]
+        assert name == "tiles" or int(re.findall(r"Li(\d+)E", kern[0][0])[1]) == nt
+
+
 def rows_of(kernel):
     """Rows of a workgroup, by the kernel's name and template arguments."""
     import re
