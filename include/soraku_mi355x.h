@@ -271,7 +271,8 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  *
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
  * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
- * exact.  hd: 16, 32, 64 or 128.  Hq: a multiple of Hkv, at most 4096; query
+ * exact; with BF16 activations a softmax weight enters its product with v with 16
+ * bits, rounded to nearest, whatever else is in the call.  hd: 16, 32, 64 or 128.  Hq: a multiple of Hkv, at most 4096; query
  * heads h G .. h G + G - 1 share key head h.  T may be 0 and is below 2^24; width *
  * page and T * Hq are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and
  * workspaces are 16-byte aligned; outputs overlap no operand.  No call allocates, waits or copies to the host, and each may

@@ -644,11 +644,12 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 //     lies in LDS row by row; the transposing LDS read gives a lane 4 keys of one dim.
 // FP32 activations: Q and P as three BF16 parts of 8 bits that add up to the FP32 value
 // exactly, three products each, so results are those of FP32 products (NP = 3).  BF16
-// activations: P rounds to BF16 once (2^-9 of a weight on average, under the output's own rounding).
+// activations: P keeps 16 bits, two parts (off by 2^-16 of a weight at most, 256 times less than the output's own
+// rounding; one part, off by 2^-8, adds as much again to it: 0.0023 of the output against 0.0017, for 269 us
+// in place of 353 below).
 //
-// 2,047 BF16 tokens over 16,384, 16 heads on 8 of 128: 265 us, 972 TFLOP/s (a large BF16 product reaches
-// 1,225 here).  The matrix cores are busy 59% of the time and the VALU (exponentials, maxima) 56%: two waves of a
-// SIMD hide only so much of one under the other.  LDS does not bound it (no bank conflicts); 16 x 16 x 32 took 310.
+// 2,047 BF16 tokens over 16,384, 16 heads on 8 of 128, with the join of its two cuts: 353 us, 1,098 TFLOP/s of the
+// three products per pair (a large BF16 product reaches 1,214 here): the matrix cores bound it.
 // 4,500 FP32 tokens with a window of 1,024: 168 us, 740 TFLOP/s of the three-part products, matrix cores 52%
 // busy: no registers are left to run a step's scores ahead.
 constexpr int KEYS = 64;                          // keys of a step
@@ -667,34 +668,37 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 // Eight FP32 values as NP BF16 fragments: cut to 8 bits, what is left cut again; the
-// third takes the rest exactly.  NP = 1 rounds to nearest.
+// third takes the rest exactly.  With two, the second is the rest rounded to nearest: off by 2^-16 of the value at most.
 template <int NP>
 __device__ __forceinline__ void parts8(const float* x, bf8* out) {
-  if constexpr (NP == 1) {
+  static_assert(NP == 2 || NP == 3, "parts of 8 bits");
+  float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[0][i] = (__bf16)x[i];
-  } else {
-    float r[8];
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i];
+  for (int p = 0; p < NP; ++p) {
+    if constexpr (NP == 2) {
+      if (p == 1) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      uint4 w;
-      uint32_t* u = &w.x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = __builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302);
-      out[p] = __builtin_bit_cast(bf8, w);
-      if (p + 1 < NP) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+        for (int i = 0; i < 8; ++i) out[1][i] = (__bf16)r[i];
+        return;
       }
+    }
+    uint4 w;
+    uint32_t* u = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302);
+    out[p] = __builtin_bit_cast(bf8, w);
+    if (p + 1 < NP) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
     }
   }
 }
 
 template <typename QT, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_tiles_kernel(AttendArgs a) {
-  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, KS = HD / 32, R = 128;
+  constexpr int NP = sizeof(QT) == 4 ? 3 : 1, PP = NP == 3 ? 3 : 2, KS = HD / 32, R = 128;   // parts of Q, of P
   constexpr int GROUP = TILE * HD * 2;            // bytes of 16 keys
   using L = TileLds<HD>;
   __shared__ __attribute__((aligned(1024))) char lds[4 * L::K];   // two slots of K, two of V
@@ -880,7 +884,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // tokens over 16,384, BF16: 287 -> 262 us; no change with three parts)
     if constexpr (AHEAD) __builtin_amdgcn_s_setprio(1);
     v16f s2[2];
-    bf8 pf[4][NP], vf[2][VU];                     // weights of the four sets of 16 keys
+    bf8 pf[4][PP], vf[2][VU];                     // weights of the four sets of 16 keys
     auto weights = [&](int g) {
       float y[8];
 #pragma unroll
@@ -888,17 +892,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         y[e] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][g % 2 * 8 + e], a.scale2, -m2));
         lr += y[e];                               // this lane's keys; a row's two lanes add up at the end
       }
-      parts8<NP>(y, pf[g]);
+      parts8<PP>(y, pf[g]);
       // formed here, under the products beside it
 #pragma unroll
-      for (int p = 0; p < NP; ++p) asm volatile("" : "+v"(pf[g][p]));
+      for (int p = 0; p < PP; ++p) asm volatile("" : "+v"(pf[g][p]));
       asm volatile("" : "+v"(lr));
     };
     auto values = [&](int q) {
 #pragma unroll
       for (int u = 0; u < VU; ++u)
 #pragma unroll
-        for (int p = NP - 1; p >= 0; --p)
+        for (int p = PP - 1; p >= 0; --p)
           o[q % VP * VU + u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[q % 2][u], pf[q / VP][p], o[q % VP * VU + u], 0, 0, 0);
     };
     auto rescale = [&]() {
