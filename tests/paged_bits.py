@@ -59,23 +59,25 @@ def low_queries(seqs, heads, hd, width=None, seed=0):
     return u, 2.0 ** 14 / math.sqrt(hd)
 
 
-def low_products(seqs, heads, hd, seed=0):
-    """FP32 queries and keys in groups of four dims (x, -x, -h, h) . (y, g, y, g) = (x - h)(y - g), h and g the first
-    8 bits of x and y: what is left of a score is the product of the low 16 bits of both sides."""
+def low_products(seqs, heads, hd, swap=False, seed=0):
+    """FP32 queries and keys whose scores are made of the products of one side's second part and the other's third.
+
+    Groups of four of the first 16 dims hold (256 + a, -256, -a, 0) . (k, k, 65792, 0) = a b with k = 65792 + b and a, b
+    0 or 1: the parts of k are 65536, 256 and b, those of 256 + a are 256 and a.  All other products of parts cancel as
+    they are added up (part by part, whole numbers up to 2^26), so a score is the number of groups with a = b = 1, exactly.
+    swap: keys and queries change places.  Returns the inputs and the scale."""
     u = Setup(seqs, *heads, hd, 16, torch.float32, torch.float32, seed=seed)
-    gen = torch.Generator().manual_seed(seed + 1)
+    g = torch.Generator().manual_seed(seed + 1)
 
-    def high(x):
-        return (x.view(torch.int32) & ~0xFFFF).view(torch.float32)
+    def bit(like):
+        return torch.randint(2, (*like.shape[:-1], 4), generator=g).float()
 
-    x = torch.rand(*u.q.shape[:-1], hd // 4, generator=gen) + 1.0
-    y = (torch.rand(*u.k.shape[:-1], hd // 4, generator=gen) + 1.0) * torch.where(
-        torch.rand(*u.k.shape[:-1], hd // 4, generator=gen) < 0.5, -1.0, 1.0)
-    h, g = high(x), high(y)
-    u.q = torch.stack((x, -x, -h, h), -1).flatten(-2)
-    u.k = torch.stack((y, g, y, g), -1).flatten(-2)
+    two, three = (u.k, u.q) if swap else (u.q, u.k)
+    a, k = bit(two), 65792.0 + bit(three)
+    two.zero_()[..., :16] = torch.stack((256.0 + a, torch.full_like(a, -256.0), -a, 0.0 * a), -1).flatten(-2)
+    three.zero_()[..., :16] = torch.stack((k, k, torch.full_like(k, 65792.0), 0.0 * k), -1).flatten(-2)
     u.mass.zero_()
-    return u, 2.0 ** 18 / math.sqrt(hd)
+    return u, 0.5
 
 
 def simulate(u, scale, window, q_parts, p_parts):
@@ -131,7 +133,7 @@ def simulate_mass(u, scale, lse, keep):
         n = int(u.lens[s])
         e, j = u.table[s, np.arange(n) // u.page], np.arange(n) % u.page
         for h in range(u.Hkv):
-            ks = [p[e, h, j] for p in cut(u.k.numpy(), 3)]
+            ks = [p[e, h, j] for p in cut(u.k.float().numpy(), 3)]
             for m in u.rows(s):
                 see = u.slot(s, m) + 1
                 for a in range(h * u.G, (h + 1) * u.G):
@@ -141,9 +143,9 @@ def simulate_mass(u, scale, lse, keep):
 
 
 def mass_bound(u, scale, lse):
-    """(exact accounts, how far one may be).  A score of hd / 16 sums of nine products each rounds once per
-    sum; exponents lose two steps and the exponential one; then one addition per term."""
+    """(exact accounts, how far one may be) with scores that are exact.  A weight: the score's scaling, the
+    difference from lse and the factor log2 e off by a step of the exponent each (3 A), the exponential (2); then one
+    addition per term."""
     want, terms = ref.mass(u, lse, scale)
-    S, _ = scores_of(u, scale, 0)
-    A = S + float(np.abs(lse).max())
-    return want, (S * 9 * u.hd / 16 + 3.0 * A + 2.0 + terms) * EPS * want
+    A = scores_of(u, scale, 0)[0] + float(np.abs(lse).max())
+    return want, (3.0 * A + 2.0 + terms) * EPS * want
