@@ -285,6 +285,7 @@ struct AttendArgs {
   float scale2;                                   // scale * log2 e: exp(s - m) = 2^(scale2 (qk - max qk))
   int window, sinks;                              // window 0: all keys
   int cut;                                        // tiles of keys per cut; cuts of a row: blockIdx.z
+  int last;                                       // the last row tile of the launch: the others follow down from it
   float* part; float* ml;                         // [cuts][T * Hq][hd], [cuts][T * Hq][2]: sums of V, (maximum times scale2, sum)
   int* count;                                     // [T * Hq]: a row's cuts to join (0: none), negative if it sees nothing
 };
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   TileAt tile;
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;   // the longest walks first
+  if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;   // the longest walks first
   const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
@@ -706,7 +707,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int h = blockIdx.x, cut = blockIdx.z;
   TileAt tile;
   // the last tiles of a sequence walk furthest: they start first
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;
+  if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;
   const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
@@ -1002,7 +1003,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if (wild) {
     __threadfence_block();                        // the stores above, by other lanes
     TileAt again;                                 // few registers are held for this through the loop
-    find_tile(c, R, gridDim.y - 1 - blockIdx.y, again);
+    find_tile(c, R, a.last - (int)blockIdx.y, again);
     const int q0 = again.len - again.n, t2 = again.tile * R, f_lo = t2 + wave * 32, f_hi = min(t2 + R, again.n * c.G);
     const int q_lo = q0 + t2 / c.G, q_hi = q0 + (f_hi - 1) / c.G;
     const Walk v = walk_of(q_lo, q_hi, a.window, a.sinks);
@@ -1048,7 +1049,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const Cache& c = a.c;
   const int h = blockIdx.x, cut = blockIdx.z;
   TileAt tile;
-  if (!find_tile(c, R, gridDim.y - 1 - blockIdx.y, tile)) return;   // the longest walks first
+  if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;   // the longest walks first
   const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
   const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);

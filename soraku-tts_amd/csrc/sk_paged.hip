@@ -18,6 +18,8 @@ using namespace sk::paged;
 
 namespace {
 
+constexpr int MOST = 65535;                       // of a grid's y and z
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // What every entry point asks of its sizes.
@@ -205,7 +207,6 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
   const Plan p = plan_attention(T, S, Hq, Hkv, hd, xdtype, kvdtype, page, width, window, sinks);
   SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= workspace_of(p, T, Hq, hd)), SK_EINVAL,
            "the workspace must hold %lld bytes", (long long)workspace_of(p, T, Hq, hd));
-  SK_CHECK(p.blocks <= 65535 && p.cuts <= 65535, SK_EINVAL, "too many rows for one call");
   AttendArgs a;
   a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, v_pages);
   a.q = q; a.out = out; a.lse = lse;
@@ -223,9 +224,8 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
       using X = decltype(x);
       using K = decltype(k);
       constexpr int HD = decltype(d)::value;
-      const dim3 grid(Hkv, p.blocks, p.cuts);
       // the kernels that share keys, with 16 NT rows and WK waves
-      auto share = [&](auto nt, auto wk) {
+      auto share = [&](dim3 grid, auto nt, auto wk) {
         constexpr int NT = decltype(nt)::value, WK = decltype(wk)::value;
         if constexpr (HD >= 32 && sizeof(K) == 2) {
           if constexpr (NT == 1 || sizeof(X) * HD <= 256)
@@ -234,16 +234,20 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
           hipLaunchKernelGGL((attend_rows_kernel<X, K, HD, NT, WK>), grid, dim3(64 * WK), 0, st, a);
         }
       };
-      if (p.tiles) {
-        if constexpr (HD >= 32 && sizeof(K) == 2)
-          hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
-      } else if (p.R == 32) {
-        share(Int<2>{}, Int<4>{});
-      } else {
-        if (p.WK == 8) share(Int<1>{}, Int<8>{});
-        else share(Int<1>{}, Int<4>{});
+      // as many row tiles per launch as a grid takes
+      for (a.last = p.blocks - 1; a.last >= 0 && err == hipSuccess; a.last -= MOST) {
+        const dim3 grid(Hkv, std::min(a.last + 1, MOST), p.cuts);
+        if (p.tiles) {
+          if constexpr (HD >= 32 && sizeof(K) == 2)
+            hipLaunchKernelGGL((attend_tiles_kernel<X, HD>), grid, dim3(256), 0, st, a);
+        } else if (p.R == 32) {
+          share(grid, Int<2>{}, Int<4>{});
+        } else {
+          if (p.WK == 8) share(grid, Int<1>{}, Int<8>{});
+          else share(grid, Int<1>{}, Int<4>{});
+        }
+        err = hipGetLastError();
       }
-      err = hipGetLastError();
       if (p.cuts == 1 || err != hipSuccess) return;
       // 4 waves per row where there are few rows with many cuts to go through
       if (p.cuts > 16) hipLaunchKernelGGL((combine_kernel<X, HD, 4>), dim3(T * Hq), dim3(256), 0, st, a, p.cuts);

@@ -241,6 +241,39 @@ def test_attention_table_slices_and_streams(ops, hip_device):
     assert torch.equal(base, out)
 
 
+@pytest.mark.parametrize("types,hd,T", [("f32", 16, 65535 * 32 + 2000), ("bf16", 32, 65535 * 128 + 3000)])
+def test_attention_of_millions_of_rows(ops, hip_device, types, hd, T):
+    """A prompt of more row tiles than a grid takes, with a window: its ends, where launches meet, and
+    rows between."""
+    xd, kd = TYPES[types]
+    window, page = 20, 4096
+    n = -(-T // page)
+    g = torch.Generator(device=hip_device).manual_seed(17)
+    k, v = (torch.randn(n, 1, page, hd, device=hip_device, generator=g).to(kd) for _ in range(2))
+    q = torch.randn(T, 1, hd, device=hip_device, generator=g).to(xd)
+    i32 = dict(dtype=torch.int32, device=hip_device)
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(18)).to(**i32)[None].contiguous()
+    out = torch.full_like(q, float("nan"))
+    lse = torch.full((T, 1), float("nan"), device=hip_device)
+    ops.paged_attention(1, 1, hd, page, None, window)(q, k, v, table, torch.tensor([0, T], **i32), torch.tensor([T], **i32),
+                                                      out=out, lse=lse)
+    assert out.isfinite().all() and lse.isfinite().all()
+    p = torch.cat([torch.arange(3000), T - 1 - torch.arange(5000), torch.randint(T, (5000,), generator=torch.Generator().manual_seed(19))])
+    p = p.to(hip_device)
+    j = p[:, None] - torch.arange(window, device=hip_device)
+    e = table[0, j.clamp_min(0) // page].long()
+    kk, vv = (x[e, 0, j.clamp_min(0) % page].double() for x in (k, v))
+    x = (kk * q[p].double()).sum(-1) * hd ** -0.5
+    x = x.masked_fill(j < 0, -np.inf)
+    want = (torch.softmax(x, -1)[..., None] * vv).sum(1)
+    wl = torch.logsumexp(x, -1)
+    # scores of at most 30, sums of hd products and 20 keys; 16-bit weights and the output's rounding
+    fine = (2.0 * (hd + 8) * 31.0 + 40.0) * 2.0 ** -24 + (2.0 ** -16 if xd == BF16 else 0.0)
+    top = vv.abs().amax(1)
+    assert ((out[p, 0].double() - want).abs() <= fine * top + HALF_STEP[xd] * (want.abs() + fine * top)).all()
+    assert ((lse[p, 0].double() - wl).abs() <= (2.0 * (hd + 8) * 31.0 + 40.0) * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("types", TYPES)
 def test_attention_graphs(ops, hip_device, types):
     """Two captured calls with workspaces, replayed in turn with eager calls

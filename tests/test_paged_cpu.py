@@ -221,6 +221,18 @@ def test_attention_plans_cover_rows_and_keys(launches):
         assert ws == ((grid[2] * (128 + 2) + 1) * c["T"] * c["Hq"] * 4 if grid[2] > 1 else 0)
 
 
+@pytest.mark.parametrize("change", [dict(T=2 ** 21 + 5, hd=16, kd=0), dict(T=2 ** 24 - 1, hd=16, kd=0), dict(T=2 ** 23 + 77, hd=32, xd=1),
+                                    dict(T=2 ** 24 - 1, S=40, hd=64), dict(T=65535 * 32, hd=16, kd=0)])
+def test_attention_of_millions_of_rows(launches, change):
+    """Row tiles past what a grid takes go into further launches; none is left out."""
+    (rc, calls, kern, ws, _), = launches([["attention", dict(dict(Hq=1, Hkv=1, S=1, width=10, stride=10, page=2 ** 20), **change)]])
+    assert rc == 0 and ws == 0
+    R = {rows_of(name) for name, _ in kern}
+    assert len(R) == 1 and all(grid[0] == grid[2] == 1 and 0 < grid[1] <= 65535 for _, grid in kern)
+    assert sum(grid[1] for _, grid in kern) * R.pop() >= change["T"]
+    assert all(grid[1] == 65535 for _, grid in kern[:-1])
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (30, 5)])
 def test_attention_kernels_of_many_heads(launches, window, sinks):
     """The GPU tests' shapes reach the kernels that they are there for."""
