@@ -272,11 +272,12 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
  * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
  * exact; with BF16 activations a softmax weight enters its product with v with 16
- * bits, rounded to nearest, whatever else is in the call.  hd: 16, 32, 64 or 128.  Hq: a multiple of Hkv, at most 4096; query
- * heads h G .. h G + G - 1 share key head h.  T may be 0 and is below 2^24; width *
- * page and T * Hq are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and
- * workspaces are 16-byte aligned; outputs overlap no operand.  No call allocates, waits or copies to the host, and each may
- * be captured into a graph. */
+ * bits, rounded to nearest, whatever else is in the call.  hd: 16, 32, 64 or 128.
+ * Hq: a multiple of Hkv, at most 4096; query heads h G .. h G + G - 1 share key head
+ * h.  S is at most 65535; T may be 0 and is below 2^24; width * page and T * Hq are
+ * at most 2^30.  q, qkv, gains, pages, outputs of xdtype and workspaces are 16-byte
+ * aligned; outputs overlap no operand.  No call allocates, waits or copies to the
+ * host, and each may be captured into a graph. */
 
 /* New tokens into the cache: qkv [T][(Hq + 2 Hkv) hd] as projected.  q and k are
  * normalised per head (RMSNorm with gains [hd]; both NULL: not) and rotated by
@@ -313,7 +314,8 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
  * [n_pages][Hkv][page].  q, lse, scale, window and sinks as in the attention call.
  * The order of sums is fixed.  Two sequences of one call that both have new tokens
  * must not share a page: each would add to accounts that the other adds to.
- * Workspace as for attention. */
+ * width * page is at most 65535 * 256 over BF16 caches with hd of 32 or more, 65535 *
+ * 128 otherwise.  Workspace as for attention. */
 int sk_op_paged_attention_mass_workspace(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd,
                                          int32_t page, int32_t width, int32_t xdtype, int32_t kvdtype,
                                          int64_t* bytes);
@@ -329,7 +331,7 @@ int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, i
  * accounts, to slots 0 .. n - 1 of the pages `to` [S][to_width] (rows to_stride
  * apart).  A page of `to` appears there once and not in `table`: old pages, which
  * other sequences may share as they share a prompt, are only read.  new_lens [S],
- * and kept [S][Hkv][keep] the old slots, -1 past n. */
+ * and kept [S][Hkv][keep] the old slots, -1 past n; S * Hkv * keep is below 2^31. */
 int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages,
                       int32_t width, int64_t table_stride, int32_t kvdtype, int32_t keep, int32_t sinks,
                       int32_t recent, void* k_pages, void* v_pages, float* mass, const int32_t* table,

@@ -25,7 +25,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // What every entry point asks of its sizes.
 int check_sizes(int32_t T, int32_t S, int32_t Hq, int32_t Hkv, int32_t hd, int32_t page, int32_t n_pages, int32_t width,
                 int64_t stride) {
-  SK_CHECK(T >= 0 && T < 1 << 24 && S > 0, SK_EINVAL, "T must be in [0, 2^24) and S positive");
+  // a row or tile finds its sequence by a pass over all S: more of them belong in several calls
+  SK_CHECK(T >= 0 && T < 1 << 24 && S > 0 && S <= MOST, SK_EINVAL, "T must be in [0, 2^24) and S in [1, %d]", MOST);
   SK_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 4096, SK_EINVAL,
            "Hq must be a positive multiple of Hkv, at most 4096");
   SK_CHECK(hd == 16 || hd == 32 || hd == 64 || hd == 128, SK_EINVAL, "hd must be a power of two in [16, 128]");
@@ -139,6 +140,11 @@ MassPlan plan_mass(int T, int S, int Hq, int Hkv, int hd, int kvdtype, int page,
   p.cut = (int)std::max<int64_t>(32, ((rows + cuts - 1) / cuts + 31) / 32 * 32);
   p.cuts = (int)std::max<int64_t>(1, (rows + p.cut - 1) / p.cut);
   return p;
+}
+int check_mass(const MassPlan& p, int S) {
+  SK_CHECK(p.blocks <= MOST && (int64_t)S * p.cuts <= MOST, SK_EINVAL, "width * page must be at most %lld for accounts",
+           (long long)MOST * p.keys);
+  return SK_OK;
 }
 int64_t workspace_of(const MassPlan& p, int S, int Hkv, int page, int width) {
   return p.cuts > 1 ? (int64_t)p.cuts * S * Hkv * page * width * 4 : 0;
@@ -264,7 +270,9 @@ int sk_op_paged_attention_mass_workspace(int32_t T, int32_t S, int32_t Hq, int32
   if (int rc = check_sizes(T, S, Hq, Hkv, hd, page, 1, width, width)) return rc;
   if (int rc = check_types(xdtype, kvdtype)) return rc;
   SK_CHECK(bytes, SK_EINVAL, "NULL operand");
-  *bytes = workspace_of(plan_mass(T, S, Hq, Hkv, hd, kvdtype, page, width), S, Hkv, page, width);
+  const MassPlan p = plan_mass(T, S, Hq, Hkv, hd, kvdtype, page, width);
+  if (int rc = check_mass(p, S)) return rc;
+  *bytes = workspace_of(p, S, Hkv, page, width);
   return SK_OK;
 }
 
@@ -280,10 +288,10 @@ int sk_op_paged_attention_mass(void* stream, int32_t T, int32_t S, int32_t Hq, i
   SK_CHECK(q && lse && k_pages && table && starts && lens && mass, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(q) && aligned16(k_pages) && aligned16(workspace), SK_EINVAL, "operands must be 16-byte aligned");
   const MassPlan p = plan_mass(T, S, Hq, Hkv, hd, kvdtype, page, width);
+  if (int rc = check_mass(p, S)) return rc;
   const int64_t need = workspace_of(p, S, Hkv, page, width);
   SK_CHECK(p.cuts == 1 || (workspace && workspace_bytes >= need), SK_EINVAL, "the workspace must hold %lld bytes",
            (long long)need);
-  SK_CHECK(p.blocks <= 65535 && (int64_t)S * p.cuts <= 65535, SK_EINVAL, "too many keys or sequences for one call");
   MassArgs a;
   a.c = cache_of(T, S, Hq, Hkv, page, n_pages, width, table_stride, starts, lens, table, k_pages, nullptr);
   a.q = q; a.lse = lse; a.mass = mass;
@@ -330,8 +338,7 @@ int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t 
            "keep must be positive, sinks and recent not negative, and their sum at most keep");
   SK_CHECK(to_width > 0 && to_stride >= to_width && (int64_t)to_width * page >= keep, SK_EINVAL,
            "the new table must have pages for keep tokens");
-  SK_CHECK(S <= 65535 && Hkv <= 65535 && (int64_t)S * Hkv * keep <= INT32_MAX, SK_EINVAL,
-           "S must be at most 65535 and S * Hkv * keep at most 2^31");
+  SK_CHECK((int64_t)S * Hkv * keep <= INT32_MAX, SK_EINVAL, "S * Hkv * keep must be below 2^31");
   SK_CHECK(k_pages && v_pages && mass && table && lens && to && new_lens && kept, SK_EINVAL, "NULL operand");
   SK_CHECK(table != to, SK_EINVAL, "the new table must have pages of its own");
   SK_CHECK(lens != new_lens, SK_EINVAL, "new_lens must not be lens");

@@ -221,6 +221,22 @@ def test_attention_plans_cover_rows_and_keys(launches):
         assert ws == ((grid[2] * (128 + 2) + 1) * c["T"] * c["Hq"] * 4 if grid[2] > 1 else 0)
 
 
+@pytest.mark.parametrize("entry", ["append", "attention", "mass", "evict"])
+def test_most_sequences(L, launches, entry):
+    """65,535 sequences run, more are refused, by the workspace queries too."""
+    from soraku_amd._lib import SK_EINVAL, SK_OK
+
+    (rc, *_), = launches([[entry, {"S": 65535, **({} if entry == "evict" else {"T": 65535})}]])
+    assert rc == SK_OK
+    name, good = ENTRY[entry]
+    for S in (65536, 2 ** 31 - 1):
+        assert getattr(L, name)(*dict(good, S=S).values()) == SK_EINVAL
+        assert "S in [1, 65535]" in L.sk_last_error().decode()
+    n = C.c_int64()
+    assert L.sk_op_paged_attention_workspace(3, 65536, 16, 8, 128, 16, 4, 0, 1, 0, 0, C.byref(n)) == SK_EINVAL
+    assert L.sk_op_paged_attention_mass_workspace(3, 65536, 16, 8, 128, 16, 4, 0, 1, C.byref(n)) == SK_EINVAL
+
+
 @pytest.mark.parametrize("change", [dict(T=2 ** 21 + 5, hd=16, kd=0), dict(T=2 ** 24 - 1, hd=16, kd=0), dict(T=2 ** 23 + 77, hd=32, xd=1),
                                     dict(T=2 ** 24 - 1, S=40, hd=64), dict(T=65535 * 32, hd=16, kd=0)])
 def test_attention_of_millions_of_rows(launches, change):
@@ -231,6 +247,22 @@ def test_attention_of_millions_of_rows(launches, change):
     assert len(R) == 1 and all(grid[0] == grid[2] == 1 and 0 < grid[1] <= 65535 for _, grid in kern)
     assert sum(grid[1] for _, grid in kern) * R.pop() >= change["T"]
     assert all(grid[1] == 65535 for _, grid in kern[:-1])
+
+
+@pytest.mark.parametrize("hd,kd,keys", [(16, 1, 128), (128, 0, 128), (128, 1, 256)])
+def test_most_slots_of_accounts(L, launches, hd, kd, keys):
+    """The limit that the header gives: refused past it, by the workspace query as by the call."""
+    from soraku_amd._lib import SK_EINVAL, SK_OK
+
+    width = 65535 * keys // 16
+    base = dict(hd=hd, kd=kd, width=width, stride=width)
+    (rc, _, kern, _, _), = launches([["mass", base]])
+    assert rc == SK_OK and kern[0][1][1] == 65535
+    n = C.c_int64()
+    assert L.sk_op_paged_attention_mass(*dict(MASS, **dict(base, width=width + 1, stride=width + 1)).values()) == SK_EINVAL
+    assert str(65535 * keys) in L.sk_last_error().decode()
+    assert L.sk_op_paged_attention_mass_workspace(3, 2, 16, 8, hd, 16, width + 1, 0, kd, C.byref(n)) == SK_EINVAL
+    assert L.sk_op_paged_attention_mass_workspace(3, 2, 16, 8, hd, 16, width, 0, kd, C.byref(n)) == SK_OK
 
 
 @pytest.mark.parametrize("window,sinks", [(0, 0), (30, 5)])
