@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 
 from . import _lib
 from ._lib import check, lib
@@ -180,11 +181,21 @@ def _need(t, name, dtype, at, shape):
     return t.data_ptr()
 
 
+def _int32(**sizes):
+    """The sizes; a foreign call would cut them down to their lowest 32 bits."""
+    for name, n in sizes.items():
+        if operator.index(n) >> 31 not in (0, -1):
+            raise ValueError(f"{name} must be a 32-bit integer, got {n}")
+    return map(operator.index, sizes.values())
+
+
 def _table(t, name, dtype, at, S):
     """(address, row stride, entries per row) of a page table."""
     if t.dtype is not dtype or t.get_device() != at or t.dim() != 2 or t.shape[0] != S:
         raise ValueError(f"{name} must be an int32 tensor [{S}, pages] on HIP device {at}")
     width, (stride, step) = t.shape[1], t.stride()
+    if (S | width) >> 31:
+        raise ValueError(f"{name} must be smaller than 2^31 x 2^31")
     if (width > 1 and step != 1) or (S > 1 and stride < width):
         raise ValueError(f"{name}'s rows must be contiguous and apart")
     return t.data_ptr(), stride if S > 1 else width, width
@@ -205,6 +216,8 @@ def _pool(k_pages, v_pages, Hkv, page, hd, codes):
 def _code(t, codes):
     if t.dtype not in codes:
         raise ValueError(f"dtype {t.dtype} not supported (float32 or bfloat16)")
+    if t.shape[0] >> 31:
+        raise ValueError("too many tokens")
     return codes[t.dtype]
 
 
@@ -236,6 +249,8 @@ def paged_append(Hq: int, Hkv: int, hd: int, page: int, eps: float):
     both None for none), rotation by ``positions * inv_freq``, k and v to
     their slots; returns q ``[T, Hq, hd]`` of qkv's dtype (``out``, if given).
     ``mass`` (accounts, ``[n_pages, Hkv, page]`` float32) is set to 0 at the new slots."""
+    Hq, Hkv, hd, page = _int32(Hq=Hq, Hkv=Hkv, hd=hd, page=page)
+
     def kernel(qkv, q_gain, k_gain, inv_freq, positions, starts, lens, table, k_pages, v_pages, mass=None, out=None):
         T = _torch()
         f32, i32 = T.f32, T.i32
@@ -262,6 +277,7 @@ def paged_attention(Hq: int, Hkv: int, hd: int, page: int, scale: float | None =
     sequences' slots, causal; with a ``window`` only the last ``window`` slots and the
     first ``sinks``.  ``scale`` defaults to hd ** -0.5.  ``lse`` ``[T, Hq]`` float32,
     if given, receives the softmax's logarithms.  Tokens that see nothing give 0 and -inf."""
+    Hq, Hkv, hd, page, window, sinks = _int32(Hq=Hq, Hkv=Hkv, hd=hd, page=page, window=window, sinks=sinks)
     scale = hd ** -0.5 if scale is None else float(scale)
 
     def kernel(q, k_pages, v_pages, table, starts, lens, out=None, lse=None):
@@ -288,6 +304,7 @@ def paged_attention_mass(Hq: int, Hkv: int, hd: int, page: int, scale: float | N
     """Adds the weight every slot got in the ``paged_attention`` call of the same
     arguments (its ``q`` and ``lse``) to ``mass`` ``[n_pages, Hkv, page]`` float32, summed over
     tokens and the query heads that share a key head; returns ``mass``."""
+    Hq, Hkv, hd, page, window, sinks = _int32(Hq=Hq, Hkv=Hkv, hd=hd, page=page, window=window, sinks=sinks)
     scale = hd ** -0.5 if scale is None else float(scale)
 
     def kernel(q, lse, k_pages, table, starts, lens, mass):
@@ -311,6 +328,8 @@ def paged_evict(Hkv: int, hd: int, page: int, keep: int, sinks: int = 0, recent:
     ``recent``, and of the others those of the largest accounts (ties to the lowest slot) move in
     order, with their accounts, to the pages of ``to`` ``[S, pages]``, none of which may be in ``table``.
     Returns the new lengths ``[S]`` and the old slots ``[S, Hkv, keep]`` (-1 past the length), int32."""
+    Hkv, hd, page, keep, sinks, recent = _int32(Hkv=Hkv, hd=hd, page=page, keep=keep, sinks=sinks, recent=recent)
+
     def kernel(k_pages, v_pages, mass, table, lens, to):
         T = _torch()
         i32 = T.i32

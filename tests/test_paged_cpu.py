@@ -129,6 +129,28 @@ def test_python_refusals():
         ops._code(torch.zeros(1, dtype=torch.float16), {torch.float32: 0})
 
 
+@pytest.mark.parametrize("big", [2 ** 31, 2 ** 32, 2 ** 32 + 64, -2 ** 32])
+def test_python_refuses_sizes_past_32_bits(big):
+    """A foreign call would take 2^32 for 0 (a window that lets every slot be seen) and 2^32 + 64 for 64."""
+    from soraku_amd import ops
+
+    makers = {ops.paged_append: dict(Hq=4, Hkv=2, hd=16, page=16, eps=1e-6),
+              ops.paged_attention: dict(Hq=4, Hkv=2, hd=16, page=16, window=8, sinks=2),
+              ops.paged_attention_mass: dict(Hq=4, Hkv=2, hd=16, page=16, window=8, sinks=2),
+              ops.paged_evict: dict(Hkv=2, hd=16, page=16, keep=16, sinks=2, recent=3)}
+    for make, good in makers.items():
+        assert callable(make(**good)) and callable(make(**{k: v if k == "eps" else np.int64(v) for k, v in good.items()}))
+        for name in good:
+            if name != "eps":
+                with pytest.raises(ValueError, match=f"{name} must be a 32-bit integer"):
+                    make(**dict(good, **{name: big}))
+    if big > 0:
+        with pytest.raises(ValueError, match="2.31"):
+            ops._table(torch.empty(1, big, dtype=torch.int32, device="meta"), "table", torch.int32, -1, 1)
+        with pytest.raises(ValueError, match="tokens"):
+            ops._code(torch.empty(big, 1, device="meta"), {torch.float32: 0})
+
+
 # ------------------------------------------------------------------ launches (stand-in HIP runtime)
 
 SCRIPT = '''
