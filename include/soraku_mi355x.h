@@ -267,7 +267,9 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * outside [0, n_pages) is no page: append drops what would go there, tokens
  * that see a key there come out of attention as NaN, accounts there are not
  * kept, eviction moves NaN from it and nothing to it.  Entries of pages that no
- * token sees may be anything.
+ * token sees may be anything.  A sequence with a length past its table has no place
+ * for its tokens: append stores none of them, they come out of attention as NaN, its
+ * accounts stay as they are; eviction goes by the slots that the table has.
  *
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
  * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
@@ -311,7 +313,8 @@ int sk_op_paged_attention(void* stream, int32_t T, int32_t S, int32_t Hq, int32_
                           void* out, float* lse, void* workspace, int64_t workspace_bytes);
 /* Adds the attention weight that every slot got from the new tokens, exp(scale q k
  * - lse) summed over tokens and the group's heads, to its account in mass
- * [n_pages][Hkv][page].  q, lse, scale, window and sinks as in the attention call.
+ * [n_pages][Hkv][page].  q, lse, scale, window and sinks as in the attention call
+ * (a token whose lse is NaN makes NaN of the accounts that it sees).
  * The order of sums is fixed.  Two sequences of one call that both have new tokens
  * must not share a page: each would add to accounts that the other adds to.
  * width * page is at most 65535 * 256 over BF16 caches with hd of 32 or more, 65535 *

@@ -12,7 +12,8 @@
 // starts, lens and table are device memory that the host does not look at, so the
 // kernels hold them in range: starts to [0, T] and not falling, lens to [0,
 // width * page], and an entry outside the pool reads page 0 with its keys counted as
-// NaN, so that rows that see it come out as NaN.
+// NaN, so that rows that see it come out as NaN.  A sequence whose length is past its table has
+// no place for all of its tokens: none is stored, and all of its pages count as outside the pool.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -134,6 +135,7 @@ __device__ __forceinline__ int page_of(const Cache& c, int j) {
   return (int)(__umulhi((uint32_t)j, c.page_mul) >> (c.page_shift - 32));
 }
 __device__ __forceinline__ int seq_len(const Cache& c, int s) { return min(max(c.lens[s], 0), c.width * c.page); }
+__device__ __forceinline__ bool too_long(const Cache& c, int s) { return c.lens[s] > c.width * c.page; }
 
 // The sequence that row m belongs to (wave-uniform; S if none): the last one that starts at or before it.
 __device__ __forceinline__ int seq_of_row(const Cache& c, int m) {
@@ -158,10 +160,12 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // Tile x of all sequences' tiles of R (token, head of the group) rows: its sequence, its number
-// there, and the sequence's first row, new tokens and length; false past the last.
+// there, the sequence's first row, new tokens and the slot of the first (slot), and the pool's pages that count
+// (none for a length past the table, whose tokens take the last slots, all of them seen); false past the last.
 // Every lane brings one sequence's numbers, in one trip to memory.
 struct TileAt {
-  int seq, tile, first, n, len;
+  int seq, tile, first, n, p0, n_pages;
+  __device__ __forceinline__ int slot(const Cache& c, int tok) const { return min(p0 + tok, c.width * c.page - 1); }
 };
 __device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, TileAt& at) {
   const int lane = threadIdx.x & 63;
@@ -170,15 +174,18 @@ __device__ __forceinline__ bool find_tile(const Cache& c, int R, int x, TileAt& 
     const int s = min(s0 + lane, c.S - 1);
     int first, n;
     seq_rows(c, s, first, n);
-    const int len = seq_len(c, s), t = s0 + lane < c.S ? (n * c.G + R - 1) / R : 0, sum = wave_scan(t);
-    const uint64_t past = __ballot(base + sum > x);
+    const bool over = too_long(c, s);
+    const int p0 = over ? max(c.width * c.page - n, 0) : seq_len(c, s) - n;
+    const int t = s0 + lane < c.S ? (n * c.G + R - 1) / R : 0, sum = wave_scan(t);
+    const uint64_t past = __ballot(base + sum > x), none = __ballot(over);
     if (past) {
       const int l = __builtin_ctzll(past);
       at.seq = s0 + l;
       at.tile = x - base - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(t, l));
       at.first = __builtin_amdgcn_readlane(first, l);
       at.n = __builtin_amdgcn_readlane(n, l);
-      at.len = __builtin_amdgcn_readlane(len, l);
+      at.p0 = __builtin_amdgcn_readlane(p0, l);
+      at.n_pages = none >> l & 1 ? 0 : c.n_pages;
       return true;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, const XT* qkv, con
   int at = -1;                                    // the slot's page, if it has one
   const int pg = page_of(c, max(slot, 0));
   if (slot >= 0 && m - first < n) at = c.table[s * c.stride + pg];
-  const bool live = at >= 0 && at < c.n_pages;
+  const bool live = at >= 0 && at < c.n_pages && !too_long(c, s);
   const size_t base = live ? (size_t)at * c.Hkv * c.page + (slot - pg * c.page) : 0;   // in rows of hd, for head 0
   __syncthreads();
   float2 t4[4];
@@ -323,12 +330,12 @@ struct TileOffsets {
   uint32_t lo, hi;
   uint64_t bad;                                   // lanes whose page is not in the pool
   // tiles t0, t0 + step ..; as pairs: t0, t0 + 1, t0 + step, t0 + step + 1 ..
-  __device__ __forceinline__ void load(const Cache& c, const int* table, const Walk& w, int t0, int step, int end, int h,
-                                       int hd, bool pairs = false) {
+  __device__ __forceinline__ void load(const Cache& c, int n_pages, const int* table, const Walk& w, int t0, int step,
+                                       int end, int h, int hd, bool pairs = false) {
     const int l = threadIdx.x & 63, t = min(t0 + (pairs ? (l >> 1) * step + (l & 1) : l * step), end - 1);
     const int j = w.tile(t) * TILE, pg = page_of(c, j);
     const int e = table[pg];
-    const bool ok = e >= 0 && e < c.n_pages;
+    const bool ok = e >= 0 && e < n_pages;
     const size_t off = (((size_t)(ok ? e : 0) * c.Hkv + h) * c.page + (j - pg * c.page)) * hd;
     lo = (uint32_t)off;
     hi = (uint32_t)(off >> 32);
@@ -489,8 +496,8 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int h = blockIdx.x, cut = blockIdx.z;
   TileAt tile;
   if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;   // the longest walks first
-  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
-  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.p0, rows = n * c.G, f0 = tile.tile * R;
+  const int p_lo = tile.slot(c, f0 / c.G), p_hi = tile.slot(c, (min(f0 + R, rows) - 1) / c.G);
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int end = min(w.n, (cut + 1) * a.cut);
   if (cut > 0 && cut * a.cut >= w.n) return;      // the first cut also answers for rows that see nothing
@@ -505,7 +512,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int f = min(f0 + j * 16 + i16, rows - 1), tok = f / c.G;
-    qp[j] = p0 + tok;
+    qp[j] = tile.slot(c, tok);
     const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
 #pragma unroll
     for (int t = 0; t < NK; ++t) {
@@ -543,7 +550,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int t_first = cut * a.cut + wave;
   bool wild = false;                              // infinities or NaN in V beside a mask
   if (t_first < end) {
-    offs.load(c, table, w, t_first, WK, end, h, HD);
+    offs.load(c, tile.n_pages, table, w, t_first, WK, end, h, HD);
     load_k(offs.at(0));
   }
   int i = 0;                                      // the tile's lane in offs
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       }
     if (++i == 64 && t + WK < end) {
       i = 0;
-      offs.load(c, table, w, t + WK, WK, end, h, HD);
+      offs.load(c, tile.n_pages, table, w, t + WK, WK, end, h, HD);
     }
     load_k(offs.at(min(i, 63)));                  // the last tile again after the last: a load without a branch
     const int k0 = w.tile(t) * TILE;
@@ -708,8 +715,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   TileAt tile;
   // the last tiles of a sequence walk furthest: they start first
   if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;
-  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
-  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.p0, rows = n * c.G, f0 = tile.tile * R;
+  const int p_lo = tile.slot(c, f0 / c.G), p_hi = tile.slot(c, (min(f0 + R, rows) - 1) / c.G);
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int begin = cut * a.cut, end = min(w.n, begin + a.cut);
   if (cut > 0 && begin >= w.n) return;            // the first cut also answers for rows that see nothing
@@ -721,7 +728,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   bf8 qf[NP][2 * KS];
   {
     const int f = min(f0 + wave * 32 + i32, rows - 1), tok = f / c.G;
-    qp = p0 + tok;
+    qp = tile.slot(c, tok);
     const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
 #pragma unroll
     for (int k = 0; k < 2 * KS; ++k) {
@@ -759,7 +766,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   size_t v_off = 0;                               // where V of the step after lies
   auto place = [&](int t) -> int {                // the step whose first tile is t; gives which of its tiles have no page
     if (at == 64) at = 0;
-    if (at == 0) offs.load(c, table, w, t, 1, end, h, HD);
+    if (at == 0) offs.load(c, tile.n_pages, table, w, t, 1, end, h, HD);
     v_off = offs.at(at + wave) * 2;
     const int none = offs.bad >> at & 15;
     at += 4;
@@ -1004,13 +1011,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __threadfence_block();                        // the stores above, by other lanes
     TileAt again;                                 // few registers are held for this through the loop
     find_tile(c, R, a.last - (int)blockIdx.y, again);
-    const int q0 = again.len - again.n, t2 = again.tile * R, f_lo = t2 + wave * 32, f_hi = min(t2 + R, again.n * c.G);
-    const int q_lo = q0 + t2 / c.G, q_hi = q0 + (f_hi - 1) / c.G;
+    const int t2 = again.tile * R, f_lo = t2 + wave * 32, f_hi = min(t2 + R, again.n * c.G);
+    const int q_lo = again.slot(c, t2 / c.G), q_hi = again.slot(c, (f_hi - 1) / c.G);
     const Walk v = walk_of(q_lo, q_hi, a.window, a.sinks);
     const int b2 = blockIdx.z * a.cut, e2 = min(v.n, b2 + a.cut);
     const int* tab = c.table + again.seq * c.stride;
     add_wild<QT, uint16_t, HD>(
-        a, h, tab, again.first, q0, f_lo, min(f_lo + 32, f_hi), v, b2, e2,
+        a, h, tab, again.first, again.p0, f_lo, min(f_lo + 32, f_hi), v, b2, e2,
         v.n <= a.cut ? nullptr : a.part + (size_t)blockIdx.z * c.T * c.Hq * HD,
         [&](int t) {
           const int t0 = b2 + (t - b2) / 4 * 4, t3 = min(t0 + 3, e2 - 1);
@@ -1050,8 +1057,8 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int h = blockIdx.x, cut = blockIdx.z;
   TileAt tile;
   if (!find_tile(c, R, a.last - (int)blockIdx.y, tile)) return;   // the longest walks first
-  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.len - n, rows = n * c.G, f0 = tile.tile * R;
-  const int p_lo = p0 + f0 / c.G, p_hi = p0 + (min(f0 + R, rows) - 1) / c.G;
+  const int seq = tile.seq, first = tile.first, n = tile.n, p0 = tile.p0, rows = n * c.G, f0 = tile.tile * R;
+  const int p_lo = tile.slot(c, f0 / c.G), p_hi = tile.slot(c, (min(f0 + R, rows) - 1) / c.G);
   const Walk w = walk_of(p_lo, p_hi, a.window, a.sinks);
   const int end = min(w.n, (cut + 1) * a.cut);
   if (cut > 0 && cut * a.cut >= w.n) return;      // the first cut also answers for rows that see nothing
@@ -1061,7 +1068,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
   const int t_first = cut * a.cut + 2 * wave;     // the wave's tiles: two of every 2 WK
   TileOffsets offs;
-  if (t_first < end) offs.load(c, table, w, t_first, 2 * WK, end, h, HD, true);
+  if (t_first < end) offs.load(c, tile.n_pages, table, w, t_first, 2 * WK, end, h, HD, true);
   const unsigned koff = i16 * HD + q4 * 8;        // elements
   const int vrow = lane / (HD / 8);
   const unsigned voff = (vrow * HD + (lane % (HD / 8) ^ 2 * L::turn16(vrow)) * 8) * 2;
@@ -1086,7 +1093,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int f = min(f0 + j * 16 + i16, rows - 1), tok = f / c.G;
-    qp[j] = p0 + tok;
+    qp[j] = tile.slot(c, tok);
     const QT* qr = static_cast<const QT*>(a.q) + ((size_t)(first + tok) * c.Hq + h * c.G + (f - tok * c.G)) * HD;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -1128,7 +1135,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (t + 2 * WK < end) {
       if (i == 64) {
         i = 0;
-        offs.load(c, table, w, t + 2 * WK, 2 * WK, end, h, HD, true);
+        offs.load(c, tile.n_pages, table, w, t + 2 * WK, 2 * WK, end, h, HD, true);
       }
       load(i, slot ^ 1, other);
     }
@@ -1328,7 +1335,7 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   seq_rows(c, seq, first, n);
   const int len = seq_len(c, seq), p0 = len - n;
   const int k0 = (blockIdx.y * 4 + wave) * NK2 * TILE;
-  if (n == 0 || k0 >= len) return;
+  if (n == 0 || k0 >= len || too_long(c, seq)) return;
   const int* table = c.table + seq * c.stride;
   const KT* kp = static_cast<const KT*>(c.k);
   float kf[NK2][NK * KW], sum[NK2];
@@ -1420,7 +1427,7 @@ __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {
   seq_rows(c, seq, first, n);
   const int len = seq_len(c, seq), p0 = len - n, rows = n * c.G;
   const int b0 = blockIdx.y * 4 * KEYS, k0 = b0 + wave * KEYS;   // first keys of the workgroup, of the wave
-  if (n == 0 || b0 >= len) return;
+  if (n == 0 || b0 >= len || too_long(c, seq)) return;
   int f_lo, f_end;
   mass_rows(a, n, p0, b0, 4 * KEYS, f_lo, f_end);
   const bool alone = f_end - f_lo <= a.cut;       // one cut: added to the accounts here
@@ -1586,7 +1593,7 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int keys) {
   int first, n, f_lo, f_hi;
   seq_rows(c, seq, first, n);
   const int len = seq_len(c, seq);
-  if (n == 0 || key >= len) return;
+  if (n == 0 || key >= len || too_long(c, seq)) return;
   mass_rows(a, n, len - n, key / keys * keys, keys, f_lo, f_hi);
   if (f_hi - f_lo <= a.cut) return;
   const int pg = page_of(c, key), page = c.table[seq * c.stride + pg];

@@ -188,6 +188,84 @@ def test_attention_pages_that_are_none(ops, hip_device, types):
     check_attention(u, *attend(ops, u, d, None, 0, 0))
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("hd", [16, 64])
+@pytest.mark.parametrize("seqs,heads", [
+    ([(1, 48), (1, 30), (1, 48), (2, 17)], (4, 2)),
+    ([(30, 48), (9, 30), (48, 48), (2, 17)], (4, 2)),
+    ([(1, 3200), (3, 900)], (4, 2)),                                            # in cuts
+    ([(150, 208), (40, 200), (208, 208), (9, 90)], (64, 64)),
+])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+def test_lengths_past_the_table(ops, hip_device, window, sinks, seqs, heads, hd, types):
+    """Sequences 0 and 2 step past their tables: their tokens are not stored and come out as NaN, what the
+    cache and its accounts hold stays, and the other sequences do not notice."""
+    xd, kd = TYPES[types]
+    u = Setup(seqs, *heads, hd, 16, xd, kd, seed=97)
+    over = torch.zeros(u.T, dtype=torch.bool)
+    for s in range(0, u.S, 2):
+        over[u.starts[s]: u.starts[s + 1]] = True
+    over = over.to(hip_device)
+    inv = (1e6 ** (-np.arange(0, hd, 2) / hd)).astype(np.float32)
+    at = torch.from_numpy(inv).to(hip_device), torch.arange(u.T, dtype=torch.int32, device=hip_device)
+
+    def run(lens):
+        d = u.on(hip_device)
+        d["lens"] = torch.tensor(lens, dtype=torch.int32, device=hip_device)
+        q = ops.paged_append(*heads, hd, 16, 1e-6)(d["qkv"], None, None, *at, d["starts"], d["lens"], d["table"], d["k"], d["v"],
+                                                   mass=d["mass"])
+        kept = {n: d[n].clone() for n in ("k", "v", "mass")}
+        out, lse = attend(ops, u, d, None, window, sinks)
+        mass = ops.paged_attention_mass(*heads, hd, 16, None, window, sinks)(
+            d["q"], lse.nan_to_num(0.0), d["k"], d["table"], d["starts"], d["lens"], d["mass"].clone())
+        return q, out, lse, mass, kept
+
+    fine = run(u.lens.tolist())
+    assert fine[1].isfinite().all()
+    for extra in (1, 37, 2 ** 31 - 1):
+        lens = [min(n + extra, 2 ** 31 - 1) if s % 2 == 0 else n for s, n in enumerate(u.lens.tolist())]
+        q, out, lse, mass, kept = run(lens)
+        assert torch.equal(q, fine[0])
+        assert out[over].isnan().all() and lse[over].isnan().all()
+        assert torch.equal(out[~over], fine[1][~over]) and torch.equal(lse[~over], fine[2][~over])
+        d = u.on(hip_device)
+        for s in range(u.S):
+            e = torch.from_numpy(u.table[s]).long().to(hip_device)
+            for n in ("k", "v", "mass"):
+                assert torch.equal(kept[n][e], (d[n] if s % 2 == 0 else fine[4][n])[e])
+            assert torch.equal(mass[e], (d["mass"] if s % 2 == 0 else fine[3])[e])
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("new", [100, 1000])
+def test_prompts_longer_than_the_table(ops, hip_device, new, types):
+    u = Setup([(5, 30), (new, new), (3, 64)], 8, 4, 64, 16, *TYPES[types], width=4, seed=99)
+    d = u.on(hip_device)
+    inv = torch.ones(32, device=hip_device)
+    ops.paged_append(8, 4, 64, 16, 1e-6)(d["qkv"], None, None, inv, torch.zeros(u.T, dtype=torch.int32, device=hip_device),
+                                         d["starts"], d["lens"], d["table"], d["k"], d["v"], mass=d["mass"])
+    for n in ("k", "v", "mass"):
+        e = torch.from_numpy(u.table[1]).long()
+        assert torch.equal(d[n].cpu()[e], getattr(u, n)[e])
+        setattr(u, n, d[n].cpu())
+    out, lse = attend(ops, u, d)
+    assert out[5: 5 + new].isnan().all() and lse[5: 5 + new].isnan().all()
+    mass = ops.paged_attention_mass(8, 4, 64, 16)(d["q"], lse.nan_to_num(0.0), d["k"], d["table"], d["starts"], d["lens"],
+                                                  d["mass"].clone())
+    assert torch.equal(mass.cpu()[e], u.mass[e])
+    for s, (lo, hi) in ((0, (0, 5)), (2, (5 + new, 8 + new))):
+        alone = Setup([u.seqs[s]], 8, 4, 64, 16, *TYPES[types], width=4)
+        alone.k, alone.v, alone.q, alone.table, alone.n_pages = u.k, u.v, u.q[lo:hi], u.table[s: s + 1], u.n_pages
+        check_attention(alone, out[lo:hi], lse[lo:hi])
+
+
+def test_evict_of_a_length_past_the_table(ops, hip_device):
+    u = Setup([(1, 48), (1, 30)], 4, 2, 64, 16, F32, BF16, spare=6, seed=98)
+    d = u.on(hip_device)
+    d["lens"][0] = 2 ** 31 - 1
+    check_evict(u, d, 33, 2, 5, *run_evict(ops, u, d, 33, 2, 5))
+
+
 def test_attention_rows_that_all_score_nothing(ops, hip_device):
     """Scores of -infinity everywhere are 0 / 0, as the formula says; one other key is enough."""
     u = Setup([(1, 20), (1, 20)], 2, 1, 64, 16, F32, F32, seed=12)
