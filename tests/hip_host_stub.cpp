@@ -18,6 +18,7 @@ std::string& calls() { static std::string s; return s; }   // one line per call
 std::string fail_name;                                     // this call fails ...
 int fail_after = -1;                                       // ... after so many of them (-1: never)
 long new_limit = -1;                                       // operator new of more bytes throws (-1: never)
+size_t arg_bytes = 0;                                      // of a launch's first argument that are written down
 hipError_t last_launch = hipSuccess;
 struct { dim3 grid, block; size_t smem; hipStream_t st; } cfg;
 
@@ -40,6 +41,7 @@ extern "C" {
 
 void stub_fail(const char* name, int after) { fail_name = name; fail_after = after; }
 void stub_new_limit(long n) { new_limit = n; }
+void stub_keep_args(long n) { arg_bytes = (size_t)n; }     // no more than the first argument has
 const char* stub_calls() { return calls().c_str(); }
 void stub_clear() { calls().clear(); }
 
@@ -57,10 +59,16 @@ hipError_t __hipPopCallConfiguration(dim3* g, dim3* b, size_t* smem, hipStream_t
   *g = cfg.grid; *b = cfg.block; *smem = cfg.smem; *st = cfg.st;
   return hipSuccess;
 }
-hipError_t hipLaunchKernel(const void* f, dim3 g, dim3 b, void**, size_t, hipStream_t) {
+hipError_t hipLaunchKernel(const void* f, dim3 g, dim3 b, void** args, size_t, hipStream_t) {
   char t[96];
   snprintf(t, sizeof(t), " %u %u %u %u ", g.x, g.y, g.z, b.x);
-  return last_launch = note("hipLaunchKernel", t + names()[f]);
+  std::string bytes = arg_bytes ? " " : "";
+  for (size_t i = 0; i < arg_bytes; ++i) {
+    char h[3];
+    snprintf(h, sizeof(h), "%02x", static_cast<const unsigned char*>(args[0])[i]);
+    bytes += h;
+  }
+  return last_launch = note("hipLaunchKernel", t + names()[f] + bytes);
 }
 hipError_t hipGetLastError() { const hipError_t e = last_launch; last_launch = hipSuccess; return e; }
 const char* hipGetErrorString(hipError_t) { return "stub error"; }

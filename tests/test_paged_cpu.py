@@ -190,10 +190,10 @@ def launches(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
                     os.path.join(ROOT, "tests", "hip_host_stub.cpp"), "-o", str(so)], check=True)
 
-    def run(cases):
+    def run(cases, script=SCRIPT):
         import json
 
-        (tmp / "s.py").write_text(SCRIPT)
+        (tmp / "s.py").write_text(script)
         (tmp / "c.json").write_text(json.dumps(cases))
         env = dict(os.environ, PYTHONPATH=os.path.join(ROOT, "tests"))
         r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "host_engine.py"), str(so), str(tmp / "s.py"),
@@ -241,6 +241,58 @@ def test_attention_plans_cover_rows_and_keys(launches):
             n = np.diff(np.concatenate(([0], cuts, [c["T"]])))
             assert sum(-(-int(x) * G // R) for x in n) <= grid[1]
         assert ws == ((grid[2] * (128 + 2) + 1) * c["T"] * c["Hq"] * 4 if grid[2] > 1 else 0)
+
+
+class AttendArgs(C.Structure):
+    """The kernels' argument (AttendArgs of sk_paged.h, a Cache first)."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "table")] + [("stride", C.c_int64), ("width", C.c_int32)] + [
+        (n, C.c_void_p) for n in ("starts", "lens")] + [(n, C.c_int32) for n in ("T", "S", "Hq", "Hkv", "G", "n_pages", "page")] + [
+        ("page_mul", C.c_uint32), ("page_shift", C.c_int32)] + [(n, C.c_void_p) for n in ("q", "out", "lse")] + [
+        ("scale2", C.c_float)] + [(n, C.c_int32) for n in ("window", "sinks", "cut", "last")] + [
+        (n, C.c_void_p) for n in ("part", "ml", "count")]
+
+
+ARGS = f"stub.stub_keep_args({C.sizeof(AttendArgs)})\n" + SCRIPT.replace("kernels(cs)", "[c[5:] + c[1:4] for c in cs]")
+
+
+def longest_walk(c, R, n, length):
+    """Key tiles that a tile of R rows of a sequence of n new tokens and that length goes through, at most."""
+    G, p0, most = c["Hq"] // c["Hkv"], length - n, 0
+    for f in range(0, n * G, R):
+        lo_slot, hi_slot = p0 + f // G, p0 + (min(f + R, n * G) - 1) // G
+        lo = (lo_slot - c["window"] + 1) // 16 if 0 < c["window"] <= lo_slot else 0
+        most = max(most, 0 if hi_slot < 0 else hi_slot // 16 + 1 - lo + min(-(-c["sinks"] // 16), lo))
+    return most
+
+
+@pytest.mark.parametrize("hd,xd,kd", [(16, 0, 0), (16, 1, 1), (32, 0, 1), (64, 1, 1), (128, 0, 0), (128, 0, 1), (128, 1, 1)])
+def test_attention_cuts_reach_the_longest_walk(launches, hd, xd, kd):
+    """Cuts are whole steps of four tiles and together as long as any walk can be, and the
+    last row tile of a launch is the one that its grid ends at."""
+    rng = np.random.default_rng(hd + xd + 2 * kd)
+    cases = []
+    for i in range(60):
+        hkv = int(rng.choice([1, 2, 8, 64]))
+        S = int(rng.choice([1, 2, 7, 40]))
+        cases.append(["attention", dict(T=S * int(rng.choice([1, 1, 5, 70, 600])), S=S, Hkv=hkv, Hq=hkv * int(rng.choice([1, 2, 8])), hd=hd, xd=xd,
+                                        kd=kd, width=(w := int(rng.choice([1, 9, 60, 300]))), stride=w, page=16 * int(rng.integers(1, 9)),
+                                        window=int(rng.choice([0, 1, 40, 700])), sinks=int(rng.choice([0, 5, 100])))])
+    some_cut = False
+    for (_, c), (rc, _, kern, _, _) in zip(cases, launches(cases, ARGS)):
+        assert rc == 0
+        name, raw, *grid = kern[0]
+        a, R, cap = AttendArgs.from_buffer_copy(bytes.fromhex(raw)), rows_of(name), c["width"] * c["page"]
+        assert (a.T, a.S, a.G, a.page, a.window, a.sinks, a.width) == (c["T"], c["S"], c["Hq"] // c["Hkv"], c["page"],
+                                                                       c["window"], c["sinks"], c["width"])
+        gx, gy, gz = (int(x) for x in grid)
+        assert a.cut > 0 and a.cut % 4 == 0 and a.last == gy - 1
+        some_cut |= gz > 1
+        n = c["T"] // c["S"]
+        for length in (cap, max(1, cap - 7), int(rng.integers(1, cap + 1)), min(cap, n)):
+            assert longest_walk(c, R, n, length) <= gz * a.cut
+            assert longest_walk(c, R, c["T"], length) <= gz * a.cut
+    assert some_cut
 
 
 @pytest.mark.parametrize("entry", ["append", "attention", "mass", "evict"])
