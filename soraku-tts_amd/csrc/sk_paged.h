@@ -319,6 +319,14 @@ __device__ __forceinline__ bool all_see(int j0, int j1, int p_lo, int p_hi, int 
   return j1 <= p_lo && (window == 0 || j0 > p_hi - window || j1 < sinks);
 }
 
+// The factor from sums that refer to the maximum m to ones for m2.  Weights refer to m scale2 as rounded, so that
+// is what counts here too: fused, the product would be off from it by half a step of an exponent that may be large.
+__device__ __forceinline__ float rescale_of(float m, float scale2, float m2) {
+#pragma clang fp contract(off)
+  const float was = m * scale2;
+  return __builtin_amdgcn_exp2f(was - m2);
+}
+
 __device__ __forceinline__ int cuts_of(const AttendArgs& a, const Walk& w, bool none) {
   const int ns = w.n <= a.cut ? 0 : (w.n + a.cut - 1) / a.cut;
   return none ? -ns : ns;
@@ -431,7 +439,7 @@ __device__ __forceinline__ void meet_rows(const AttendArgs& a, const float* po, 
     const float m2 = mx == -INFINITY ? LOWEST : mx * a.scale2;
 #pragma unroll
     for (int u = 0; u < WK; ++u) {
-      f[u] = __builtin_amdgcn_exp2f(fmaf(pm[u * R + tid], a.scale2, -m2));
+      f[u] = rescale_of(pm[u * R + tid], a.scale2, m2);
       l = fmaf(f[u], pl[u * R + tid], l);
     }
     const int row = f0 + tid, tok = row / c.G;
@@ -598,7 +606,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       mx = max4(mx);
       const float mn = fmaxf(mr[j], mx);
       const float m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
-      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
+      const float sc = mr[j] == mn ? 1.f : rescale_of(mr[j], a.scale2, m2);
       float sum = 0.f;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
@@ -1184,7 +1192,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
         for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][g][v]);
       const float mn = fmaxf(mr[j], max4(mx)), m2 = mn == -INFINITY ? 0.f : mn * a.scale2;
-      const float sc = mr[j] == mn ? 1.f : __builtin_amdgcn_exp2f(fmaf(mr[j], a.scale2, -m2));
+      const float sc = mr[j] == mn ? 1.f : rescale_of(mr[j], a.scale2, m2);
       float y[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

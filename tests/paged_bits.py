@@ -29,9 +29,9 @@ def cut(x, n):
     return out
 
 
-def near_ties(seqs, heads, hd, xd, kd, width=None, seed=0):
-    """Scores that FP32 and BF16 products give exactly, close to each other, and values of -1 and 1: a
-    row's result is a difference of weights.  Returns the inputs and the scale."""
+def near_ties(seqs, heads, hd, xd, kd, width=None, seed=0, level=0):
+    """Scores that FP32 and BF16 products give exactly, close to each other (and to level^2 / 16), and values of -1 and
+    1: a row's result is a difference of weights.  Returns the inputs and the scale."""
     u = Setup(seqs, *heads, hd, 16, xd, kd, width=width, seed=seed)
     g = torch.Generator().manual_seed(seed + 1)
 
@@ -40,6 +40,8 @@ def near_ties(seqs, heads, hd, xd, kd, width=None, seed=0):
 
     u.q, u.k = pick(u.q, [-0.5, 0.0, 0.5]), pick(u.k, [-1.0, -0.5, 0.0, 0.5, 1.0])
     u.v = pick(u.v, [-1.0, 1.0])
+    if level:
+        u.q[..., -1], u.k[..., -1] = level, level
     return u, 2.0 ** -4
 
 
@@ -99,12 +101,13 @@ def simulate(u, scale, window, q_parts, p_parts):
 
 def out_bound(u, scale, window):
     """(exact out, how far an output may be) with scores that are exact.  A weight: the factor log2 e and
-    its product off by a step of the exponent, the difference from the maximum and that maximum's own
-    rounding by as much (5 S steps of 2^-24, S the largest score), the exponential and up to one change of
+    its product off by a step of the exponent, the difference from the maximum by as much, and that of an
+    earlier maximum (5 S steps of 2^-24, S the largest difference of two scores of a row: weights and sums refer to one and the
+    same rounded maximum, so its own size does not count), the exponential and up to one change of
     the maximum (8).  Those count once in the sum over values, once in the sum of weights; n additions
     and the factors in common follow (8).  BF16 activations: weights of 16 bits, 2^-16 of each, and the output's rounding."""
     want, _, weight, size = ref.attention(u, scale, window, 0)
-    S, n = scores_of(u, scale, window)
+    _, S, n = scores_of(u, scale, window)
     fine = (2.0 * (5.0 * S + 8.0) + n + 8.0) * EPS * weight
     if u.xd == torch.bfloat16:
         fine = fine + 2.0 ** -16 * weight
@@ -113,16 +116,18 @@ def out_bound(u, scale, window):
 
 
 def scores_of(u, scale, window):
-    """The largest |score| that a row sees, and the most keys that one sees."""
-    top, most, q = 0.0, 0, u.q.double().numpy()
+    """The largest |score| that a row sees, the largest difference of two of a row, and the most keys that one sees."""
+    top, apart, most, q = 0.0, 0.0, 0, u.q.double().numpy()
     for s in range(u.S):
         for h in range(u.Hkv):
             k = u.keys(u.k, s, h, int(u.lens[s]))
             for m in u.rows(s):
                 see = ref.seen(u.slot(s, m), window, 0)
-                most = max(most, len(see))
-                top = max(top, float(np.abs(scale * (k[see] @ q[m, h * u.G: (h + 1) * u.G].T)).max(initial=0.0)))
-    return top, most
+                if not see:
+                    continue
+                x = scale * (k[see] @ q[m, h * u.G: (h + 1) * u.G].T)
+                top, apart, most = max(top, float(np.abs(x).max())), max(apart, float(np.ptp(x, 0).max())), max(most, len(see))
+    return top, apart, most
 
 
 def simulate_mass(u, scale, lse, keep):

@@ -46,6 +46,16 @@ def test_weights(ops, hip_device, types, shape, hd):
     check(attend(ops, hip_device, u, scale, 2)[0], *bits.out_bound(u, scale, 2))
 
 
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("shape", [*SHAPES, "cuts"])
+@pytest.mark.parametrize("types", TYPES)
+def test_large_scores(ops, hip_device, types, shape, hd):
+    """Scores around 1,024: the differences decide, in every wave and cut and across them."""
+    seqs, heads = dict(SHAPES, cuts=([(1, 700), (1, 430)], (4, 2)))[shape]
+    u, scale = bits.near_ties(seqs, heads, hd, *TYPES[types], seed=hd, level=128)
+    check(attend(ops, hip_device, u, scale, 0)[0], *bits.out_bound(u, scale, 0))
+
+
 @pytest.mark.parametrize("hd", [32, 64, 128])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_queries(ops, hip_device, shape, hd):
