@@ -9,7 +9,7 @@ namespace sk {
 // 16 bytes per lane from g straight into LDS at l + 16 * lane (l wave-uniform).
 // Written as assembly because with the builtin the compiler waits for every
 // load in flight (vmcnt(0)) before the next LDS read, whichever part of the
-// ring it reads; the loop below does the waiting itself (stage_sync).  M0 holds
+// ring it reads; callers' loops do the waiting themselves (stage_sync).  M0 holds
 // the LDS address and is declared overwritten: a value that the compiler keeps
 // there is set again afterwards (it does so, although it warns that M0 is a
 // reserved register).  The statement has no outputs: nothing is

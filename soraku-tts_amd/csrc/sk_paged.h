@@ -662,11 +662,12 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // exactly, three products each, so results are those of FP32 products (NP = 3).  BF16
 // activations: P keeps 16 bits, two parts (off by 2^-16 of a weight at most, 256 times less than the output's own
 // rounding; one part, off by 2^-8, adds as much again to it: 0.0023 of the output against 0.0017, for 269 us
-// in place of 353 below).
+// in place of 353 to 372 below).
 //
-// 2,047 BF16 tokens over 16,384, 16 heads on 8 of 128, with the join of its two cuts: 353 us, 1,098 TFLOP/s of the
-// three products per pair (a large BF16 product reaches 1,214 here): the matrix cores bound it.
-// 4,500 FP32 tokens with a window of 1,024: 168 us, 740 TFLOP/s of the three-part products, matrix cores 52%
+// 2,047 BF16 tokens over 16,384, 16 heads on 8 of 128, with the join of its two cuts: 353 to 372 us by the
+// card, 1,040 to 1,098 TFLOP/s of the three products per pair (a large BF16 product reaches 1,200 here).  The matrix cores
+// are busy 68% of the time, the VALU (exponentials, maxima, parts) 60%.  LDS does not bound it (no bank conflicts).
+// 4,500 FP32 tokens with a window of 1,024: 171 us, 725 TFLOP/s of the three-part products, matrix cores 52%
 // busy: no registers are left to run a step's scores ahead.
 constexpr int KEYS = 64;                          // keys of a step
 
@@ -1049,8 +1050,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // take 1,024 cycles of a SIMD per 4 KB of the cache, these 64 to 192 (with BF16 activations P keeps 16
 // bits, two parts: it costs nothing here).  K goes from the pages to registers as fragments, V to
 // two slots of LDS of the wave's own, both a step ahead.
-// 32 rows of 328 to 657 tokens, FP32 on BF16: 16.8 us for 65 MB, one workgroup per CU at what it draws (12.7 at
-// a large copy's rate); two rows of 30,720 and 61,441 in 16 cuts: 66 us, 5.7 TB/s.
+// 32 rows of 328 to 657 tokens, FP32 on BF16: 17 us for 65 MB, one workgroup per CU at what it draws (10.7 at
+// the 6.1 TB/s of a pure read); two rows of 30,720 and 61,441 in 16 cuts: 66 us, 5.7 TB/s.
 template <typename QT, int HD, int NT, int WK>
 __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_few_kernel(AttendArgs a) {
   constexpr int NP = sizeof(QT) == 4 ? 3 : 1, PP = NP == 3 ? 3 : 2;   // parts of Q, of P
@@ -1246,7 +1247,7 @@ __global__ __launch_bounds__(WK * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // Joins the cuts of rows that have several (at most 64); WPR waves per row (token, query head),
 // half a wave per cut and 16 bytes per lane, the parts of a wave's cuts loading together.
 // What the kernel before left in `count` spares the way to the row's sequence (2,047
-// tokens: 25 -> 13 us).
+// tokens: 25 -> 17 us).
 template <typename QT, int HD, int WPR>
 __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a, int cuts) {
   constexpr int NL = HD / 4, PER = 64 / NL < 2 ? 1 : 2, U = 4;   // lanes of a part, cuts of a wave at a time, loads under way
@@ -1417,7 +1418,7 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
 // Many rows on few keys are cut over workgroups, whose sums mass_join_kernel adds in order.
 //
 // 32 rows of 2,400 to 4,800 tokens, FP32 on BF16: 52 us, 244 MB at 4.7 TB/s.  Prompts of 900 and 1,800 over
-// 1,800 and 3,600: 90 + 5 us, 830 TFLOP/s of the three-part products, matrix cores 48% busy beside one exponential
+// 1,800 and 3,600: 92 + 5 us, 810 TFLOP/s of the three-part products, matrix cores 48% busy beside one exponential
 // per weight and the parts (three waves per SIMD spill: 109; cuts for fewer than twelve workgroups per CU: 132 to 140).
 template <typename QT, typename KT, int HD, int N>
 __global__ __launch_bounds__(256) void mass_tiles_kernel(MassArgs a) {

@@ -148,7 +148,9 @@ def sample(V: int, bos_id: int, eos_id: int, pad_id: int):
 # Pools k_pages / v_pages [n_pages, Hkv, page, hd] (float32 or bfloat16), table
 # [S, width] int32 (any row stride, so a slice of a wider one will do), starts
 # [S + 1] and lens [S] int32, all on the HIP device: sequence s's new tokens are
-# the packed rows starts[s]:starts[s + 1] and lens[s] its length with them.
+# the packed rows starts[s]:starts[s + 1] and lens[s] its length with them.  Calls are
+# planned from rows per sequence and width: single tokens and chunks belong in calls of their
+# own, and a wide table is passed as a slice that the longest sequence fills.
 # include/soraku_mi355x.h holds the whole contract.
 #
 # A single-token call runs for 4 to 25 us on the GPU, so the host's part is kept
