@@ -260,7 +260,8 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * rows starts[s] .. starts[s + 1] of T, and lens[s] is its length with them:
  * token i of n has slot lens[s] - n + i.  Sequences without new tokens and
  * lengths of 0 are fine; rows from starts[S] on are padding and left alone.
- * table, starts and lens are device int32.
+ * table, starts and lens are device int32; the pages of a sequence that append or
+ * accounts write to are different ones.
  *
  * The host does not look at device memory, so the kernels hold what they find
  * there in range: lens to [0, width * page], starts to [0, T].  A table entry
@@ -274,12 +275,12 @@ int sk_op_sample(void* stream, int32_t rows, int32_t V, const float* logits, flo
  * xdtype / kvdtype: activations and cache, SK_F32 / SK_F32, SK_F32 / SK_BF16 or
  * SK_BF16 / SK_BF16; sums and softmax are FP32, products of FP32 activations
  * exact; with BF16 activations a softmax weight enters its product with v with 16
- * bits, rounded to nearest, whatever else is in the call.  hd: 16, 32, 64 or 128.
- * Hq: a multiple of Hkv, at most 4096; query heads h G .. h G + G - 1 share key head
- * h.  S is at most 65535; T may be 0 and is below 2^24; width * page and T * Hq are
- * at most 2^30.  q, qkv, gains, pages, outputs of xdtype and workspaces are 16-byte
- * aligned; outputs overlap no operand.  No call allocates, waits or copies to the
- * host, and each may be captured into a graph.
+ * bits (hd 16: 32), rounded to nearest, whatever else is in the call.  hd: 16, 32,
+ * 64 or 128.  Hq: a multiple of Hkv, at most 4096; query heads h G .. h G + G - 1
+ * share key head h.  S is at most 65535; T may be 0 and is below 2^24; width * page
+ * and T * Hq are at most 2^30.  q, qkv, gains, pages, outputs of xdtype and workspaces
+ * are 16-byte aligned; outputs overlap no operand.  No call allocates, waits or copies
+ * to the host, and each may be captured into a graph.
  *
  * How attention and accounts are cut up is planned for the whole call, from the
  * average of new tokens, T / S, and from width.  So single tokens and chunks belong
