@@ -40,6 +40,9 @@ extern "C" {
 /* ---- element types --------------------------------------------------- */
 #define SK_F32  0
 #define SK_BF16 1
+/* ---- what a projection does with its sums ------------------------------ */
+#define SK_ACT_NONE   0
+#define SK_ACT_SWIGLU 1
 
 /* Model dimensions and special ids (SorakuV2Config model.py:34-63 plus the
  * Qwen3 text config).  audio_vocab = codebook_size + 3 (model.py:61-63). */
@@ -348,6 +351,36 @@ int sk_op_paged_evict(void* stream, int32_t S, int32_t Hkv, int32_t hd, int32_t 
                       int32_t recent, void* k_pages, void* v_pages, float* mass, const int32_t* table,
                       const int32_t* lens, const int32_t* to, int64_t to_stride, int32_t to_width,
                       int32_t* new_lens, int32_t* kept);
+
+/* ---- operator API: projections with 8-bit weights -----------------------
+ * Matrices of one byte per element for programs that drive layers one operator at a
+ * time; no counterpart in the reference, whose weights are FP32 or BF16.
+ *
+ * A row t of K values has codes q = 127 t / max|t|, rounded to the nearest whole number
+ * (exactly; ties to even), and a scale max|t| / 127: it stands for q * scale.  A row of
+ * zeros has scale 0; one with an infinity or NaN has codes 0 and scale NaN.  A row's codes
+ * take Kp bytes, K rounded up to a multiple of 128, zeros behind K.  K is at most 130,944.
+ * xdtype is SK_F32 or SK_BF16; operands are 16-byte aligned but scales, bias and odd rows
+ * within them.  No call allocates, waits or copies to the host, and each may be captured into a
+ * graph. */
+
+/* Codes [R][Kp] and scales [R] of R rows x [R][K] of xdtype, for weights at load time.  R may be 0
+ * and is below 2^24. */
+int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const void* x, int8_t* codes, float* scales);
+/* out [M][N] = act(x W^T + bias) + residual with W [N][K] as codes [N][Kp] and scales [N]; bias [N] and residual
+ * [M][N] may be NULL.  With SK_ACT_SWIGLU W has 2 N rows, gate rows first, bias 2 N, and out is silu(gate) * up (+
+ * residual).  x, residual and out are of xdtype; out may be residual itself (sums in place), and overlaps no other operand.
+ * The rows of x become codes on the way; with eps >= 0 x is normalised first (RMSNorm with gain [K], or NULL for
+ * none): then fp32(x gain) is coded and the norm's factor goes into the scale.  Products are summed
+ * in whole numbers, exactly, so a row's result does not hang on what else is in the call; scales, bias, act
+ * and residual follow in FP32, rounded once at the end.  A row of x with an infinity or NaN gives NaN.  Codes of W
+ * may be any bytes, -128 too, whoever made them (behind K they meet zeros).
+ * M may be 0 and is below 2^24; N is at most 2^20.  The workspace holds the bytes that _workspace gives for the same
+ * sizes (where that is 0 it may be NULL) and belongs to the call until it has run. */
+int sk_op_int8_linear_workspace(int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act, int64_t* bytes);
+int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act, float eps,
+                      const void* x, const float* gain, const int8_t* codes, const float* scales, const float* bias,
+                      const void* residual, void* out, void* workspace, int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

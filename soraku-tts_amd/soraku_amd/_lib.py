@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "libsoraku_mi355x.so")
 
 SK_OK, SK_EINVAL, SK_ENOWEIGHT, SK_ENOCAPTURE, SK_EKVFULL, SK_EHIP, SK_ESTATE = 0, -1, -2, -3, -4, -5, -6
 SK_F32, SK_BF16 = 0, 1
+SK_ACT_NONE, SK_ACT_SWIGLU = 0, 1
 
 ERROR_NAMES = {
     SK_EINVAL: "SK_EINVAL", SK_ENOWEIGHT: "SK_ENOWEIGHT", SK_ENOCAPTURE: "SK_ENOCAPTURE",
@@ -95,6 +96,9 @@ PROTOTYPES = {
     "sk_op_paged_attention_mass_workspace": (_I, [*[_I] * 9, _PI64]),
     "sk_op_paged_attention_mass": (_I, [_P, *[_I] * 8, _L, _I, _I, _F, _I, _I, *[_P] * 8, _L]),
     "sk_op_paged_evict": (_I, [_P, *[_I] * 6, _L, *[_I] * 4, *[_P] * 6, _L, _I, _P, _P]),
+    "sk_op_int8_rows": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "sk_op_int8_linear_workspace": (_I, [*[_I] * 5, _PI64]),
+    "sk_op_int8_linear": (_I, [_P, *[_I] * 5, _F, *[_P] * 8, _L]),
 }
 
 

@@ -158,12 +158,13 @@ def sample(V: int, bos_id: int, eos_id: int, pad_id: int):
 # objects.
 
 class _Torch:
-    """What the paged operators use of torch, looked up once."""
+    """What these operators use of torch, looked up once."""
 
     def __init__(self):
         import torch
 
         self.f32, self.bf16, self.i32, self.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
+        self.i8 = torch.int8
         self.empty, self.empty_like, self.on = torch.empty, torch.empty_like, torch.cuda.device
         self.stream, self.device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self.codes = {torch.float32: _lib.SK_F32, torch.bfloat16: _lib.SK_BF16}
@@ -345,4 +346,76 @@ def paged_evict(Hkv: int, hd: int, page: int, keep: int, sinks: int = 0, recent:
               _need(mass, "mass", T.f32, at, (n, Hkv, page)), tp, _need(lens, "lens", i32, at, (S,)), dp, to_stride,
               to_width, new_lens.data_ptr(), kept.data_ptr())
         return new_lens, kept
+    return kernel
+
+
+# ---- projections with 8-bit weights (no counterpart in the reference) ----
+# A matrix [N, K] is held as codes [N, Kp] int8 (Kp: K up to a multiple of 128, zeros behind)
+# and scales [N] float32, one per row; int8_rows makes them, once, when weights are loaded.
+# Activations are float32 or bfloat16 and become codes, row by row, inside int8_linear.
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(*sizes) -> int:
+    n = C.c_int64()
+    check(lib().sk_op_int8_linear_workspace(*sizes, C.byref(n)))
+    return n.value
+
+
+def _matrix(t, name, K, codes):
+    """(device number, rows, type code) of a contiguous [rows, K] tensor of float32 or bfloat16."""
+    if not t.is_cuda:
+        raise ValueError("operands must live on the HIP device")
+    if t.dim() != 2 or t.shape[1] != K or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor [rows, {K}], got {tuple(t.shape)}"
+                         f"{'' if t.is_contiguous() else ', not contiguous'}")
+    return t.get_device(), t.shape[0], _code(t, codes)
+
+
+def int8_rows(K: int):
+    """``kernel(x[R, K]) -> codes [R, Kp] int8, scales [R] float32``: each row as the nearest whole
+    numbers of 127 x / max|x| and the scale max|x| / 127."""
+    K, = _int32(K=K)
+
+    def kernel(x):
+        T = _torch()
+        at, rows, xd = _matrix(x, "x", K, T.codes)
+        codes = T.empty((rows, -(-K // 128) * 128), device=x.device, dtype=T.i8)
+        scales = T.empty((rows,), device=x.device, dtype=T.f32)
+        _call(T, T.lib.sk_op_int8_rows, at, rows, K, xd, x.data_ptr(), codes.data_ptr(), scales.data_ptr())
+        return codes, scales
+    return kernel
+
+
+def int8_linear(N: int, K: int, act: str | None = None, eps: float | None = None):
+    """out ``[M, N]`` = act(x W^T + bias) + residual with W as ``codes`` [N, Kp] and ``scales`` [N] of
+    ``int8_rows``; of x's dtype.  ``act="swiglu"``: W has 2 N rows, gate rows first, and act is
+    silu(gate) * up.  With ``eps`` x is normalised first (RMSNorm, ``gain`` [K] or none).  ``out`` may be
+    ``residual`` itself."""
+    N, K = _int32(N=N, K=K)
+    if act not in (None, "swiglu"):
+        raise ValueError(f"act must be None or 'swiglu', got {act!r}")
+    both, kp = (2 * N if act else N), -(-K // 128) * 128
+    act = _lib.SK_ACT_SWIGLU if act else _lib.SK_ACT_NONE
+    if eps is not None and not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    eps = -1.0 if eps is None else float(eps)
+
+    def kernel(x, codes, scales, gain=None, bias=None, residual=None, out=None):
+        T = _torch()
+        f32, dt = T.f32, x.dtype
+        at, rows, xd = _matrix(x, "x", K, T.codes)
+        shape = (rows, N)
+        if out is None:
+            out = T.empty(shape, device=x.device, dtype=dt)
+            op = out.data_ptr()
+        else:
+            op = _need(out, "out", dt, at, shape)
+        size = _linear_workspace(rows, N, K, xd, act)
+        ws = T.empty(size, device=x.device, dtype=T.u8) if size else None
+        _call(T, T.lib.sk_op_int8_linear, at, rows, N, K, xd, act, eps, x.data_ptr(),
+              None if gain is None else _need(gain, "gain", f32, at, (K,)), _need(codes, "codes", T.i8, at, (both, kp)),
+              _need(scales, "scales", f32, at, (both,)), None if bias is None else _need(bias, "bias", f32, at, (both,)),
+              None if residual is None else _need(residual, "residual", dt, at, shape), op,
+              ws.data_ptr() if size else None, size)
+        return out
     return kernel
