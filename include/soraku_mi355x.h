@@ -382,6 +382,31 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
                       const void* x, const float* gain, const int8_t* codes, const float* scales, const float* bias,
                       const void* residual, void* out, void* workspace, int64_t workspace_bytes);
 
+/* ---- operator API: sampling by row --------------------------------------
+ * sk_op_sample for a batch: every row of logits with its own parameters, read from device memory when the call runs
+ * (so a captured graph follows them), over vocabularies of up to 2^20, with min-p and a mask of bits.
+ *
+ * logits are R rows of V values of dtype (SK_F32 or SK_BF16), rows stride elements apart; with cfg_scale [R] they are
+ * 2 R rows, cond and uncond of each in turn, merged as uncond + cfg_scale (cond - uncond) in FP32, each
+ * operation rounded.  Candidates of a row are its finite values; with allowed, those whose bit (id % 32 of word
+ * id / 32) is set, words allowed_stride apart by row (0: one row for all).  They are divided by temperature[r] in
+ * FP32 (results held to the finite range); a temperature that is not above 0 takes the largest one, of equal ones that of the lowest id.
+ *
+ * In the order of values, largest first, equal ones by the lower id: top_k[r] in [1, candidates) keeps those
+ * down to the k-th's value (all that equal it); top_p[r] in (0, 1) of these the first ones up to and with the one
+ * whose sum of weights e^(x - largest) passes top_p of their whole; min_p[r] in (0, 1] of these the ones with a weight of at
+ * least min_p.  Other values of these, and NULL arrays, filter nothing (temperature: 1).  token[r] is
+ * the first kept one whose sum passes u[r] of the kept sum; u is in [0, 1) (below it counts as 0, above as the last one).  Sums are exact
+ * sums of weights rounded to 2^-44 of the largest's power of two or finer (2^-42 past 2^19 values).  logprob (may be NULL): the
+ * logarithm of the drawn one's part of the kept sum, 0 when greedy; kept (may be NULL): how many were kept.  A row without candidates
+ * gives -1, -infinity and 0.  R may be 0 and is at most 65535.  No call allocates, waits or copies to the host.  Workspace as for
+ * the operators above. */
+int sk_op_sample_rows_workspace(int32_t R, int32_t V, int32_t dtype, int64_t* bytes);
+int sk_op_sample_rows(void* stream, int32_t R, int32_t V, int32_t dtype, const void* logits, int64_t stride,
+                      const double* u, const float* temperature, const int32_t* top_k, const float* top_p,
+                      const float* min_p, const float* cfg_scale, const uint32_t* allowed, int64_t allowed_stride,
+                      int64_t* token, float* logprob, int32_t* kept, void* workspace, int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

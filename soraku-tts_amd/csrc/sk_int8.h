@@ -21,6 +21,9 @@
 
 #include "sk_lds.h"
 
+// Each operation rounds by itself (fused ones are written as such): all kernels give the same bits.
+#pragma clang fp contract(off)
+
 namespace sk {
 namespace int8 {
 
@@ -74,7 +77,7 @@ __device__ __forceinline__ float weigh8(const float* gain, int k, int K, bool wh
   float g[8];
   load8<float>(gain, k, K, whole, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = __fmul_rn(t[i], g[i]);
+  for (int i = 0; i < 8; ++i) t[i] *= g[i];
   return squares;
 }
 // The largest |t| as bits: NaN above infinity above every number.
@@ -140,8 +143,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 constexpr int BLOCK = 512;
 __device__ __forceinline__ float norm_of(const float* blocks, int K, float eps) {
   float s = 0.f;
-  for (int b = 0; b * BLOCK < K; ++b) s = __fadd_rn(s, blocks[b]);
-  return 1.f / sqrtf(__fadd_rn(s / (float)K, eps));
+  for (int b = 0; b * BLOCK < K; ++b) s += blocks[b];
+  return 1.f / sqrtf(s / (float)K + eps);
 }
 
 struct RowsArgs {
@@ -229,8 +232,7 @@ struct LinearArgs {
 
 __device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
 
-// Four neighbouring outputs n .. n + 3 of row m from their sums; every operation is rounded by
-// itself, so that all kernels give the same bits.
+// Four neighbouring outputs n .. n + 3 of row m from their sums.
 template <typename X, bool SWIGLU>
 __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i acc, v4i up) {
   if (m >= a.M || n >= a.N) return;
@@ -241,12 +243,12 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i a
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = min(n + i, a.N - 1);
-    y[i] = __fmul_rn(__fmul_rn((float)acc[i], s), a.ws[c]);
-    if (a.bias) y[i] = __fadd_rn(y[i], a.bias[c]);
+    y[i] = (float)acc[i] * s * a.ws[c];
+    if (a.bias) y[i] += a.bias[c];
     if constexpr (SWIGLU) {
-      float u = __fmul_rn(__fmul_rn((float)up[i], s), a.ws[a.N + c]);
-      if (a.bias) u = __fadd_rn(u, a.bias[a.N + c]);
-      y[i] = __fmul_rn(silu(y[i]), u);
+      float u = (float)up[i] * s * a.ws[a.N + c];
+      if (a.bias) u += a.bias[a.N + c];
+      y[i] = silu(y[i]) * u;
     }
   }
   X* o = static_cast<X*>(a.out) + at;
@@ -255,7 +257,7 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i a
     if constexpr (sizeof(X) == 4) {
       if (a.res) {
         const float4 v = *reinterpret_cast<const float4*>(re);
-        y[0] = __fadd_rn(y[0], v.x); y[1] = __fadd_rn(y[1], v.y); y[2] = __fadd_rn(y[2], v.z); y[3] = __fadd_rn(y[3], v.w);
+        y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
       }
       *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
     } else {
@@ -264,7 +266,7 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i a
         r[0] = __uint_as_float(v.x << 16); r[1] = __uint_as_float(v.x & 0xffff0000u);
         r[2] = __uint_as_float(v.y << 16); r[3] = __uint_as_float(v.y & 0xffff0000u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = __fadd_rn(y[i], r[i]);
+        for (int i = 0; i < 4; ++i) y[i] += r[i];
       }
       *reinterpret_cast<uint2*>(o) = make_uint2((uint32_t)from_f<X>(y[0]) | (uint32_t)from_f<X>(y[1]) << 16,
                                                 (uint32_t)from_f<X>(y[2]) | (uint32_t)from_f<X>(y[3]) << 16);
@@ -272,7 +274,7 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i a
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) o[i] = from_f<X>(a.res ? __fadd_rn(y[i], to_f<X>(re[i])) : y[i]);
+      if (n + i < a.N) o[i] = from_f<X>(a.res ? y[i] + to_f<X>(re[i]) : y[i]);
   }
 }
 

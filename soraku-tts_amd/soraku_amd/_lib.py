@@ -99,6 +99,8 @@ PROTOTYPES = {
     "sk_op_int8_rows": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "sk_op_int8_linear_workspace": (_I, [*[_I] * 5, _PI64]),
     "sk_op_int8_linear": (_I, [_P, *[_I] * 5, _F, *[_P] * 8, _L]),
+    "sk_op_sample_rows_workspace": (_I, [_I, _I, _I, _PI64]),
+    "sk_op_sample_rows": (_I, [_P, _I, _I, _I, _P, _L, *[_P] * 7, _L, *[_P] * 4, _L]),
 }
 
 

@@ -164,7 +164,7 @@ class _Torch:
         import torch
 
         self.f32, self.bf16, self.i32, self.u8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8
-        self.i8 = torch.int8
+        self.i8, self.i64, self.f64 = torch.int8, torch.int64, torch.float64
         self.empty, self.empty_like, self.on = torch.empty, torch.empty_like, torch.cuda.device
         self.stream, self.device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         self.codes = {torch.float32: _lib.SK_F32, torch.bfloat16: _lib.SK_BF16}
@@ -417,5 +417,69 @@ def int8_linear(N: int, K: int, act: str | None = None, eps: float | None = None
               _need(scales, "scales", f32, at, (both,)), None if bias is None else _need(bias, "bias", f32, at, (both,)),
               None if residual is None else _need(residual, "residual", dt, at, shape), op,
               ws.data_ptr() if size else None, size)
+        return out
+    return kernel
+
+
+# ---- sampling by row (sample for a batch, model.py:686-708) ----
+
+@functools.lru_cache(maxsize=1024)
+def _sample_workspace(*sizes) -> int:
+    n = C.c_int64()
+    check(lib().sk_op_sample_rows_workspace(*sizes, C.byref(n)))
+    return n.value
+
+
+def sample_rows(V: int, cfg: bool = False):
+    """One id per row of logits ``[R, V]`` (float32 or bfloat16; rows may be apart) from the uniform draws
+    ``u`` [R] float64: ``kernel(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
+    cfg_scale=None, allowed=None, out=None, logprob=None, kept=None) -> int64[R]``.
+
+    Parameters are tensors [R] on the device (``top_k`` int32, the others float32) or None for none of
+    it; a temperature that is not above 0 is greedy.  With ``cfg`` the logits are ``[R, 2, V]``, cond and
+    uncond, merged with ``cfg_scale``.  ``allowed``: bits of the ids that may be drawn, int32 ``[R or 1, ceil(V / 32)]``.
+    ``logprob`` [R] float32 and ``kept`` [R] int32, if given, receive the drawn id's log-probability among the
+    kept ones, and their number.  A row without candidates gives -1."""
+    V, = _int32(V=V)
+    words = (V + 31) // 32
+
+    def kernel(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, cfg_scale=None, allowed=None, out=None,
+               logprob=None, kept=None):
+        T = _torch()
+        f32, i32 = T.f32, T.i32
+        if not logits.is_cuda:
+            raise ValueError("operands must live on the HIP device")
+        at, dim, shape, step = logits.get_device(), 3 if cfg else 2, logits.shape, logits.stride()
+        if len(shape) != dim or shape[-1] != V or (cfg and shape[1] != 2):
+            raise ValueError(f"logits must be [rows, {'2, ' if cfg else ''}{V}], got {tuple(shape)}")
+        rows, dt = shape[0], _code(logits, T.codes)
+        stride = step[-2] if cfg or rows > 1 else V
+        if (V > 1 and step[-1] != 1) or stride < V or (cfg and rows > 1 and step[0] != 2 * stride):
+            raise ValueError("logits' rows must be contiguous and evenly apart")
+        if cfg != (cfg_scale is not None):
+            raise ValueError("cfg_scale comes with cfg")
+        n = (rows,)
+        if out is None:
+            out = T.empty(n, device=logits.device, dtype=T.i64)
+            op = out.data_ptr()
+        else:
+            op = _need(out, "out", T.i64, at, n)
+        apart = 0
+        if allowed is not None:
+            if allowed.dim() != 2 or allowed.shape[0] not in (1, rows):
+                raise ValueError(f"allowed must be int32 [{rows} or 1, {words}]")
+            _need(allowed, "allowed", i32, at, (allowed.shape[0], words))
+            apart = words if allowed.shape[0] == rows else 0
+        size = _sample_workspace(rows, V, dt)
+        ws = T.empty(size, device=logits.device, dtype=T.u8) if size else None
+        _call(T, T.lib.sk_op_sample_rows, at, rows, V, dt, logits.data_ptr(), stride, _need(u, "u", T.f64, at, n),
+              None if temperature is None else _need(temperature, "temperature", f32, at, n),
+              None if top_k is None else _need(top_k, "top_k", i32, at, n),
+              None if top_p is None else _need(top_p, "top_p", f32, at, n),
+              None if min_p is None else _need(min_p, "min_p", f32, at, n),
+              None if cfg_scale is None else _need(cfg_scale, "cfg_scale", f32, at, n),
+              None if allowed is None else allowed.data_ptr(), apart, op,
+              None if logprob is None else _need(logprob, "logprob", f32, at, n),
+              None if kept is None else _need(kept, "kept", i32, at, n), ws.data_ptr() if size else None, size)
         return out
     return kernel
