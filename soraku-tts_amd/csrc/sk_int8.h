@@ -28,6 +28,7 @@ namespace sk {
 namespace int8 {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr int GROUP = 128;                        // codes of a row: whole groups of these
 
@@ -42,26 +43,26 @@ template <> __device__ __forceinline__ uint16_t from_f<uint16_t>(float v) {
 
 // ------------------------------------------------------------ codes of a row
 
-// 8 neighbouring values of a row from k on, 0 past K.  `whole`: K is a multiple
-// of 8 and rows are 16-byte aligned.
-template <typename X>
-__device__ __forceinline__ void load8(const X* row, int k, int K, bool whole, float (&t)[8]) {
-  if (whole) {
-    if (k >= K) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = 0.f;
-    } else if constexpr (sizeof(X) == 2) {
-      const uint4 v = *reinterpret_cast<const uint4*>(row + k);
+// 8 neighbouring values of a row from k on, 0 past K.  WHOLE: K is a multiple of 8, so
+// that rows are aligned for pieces of 8.
+template <typename X, bool WHOLE>
+__device__ __forceinline__ void load8(const X* row, int k, int K, float (&t)[8]) {
+  if constexpr (WHOLE) {                          // past K the last piece is loaded, and not taken
+    const X* p = row + min(k, K - 8);
+    if constexpr (sizeof(X) == 2) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        t[2 * i] = __uint_as_float(w[i] << 16);
-        t[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        const uint32_t x = k < K ? w[i] : 0u;
+        t[2 * i] = __uint_as_float(x << 16);
+        t[2 * i + 1] = __uint_as_float(x & 0xffff0000u);
       }
     } else {
-      const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
-      t[0] = a.x; t[1] = a.y; t[2] = a.z; t[3] = a.w;
-      t[4] = b.x; t[5] = b.y; t[6] = b.z; t[7] = b.w;
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = k < K ? x[i] : 0.f;
     }
   } else {
 #pragma unroll
@@ -69,15 +70,19 @@ __device__ __forceinline__ void load8(const X* row, int k, int K, bool whole, fl
   }
 }
 // x^2 of 8 values, and t times the gain (rounded to FP32: the definition's one rounding).
-__device__ __forceinline__ float weigh8(const float* gain, int k, int K, bool whole, float (&t)[8]) {
+enum { PLAIN = 0, NORM = 1, GAIN = 2 };           // what becomes of a row first: nothing, a norm, a norm with a gain
+template <bool WHOLE, int MODE>
+__device__ __forceinline__ float weigh8(const float* gain, int k, int K, float (&t)[8]) {
   float squares = 0.f;
+  if constexpr (MODE != PLAIN)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) squares = fmaf(t[i], t[i], squares);
-  if (!gain) return squares;
-  float g[8];
-  load8<float>(gain, k, K, whole, g);
+    for (int i = 0; i < 8; ++i) squares = fmaf(t[i], t[i], squares);
+  if constexpr (MODE == GAIN) {
+    float g[8];
+    load8<float, WHOLE>(gain, k, K, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] *= g[i];
+    for (int i = 0; i < 8; ++i) t[i] *= g[i];
+  }
   return squares;
 }
 // The largest |t| as bits: NaN above infinity above every number.
@@ -87,54 +92,79 @@ __device__ __forceinline__ uint32_t top8(const float (&t)[8], uint32_t top) {
   return top;
 }
 
-// How a row with this largest |t| is coded.  Rows of less than 2^-60 are
-// multiplied by 2^80 first (exact), so that 127 / top is a number.
+// How a row with this largest |t| is coded.  Rows of less than 2^-60 or more than 2^100 are multiplied by a
+// power of two first (exact but for values that are no code), so that nothing below over- or underflows.
 struct Coder {
   float r, up, top;                               // 127 / (top up), up, top up
   float scale;                                    // top / 127
   __device__ explicit Coder(uint32_t bits) {
     const float t = __uint_as_float(bits);
     const bool bad = bits >= 0x7f800000u;
-    up = t < 0x1p-60f ? 0x1p80f : 1.f;
+    up = t < 0x1p-60f ? 0x1p80f : t > 0x1p100f ? 0x1p-20f : 1.f;
     top = t * up;
     r = bad || bits == 0 ? 0.f : 127.f / top;
     scale = bad ? __uint_as_float(0x7fc00000u) : t / 127.f;
-    if (bad) up = 0.f;                            // its values: 0 times r is no code either way
   }
-  // The nearest whole number of 127 t / top.  The rounded product is off by at most
-  // 127 * 2^-23 = 1.5e-5; within 1e-4 of a middle l + 1/2, 254 t and (2 l + 1) top (at most 33
-  // bits each) are compared in 64 bits, exactly.
-  __device__ __forceinline__ int code(float t) const {
-    const float f = t * up * r, q = rintf(f), d = f - q;
-    int c = (int)q;
-    if (fabsf(d) > 0.4999f) {
-      const int l = d > 0.f ? c : c - 1;
-      const double a = 254.0 * (double)(t * up), b = (2.0 * l + 1.0) * (double)top;
-      c = a > b ? l + 1 : a < b ? l : l + (l & 1);
-    }
-    return c;
+  // The nearest whole number of 127 t / top, t multiplied by up, exactly.  With the middle m = floor(t r) + 1/2 (floor
+  // of the rounded product may be one off next to a whole number, where the other side of m decides alike), m top
+  // is ph + pl exactly; 127 t - ph is rounded where it is far from 0, and exact where it matters: next to a
+  // middle it is below 2^-13 top, a multiple of t's last place.
+  __device__ __forceinline__ int exact(float t) const {
+    const float l = floorf(t * r), m = l + 0.5f;
+    const float ph = m * top, pl = fmaf(m, top, -ph), d = fmaf(127.f, t, -ph);
+    const int c = (int)l;
+    return c + (d > pl ? 1 : d < pl ? 0 : (c & 1));
   }
-  // 8 codes; of a row that has none (r = 0: zeros, infinities, NaN) zeros.
-  __device__ __forceinline__ uint2 code8(const float (&t)[8]) const {
-    uint32_t w[2] = {0, 0};
-    if (r != 0.f) {
+  // Values as the others want them.
+  __device__ __forceinline__ void scale8(float (&t)[8]) const {
+    if (up != 1.f)                                // the row's: all lanes alike
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t)(code(t[i]) & 0xff) << (8 * (i % 4));
+      for (int i = 0; i < 8; ++i) t[i] *= up;
+  }
+  // 8 codes; of a row that has none (r = 0: zeros, infinities, NaN) zeros.  The rounded product t r is off by at
+  // most 127 * 2^-23 = 1.5e-5; adding 1.5 * 2^23 rounds it to a whole number, which the sum's lowest
+  // byte holds.  Where one of a wave's is within 1e-4 of a middle, as quotients of BF16 values often are, they
+  // are taken exactly (12,288 x 2048 in BF16: most waves).
+  __device__ __forceinline__ uint2 code8(const float (&t)[8]) const {
+    constexpr float MAGIC = 12582912.f;
+    uint32_t q[8];
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = t[i] * r, s = f + MAGIC;
+      q[i] = __float_as_uint(s);
+      far = fmaxf(far, fabsf(f - (s - MAGIC)));
     }
-    return make_uint2(w[0], w[1]);
+    if (__any(far > 0.4999f)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = (uint32_t)exact(t[i]);
+    }
+    auto pack = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+    };
+    const uint32_t some = r != 0.f ? ~0u : 0u;
+    return make_uint2(pack(q[0], q[1], q[2], q[3]) & some, pack(q[4], q[5], q[6], q[7]) & some);
   }
 };
 
-// Over a wave, in every lane.
+// Over a wave, in every lane: 16 neighbours by exchanges in registers, then the four groups.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
+  v = max(v, (uint32_t)dpp<0xb1>((int)v));        // quad_perm [1,0,3,2]
+  v = max(v, (uint32_t)dpp<0x4e>((int)v));        // quad_perm [2,3,0,1]
+  v = max(v, (uint32_t)dpp<0x141>((int)v));       // row_half_mirror
+  v = max(v, (uint32_t)dpp<0x140>((int)v));       // row_mirror
+  auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+  return max(max(at(0), at(16)), max(at(32), at(48)));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  v += __int_as_float(dpp<0xb1>(__float_as_int(v)));
+  v += __int_as_float(dpp<0x4e>(__float_as_int(v)));
+  v += __int_as_float(dpp<0x141>(__float_as_int(v)));
+  v += __int_as_float(dpp<0x140>(__float_as_int(v)));
+  auto at = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+  return (at(0) + at(16)) + (at(32) + at(48));
 }
 
 // Sums of squares have one order whatever holds the row, so that a row's norm does not
@@ -151,45 +181,39 @@ struct RowsArgs {
   const void* x; const float* gain; float eps;    // eps < 0: not normalised
   int R, K, Kp;
   int8_t* codes; float* scales;
-  int* zero; int n_zero;                          // words that the launch also sets to 0 (tickets of the product)
 };
 
 // Codes of R rows: W waves per row, C chunks of 512 W values held in registers (C = 0:
 // any K, read twice).  Bytes bound it: each value read once (the second read of C = 0
 // comes from cache) and each code written once.
-template <typename X, int W, int C>
+template <typename X, int W, int C, bool WHOLE, int MODE>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (blockIdx.x == 0)
-    for (int i = tid; i < a.n_zero; i += 256) a.zero[i] = 0;
   const int row = blockIdx.x * (4 / W) + wave / W;
   if (W < 4 && row >= a.R) return;                // whole waves, and no barrier below for W = 1
-  const bool whole = a.K % 8 == 0;
   const X* x = static_cast<const X*>(a.x) + (size_t)row * a.K;
   const int k0 = (wave % W * 64 + lane) * 8;
-  const float* gain = a.eps >= 0.f ? a.gain : nullptr;
   constexpr int STEP = W * BLOCK, R = 4 / W;       // values per step, rows per workgroup
   __shared__ float blocks[R][C ? C * W : (1 << 17) / BLOCK];
   float* mine = blocks[wave / W];
-  const bool norm = a.eps >= 0.f;
   uint32_t top = 0;
   float t[C ? C : 1][8];
   auto take = [&](int k, float (&v)[8]) {
-    float s = weigh8(gain, k, a.K, whole, v);
+    float s = weigh8<WHOLE, MODE>(a.gain, k, a.K, v);
     top = top8(v, top);
-    if (norm) {
+    if constexpr (MODE != PLAIN) {
       s = wave_sum(s);
       if (lane == 0) mine[k / BLOCK] = s;
     }
   };
   if constexpr (C > 0) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) load8<X>(x, k0 + c * STEP, a.K, whole, t[c]);
+    for (int c = 0; c < C; ++c) load8<X, WHOLE>(x, k0 + c * STEP, a.K, t[c]);
 #pragma unroll
     for (int c = 0; c < C; ++c) take(k0 + c * STEP, t[c]);
   } else {
     for (int k = k0; k - lane * 8 < a.K; k += STEP) {   // whole waves
-      load8<X>(x, k, a.K, whole, t[0]);
+      load8<X, WHOLE>(x, k, a.K, t[0]);
       take(k, t[0]);
     }
   }
@@ -201,18 +225,21 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
   }
   const Coder coder(top);
-  if (wave % W == 0 && lane == 0) a.scales[row] = norm ? coder.scale * norm_of(mine, a.K, a.eps) : coder.scale;
+  if (wave % W == 0 && lane == 0) a.scales[row] = MODE != PLAIN ? coder.scale * norm_of(mine, a.K, a.eps) : coder.scale;
   int8_t* q = a.codes + (size_t)row * a.Kp;
   if constexpr (C > 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int k = k0 + c * STEP;
-      if (k < a.Kp) *reinterpret_cast<uint2*>(q + k) = coder.code8(t[c]);
+      coder.scale8(t[c]);
+      const uint2 v = coder.code8(t[c]);
+      if (k < a.Kp) *reinterpret_cast<uint2*>(q + k) = v;
     }
   } else {
     for (int k = k0; k < a.Kp; k += STEP) {
-      load8<X>(x, k, a.K, whole, t[0]);
-      weigh8(gain, k, a.K, whole, t[0]);
+      load8<X, WHOLE>(x, k, a.K, t[0]);
+      weigh8<WHOLE, MODE>(a.gain, k, a.K, t[0]);
+      coder.scale8(t[0]);
       *reinterpret_cast<uint2*>(q + k) = coder.code8(t[0]);
     }
   }
@@ -226,54 +253,63 @@ struct LinearArgs {
   const float* bias;                              // [N] (SwiGLU: [2 N]) or null
   const void* res; void* out;                     // [M][N] of X; res may be null, or out itself
   int M, N, Kp;
-  int mt, nt, ksplit, gm;                         // tiles along M and N, cuts of K; tiles along M per group
-  int* part; int* ticket;                         // ksplit > 1: sums of the cuts, arrivals per tile
+  int mt, nt, gm;                                 // tiles along M and N, tiles along M per group
 };
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
+// g / (1 + e^-g) with the GPU's own powers of two and reciprocals (each within a step of the result): t = -g log2(e)
+// in two parts, 2^t_hi (1 + t_lo ln 2).  Below -87 it is 0.
+__device__ __forceinline__ float silu(float g) {
+  constexpr float L = 1.44269504088896341f, L2 = 1.92596299e-8f, LN2 = 0.693147181f;   // log2(e) = L + L2
+  const float h = __builtin_amdgcn_fmed3f(g, -150.f, 150.f);   // past those e is 0 or infinite
+  const float t = -h * L, lo = fmaf(-h, L2, fmaf(-h, L, -t));
+  const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, LN2, 1.f);
+  return g * __builtin_amdgcn_rcpf(1.f + e);
+}
+// act of sums of row m (scale s) and column c (scale w, bias b; SwiGLU: and of its up column).
+template <bool SWIGLU>
+__device__ __forceinline__ float act_of(int acc, int up, float s, float w, float w2, float b, float b2) {
+  const float y = (float)acc * s * w + b;
+  if constexpr (SWIGLU) return silu(y) * ((float)up * s * w2 + b2);
+  else return y;
+}
 
-// Four neighbouring outputs n .. n + 3 of row m from their sums.
-template <typename X, bool SWIGLU>
-__device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i acc, v4i up) {
+// C (4 or 8) neighbouring outputs n .. n + C - 1 of row m before the residual.
+template <typename X, int C>
+__device__ __forceinline__ void emit(const LinearArgs& a, int m, int n, float (&y)[C]) {
   if (m >= a.M || n >= a.N) return;
-  const float s = a.as[m];
   const size_t at = (size_t)m * a.N + n;
-  const bool four = (a.N & 3) == 0;               // then rows are 16-byte (BF16 8-byte) aligned, and n + 3 < N
-  float y[4], r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = min(n + i, a.N - 1);
-    y[i] = (float)acc[i] * s * a.ws[c];
-    if (a.bias) y[i] += a.bias[c];
-    if constexpr (SWIGLU) {
-      float u = (float)up[i] * s * a.ws[a.N + c];
-      if (a.bias) u += a.bias[a.N + c];
-      y[i] = silu(y[i]) * u;
-    }
-  }
   X* o = static_cast<X*>(a.out) + at;
   const X* re = static_cast<const X*>(a.res) + at;
-  if (four) {
+  if (a.N % C == 0) {                             // then n + C <= N, and rows are aligned for pieces of C
     if constexpr (sizeof(X) == 4) {
       if (a.res) {
-        const float4 v = *reinterpret_cast<const float4*>(re);
-        y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
-      }
-      *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
-    } else {
-      if (a.res) {
-        const uint2 v = *reinterpret_cast<const uint2*>(re);
-        r[0] = __uint_as_float(v.x << 16); r[1] = __uint_as_float(v.x & 0xffff0000u);
-        r[2] = __uint_as_float(v.y << 16); r[3] = __uint_as_float(v.y & 0xffff0000u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] += r[i];
+        for (int i = 0; i < C / 4; ++i) {
+          const float4 v = reinterpret_cast<const float4*>(re)[i];
+          y[4 * i] += v.x; y[4 * i + 1] += v.y; y[4 * i + 2] += v.z; y[4 * i + 3] += v.w;
+        }
       }
-      *reinterpret_cast<uint2*>(o) = make_uint2((uint32_t)from_f<X>(y[0]) | (uint32_t)from_f<X>(y[1]) << 16,
-                                                (uint32_t)from_f<X>(y[2]) | (uint32_t)from_f<X>(y[3]) << 16);
+#pragma unroll
+      for (int i = 0; i < C / 4; ++i)
+        reinterpret_cast<float4*>(o)[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+    } else {
+      typedef uint32_t Piece __attribute__((ext_vector_type(C / 2)));
+      if (a.res) {
+        const Piece v = *reinterpret_cast<const Piece*>(re);
+#pragma unroll
+        for (int i = 0; i < C / 2; ++i) {
+          y[2 * i] += __uint_as_float(v[i] << 16);
+          y[2 * i + 1] += __uint_as_float(v[i] & 0xffff0000u);
+        }
+      }
+      Piece v;
+#pragma unroll
+      for (int i = 0; i < C / 2; ++i) v[i] = (uint32_t)from_f<X>(y[2 * i]) | (uint32_t)from_f<X>(y[2 * i + 1]) << 16;
+      *reinterpret_cast<Piece*>(o) = v;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < C; ++i)
       if (n + i < a.N) o[i] = from_f<X>(a.res ? y[i] + to_f<X>(re[i]) : y[i]);
   }
 }
@@ -284,15 +320,16 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, v4i a
 // so that the 16 rows of a matrix fragment lie in different banks.  S stages in a ring with one
 // barrier each.  The matrix cores take the weights as their row operand, so a lane ends up
 // with 4 neighbouring columns of one row.  Rows past M or N are clamped on load and not stored.
-template <typename X, bool SWIGLU, int BM, int BN, int WM, int WN, int S>
+template <typename X, bool SWIGLU, int BM, int BN, int WM, int WN, int S, int H>
 __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
-  constexpr int W = WM * WN, ROWS = BM + BN, PER = ROWS / 8 / W;   // loads of 8 rows, of them per wave
-  static_assert(ROWS % (8 * W) == 0, "every wave loads alike");
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16, STAGE = ROWS * 128;
+  constexpr int W = WM * WN, ROWS = BM + BN, LR = 16 / H, PER = ROWS / LR / W;   // rows per load, loads per wave
+  static_assert(ROWS % (LR * W) == 0 && BM % 16 == 0, "every wave loads alike");
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, RB = 64 * H, STAGE = ROWS * RB;
   static_assert(!SWIGLU || TN % 2 == 0, "every wave holds gate and up of its columns");
   __shared__ __attribute__((aligned(1024))) char lds[S * STAGE];
+  __shared__ __attribute__((aligned(16))) float row_s[BM], col_s[BN], col_b[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane & 15, q4 = lane >> 4;
+  const int i32 = lane & 31, hi = lane >> 5;
 
   // Tile of this workgroup: an XCD's workgroups (every eighth) take a run of tiles, in groups
   // of gm along M with M fastest, so that the tiles it works on at a time share panels in its L2.
@@ -304,20 +341,21 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   constexpr int NC = SWIGLU ? BN / 2 : BN;
   const int n0 = gr / gm * NC;
 
-  const int Kp = a.Kp, nst = Kp / 128;
+  const int Kp = a.Kp, nst = Kp / RB;
+  auto turn = [](int row) { return H == 1 ? row >> 2 & 3 : row >> 1 & 7; };
   const char* gb[PER];
   unsigned voff[PER];
 #pragma unroll
   for (int c = 0; c < PER; ++c) {
-    const int g = wave * PER + c;                 // rows 8 g .. 8 g + 7 of the stage
+    const int g = wave * PER + c;                 // rows LR g .. LR (g + 1) - 1 of the stage
     const char* base;
     int first, last;
-    if (g < BM / 8) {
+    if (g < BM / LR) {
       base = reinterpret_cast<const char*>(a.a);
-      first = m0 + g * 8;
+      first = m0 + g * LR;
       last = a.M - 1;
     } else {
-      const int b = g * 8 - BM;                   // row of the weights' part
+      const int b = g * LR - BM;                 // row of the weights' part
       base = reinterpret_cast<const char*>(a.w);
       if (SWIGLU && b >= NC) base += (size_t)a.N * Kp;
       first = n0 + (SWIGLU && b >= NC ? b - NC : b);
@@ -325,86 +363,159 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
     }
     const int r0 = min(first, last);
     gb[c] = base + (size_t)r0 * Kp;
-    voff[c] = (unsigned)((min(first + (lane >> 3), last) - r0) * Kp + (((lane & 7) ^ (lane >> 3)) * 16));
+    const int lr = lane / (4 * H), row = g * LR + lr;
+    voff[c] = (unsigned)((min(first + lr, last) - r0) * Kp + ((lane & (4 * H - 1)) ^ turn(row)) * 16);
   }
-  auto issue = [&](int s) {
-    const char* l = lds + (s % S) * STAGE + wave * PER * 1024;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) lds_load16(gb[c] + (size_t)s * 128, voff[c], l + c * 1024);
+  auto issue = [&](int s, int c) {
+    lds_load16(gb[c] + (size_t)s * RB, voff[c], lds + (s % S) * STAGE + (wave * PER + c) * 1024);
   };
+  for (int i = tid; i < BM; i += W * 64) row_s[i] = a.as[min(m0 + i, a.M - 1)];
+  for (int i = tid; i < BN; i += W * 64) {
+    const int c = (SWIGLU && i >= NC ? a.N : 0) + min(n0 + (SWIGLU && i >= NC ? i - NC : i), a.N - 1);
+    col_s[i] = a.ws[c];
+    col_b[i] = a.bias ? a.bias[c] : 0.f;
+  }
   const int wm = wave / WN, wn = wave % WN;
   // first row in the weights' part of column group j of this wave
   auto col = [&](int j) {
-    if constexpr (SWIGLU) return j < TN / 2 ? (wn * (TN / 2) + j) * 16 : NC + (wn * (TN / 2) + j - TN / 2) * 16;
-    else return (wn * TN + j) * 16;
+    if constexpr (SWIGLU) return j < TN / 2 ? (wn * (TN / 2) + j) * 32 : NC + (wn * (TN / 2) + j - TN / 2) * 32;
+    else return (wn * TN + j) * 32;
   };
-  v4i acc[TM][TN];
+  v16i acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s)
-    if (s < nst) issue(s);
-  for (int s = 0; s < nst; ++s) {
-    const int ahead = nst - 1 - s;
-    if (ahead >= S - 2) stage_sync<PER * (S - 2)>();
-    else if (S > 3 && ahead == 1) stage_sync<(S > 3 ? PER : 0)>();
-    else stage_sync<0>();
-    if (s + S - 1 < nst) issue(s + S - 1);
-    const char* l = lds + (s % S) * STAGE + i16 * 128;
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+  // A stage's fragments come in four quarters of 32 codes, each a quarter ahead of its products, read
+  // between the products of the one before.  While the last one's products run, the
+  // stage's place in the ring is free for its next loads and the next stage's first quarter is on its way.
+  v4i af[2][TM], bf[2][TN];
+  auto piece = [&](int s, int q) { return lds + (s % S) * STAGE + i32 * RB + ((q * 2 + hi) ^ turn(i32)) * 16; };
+  auto fetch = [&](const char* l, int set, int f) {   // fragment f of a quarter
+    if (f < TN) bf[set][f] = *reinterpret_cast<const v4i*>(l + (BM + col(f)) * RB);
+    else af[set][f - TN] = *reinterpret_cast<const v4i*>(l + (wm * TM + f - TN) * 32 * RB);
+  };
+  // Loads are spread over the products too: a wave that issues all of a stage's at once stands in line for
+  // the memory pipe, and its matrix core idles.
+  constexpr int P = TM * TN, L0 = (PER + 1) / 2;  // products of a piece; loads in the stage's last piece, the others in the next one's first
+  auto multiply = [&](int set, const char* l, int load, int c0, int c1) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const char* lk = l + (((kb * 4 + q4) ^ (i16 & 7)) * 16);
-      v4i af[TM], bf[TN];
+    for (int p = 0; p < P; ++p) {
+      const int i = p / TN, j = p % TN;
+      acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[set][j], af[set][i], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) af[i] = *reinterpret_cast<const v4i*>(lk + (wm * TM + i) * 2048);
+      for (int f = 0; f < TM + TN; ++f)
+        if (f * P / (TM + TN) == p) fetch(l, set ^ 1, f);
+      if (load >= 0) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) bf[j] = *reinterpret_cast<const v4i*>(lk + (BM + col(j)) * 128);
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af[i], acc[i][j], 0, 0, 0);
+        for (int c = c0; c < c1; ++c)
+          if ((2 * (c - c0) + 1) * P / (2 * (c1 - c0)) == p) issue(load, c);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // stages in flight behind the one that is waited for: at most S - 1 (first wait), then S - 2
+  auto arrive = [&](int behind) {
+    if (S > 4 && behind >= 4) stage_sync<(S > 4 ? 4 : 0) * PER>();
+    else if (S > 3 && behind >= 3) stage_sync<(S > 3 ? 3 : 0) * PER>();
+    else if (S > 2 && behind >= 2) stage_sync<(S > 2 ? 2 : 0) * PER>();
+    else if (behind >= 1) stage_sync<PER>();
+    else stage_sync<0>();
+  };
+  static_assert(S >= 2 && S <= 5, "arrive() counts up to four stages");
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (s < nst) {
+#pragma unroll
+      for (int c = 0; c < PER; ++c) issue(s, c);
+    }
+  arrive(min(S, nst) - 1);
+#pragma unroll
+  for (int f = 0; f < TM + TN; ++f) fetch(piece(0, 0), 0, f);
+  constexpr int Q = 2 * H;                        // pieces of a stage
+  for (int s = 0; s < nst; ++s) {
+    // stage s - 1 + S goes on into the place of stage s - 1
+    multiply(0, piece(s, 1), s && s - 1 + S < nst ? s - 1 + S : -1, L0, PER);
+#pragma unroll
+    for (int q = 1; q < Q - 1; ++q) multiply(q & 1, piece(s, q + 1), -1, 0, 0);
+    if (s + 1 < nst) arrive(min(S - 2, nst - 2 - s));
+    multiply(1, piece(s + 1, 0), s + S < nst ? s + S : -1, 0, L0);   // past the last stage: read and not used
   }
+  // Lane: row m = lane % 32 of each 32 x 32 tile, columns 8 g + 4 (lane / 32) .. + 3 for g in 0 .. 3.  Through the
+  // wave's own part of LDS, so that stores are of whole pieces of rows: as they lie they are
+  // 8 or 16 bytes of 32 rows each (8192 x 8192 outputs in BF16: 75 us).
+  constexpr int TO = SWIGLU ? TN / 2 : TN;        // tiles out
+  constexpr int CJ = TO % 2 == 0 && W * 32 * 68 * 4 <= S * STAGE ? 2 : 1, CW = CJ * 32, LD = CW + 4;   // of them, and columns, at a time
+  static_assert(W * 32 * LD * 4 <= S * STAGE, "the waves' parts lie in the ring");
+  float* part = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+  __syncthreads();                                // the ring is read
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = m0 + (wm * TM + i) * 16 + i16;
+    const int r0 = (wm * TM + i) * 32;
+    const float sc = row_s[r0 + i32];
 #pragma unroll
-    for (int j = 0; j < (SWIGLU ? TN / 2 : TN); ++j)
-      finish4<X, SWIGLU>(a, m, n0 + col(j) + q4 * 4, acc[i][j], acc[i][SWIGLU ? j + TN / 2 : j]);
+    for (int j0 = 0; j0 < TO; j0 += CJ) {
+#pragma unroll
+      for (int j = j0; j < j0 + CJ; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = col(j) + g * 8 + hi * 4;
+          const float4 w = *reinterpret_cast<const float4*>(col_s + c), b = *reinterpret_cast<const float4*>(col_b + c);
+          float4 w2 = w, b2 = b;
+          if constexpr (SWIGLU) {
+            w2 = *reinterpret_cast<const float4*>(col_s + NC + c);
+            b2 = *reinterpret_cast<const float4*>(col_b + NC + c);
+          }
+          const v16i &y = acc[i][j], &u = acc[i][SWIGLU ? j + TN / 2 : j];
+          float4 o;
+          o.x = act_of<SWIGLU>(y[4 * g], u[4 * g], sc, w.x, w2.x, b.x, b2.x);
+          o.y = act_of<SWIGLU>(y[4 * g + 1], u[4 * g + 1], sc, w.y, w2.y, b.y, b2.y);
+          o.z = act_of<SWIGLU>(y[4 * g + 2], u[4 * g + 2], sc, w.z, w2.z, b.z, b2.z);
+          o.w = act_of<SWIGLU>(y[4 * g + 3], u[4 * g + 3], sc, w.w, w2.w, b.w, b2.w);
+          *reinterpret_cast<float4*>(part + i32 * LD + (j - j0) * 32 + g * 8 + hi * 4) = o;
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < 32 * CW / 8 / 64; ++e) {
+        const int r = (e * 64 + lane) / (CW / 8), c = (e * 64 + lane) % (CW / 8) * 8;
+        const float4 lo = *reinterpret_cast<const float4*>(part + r * LD + c), up = *reinterpret_cast<const float4*>(part + r * LD + c + 4);
+        float o[8] = {lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
+        emit<X, 8>(a, m0 + r0 + r, n0 + col(j0) + c, o);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
 // Products of few rows: a workgroup has NT tiles of 16 weight rows (SwiGLU: half of them gate,
 // half the same rows of up) and MT tiles of 16 activation rows, and its W waves take every W-th
 // unit of 128 codes; their sums meet in LDS.  The weights' bytes bound it: they go
-// straight to registers as matrix fragments, D units ahead, and are read once for all
-// rows.  K may be cut over ksplit workgroups; the last one to arrive adds the cuts up.
+// straight to registers as matrix fragments, D units ahead, and are read once for all rows.
 //
 // FUSED (up to 8 rows, a power of two times K at most 16,384): the workgroup codes the
 // activations' rows itself, each into its own LDS, which saves the launch that writes them;
 // the weights' first units are on their way meanwhile.
-template <typename X, bool SWIGLU, bool FUSED, int MT, int NT, int W>
+template <typename X, bool SWIGLU, bool FUSED, bool WHOLE, int MT, int NT, int W, int D>
 __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
   static_assert(!SWIGLU || NT % 2 == 0, "gate and up of the same columns");
   static_assert(!FUSED || (MT == 1 && W == 8), "8 waves code up to 8 rows");
-  constexpr int D = 2, NC = (SWIGLU ? NT / 2 : NT) * 16;
+  constexpr int NC = (SWIGLU ? NT / 2 : NT) * 16;
   extern __shared__ __attribute__((aligned(16))) char dyn[];   // FUSED: codes, rows Kp + 16 apart; then the waves' sums
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane & 15, q4 = lane >> 4;
-  const int tile = blockIdx.x / a.ksplit, ks = blockIdx.x - tile * a.ksplit;
-  const int n0 = tile * NC, m0 = blockIdx.y * (MT * 16);
+  const int n0 = blockIdx.x * NC, m0 = blockIdx.y * (MT * 16);
   const int Kp = a.Kp, units = Kp / 128;
-  const int u0 = (int)((int64_t)units * ks / a.ksplit), nu = (int)((int64_t)units * (ks + 1) / a.ksplit) - u0;
-  const int mine = nu > wave ? (nu - wave + W - 1) / W : 0;
+  const int mine = units > wave ? (units - wave + W - 1) / W : 0;
 
   const int8_t* wp[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const bool is_up = SWIGLU && j >= NT / 2;
     const int n = min(n0 + (is_up ? j - NT / 2 : j) * 16 + i16, a.N - 1);
-    wp[j] = a.w + ((size_t)(is_up ? a.N : 0) + n) * Kp + (size_t)(u0 + wave) * 128 + q4 * 16;
+    wp[j] = a.w + ((size_t)(is_up ? a.N : 0) + n) * Kp + wave * 128 + q4 * 16;
   }
   v4i b[D][NT][2];
   auto load_w = [&](int d, int i) {
@@ -432,7 +543,7 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
     __shared__ float blocks[8 * C];               // of a row: its waves' C
     const int rows2 = a.M > 4 ? 8 : a.M > 2 ? 4 : a.M;   // rows up to a power of two
     const int wpr = 8 / rows2, row = wave / wpr, step = wpr * BLOCK;
-    const bool whole = r.K % 8 == 0, norm = r.eps >= 0.f;
+    const bool norm = r.eps >= 0.f;
     const float* gain = norm ? r.gain : nullptr;
     const int k0 = (wave % wpr * 64 + lane) * 8;
     float t[C][8];
@@ -441,11 +552,13 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
       const X* x = static_cast<const X*>(r.x) + (size_t)row * r.K;
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        if (c * step < r.K) load8<X>(x, k0 + c * step, r.K, whole, t[c]);
+        if (c * step < r.K) load8<X, WHOLE>(x, k0 + c * step, r.K, t[c]);
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (c * step < r.K) {
-          float s = weigh8(gain, k0 + c * step, r.K, whole, t[c]);
+          const int k = k0 + c * step;
+          float s = norm ? weigh8<WHOLE, NORM>(nullptr, k, r.K, t[c]) : 0.f;
+          if (gain) weigh8<WHOLE, GAIN>(gain, k, r.K, t[c]);
           top = top8(t[c], top);
           if (norm) {
             s = wave_sum(s);
@@ -464,7 +577,11 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int k = k0 + c * step;
-        if (k < Kp) *reinterpret_cast<uint2*>(dyn + (size_t)row * (Kp + 16) + k) = coder.code8(t[c]);
+        if (c * step < Kp) {
+          coder.scale8(t[c]);
+          const uint2 v = coder.code8(t[c]);
+          if (k < Kp) *reinterpret_cast<uint2*>(dyn + (size_t)row * (Kp + 16) + k) = v;
+        }
       }
     }
     __syncthreads();
@@ -472,7 +589,7 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
   } else {
 #pragma unroll
     for (int j = 0; j < MT; ++j)
-      ap[j] = a.a + (size_t)min(m0 + j * 16 + i16, a.M - 1) * Kp + (size_t)(u0 + wave) * 128 + q4 * 16;
+      ap[j] = a.a + (size_t)min(m0 + j * 16 + i16, a.M - 1) * Kp + wave * 128 + q4 * 16;
 #pragma unroll
     for (int d = 0; d < D; ++d)
       if (d < mine) load_a(d, d);
@@ -516,32 +633,22 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
     for (int w = 1; w < W; ++w) s += sum[w * VECS + e];
     return s;
   };
-  const bool cut = !FUSED && a.ksplit > 1;
-  const size_t all = (size_t)blockIdx.y * (gridDim.x / a.ksplit) + tile;
-  v4i* part = reinterpret_cast<v4i*>(a.part) + all * a.ksplit * VECS;
-  if (cut) {
-    for (int e = tid; e < VECS; e += W * 64) part[(size_t)ks * VECS + e] = add_waves(e);
-    __threadfence();
-    __shared__ int arrived;
-    __syncthreads();
-    if (tid == 0) arrived = __hip_atomic_fetch_add(a.ticket + all, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (arrived != a.ksplit - 1) return;
-    __threadfence();
-  }
-  auto total = [&](int e) {
-    if (!cut) return add_waves(e);
-    v4i s = part[e];
-    for (int c = 1; c < a.ksplit; ++c) s += part[(size_t)c * VECS + e];
-    return s;
-  };
   if constexpr (FUSED) a.as = row_scale;
   constexpr int OT = SWIGLU ? NT / 2 : NT;        // output tiles
   for (int e = tid; e < MT * OT * 64; e += W * 64) {
     const int l = e & 63, j = e / 64 % OT, i = e / 64 / OT;
-    const v4i y = total((i * NT + j) * 64 + l);
-    const v4i up = SWIGLU ? total((i * NT + j + NT / 2) * 64 + l) : y;
-    finish4<X, SWIGLU>(a, m0 + i * 16 + (l & 15), n0 + j * 16 + (l >> 4) * 4, y, up);
+    const v4i y = add_waves((i * NT + j) * 64 + l);
+    const v4i up = SWIGLU ? add_waves((i * NT + j + NT / 2) * 64 + l) : y;
+    const int m = m0 + i * 16 + (l & 15), n = n0 + j * 16 + (l >> 4) * 4;
+    float out[4];
+    const float sc = a.as[min(m, a.M - 1)];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int c = min(n + v, a.N - 1);
+      out[v] = act_of<SWIGLU>(y[v], up[v], sc, a.ws[c], SWIGLU ? a.ws[a.N + c] : 0.f, a.bias ? a.bias[c] : 0.f,
+                              SWIGLU && a.bias ? a.bias[a.N + c] : 0.f);
+    }
+    emit<X, 4>(a, m, n, out);
   }
 }
 

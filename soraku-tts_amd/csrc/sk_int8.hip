@@ -33,78 +33,111 @@ int check_linear(int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act) {
   return check_type(xdtype);
 }
 
-template <typename X, int W>
-void launch_rows_w(const RowsArgs& a, hipStream_t st) {
-  const dim3 grid((a.R + 4 / W - 1) / (4 / W));
-  switch ((a.Kp + W * 512 - 1) / (W * 512)) {
-    case 1: hipLaunchKernelGGL((rows_kernel<X, W, 1>), grid, dim3(256), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((rows_kernel<X, W, 2>), grid, dim3(256), 0, st, a); break;
-    case 3:
-    case 4: hipLaunchKernelGGL((rows_kernel<X, W, 4>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((rows_kernel<X, W, 0>), grid, dim3(256), 0, st, a); break;
+// A wave per row where rows are short and many (12,288 of 2,048), four where not, so that 32 rows spread
+// over as many CUs; up to 8,192 values stay in registers.
+template <typename X, int MODE>
+void launch_rows_as(const RowsArgs& a, hipStream_t st) {
+  auto go = [&](auto kernel, int per) { hipLaunchKernelGGL(kernel, dim3((a.R + per - 1) / per), dim3(256), 0, st, a); };
+  if (a.K % 8 != 0) go(rows_kernel<X, 4, 0, false, MODE>, 1);
+  else if (a.Kp <= 2048 && a.R >= 1024) {
+    if (a.Kp <= 512) go(rows_kernel<X, 1, 1, true, MODE>, 4);
+    else if (a.Kp <= 1024) go(rows_kernel<X, 1, 2, true, MODE>, 4);
+    else go(rows_kernel<X, 1, 4, true, MODE>, 4);
+  } else {
+    if (a.Kp <= 2048) go(rows_kernel<X, 4, 1, true, MODE>, 1);
+    else if (a.Kp <= 4096) go(rows_kernel<X, 4, 2, true, MODE>, 1);
+    else if (a.Kp <= 8192) go(rows_kernel<X, 4, 4, true, MODE>, 1);
+    else go(rows_kernel<X, 4, 0, true, MODE>, 1);
   }
 }
 template <typename X>
 void launch_rows(const RowsArgs& a, hipStream_t st) {
-  if (a.Kp <= 2048 && a.R >= 1024) launch_rows_w<X, 1>(a, st);
-  else launch_rows_w<X, 4>(a, st);
+  if (a.eps < 0.f) launch_rows_as<X, PLAIN>(a, st);
+  else if (a.gain) launch_rows_as<X, GAIN>(a, st);
+  else launch_rows_as<X, NORM>(a, st);
 }
 
-// How a product is computed.
+// How a product is computed: by a workgroup per 16 columns and up to 32 rows, which
+// may code the rows itself, or in tiles.
 struct Plan {
   bool fused, few;
-  int bm, bn, ksplit;                             // tile (few: 16 MT x 16 NT), cuts of K
+  int tile, bm, bn;                               // of TILES; rows and columns (SwiGLU: gate and up together) of a workgroup
 };
+// Estimated us of a launch of tiles when a CU has r of them, of u stages: fix + r round + u lat + (r - 1) u thr, fitted
+// to 207 times (33 to 7,680 rows, the trunks' projections and odd ones; rms error 7 to 24%).  The tile chosen is on
+// average within 6% of the fastest (SwiGLU 3%).  E.g. 7,680 rows of 2 x 6144 x 2048: 256 x 256 204 us, 128 x 128 231;
+// 774 of 4096 x 1024: 64 x 128 9.2, 128 x 128 10.0, 256 x 256 15.6; 64 of 2048 x 6144: 64 x 64 15.4, 64 x 128 21.6.
+struct Tile { int bm, bn; float fix, round, lat, thr, fix2, round2, lat2, thr2; };   // 2: SwiGLU
+constexpr Tile TILES[] = {{256, 256, 0.f, 7.19f, 1.10f, 2.28f, 0.f, 8.47f, 1.15f, 1.87f},
+                          {192, 256, 0.f, 7.00f, .92f, 1.53f, 0.f, 7.23f, 1.00f, 1.40f},
+                          {128, 128, .98f, 4.06f, .56f, .37f, 2.16f, 1.92f, .62f, .49f},
+                          {64, 128, 2.07f, 1.73f, .41f, .26f, 2.27f, .75f, .44f, .31f},
+                          {64, 64, 1.93f, 1.35f, .26f, .18f, 2.31f, 1.04f, .42f, .19f}};
+// Up to 32 rows the weights' bytes bound a product and tiles of 64 rows would be half empty (32 rows of 2048 x
+// 6144: 10.1 us, in tiles 15.4; 64: 15.6 and 15.4).  Up to 8 the workgroups code the rows themselves where each wave
+// then has at most 2,048 values (2 rows x 4096 x 2048: 6.5 us, with a launch for the codes 8 in two).
 Plan plan_linear(int M, int N, int K, bool swiglu) {
   const int rows2 = M > 4 ? 8 : M > 2 ? 4 : M;
   Plan p{};
-  p.ksplit = 1;
-  p.few = M <= 64;
+  p.few = M <= 32;
   p.fused = M <= 8 && rows2 * K <= 16384;
   if (p.few) {
-    p.bm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    p.bn = swiglu ? 32 : 16;
-  } else {
-    p.bm = p.bn = 128;
+    p.bm = M <= 16 ? 16 : 32;
+    // wide ones read their rows' codes less often (32 rows of 2 x 6144 x 2048: 8.4 us, 9.9 by 16 columns)
+    p.bn = !swiglu ? 16 : !p.fused && N >= 4096 ? 64 : 32;
+    return p;
+  }
+  float best = 1e30f;
+  for (int i = 0; i < (int)(sizeof(TILES) / sizeof(Tile)); ++i) {
+    const Tile& t = TILES[i];
+    const int nc = swiglu ? t.bn / 2 : t.bn;
+    const int64_t tiles = (int64_t)((M + t.bm - 1) / t.bm) * ((N + nc - 1) / nc);
+    const float r = (float)((tiles + 255) / 256), u = (float)(padded(K) / 128);
+    const float us = swiglu ? t.fix2 + r * t.round2 + u * (t.lat2 + (r - 1) * t.thr2) : t.fix + r * t.round + u * (t.lat + (r - 1) * t.thr);
+    if (us < best) { best = us; p.tile = i; p.bm = t.bm; p.bn = t.bn; }
   }
   return p;
 }
 int cols_of(const Plan& p, bool swiglu) { return swiglu ? p.bn / 2 : p.bn; }
-int64_t tiles_of(const Plan& p, int M, int N, bool swiglu) {
-  const int nc = cols_of(p, swiglu);
-  return (int64_t)((M + p.bm - 1) / p.bm) * ((N + nc - 1) / nc);
-}
-// Workspace: the activations' codes, their scales, then tickets and sums of the cuts.
-struct Space { int64_t scales, tickets, parts, bytes; };
-Space space_of(const Plan& p, int M, int N, int K, bool swiglu) {
-  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  Space s{};
-  if (p.fused || M == 0) return s;
-  const int64_t tiles = tiles_of(p, M, N, swiglu);
-  s.scales = up((int64_t)M * padded(K));
-  s.tickets = s.scales + up((int64_t)M * 4);
-  s.parts = s.tickets + (p.ksplit > 1 ? up(tiles * 4) : 0);
-  s.bytes = s.parts + (p.ksplit > 1 ? tiles * p.ksplit * p.bm * p.bn * 4 : 0);
-  return s;
-}
+// Workspace: the activations' codes, then their scales.
+int64_t codes_of(int M, int K) { return ((int64_t)M * padded(K) + 255) / 256 * 256; }
+int64_t space_of(const Plan& p, int M, int K) { return p.fused || M == 0 ? 0 : codes_of(M, K) + (int64_t)M * 4; }
 
 template <typename X, bool SWIGLU>
-void launch_few(const Plan& p, LinearArgs a, const RowsArgs& r, hipStream_t st) {
-  const dim3 grid(a.nt * a.ksplit, a.mt);
-  constexpr int NT = SWIGLU ? 2 : 1;
-  auto go = [&](auto kernel, int W, int MT, bool fused) {
+void launch_few(const Plan& p, const LinearArgs& a, const RowsArgs& r, hipStream_t st) {
+  auto go = [&](auto kernel, int MT, int NT, bool fused) {
     const size_t codes = fused ? (size_t)a.M * (a.Kp + 16) : 0;
-    hipLaunchKernelGGL(kernel, grid, dim3(W * 64), std::max<size_t>(codes, (size_t)W * MT * NT * 1024), st, a, r);
+    hipLaunchKernelGGL(kernel, dim3(a.nt, a.mt), dim3(512), std::max<size_t>(codes, (size_t)8 * MT * NT * 1024), st, a, r);
   };
-  if (p.fused) go(few_kernel<X, SWIGLU, true, 1, NT, 8>, 8, 1, true);
-  else if (p.bm == 16) go(few_kernel<X, SWIGLU, false, 1, NT, 8>, 8, 1, false);
-  else if (p.bm == 32) go(few_kernel<X, SWIGLU, false, 2, NT, 8>, 8, 2, false);
-  else go(few_kernel<X, SWIGLU, false, 4, NT, 4>, 4, 4, false);
+  constexpr int NT = SWIGLU ? 2 : 1;
+  if (p.fused) {
+    if (r.K % 8 == 0) go(few_kernel<X, SWIGLU, true, true, 1, NT, 8, 2>, 1, NT, true);
+    else go(few_kernel<X, SWIGLU, true, false, 1, NT, 8, 2>, 1, NT, true);
+  }
+  else if (p.bm == 16) {
+    if (p.bn == 64) { if constexpr (SWIGLU) go(few_kernel<X, SWIGLU, false, true, 1, 4, 8, 2>, 1, 4, false); }
+    else go(few_kernel<X, SWIGLU, false, true, 1, NT, 8, 2>, 1, NT, false);
+  } else {
+    if (p.bn == 64) { if constexpr (SWIGLU) go(few_kernel<X, SWIGLU, false, true, 2, 4, 8, 2>, 2, 4, false); }
+    else go(few_kernel<X, SWIGLU, false, true, 2, NT, 8, 2>, 2, NT, false);
+  }
 }
 template <typename X, bool SWIGLU>
-void launch_tiles(const Plan&, const LinearArgs& a, hipStream_t st) {
-  const int tiles = a.mt * a.nt;
-  hipLaunchKernelGGL((tiles_kernel<X, SWIGLU, 128, 128, 2, 2, 3>), dim3((tiles + 7) / 8 * 8), dim3(256), 0, st, a);
+void launch_tiles(const Plan& p, const LinearArgs& a, hipStream_t st) {
+  auto go = [&](auto kernel, int waves) {
+    const int64_t tiles = (int64_t)a.mt * a.nt;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(waves * 64), 0, st, a);
+  };
+  switch (p.tile) {
+    case 0: go(tiles_kernel<X, SWIGLU, 256, 256, 4, 4, 2, 2>, 16); break;
+    case 1: go(tiles_kernel<X, SWIGLU, 192, 256, 2, 4, 2, 2>, 8); break;
+    case 2: go(tiles_kernel<X, SWIGLU, 128, 128, 2, 2, 2, 2>, 4); break;
+    case 3: go(tiles_kernel<X, SWIGLU, 64, 128, 2, 2, 2, 2>, 4); break;
+    default:
+      if constexpr (SWIGLU) go(tiles_kernel<X, SWIGLU, 64, 64, 2, 1, 3, 2>, 2);
+      else go(tiles_kernel<X, SWIGLU, 64, 64, 2, 2, 4, 2>, 4);
+      break;
+  }
 }
 
 template <typename X>
@@ -130,7 +163,7 @@ int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const vo
   if (R == 0) return SK_OK;
   SK_CHECK(x && codes && scales, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(x) && aligned16(codes), SK_EINVAL, "operands must be 16-byte aligned");
-  const RowsArgs a{x, nullptr, -1.f, R, K, padded(K), codes, scales, nullptr, 0};
+  const RowsArgs a{x, nullptr, -1.f, R, K, padded(K), codes, scales};
   if (xdtype == SK_BF16) launch_rows<uint16_t>(a, (hipStream_t)stream);
   else launch_rows<float>(a, (hipStream_t)stream);
   SK_HIP(hipGetLastError());
@@ -140,8 +173,7 @@ int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const vo
 int sk_op_int8_linear_workspace(int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act, int64_t* bytes) {
   if (int rc = check_linear(M, N, K, xdtype, act)) return rc;
   SK_CHECK(bytes, SK_EINVAL, "NULL operand");
-  const bool swiglu = act == SK_ACT_SWIGLU;
-  *bytes = space_of(plan_linear(M, N, K, swiglu), M, N, K, swiglu).bytes;
+  *bytes = space_of(plan_linear(M, N, K, act == SK_ACT_SWIGLU), M, K);
   return SK_OK;
 }
 
@@ -159,20 +191,19 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
   SK_CHECK(out != x, SK_EINVAL, "out must not be x");
   const bool swiglu = act == SK_ACT_SWIGLU;
   const Plan p = plan_linear(M, N, K, swiglu);
-  const Space s = space_of(p, M, N, K, swiglu);
-  SK_CHECK(s.bytes == 0 || (workspace && workspace_bytes >= s.bytes), SK_EINVAL, "the workspace must hold %lld bytes",
-           (long long)s.bytes);
+  const int64_t need = space_of(p, M, K);
+  SK_CHECK(need == 0 || (workspace && workspace_bytes >= need), SK_EINVAL, "the workspace must hold %lld bytes",
+           (long long)need);
   char* ws = static_cast<char*>(workspace);
   const int nc = cols_of(p, swiglu);
   LinearArgs a{};
   a.a = p.fused ? nullptr : (int8_t*)ws;
-  a.as = p.fused ? nullptr : (float*)(ws + s.scales);
+  a.as = p.fused ? nullptr : (float*)(ws + codes_of(M, K));
   a.w = codes; a.ws = scales; a.bias = bias; a.res = residual; a.out = out;
   a.M = M; a.N = N; a.Kp = padded(K);
-  a.mt = (M + p.bm - 1) / p.bm; a.nt = (N + nc - 1) / nc; a.ksplit = p.ksplit; a.gm = 8;
-  if (p.ksplit > 1) { a.ticket = (int*)(ws + s.tickets); a.part = (int*)(ws + s.parts); }
-  const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as), a.ticket,
-                   p.ksplit > 1 ? a.mt * a.nt : 0};
+  a.mt = (M + p.bm - 1) / p.bm; a.nt = (N + nc - 1) / nc; a.gm = 8;
+  SK_CHECK((int64_t)a.mt * a.nt < INT32_MAX - 8, SK_EINVAL, "M * N is too large: several calls are needed");
+  const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as)};
   return xdtype == SK_BF16 ? run_linear<uint16_t>((hipStream_t)stream, p, a, r, swiglu)
                            : run_linear<float>((hipStream_t)stream, p, a, r, swiglu);
 }
