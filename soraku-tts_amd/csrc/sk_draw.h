@@ -8,7 +8,7 @@
 // whose sum passes u times the sum of the kept.  So nothing needs the whole order, only the places
 // where counts or sums of the largest values pass a bound:
 //
-// * a histogram of y (32 buckets per power of two of the weight) with counts and sums
+// * a histogram of y (64 buckets per power of two of the weight) with counts and sums
 //   tells the few buckets in which the bounds are passed;
 // * their values alone are listed and sorted, and the bounds are found in the list by
 //   bisection;
@@ -32,9 +32,9 @@ namespace sk {
 namespace draw {
 
 constexpr int NT = 1024;                          // threads of a workgroup
-constexpr int NB = 1536;                          // buckets: e = ref - t below 48
-constexpr int PER_BIT = 32;                       // buckets per power of two
-constexpr int CAP = 4096;                         // values of the list
+constexpr int PER_BIT = 64, FINE = 20 * PER_BIT;  // buckets per power of two of the weight, for the first 20 of them,
+constexpr int STEP = 8, NB = FINE + 28 * PER_BIT / STEP;   // then an eighth as many, down to 2^-48
+constexpr int CAP = 2048;                         // values of the list
 constexpr int DIGITS = 2048;                      // of 11, 11 and 10 bits of a key
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
@@ -65,12 +65,15 @@ template <typename X> __device__ __forceinline__ float to_f(X v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<uint16_t>(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
-// One row's values as keys: larger values have larger keys, 0 is no candidate.
-template <typename X>
+// One row's values as keys: larger values have larger keys, 0 is no candidate.  Keys of x, before the division, are enough
+// wherever an order or a threshold is all that is asked: division by T > 0 keeps the order (but makes equals of some).
+// WIDE: rows begin at multiples of 16 bytes and are whole pieces of 16, so that a load takes 4 or 8 values.
+template <typename X, bool WIDE>
 struct Row {
   const X* cond; const X* uncond;
   const uint32_t* allowed;
   float s, T;
+  double inv;                                     // 1 / T, or 0: divide
   int V;
   __device__ Row(const Args& a, int r) {
     const X* l = static_cast<const X*>(a.logits);
@@ -79,23 +82,65 @@ struct Row {
     allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride : nullptr;
     s = a.cfg ? a.cfg[r] : 0.f;
     T = a.temperature ? a.temperature[r] : 1.f;
+    inv = !(T > 0.f) ? 1.0 : T > 0x1p-20f && T < 0x1p20f ? 1.0 / (double)T : 0.0;   // (greedy: x itself)
     V = a.V;
   }
-  __device__ __forceinline__ uint32_t key(int v) const {
-    float x = to_f<X>(cond[v]);
+  // x / T rounded to FP32, held to the finite range.  By the reciprocal in 64 bits that is the same: its product is within
+  // 2^-52 of the quotient, and a quotient of two 24-bit numbers is no middle of two FP32 numbers and lies at least
+  // 2^-49 from any (x - T m is a multiple of the last place of a 49-bit product).  Results below the normal range
+  // have fewer bits, so those are divided, and so is by temperatures that could make them of ordinary x.
+  __device__ __forceinline__ float divided(float x) const {
+    float y = (float)((double)x * inv);
+    if (fabsf(y) < 0x1p-100f && x != 0.f) y = T > 0.f ? x / T : x;
+    return __builtin_amdgcn_fmed3f(y, -3.402823466e38f, 3.402823466e38f);
+  }
+  // x of an id; NaN: no candidate
+  __device__ __forceinline__ float x_of(X c, X uc, uint32_t word, int v) const {
+    float x = to_f<X>(c);
     if (uncond) {
-      const float u = to_f<X>(uncond[v]);
+      const float u = to_f<X>(uc);
       x = u + s * (x - u);
     }
-    const bool ok = fabsf(x) <= 3.402823466e38f && (!allowed || (allowed[v >> 5] >> (v & 31) & 1u));
-    if (T > 0.f) x = fminf(fmaxf(x / T, -3.402823466e38f), 3.402823466e38f);
-    return ok ? key_of(x) : 0u;
+    return fabsf(x) <= 3.402823466e38f && (word >> (v & 31) & 1u) ? x : __uint_as_float(0x7fc00000u);
+  }
+  // the key of y
+  __device__ __forceinline__ uint32_t key(int v) const {
+    const float x = x_of(cond[v], uncond ? uncond[v] : X(0), allowed ? allowed[v >> 5] : ~0u, v);
+    return x == x ? key_of(divided(x)) : 0u;
+  }
+  // f(id, x) of values v0 .. v1 (x NaN: no candidate), 16 values of a thread (8 of them one by one) on their way at a time.  WIDE: v0
+  // and v1 are at whole pieces.
+  template <typename F>
+  __device__ __forceinline__ void each(int v0, int v1, F f) const {
+    constexpr int P = WIDE ? 16 / (int)sizeof(X) : 1, U = WIDE ? 16 / P : 8;
+    struct alignas(P * sizeof(X)) Piece { X x[P]; };
+    for (int at = v0; at < v1; at += U * P * NT) {
+      Piece c[U], u[U];
+      uint32_t word[U];
+      int v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        v[i] = at + (i * NT + (int)threadIdx.x) * P;
+        const int l = min(v[i], v1 - P);
+        c[i] = *reinterpret_cast<const Piece*>(cond + l);
+        if (uncond) u[i] = *reinterpret_cast<const Piece*>(uncond + l);
+        else u[i] = c[i];
+        word[i] = allowed ? allowed[l >> 5] : ~0u;   // a piece's bits lie in one word
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v[i] < v1) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            f(v[i] + j, x_of(c[i].x[j], u[i].x[j], word[i], v[i] + j));
+          }
+        }
+    }
   }
 };
 
-// e = ref - t of a key, and its weight 2^-e in units of 2^-bits, rounded to nearest: e = n + f,
-// 2^-f by the exponential series in f ln 2 (|f ln 2| <= 0.347, terms to the 12th: 1e-16).
 __device__ __forceinline__ double log2_of(uint32_t key) { return (double)value_of(key) * LOG2E; }
+// 2^-e, e = n + f: 2^-f by the exponential series in f ln 2 (|f ln 2| <= 0.347, terms to the 12th: 1e-16).
 __device__ __forceinline__ double power(double e) {
   const double n = rint(e), z = (n - e) * LN2;
   double p = 1.0 / 479001600.0;
@@ -113,142 +158,191 @@ __device__ __forceinline__ double power(double e) {
   p = fma(p, z, 1.0);
   return ldexp(p, -(int)n);
 }
-// e at most bits + 2, past which a weight is 0
-__device__ __forceinline__ unsigned long long weight(double e, int bits) {
-  if (!(e <= bits + 2)) return 0;
-  const double x = ldexp(power(e), bits) + 0x1p52;   // the sum's last bits are the whole number
+// The weight 2^-e of a value b steps below ref, in units of 2^-bits, rounded to nearest: with e = (b + f) / 64, f in 0 .. 1
+// but for the step's rounding, 2^(-b / 64) from a table of 64 and the exponential series in -f ln 2 / 64 (to the 6th: 1e-17).
+__device__ __forceinline__ unsigned long long weight(double e, int b, int bits, const double* roots) {
+  constexpr double C = -LN2 / PER_BIT;
+  const double z = fma(e, (double)PER_BIT, -(double)b) * C;
+  double p = fma(1.0 / 720.0, z, 1.0 / 120.0);
+  p = fma(p, z, 1.0 / 24.0);
+  p = fma(p, z, 1.0 / 6.0);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0) * roots[b & (PER_BIT - 1)];
+  const double x = ldexp(p, bits - b / PER_BIT) + 0x1p52;   // the sum's last bits are the whole number
   return (unsigned long long)__double_as_longlong(x) & 0xfffffffffffffull;
 }
-// The bucket of t: whole numbers are compared, so that t has the same one whichever ref it is counted from.
-__device__ __forceinline__ int bucket(double ref, double t) {
-  const double d = ref * PER_BIT - floor(t * PER_BIT) - 1.0;
-  return d >= NB - 1 ? NB - 1 : d > 0.0 ? (int)d : 0;
-}
-// A value's weight: 0 in the last bucket, which has all that is far below.
-__device__ __forceinline__ unsigned long long weight_of(double ref, double t, int b, int bits) {
-  return b < NB - 1 ? weight(ref - t, bits) : 0;
-}
+constexpr int LAST = FINE + (NB - 1 - FINE) * STEP;   // the first step of the last bucket, which has all that is far below
+__device__ __forceinline__ int bucket_of(int b) { return b < FINE ? b : FINE + (b - FINE) / STEP; }
+// Where a row's values lie below its reference.  Steps of y are the same number for the same value wherever they are asked,
+// larger for larger values, and counted down from 64 ref, ref a whole number, so counts from the refs of two slices are whole
+// numbers apart.  FP32 does for that up to |y| of 4096 (steps within 0.05 of those of 64 bits).  Past it (a temperature of 1 /
+// 1000, values of a mask's making) ref is the largest value itself, and its row is one workgroup's.
+struct Scale {
+  double ref, from, off;                          // in powers of two; e = (from - y) log2(e) + off
+  float ref64;                                    // 64 ref
+  bool wild;
+  static __device__ __forceinline__ float steps(float y) { return floorf(y * (float)(LOG2E * PER_BIT)); }
+  __device__ explicit Scale(float y) {
+    wild = !(fabsf(y) < 4096.f);
+    const float whole = floorf(steps(y) * (1.f / PER_BIT)) + 1.f;
+    ref64 = whole * PER_BIT;
+    ref = wild ? (double)y * LOG2E : (double)whole;
+    from = wild ? (double)y : 0.0;
+    off = wild ? 0.0 : ref;
+  }
+  // powers of two below ref
+  __device__ __forceinline__ double e(float y) const { return fma(from - (double)y, LOG2E, off); }
+  // whole steps below ref, at most LAST
+  __device__ __forceinline__ int below(float y) const {
+    if (wild) return (int)fmin(e(y) * PER_BIT, (double)LAST);
+    return (int)__builtin_amdgcn_fmed3f(ref64 - steps(y) - 1.f, 0.f, (float)LAST);
+  }
+  __device__ __forceinline__ int bucket(float y) const { return bucket_of(below(y)); }
+  // The bucket of the least value that min-p keeps, give (-1) or take (1) rounding.
+  __device__ __forceinline__ int least(float top, double m, double side) const {
+    const double d = e(top) - log2(m) + side * 1e-3;
+    return bucket_of((int)fmin(fmax(d * PER_BIT, 0.0), (double)LAST));
+  }
+  // A value's weight: 0 in the last bucket.
+  __device__ __forceinline__ unsigned long long weight(float y, int bits, const double* roots) const {
+    const int b = below(y);
+    return b < LAST ? draw::weight(e(y), b, bits, roots) : 0;
+  }
+};
 
 // The workgroup's shared memory.
 struct Shared {
+  double roots[PER_BIT];                          // 2^(-i / 64)
   unsigned long long mass[NB + 1];                // of a bucket, then of all before it
-  unsigned long long list[CAP], sum[CAP];
+  alignas(16) unsigned long long list[2 * CAP];   // then their sums (digit by digit: histograms)
   unsigned count[NB + 1];
   unsigned long long wave64[16];
   unsigned wave32[16];
   unsigned listed;
-  int flag;
-  struct { int lo, hi, pos; unsigned cp; unsigned long long mp; } range[4];
+  int flag, found;
+  // ranges of buckets: first and last, the keys of x between them, where they begin in the list, what lies before them
+  struct { int lo, hi, pos; uint32_t least, most; unsigned cp; unsigned long long mp; } range[4];
   int lo[4], hi[4], ranges, total;
   // digit by digit
   struct { unsigned prefix; unsigned cp; unsigned long long mp; unsigned cnt; unsigned long long mass; } at;
 };
-static_assert(sizeof(unsigned long long) * CAP * 2 >= DIGITS * 12, "digits' histograms lie in the list's place");
+static_assert(CAP * 16 >= (DIGITS + 1) * 12, "digits' histograms lie in the list's place");
 
+// Exchanges between a wave's lanes in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned moved(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long moved(unsigned long long v) {
+  return (unsigned long long)moved<CTRL, ROWS>((unsigned)(v >> 32)) << 32 | moved<CTRL, ROWS>((unsigned)v);
+}
+// f of this lane's and all lower lanes' values, 0 being its neutral one: within rows of 16 lanes (shifted by 1, 2, 4, 8),
+// then the last of a row into the next ones.
 template <typename T, typename F>
-__device__ __forceinline__ T wave_all(T v, F f) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = f(v, (T)__shfl_xor(v, o));
+__device__ __forceinline__ T wave_incl(T v, F f) {
+  v = f(v, moved<0x111, 0xf>(v));
+  v = f(v, moved<0x112, 0xf>(v));
+  v = f(v, moved<0x114, 0xf>(v));
+  v = f(v, moved<0x118, 0xf>(v));
+  v = f(v, moved<0x142, 0xa>(v));                 // row_bcast15 into rows 1 and 3
+  v = f(v, moved<0x143, 0xc>(v));                 // row_bcast31 into rows 2 and 3
   return v;
 }
-__device__ __forceinline__ unsigned long long wave_incl(unsigned long long v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
+__device__ __forceinline__ unsigned at_lane(unsigned v, int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ unsigned long long at_lane(unsigned long long v, int l) {
+  return (unsigned long long)at_lane((unsigned)(v >> 32), l) << 32 | at_lane((unsigned)v, l);
 }
+struct Plus { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
+struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
+template <typename T, typename F>
+__device__ __forceinline__ T wave_all(T v, F f) { return at_lane(wave_incl(v, f), 63); }
 
-// Largest of a value over the workgroup, in every thread.
-__device__ __forceinline__ unsigned long long block_max(unsigned long long v, Shared& s) {
-  v = wave_all(v, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
+// The largest of a and the sum of b over the workgroup, in every thread.
+__device__ __forceinline__ void block_max_sum(unsigned long long& a, unsigned& b, Shared& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  a = wave_all(a, Larger{});
+  b = wave_all(b, Plus{});
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave64[threadIdx.x >> 6] = v;
+  if (lane == 0) { s.wave64[wave] = a; s.wave32[wave] = b; }
   __syncthreads();
-  v = s.wave64[0];
-  for (int w = 1; w < NT / 64; ++w) v = s.wave64[w] > v ? s.wave64[w] : v;
-  return v;
+  a = wave_all(lane < 16 ? s.wave64[lane] : 0, Larger{});
+  b = wave_all(lane < 16 ? s.wave32[lane] : 0, Plus{});
 }
-__device__ __forceinline__ unsigned block_sum(unsigned v, Shared& s) {
-  v = wave_all(v, [](unsigned a, unsigned b) { return a + b; });
+// The sum over the workgroup, in every thread.
+__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, Shared& s) {
+  const int lane = threadIdx.x & 63;
+  v = wave_all(v, Plus{});
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave32[threadIdx.x >> 6] = v;
+  if (lane == 0) s.wave64[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0;
-  for (int w = 0; w < NT / 64; ++w) v += s.wave32[w];
-  return v;
+  return wave_all(lane < 16 ? s.wave64[lane] : 0, Plus{});
 }
-// Exclusive sums of a[0 .. n) in place and the whole at a[n]; n at most 4 NT.
-template <typename T>
-__device__ __forceinline__ void block_scan(T* a, int n, Shared& s) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (n + NT - 1) / NT, at = tid * per;
-  T v[4], mine = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = i < per && at + i < n ? a[at + i] : T(0);
-    mine += v[i];
-  }
-  const unsigned long long incl = wave_incl(mine, lane);
+// Exclusive sums of count[0 .. n) and mass[0 .. n) in place, and the wholes at n; n at most 2 NT.
+__device__ __forceinline__ void block_scan(unsigned* count, unsigned long long* mass, int n, Shared& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x * 2;
+  const bool on0 = at < n, on1 = at + 1 < n;
+  const unsigned c0 = on0 ? count[at] : 0, c1 = on1 ? count[at + 1] : 0;
+  const unsigned long long m0 = on0 ? mass[at] : 0, m1 = on1 ? mass[at + 1] : 0;
+  unsigned c = wave_incl(c0 + c1, Plus{});
+  unsigned long long m = wave_incl(m0 + m1, Plus{});
+  if (lane == 63) { s.wave32[wave] = c; s.wave64[wave] = m; }
   __syncthreads();
-  if (lane == 63) s.wave64[wave] = incl;
-  __syncthreads();
-  unsigned long long base = 0, all = 0;
-  for (int w = 0; w < NT / 64; ++w) {
-    if (w < wave) base += s.wave64[w];
-    all += s.wave64[w];
-  }
-  T x = (T)(base + incl) - mine;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < per && at + i < n) a[at + i] = x;
-    x += v[i];
-  }
-  if (tid == 0) a[n] = (T)all;
+  // lane w: all of the waves before w + 1
+  const unsigned wc = wave_incl(lane < 16 ? s.wave32[lane] : 0, Plus{});
+  const unsigned long long wm = wave_incl(lane < 16 ? s.wave64[lane] : 0, Plus{});
+  if (wave) { c += at_lane(wc, wave - 1); m += at_lane(wm, wave - 1); }
+  c -= c0 + c1;
+  m -= m0 + m1;
+  if (on0) { count[at] = c; mass[at] = m; }
+  if (on1) { count[at + 1] = c + c0; mass[at + 1] = m + m0; }
+  if (threadIdx.x == 0) { count[n] = at_lane(wc, 15); mass[n] = at_lane(wm, 15); }
   __syncthreads();
 }
 
-// The largest key, the lowest id that has it, and how many candidates values v0 .. v1 hold.
-template <typename X>
-__device__ void survey(const Row<X>& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
+// The largest key of x, the lowest id that has it, and how many candidates values v0 .. v1 hold.
+template <typename X, bool WIDE>
+__device__ void survey(const Row<X, WIDE>& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
   unsigned long long b = 0;
   unsigned c = 0;
-  for (int v = v0 + threadIdx.x; v < v1; v += NT) {
-    const uint32_t k = row.key(v);
-    const unsigned long long x = (unsigned long long)k << 32 | (uint32_t)~v;
-    if (k) { ++c; b = x > b ? x : b; }
-  }
-  best = block_max(b, s);
-  n = (int)block_sum(c, s);
+  row.each(v0, v1, [&](int v, float x) {
+    const unsigned long long k = x == x ? (unsigned long long)key_of(x) << 32 | (uint32_t)~v : 0ull;
+    c += x == x;
+    b = k > b ? k : b;
+  });
+  block_max_sum(b, c, s);
+  best = b;
+  n = (int)c;
 }
-__device__ __forceinline__ double ref_of(unsigned long long best) { return floor(log2_of((uint32_t)(best >> 32))) + 1.0; }
-
-// Counts and sums by bucket of values v0 .. v1 in s.count and s.mass.
-template <typename X>
-__device__ void histogram(const Row<X>& row, int v0, int v1, double ref, int bits, Shared& s) {
+// Counts and (with sums) sums of weights by bucket of values v0 .. v1 in s.count and s.mass.
+template <typename X, bool WIDE>
+__device__ void histogram(const Row<X, WIDE>& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
   for (int i = threadIdx.x; i < NB; i += NT) { s.count[i] = 0; s.mass[i] = 0; }
   __syncthreads();
-  for (int v = v0 + threadIdx.x; v < v1; v += NT) {
-    const uint32_t k = row.key(v);
-    if (!k) continue;
-    const double t = log2_of(k);
-    const int b = bucket(ref, t);
-    atomicAdd(&s.count[b], 1u);
-    if (b < NB - 1) atomicAdd(&s.mass[b], weight(ref - t, bits));
-  }
+  row.each(v0, v1, [&](int, float x) {
+    const float y = row.divided(x);
+    const int d = at.below(y), b = bucket_of(d);
+    const unsigned long long w = sums ? weight(at.e(y), d, bits, s.roots) : 0;
+    if (x == x) {
+      atomicAdd(&s.count[b], 1u);
+      if (sums && d < LAST) atomicAdd(&s.mass[b], w);
+    }
+  });
   __syncthreads();
 }
+
+// Whether a row is listed down to its k-th value (or whole, where it has fewer than k).
+__device__ __forceinline__ bool lists(const Args& a, int r) { return a.top_k && a.top_k[r] > 0 && a.top_k[r] <= CAP / 2; }
 
 // The parameters of a row as the definitions read them.
 struct Params {
   double p, m, u;                                 // p in (0, 1) or 0: none; m in (0, 1] or 0: none
   int k;                                          // 0: none
-  bool greedy;
+  bool greedy, list;                              // list: all that top-k leaves is listed, and no sums are asked of the histogram
   __device__ Params(const Args& a, int r, int n) {
     const float T = a.temperature ? a.temperature[r] : 1.f;
     greedy = !(T > 0.f);
     k = a.top_k ? a.top_k[r] : 0;
+    list = lists(a, r);
     if (k <= 0 || k >= n) k = 0;
     const float tp = a.top_p ? a.top_p[r] : 0.f, mp = a.min_p ? a.min_p[r] : 0.f;
     p = tp > 0.f && tp < 1.f ? (double)tp : 0.0;
@@ -268,100 +362,149 @@ __device__ __forceinline__ bool heavy(uint32_t key, uint32_t top, double m) {
   return power(fmin(log2_of(top) - log2_of(key), 1000.0)) >= m;
 }
 
-// The t down to which weights are kept, give (1) or take (-1) rounding.
-__device__ __forceinline__ double least_t(double m, double top, double side) {
-  return fmin(top + log2(m) + side * (1e-6 + fabs(top) * 0x1p-50), top);
-}
-
-// Bucket b with mass[b] <= T < mass[b + 1] (sums of all before).
-__device__ int find_mass(const Shared& s, unsigned long long T) {
-  int lo = 0, hi = NB - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (s.mass[mid + 1] > T) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-// Bucket b with count[b] <= c < count[b + 1].
-__device__ int find_count(const Shared& s, unsigned c) {
-  int lo = 0, hi = NB - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (s.count[mid + 1] > c) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-
-// One thread: the buckets in which the row's bounds are passed, as ranges in s.range; s.total is
-// the number of values that they hold.  The whole that top-p takes its part of, and the kept sum that the draw
-// takes its part of, are known up to the bucket in which the bound before lies, so theirs may be several.
-__device__ void plan(const Params& q, double ref, double top, Shared& s) {
-  int (&lo)[4] = s.lo, (&hi)[4] = s.hi, n = 0;    // in shared memory: indexed as the run goes
-  unsigned long long w_lo = s.mass[NB], w_hi = s.mass[NB];
+// The buckets in which the row's bounds are passed, as ranges in s.range; s.total is the number of values
+// that they hold.  The whole that top-p takes its part of, and the kept sum that the draw takes its part of, are
+// known up to the bucket in which the bound before lies, so theirs may be several.  All threads:
+// each looks at two buckets.
+template <typename X, bool WIDE>
+__device__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, float top, Shared& s) {
+  // the buckets b with a[b] <= x < a[b + 1] (sums of all before) for lo and hi
+  auto find = [&](const auto* a, auto lo, auto hi, int& lo_b, int& hi_b, int i) {
+    for (int b = threadIdx.x; b < NB; b += NT) {
+      const auto x = a[b], y = a[b + 1];
+      if (x <= lo && lo < y) s.lo[i] = b;
+      if (x <= hi && hi < y) s.hi[i] = b;
+    }
+    __syncthreads();
+    lo_b = s.lo[i];
+    hi_b = s.hi[i];
+  };
+  constexpr int NONE = 1 << 20;
+  int lo[4] = {NONE, NONE, NONE, NONE}, hi[4] = {NONE, NONE, NONE, NONE};   // of k, p, min-p, the draw
+  unsigned long long w_lo = s.mass[NB], w_hi = w_lo;
   if (q.k) {
-    const int b = find_count(s, q.k - 1);
-    lo[n] = hi[n] = b; ++n;
-    w_lo = s.mass[b]; w_hi = s.mass[b + 1];
+    find(s.count, (unsigned)(q.k - 1), (unsigned)(q.k - 1), lo[0], hi[0], 0);
+    w_lo = s.mass[lo[0]]; w_hi = s.mass[lo[0] + 1];
   }
-  unsigned long long k_lo = w_lo, k_hi = w_hi;    // of the kept sum
-  if (q.p > 0.0) {
-    lo[n] = find_mass(s, part_of(q.p, w_lo));
-    hi[n] = find_mass(s, part_of(q.p, w_hi));
-    k_lo = s.mass[lo[n]]; k_hi = s.mass[hi[n] + 1];
-    ++n;
-  }
-  if (q.m > 0.0) {
-    lo[n] = bucket(ref, least_t(q.m, top, 1.0)); hi[n] = bucket(ref, least_t(q.m, top, -1.0));
-    k_lo = min(k_lo, s.mass[lo[n]]); k_hi = min(k_hi, s.mass[hi[n] + 1]);
-    ++n;
-  }
-  lo[n] = find_mass(s, part_of(q.u, k_lo));
-  hi[n] = find_mass(s, part_of(q.u, k_hi));
-  ++n;
-  for (int i = 1; i < n; ++i)                     // by their first bucket
-    for (int j = i; j > 0 && lo[j] < lo[j - 1]; --j) {
-      const int a = lo[j], b = hi[j];
-      lo[j] = lo[j - 1]; hi[j] = hi[j - 1]; lo[j - 1] = a; hi[j - 1] = b;
+  if (q.list) {                                   // one range from the first bucket on
+    lo[0] = 0;
+    if (!q.k) hi[0] = NB - 1;
+  } else {
+    unsigned long long k_lo = w_lo, k_hi = w_hi;  // of the kept sum
+    if (q.p > 0.0) {
+      find(s.mass, part_of(q.p, w_lo), part_of(q.p, w_hi), lo[1], hi[1], 1);
+      k_lo = s.mass[lo[1]]; k_hi = s.mass[hi[1] + 1];
     }
-  int r = 0;
-  for (int i = 1; i < n; ++i) {                   // overlapping ones become one
-    if (lo[i] <= hi[r] + 1) hi[r] = max(hi[r], hi[i]);
-    else { ++r; lo[r] = lo[i]; hi[r] = hi[i]; }
+    if (q.m > 0.0) {
+      lo[2] = at.least(top, q.m, -1.0); hi[2] = at.least(top, q.m, 1.0);
+      k_lo = min(k_lo, s.mass[lo[2]]); k_hi = min(k_hi, s.mass[hi[2] + 1]);
+    }
+    find(s.mass, part_of(q.u, k_lo), part_of(q.u, k_hi), lo[3], hi[3], 3);
   }
-  unsigned total = 0;
-  for (int i = 0; i <= r; ++i) {
-    s.range[i].lo = lo[i]; s.range[i].hi = hi[i];
-    s.range[i].pos = (int)total;
-    s.range[i].cp = s.count[lo[i]]; s.range[i].mp = s.mass[lo[i]];
-    total += s.count[hi[i] + 1] - s.count[lo[i]];
+  // by their first bucket
+  auto order = [&](int i, int j) {
+    if (lo[j] < lo[i]) {
+      const int a = lo[i], b = hi[i];
+      lo[i] = lo[j]; hi[i] = hi[j]; lo[j] = a; hi[j] = b;
+    }
+  };
+  order(0, 1); order(2, 3); order(0, 2); order(1, 3); order(1, 2);
+  if (threadIdx.x == 0) {
+    unsigned total = 0;
+    int r = 0, l = lo[0], h = hi[0];
+    auto put = [&]() {
+      const unsigned c = s.count[l];
+      s.range[r].lo = l; s.range[r].hi = h;
+      s.range[r].pos = (int)total;
+      s.range[r].cp = c; s.range[r].mp = s.mass[l];
+      total += s.count[h + 1] - c;
+      ++r;
+    };
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (lo[i] != NONE) {
+        if (lo[i] <= h + 1) h = max(h, hi[i]);    // overlapping ones become one
+        else { put(); l = lo[i]; h = hi[i]; }
+      }
+    put();
+    s.ranges = r;
+    s.total = (int)total;
+    s.listed = 0;
   }
-  s.ranges = r + 1;
-  s.total = (int)total;
+  __syncthreads();
+  // the keys of x that a range begins and ends with: the largest whose bucket is at least lo, the least whose
+  // bucket is at most hi; a wave for each, which tries 64 keys at a time
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave < 2 * s.ranges) {
+    const int i = wave / 2, lo_b = s.range[i].lo, hi_b = s.range[i].hi;
+    // keys before `from` are on this side of the border, from `from + size` on they are not (border: the first
+    // key whose bucket is at most hi, or the first whose bucket is below lo)
+    uint32_t from = 0x00800000u, size = 0xff800000u - 0x00800000u;   // of the finite numbers
+    while (size) {
+      const uint32_t part = size / 64 + 1, end = from + size;   // lane l asks of key from + (l + 1) part - 1
+      const uint64_t key = (uint64_t)from + (lane + 1) * (uint64_t)part - 1;
+      const int b = at.bucket(row.divided(value_of((uint32_t)min(key, (uint64_t)(end - 1)))));
+      const bool past = key >= end || (wave & 1 ? b <= hi_b : b < lo_b);   // 64 parts are more than size: one is past
+      from += __builtin_ctzll(__ballot(past)) * part;
+      size = min(part - 1, end - from);
+    }
+    if (lane == 0) {
+      if (wave & 1) s.range[i].least = (uint32_t)from;
+      else s.range[i].most = (uint32_t)from - 1;
+    }
+  }
+  __syncthreads();
 }
 
-// Adds the values of v0 .. v1 that lie in the ranges to a list.
-template <typename X>
-__device__ void gather(const Row<X>& row, int v0, int v1, double ref, const Shared& s, unsigned long long* list, unsigned* listed) {
-  const int nr = s.ranges;
-  for (int v = v0 + threadIdx.x; v < v1; v += NT) {
-    const uint32_t k = row.key(v);
-    if (!k) continue;
-    const int b = bucket(ref, log2_of(k));
+// Puts the values of v0 .. v1 that lie in the ranges into s.list, s.listed of them.
+template <typename X, bool WIDE>
+__device__ void gather(const Row<X, WIDE>& row, int v0, int v1, Shared& s) {
+  float least[4], most[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool is = i < s.ranges;
+    least[i] = is ? value_of(s.range[i].least) : INFINITY;
+    most[i] = is ? value_of(s.range[i].most) : 0.f;
+  }
+  row.each(v0, v1, [&](int v, float x) {
     bool in = false;
-    for (int i = 0; i < nr; ++i) in |= b >= s.range[i].lo && b <= s.range[i].hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in |= x >= least[i] && x <= most[i];
     if (in) {
-      const unsigned at = atomicAdd(listed, 1u);
-      if (at < CAP) list[at] = (unsigned long long)k << 32 | (uint32_t)~v;
+      const unsigned at = atomicAdd(&s.listed, 1u);
+      if (at < CAP) s.list[at] = (unsigned long long)key_of(row.divided(x)) << 32 | (uint32_t)~v;
     }
-  }
+  });
+  __syncthreads();
 }
 
-// s.list[0 .. n), largest first; n at most CAP.
+// s.list[0 .. n), largest first; n at most CAP.  Up to 1,024 values each finds its place by counting the
+// larger ones, NT / P threads to a value (181 values: 2,000 clocks, by the network, whose steps are a barrier
+// each, 17,600).
 __device__ void sort_list(int n, Shared& s) {
   int P = 2;
   while (P < n) P <<= 1;
+  if (P <= NT) {
+    const int per = NT / P < 64 ? NT / P : 64, i = threadIdx.x / per, part = threadIdx.x % per;
+    unsigned long long x = 0;
+    unsigned place = 0;
+    if (threadIdx.x == 0 && (n & 1)) s.list[n] = 0;
+    __syncthreads();
+    if (i < n) {
+      const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(s.list);
+      x = s.list[i];
+#pragma unroll 8
+      for (int j = part; j < (n + 1) / 2; j += per) {
+        const ulonglong2 y = pairs[j];
+        place += (y.x > x) + (y.y > x);
+      }
+    }
+    for (int o = per / 2; o; o >>= 1) place += __shfl_xor(place, o);
+    __syncthreads();
+    if (i < n && part == 0) s.list[place] = x;
+    __syncthreads();
+    return;
+  }
   for (int i = n + threadIdx.x; i < P; i += NT) s.list[i] = 0;
   __syncthreads();
   for (int k = 2; k <= P; k <<= 1)
@@ -383,59 +526,58 @@ __device__ void answer(const Args& a, int r, int token, double logprob, int kept
   if (a.kept) a.kept[r] = kept;
 }
 // ln of the drawn one's part of the kept sum.
-__device__ __forceinline__ double part_log(uint32_t key, double ref, unsigned long long kept, int bits) {
-  return (log2_of(key) - ref + bits) * LN2 - log((double)kept);
+__device__ __forceinline__ double part_log(uint32_t key, const Scale& at, unsigned long long kept, int bits) {
+  return (bits - at.e(value_of(key))) * LN2 - log((double)kept);
 }
 
 // The row's answer from the sorted list of its ranges.
-__device__ void finish_list(const Args& a, int r, const Params& q, double ref, unsigned long long best, int n, Shared& s) {
-  const int total = s.total;
-  for (int i = threadIdx.x; i < total; i += NT) {
-    const double t = log2_of((uint32_t)(s.list[i] >> 32));
-    s.sum[i] = weight_of(ref, t, bucket(ref, t), a.bits);
-  }
-  __syncthreads();
-  // sums up to and with each: four to a thread
+__device__ void finish_list(const Args& a, int r, const Params& q, const Scale& scale, uint32_t top, int n, Shared& s) {
+  const int total = s.total, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned long long* sum_at = s.list + CAP;
+  // sums up to and with each, `per` neighbours to a thread
+  const int per = (total + NT - 1) / NT;
   {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned long long v[CAP / NT], mine = 0;
 #pragma unroll
     for (int i = 0; i < CAP / NT; ++i) {
-      const int at = tid * (CAP / NT) + i;
-      v[i] = at < total ? s.sum[at] : 0;
+      const int at = tid * per + i;
+      v[i] = 0;
+      if (i < per && at < total) {
+        const uint32_t key = (uint32_t)(s.list[at] >> 32);
+        v[i] = scale.weight(value_of(key), a.bits, s.roots);
+      }
       mine += v[i];
     }
-    const unsigned long long incl = wave_incl(mine, lane);
-    __syncthreads();
+    const unsigned long long incl = wave_incl(mine, Plus{});
     if (lane == 63) s.wave64[wave] = incl;
     __syncthreads();
     unsigned long long x = incl - mine;
     for (int w = 0; w < wave; ++w) x += s.wave64[w];
 #pragma unroll
     for (int i = 0; i < CAP / NT; ++i) {
-      const int at = tid * (CAP / NT) + i;
+      const int at = tid * per + i;
       x += v[i];
-      if (at < total) s.sum[at] = x;
+      if (i < per && at < total) sum_at[at] = x;
     }
   }
   __syncthreads();
-  if (threadIdx.x) return;
-  const uint32_t top = (uint32_t)(best >> 32);
+  if (wave) return;
+  // one wave from here on
   auto end_of = [&](int i) { return i + 1 < s.ranges ? s.range[i + 1].pos : total; };
   // sum of all up to and with list entry i of range g
   auto upto = [&](int g, int i) {
     const int p = s.range[g].pos;
-    return s.range[g].mp + s.sum[i] - (p ? s.sum[p - 1] : 0);
+    return s.range[g].mp + sum_at[i] - (p ? sum_at[p - 1] : 0);
   };
-  // first entry of range g for which `past` holds (it holds from some entry on), or its end
+  // first entry of range g for which `past` holds (it holds from some entry on), or its end; 64 at a time
   auto first = [&](int g, auto past) {
-    int lo = s.range[g].pos, hi = end_of(g);
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (past(mid)) hi = mid;
-      else lo = mid + 1;
+    int from = s.range[g].pos, size = end_of(g) - from;
+    while (size) {
+      const int part = size / 64 + 1, at = from + (lane + 1) * part - 1, end = from + size;
+      from += __builtin_ctzll(__ballot(at >= end || past(at))) * part;   // 64 parts are more than size: one is past
+      size = min(part - 1, end - from);
     }
-    return lo;
+    return from;
   };
   // (values, sum) of all before entry i of range g
   auto before = [&](int g, int i, unsigned& c, unsigned long long& w) {
@@ -453,7 +595,7 @@ __device__ void finish_list(const Args& a, int r, const Params& q, double ref, u
     return g;
   };
   unsigned kept = (unsigned)n;
-  unsigned long long sum = s.mass[NB];
+  unsigned long long sum = q.list ? sum_at[total - 1] : s.mass[NB];
   if (q.k) {
     const int g = range_of_count(q.k - 1), at = s.range[g].pos + (int)(q.k - 1 - s.range[g].cp);
     const uint32_t cut = (uint32_t)(s.list[at] >> 32);
@@ -470,7 +612,7 @@ __device__ void finish_list(const Args& a, int r, const Params& q, double ref, u
   }
   if (q.m > 0.0) {
     // its range holds the bucket of the bound
-    const int b = bucket(ref, least_t(q.m, log2_of(top), 1.0));
+    const int b = scale.least(value_of(top), q.m, -1.0);
     int g = 0;
     while (g + 1 < s.ranges && s.range[g + 1].lo <= b) ++g;
     unsigned c;
@@ -480,15 +622,14 @@ __device__ void finish_list(const Args& a, int r, const Params& q, double ref, u
   }
   const unsigned long long T = part_of(q.u, sum);
   const int g = range_of_mass(T);
-  int i = min(first(g, [&](int i) { return upto(g, i) > T; }), end_of(g) - 1);
-  const uint32_t key = (uint32_t)(s.list[i] >> 32);
-  answer(a, r, (int)~(uint32_t)s.list[i], part_log(key, ref, sum, a.bits), (int)kept);
+  const int i = min(first(g, [&](int i) { return upto(g, i) > T; }), end_of(g) - 1);
+  if (lane == 0) answer(a, r, (int)~(uint32_t)s.list[i], part_log((uint32_t)(s.list[i] >> 32), scale, sum, a.bits), (int)kept);
 }
 
 // Digit by digit: the value at which the count of the largest (by_count) or their sum passes T, in
 // s.at: its key, the count and sum of all above it, and its own.
-template <typename X>
-__device__ void descend(const Row<X>& row, double ref, int bits, bool by_count, unsigned long long T, Shared& s) {
+template <typename X, bool WIDE>
+__device__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bits, bool by_count, unsigned long long T, Shared& s) {
   unsigned long long* mass = s.list;              // [DIGITS + 1], then counts
   unsigned* count = reinterpret_cast<unsigned*>(s.list + DIGITS + 1);
   uint32_t prefix = 0, mask = 0;
@@ -505,15 +646,14 @@ __device__ void descend(const Row<X>& row, double ref, int bits, bool by_count, 
       const int d = digits - 1 - (int)(k >> shift & (digits - 1));
       unsigned long long w = 0;
       if (on) {
-        const double t = log2_of(k);
-        w = weight_of(ref, t, bucket(ref, t), bits);
+        w = scale.weight(value_of(k), bits, s.roots);
       }
       // where a wave's values all have one digit, as equal logits do, one lane adds for all
       const unsigned long long who = __ballot(on);
       if (!who) continue;
       const int d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(who));
       if (__ballot(on && d == d0) == who) {
-        w = wave_all(w, [](unsigned long long x, unsigned long long y) { return x + y; });
+        w = wave_all(w, Plus{});
         if ((threadIdx.x & 63) == 0) {
           atomicAdd(&count[d0], (unsigned)__popcll(who));
           atomicAdd(&mass[d0], w);
@@ -524,8 +664,7 @@ __device__ void descend(const Row<X>& row, double ref, int bits, bool by_count, 
       }
     }
     __syncthreads();
-    block_scan(mass, digits, s);
-    block_scan(count, digits, s);
+    block_scan(count, mass, digits, s);
     if (threadIdx.x == 0) {
       int lo = 0, hi = digits - 1;
       while (lo < hi) {
@@ -547,21 +686,21 @@ __device__ void descend(const Row<X>& row, double ref, int bits, bool by_count, 
 }
 
 // The row's answer where the list does not hold its ranges.
-template <typename X>
-__device__ void finish_digits(const Args& a, int r, const Row<X>& row, const Params& q, double ref, unsigned long long best,
+template <typename X, bool WIDE>
+__device__ void finish_digits(const Args& a, int r, const Row<X, WIDE>& row, const Params& q, const Scale& scale, uint32_t top,
                               int n, Shared& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   unsigned kept = (unsigned)n;
-  unsigned long long sum = s.mass[NB];
+  unsigned long long sum = s.mass[NB];            // (with q.list there is a k: the list holds any row of fewer)
   if (q.k) {
-    descend(row, ref, a.bits, true, q.k - 1, s);
+    descend(row, scale, a.bits, true, q.k - 1, s);
     kept = s.at.cp + s.at.cnt;
     sum = s.at.mp + s.at.mass;
   }
   if (q.p > 0.0) {
     const unsigned long long T = part_of(q.p, sum);
     __syncthreads();
-    descend(row, ref, a.bits, false, T, s);
+    descend(row, scale, a.bits, false, T, s);
     // of the equal values so many that the sum passes T
     const unsigned long long w = s.at.cnt ? s.at.mass / s.at.cnt : 0;
     unsigned c = w ? (unsigned)min((T - s.at.mp) / w + 1, (unsigned long long)s.at.cnt) : s.at.cnt;
@@ -572,24 +711,18 @@ __device__ void finish_digits(const Args& a, int r, const Row<X>& row, const Par
     unsigned long long w = 0;
     for (int v = tid; v < row.V; v += NT) {
       const uint32_t k = row.key(v);
-      if (k && heavy(k, (uint32_t)(best >> 32), q.m)) {
-        const double t = log2_of(k);
+      if (k && heavy(k, top, q.m)) {
         ++c;
-        w += weight_of(ref, t, bucket(ref, t), a.bits);
+        w += scale.weight(value_of(k), a.bits, s.roots);
       }
     }
-    c = block_sum(c, s);
-    w = wave_all(w, [](unsigned long long x, unsigned long long y) { return x + y; });
-    __syncthreads();
-    if (lane == 0) s.wave64[wave] = w;
-    __syncthreads();
-    w = 0;
-    for (int i = 0; i < NT / 64; ++i) w += s.wave64[i];
+    c = (unsigned)block_sum(c, s);
+    w = block_sum(w, s);
     if (c < kept) { kept = c; sum = w; }
   }
   const unsigned long long T = part_of(q.u, sum);
   __syncthreads();
-  descend(row, ref, a.bits, false, T, s);
+  descend(row, scale, a.bits, false, T, s);
   const uint32_t key = s.at.prefix;
   const unsigned long long w = s.at.cnt ? s.at.mass / s.at.cnt : 0;
   const unsigned long long nth = w ? (T - s.at.mp) / w : 0;   // from 0, among the equal ones by id
@@ -607,7 +740,7 @@ __device__ void finish_digits(const Args& a, int r, const Row<X>& row, const Par
       const bool is = v < v1 && row.key(v) == key;
       const unsigned long long who = __ballot(is);
       const unsigned mine = ahead + (unsigned)__popcll(who & ((1ull << lane) - 1));
-      if (is && mine == nth) answer(a, r, v, part_log(key, ref, sum, a.bits), (int)kept);
+      if (is && mine == nth) answer(a, r, v, part_log(key, scale, sum, a.bits), (int)kept);
       ahead += (unsigned)__popcll(who);
     }
   }
@@ -621,33 +754,29 @@ __device__ bool finish_early(const Args& a, int r, const Params& q, unsigned lon
 }
 
 // A whole row in one workgroup.
-template <typename X>
+template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   __shared__ Shared s;
+  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
   const int r = blockIdx.x;
-  const Row<X> row(a, r);
+  const Row<X, WIDE> row(a, r);
   unsigned long long best;
   int n;
   survey(row, 0, a.V, s, best, n);
   const Params q(a, r, n);
   if (finish_early(a, r, q, best, n)) return;
-  const double ref = ref_of(best);
-  histogram(row, 0, a.V, ref, a.bits, s);
-  block_scan(s.mass, NB, s);
-  block_scan(s.count, NB, s);
-  if (threadIdx.x == 0) {
-    plan(q, ref, log2_of((uint32_t)(best >> 32)), s);
-    s.listed = 0;
-  }
-  __syncthreads();
+  const uint32_t top = key_of(row.divided(value_of((uint32_t)(best >> 32))));
+  const Scale scale(value_of(top));
+  histogram(row, 0, a.V, scale, a.bits, !q.list, s);
+  block_scan(s.count, s.mass, NB, s);
+  plan(row, q, scale, value_of(top), s);
   if (s.total > CAP) {
-    finish_digits(a, r, row, q, ref, best, n, s);
+    finish_digits(a, r, row, q, scale, top, n, s);
     return;
   }
-  gather(row, 0, a.V, ref, s, s.list, &s.listed);
-  __syncthreads();
+  gather(row, 0, a.V, s);
   sort_list(s.total, s);
-  finish_list(a, r, q, ref, best, n, s);
+  finish_list(a, r, q, scale, top, n, s);
 }
 
 // A row over several workgroups, in two launches.  The first leaves each slice's histogram,
@@ -672,94 +801,124 @@ struct RowSpace {
   }
 };
 
-template <typename X>
+template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
   __shared__ Shared s;
+  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
-  const Row<X> row(a, r);
+  const Row<X, WIDE> row(a, r);
   const RowSpace w(a, r);
   const int v0 = g * a.slice, v1 = min(v0 + a.slice, a.V);
   unsigned long long best;
   int n;
   survey(row, v0, v1, s, best, n);
-  const double ref = n ? ref_of(best) : 0.0;
+  const Scale scale(n ? row.divided(value_of((uint32_t)(best >> 32))) : 0.f);
   if (threadIdx.x == 0) {
-    w.info[g] = {ref, best, n, 0};
+    w.info[g] = {scale.ref, best, n, 0};
     if (g == 0) { *w.listed = 0; *w.arrived = 0; }
   }
-  if (n == 0 || !(row.T > 0.f)) return;           // nothing of it is read
-  histogram(row, v0, v1, ref, a.bits, s);
+  if (n == 0 || !(row.T > 0.f) || scale.wild) return;   // nothing of it is read
+  histogram(row, v0, v1, scale, a.bits, !lists(a, r), s);
   for (int i = threadIdx.x; i < NB; i += NT) {
     w.count[(size_t)g * NB + i] = s.count[i];
     w.mass[(size_t)g * NB + i] = s.mass[i];
   }
 }
 
-template <typename X>
+template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   __shared__ Shared s;
+  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
-  const Row<X> row(a, r);
+  const Row<X, WIDE> row(a, r);
   const RowSpace w(a, r);
+  SliceInfo* info = reinterpret_cast<SliceInfo*>(s.list);   // of all slices, here
+  for (int i = threadIdx.x; i < a.slices; i += NT) info[i] = w.info[i];
+  __syncthreads();
   unsigned long long best = 0;
   int n = 0;
   for (int i = 0; i < a.slices; ++i) {
-    const SliceInfo f = w.info[i];
-    best = f.best > best ? f.best : best;
-    n += f.n;
+    best = info[i].best > best ? info[i].best : best;
+    n += info[i].n;
   }
   const Params q(a, r, n);
   if (n == 0 || q.greedy) {
     if (g == 0) finish_early(a, r, q, best, n);
     return;
   }
-  const double ref = ref_of(best), top = log2_of((uint32_t)(best >> 32));
-  // Past 2^40 the slices' refs need not be whole numbers apart: one workgroup takes the row.
-  const bool alone = !(fabs(ref) < 0x1p40);
+  const uint32_t top = key_of(row.divided(value_of((uint32_t)(best >> 32))));
+  const Scale scale(value_of(top));
+  const bool alone = scale.wild;
   if (alone && g) return;
   if (alone) {
-    histogram(row, 0, a.V, ref, a.bits, s);
+    histogram(row, 0, a.V, scale, a.bits, !q.list, s);
   } else {
+    // A slice's ref is `up` powers of two lower, so its steps lie 64 up further below the row's: a fine bucket has one of
+    // the slice's fine ones, a wide one one of its wide ones or eight of its fine ones.
+    constexpr int GROUP = 5;                      // slices whose loads are on their way together
     for (int b = threadIdx.x; b < NB; b += NT) {
       unsigned c = 0;
       unsigned long long m = 0;
-      for (int i = 0; i < a.slices; ++i) {
-        const SliceInfo f = w.info[i];
-        const double up = ref - f.ref;            // a whole number
-        if (!f.n || up >= NB / PER_BIT) continue;
-        const int at = b - (int)up * PER_BIT;
-        if (at >= 0 && b < NB - 1) {
-          c += w.count[(size_t)i * NB + at];
-          m += w.mass[(size_t)i * NB + at] >> (int)up;
+      for (int i0 = 0; i0 < a.slices; i0 += GROUP) {
+        unsigned x[GROUP];
+        unsigned long long y[GROUP];
+        int from[GROUP], by[GROUP];
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+          const int i = min(i0 + j, a.slices - 1);
+          const double up = scale.ref - info[i].ref;   // a whole number, or beyond all buckets
+          const bool near = i0 + j < a.slices && info[i].n && up < 48.0 && b < NB - 1;   // the last bucket has the rest
+          by[j] = near ? (int)up : 0;
+          const int d = (b < FINE ? b : FINE + (b - FINE) * STEP) - by[j] * PER_BIT;
+          from[j] = !near || d < 0 ? -1 : d;
+          const size_t at = (size_t)i * NB + max(bucket_of(max(d, 0)), 0);
+          x[j] = w.count[at];                     // a slice without candidates left none: loaded, not taken
+          y[j] = w.mass[at];
         }
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j)
+          if (from[j] >= 0) {
+            c += x[j];
+            m += y[j] >> by[j];
+            if (b >= FINE && from[j] < FINE)
+              for (int k = 1; k < STEP; ++k) {
+                const size_t at = (size_t)(i0 + j) * NB + from[j] + k;
+                c += w.count[at];
+                m += w.mass[at] >> by[j];
+              }
+          }
       }
       s.count[b] = c;
       s.mass[b] = m;
     }
     __syncthreads();
   }
-  block_scan(s.mass, NB, s);
-  block_scan(s.count, NB, s);
-  if (threadIdx.x == 0) {
-    s.count[NB] = n;                              // the last bucket has the rest
-    plan(q, ref, top, s);
-  }
+  block_scan(s.count, s.mass, NB, s);
+  if (threadIdx.x == 0) s.count[NB] = n;
   __syncthreads();
+  plan(row, q, scale, value_of(top), s);
   if (s.total > CAP) {
-    if (g == 0) finish_digits(a, r, row, q, ref, best, n, s);
+    if (g == 0) finish_digits(a, r, row, q, scale, top, n, s);
     return;
   }
-  gather(row, alone ? 0 : g * a.slice, alone ? a.V : min((g + 1) * a.slice, a.V), ref, s, w.list, w.listed);
-  __threadfence();
+  // The list passes between workgroups of one launch, on whatever XCD they run: its stores and loads are of device
+  // scope, which pass the L2s by, and done before the arrival is counted.  (Plain stores and a fence write
+  // back the whole L2 for every workgroup.)
+  gather(row, alone ? 0 : g * a.slice, alone ? a.V : min((g + 1) * a.slice, a.V), s);
+  if (threadIdx.x == 0) s.found = (int)atomicAdd(w.listed, s.listed);
+  __syncthreads();
+  for (int i = threadIdx.x; i < (int)s.listed; i += NT)
+    __hip_atomic_store(w.list + s.found + i, s.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
     s.flag = alone || (int)__hip_atomic_fetch_add(w.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.slices - 1;
   __syncthreads();
   if (!s.flag) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < s.total; i += NT) s.list[i] = w.list[i];
+  for (int i = threadIdx.x; i < s.total; i += NT) s.list[i] = __hip_atomic_load(w.list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
   sort_list(s.total, s);
-  finish_list(a, r, q, ref, best, n, s);
+  finish_list(a, r, q, scale, top, n, s);
 }
 
 }  // namespace draw

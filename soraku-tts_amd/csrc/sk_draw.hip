@@ -25,13 +25,28 @@ int check_sizes(int32_t R, int32_t V, int32_t dtype) {
 // Workgroups per row.
 int slices_of(int R, int V) {
   if (V <= 16384) return 1;
-  return std::max((V + 65535) / 65536, std::min(10, 256 / std::max(R, 1)));
+  return std::max((V + 65535) / 65536, std::min(10, 512 / std::max(R, 1)));
 }
 // Sums of V weights of up to 2^bits stay below 2^63.
 int bits_of(int V) {
   int b = 0;
   while ((1 << b) < V) ++b;
   return std::min(46, 62 - b);
+}
+
+template <typename X, bool WIDE>
+int run(const Args& a, hipStream_t st) {
+  if (a.slices == 1) {
+    hipLaunchKernelGGL((row_kernel<X, WIDE>), dim3(a.R), dim3(NT), 0, st, a);
+    SK_HIP(hipGetLastError());
+    return SK_OK;
+  }
+  const dim3 grid(a.slices, a.R);
+  hipLaunchKernelGGL((slice_kernel<X, WIDE>), grid, dim3(NT), 0, st, a);
+  SK_HIP(hipGetLastError());
+  hipLaunchKernelGGL((pick_kernel<X, WIDE>), grid, dim3(NT), 0, st, a);
+  SK_HIP(hipGetLastError());
+  return SK_OK;
 }
 
 }  // namespace
@@ -59,24 +74,15 @@ int sk_op_sample_rows(void* stream, int32_t R, int32_t V, int32_t dtype, const v
   SK_CHECK(((uintptr_t)workspace & 15) == 0, SK_EINVAL, "the workspace must be 16-byte aligned");
   Args a{logits, stride, u, temperature, top_k, top_p, min_p, cfg_scale, allowed, allowed_stride, R, V, bits_of(V),
          slices_of(R, V), 0, token, logprob, kept, (char*)workspace};
-  a.slice = (V + a.slices - 1) / a.slices;
+  // whole pieces of 16 bytes to a slice
+  a.slice = ((V + a.slices - 1) / a.slices + 7) / 8 * 8;
+  const int64_t need = a.slices > 1 ? (int64_t)R * RowSpace::bytes(a.slices) : 0;
+  SK_CHECK(need == 0 || (workspace && workspace_bytes >= need), SK_EINVAL, "the workspace must hold %lld bytes", (long long)need);
+  const int64_t size = dtype == SK_BF16 ? 2 : 4;
+  const bool wide = (uintptr_t)logits % 16 == 0 && stride * size % 16 == 0 && V * size % 16 == 0;
   const hipStream_t st = (hipStream_t)stream;
-  if (a.slices == 1) {
-    if (dtype == SK_BF16) hipLaunchKernelGGL(row_kernel<uint16_t>, dim3(R), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL(row_kernel<float>, dim3(R), dim3(NT), 0, st, a);
-    SK_HIP(hipGetLastError());
-    return SK_OK;
-  }
-  const int64_t need = (int64_t)R * RowSpace::bytes(a.slices);
-  SK_CHECK(workspace && workspace_bytes >= need, SK_EINVAL, "the workspace must hold %lld bytes", (long long)need);
-  const dim3 grid(a.slices, R);
-  if (dtype == SK_BF16) hipLaunchKernelGGL(slice_kernel<uint16_t>, grid, dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL(slice_kernel<float>, grid, dim3(NT), 0, st, a);
-  SK_HIP(hipGetLastError());
-  if (dtype == SK_BF16) hipLaunchKernelGGL(pick_kernel<uint16_t>, grid, dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL(pick_kernel<float>, grid, dim3(NT), 0, st, a);
-  SK_HIP(hipGetLastError());
-  return SK_OK;
+  if (dtype == SK_BF16) return wide ? run<uint16_t, true>(a, st) : run<uint16_t, false>(a, st);
+  return wide ? run<float, true>(a, st) : run<float, false>(a, st);
 }
 
 }  // extern "C"
