@@ -35,6 +35,7 @@ constexpr int NT = 1024;                          // threads of a workgroup
 constexpr int PER_BIT = 64, FINE = 20 * PER_BIT;  // buckets per power of two of the weight, for the first 20 of them,
 constexpr int STEP = 8, NB = FINE + 28 * PER_BIT / STEP;   // then an eighth as many, down to 2^-48
 constexpr int CAP = 2048;                         // values of the list
+constexpr int SHORT = 4096;                       // values of a row that is read once more rather than searched for borders
 constexpr int DIGITS = 2048;                      // of 11, 11 and 10 bits of a key
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
@@ -65,6 +66,23 @@ template <typename X> __device__ __forceinline__ float to_f(X v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<uint16_t>(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
+// A row's parameters as they lie in memory: loaded before anything waits.
+struct Given {
+  float T, s, p, m;
+  int k;
+  double u;
+  __device__ Given(const Args& a, int r) {
+    T = a.temperature ? a.temperature[r] : 1.f;
+    s = a.cfg ? a.cfg[r] : 0.f;
+    p = a.top_p ? a.top_p[r] : 0.f;
+    m = a.min_p ? a.min_p[r] : 0.f;
+    k = a.top_k ? a.top_k[r] : 0;
+    u = a.u[r];
+  }
+  // Whether the row is listed down to its k-th value (or whole, where it has fewer than k).
+  __device__ bool lists() const { return k > 0 && k <= CAP / 2; }
+};
+
 // One row's values as keys: larger values have larger keys, 0 is no candidate.  Keys of x, before the division, are enough
 // wherever an order or a threshold is all that is asked: division by T > 0 keeps the order (but makes equals of some).
 // WIDE: rows begin at multiples of 16 bytes and are whole pieces of 16, so that a load takes 4 or 8 values.
@@ -75,13 +93,13 @@ struct Row {
   float s, T;
   double inv;                                     // 1 / T, or 0: divide
   int V;
-  __device__ Row(const Args& a, int r) {
+  __device__ Row(const Args& a, const Given& g, int r) {
     const X* l = static_cast<const X*>(a.logits);
     cond = l + (size_t)(a.cfg ? 2 * (size_t)r : r) * a.stride;
     uncond = a.cfg ? cond + a.stride : nullptr;
     allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride : nullptr;
-    s = a.cfg ? a.cfg[r] : 0.f;
-    T = a.temperature ? a.temperature[r] : 1.f;
+    s = g.s;
+    T = g.T;
     inv = !(T > 0.f) ? 1.0 : T > 0x1p-20f && T < 0x1p20f ? 1.0 / (double)T : 0.0;   // (greedy: x itself)
     V = a.V;
   }
@@ -94,18 +112,14 @@ struct Row {
     if (fabsf(y) < 0x1p-100f && x != 0.f) y = T > 0.f ? x / T : x;
     return __builtin_amdgcn_fmed3f(y, -3.402823466e38f, 3.402823466e38f);
   }
-  // x of an id; NaN: no candidate
-  __device__ __forceinline__ float x_of(X c, X uc, uint32_t word, int v) const {
-    float x = to_f<X>(c);
-    if (uncond) {
-      const float u = to_f<X>(uc);
-      x = u + s * (x - u);
-    }
-    return fabsf(x) <= 3.402823466e38f && (word >> (v & 31) & 1u) ? x : __uint_as_float(0x7fc00000u);
+  // x of cond and uncond; NaN: no candidate
+  __device__ __forceinline__ float x_of(float x, float u, bool on) const {
+    if (uncond) x = u + s * (x - u);
+    return fabsf(x) <= 3.402823466e38f && on ? x : __uint_as_float(0x7fc00000u);
   }
   // the key of y
   __device__ __forceinline__ uint32_t key(int v) const {
-    const float x = x_of(cond[v], uncond ? uncond[v] : X(0), allowed ? allowed[v >> 5] : ~0u, v);
+    const float x = x_of(to_f<X>(cond[v]), uncond ? to_f<X>(uncond[v]) : 0.f, !allowed || (allowed[v >> 5] >> (v & 31) & 1u));
     return x == x ? key_of(divided(x)) : 0u;
   }
   // f(id, x) of values v0 .. v1 (x NaN: no candidate), 16 values of a thread (8 of them one by one) on their way at a time.  WIDE: v0
@@ -113,28 +127,37 @@ struct Row {
   template <typename F>
   __device__ __forceinline__ void each(int v0, int v1, F f) const {
     constexpr int P = WIDE ? 16 / (int)sizeof(X) : 1, U = WIDE ? 16 / P : 8;
-    struct alignas(P * sizeof(X)) Piece { X x[P]; };
+    auto load = [](const X* p) {
+      if constexpr (WIDE) return *reinterpret_cast<const uint4*>(p);
+      else return to_f<X>(*p);
+    };
+    auto part = [](const auto& w, int j) {        // value j of a piece
+      if constexpr (!WIDE) return w;
+      else if constexpr (sizeof(X) == 4) return __uint_as_float(j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w);
+      else {
+        const uint32_t pair = j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w;
+        return __uint_as_float(j & 1 ? pair & 0xffff0000u : pair << 16);
+      }
+    };
+    using Piece = decltype(load(cond));
     for (int at = v0; at < v1; at += U * P * NT) {
       Piece c[U], u[U];
-      uint32_t word[U];
-      int v[U];
+      uint32_t bits[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        v[i] = at + (i * NT + (int)threadIdx.x) * P;
-        const int l = min(v[i], v1 - P);
-        c[i] = *reinterpret_cast<const Piece*>(cond + l);
-        if (uncond) u[i] = *reinterpret_cast<const Piece*>(uncond + l);
-        else u[i] = c[i];
-        word[i] = allowed ? allowed[l >> 5] : ~0u;   // a piece's bits lie in one word
+        const int l = min(at + (i * NT + (int)threadIdx.x) * P, v1 - P);
+        c[i] = load(cond + l);
+        u[i] = uncond ? load(uncond + l) : c[i];
+        bits[i] = allowed ? allowed[l >> 5] >> (l & 31) : ~0u;   // a piece's bits lie in one word
       }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v[i] < v1) {
+      for (int i = 0; i < U; ++i) {
+        const int v = at + (i * NT + (int)threadIdx.x) * P;
+        if (v < v1) {
 #pragma unroll
-          for (int j = 0; j < P; ++j) {
-            f(v[i] + j, x_of(c[i].x[j], u[i].x[j], word[i], v[i] + j));
-          }
+          for (int j = 0; j < P; ++j) f(v + j, x_of(part(c[i], j), part(u[i], j), bits[i] >> j & 1u));
         }
+      }
     }
   }
 };
@@ -330,25 +353,18 @@ __device__ void histogram(const Row<X, WIDE>& row, int v0, int v1, const Scale& 
   __syncthreads();
 }
 
-// Whether a row is listed down to its k-th value (or whole, where it has fewer than k).
-__device__ __forceinline__ bool lists(const Args& a, int r) { return a.top_k && a.top_k[r] > 0 && a.top_k[r] <= CAP / 2; }
-
-// The parameters of a row as the definitions read them.
+// As the definitions read them, with n candidates.
 struct Params {
   double p, m, u;                                 // p in (0, 1) or 0: none; m in (0, 1] or 0: none
   int k;                                          // 0: none
   bool greedy, list;                              // list: all that top-k leaves is listed, and no sums are asked of the histogram
-  __device__ Params(const Args& a, int r, int n) {
-    const float T = a.temperature ? a.temperature[r] : 1.f;
-    greedy = !(T > 0.f);
-    k = a.top_k ? a.top_k[r] : 0;
-    list = lists(a, r);
-    if (k <= 0 || k >= n) k = 0;
-    const float tp = a.top_p ? a.top_p[r] : 0.f, mp = a.min_p ? a.min_p[r] : 0.f;
-    p = tp > 0.f && tp < 1.f ? (double)tp : 0.0;
-    m = mp > 0.f && mp <= 1.f ? (double)mp : 0.0;
-    u = a.u[r];
-    u = u > 0.0 ? fmin(u, 1.0) : 0.0;             // NaN and less than 0: 0
+  __device__ Params(const Given& g, int n) {
+    greedy = !(g.T > 0.f);
+    list = g.lists();
+    k = g.k > 0 && g.k < n ? g.k : 0;
+    p = g.p > 0.f && g.p < 1.f ? (double)g.p : 0.0;
+    m = g.m > 0.f && g.m <= 1.f ? (double)g.m : 0.0;
+    u = g.u > 0.0 ? fmin(g.u, 1.0) : 0.0;         // NaN and less than 0: 0
   }
 };
 // Largest whole number not above part * all, and below all.
@@ -432,6 +448,7 @@ __device__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, 
     s.listed = 0;
   }
   __syncthreads();
+  if (row.V <= SHORT) return;
   // the keys of x that a range begins and ends with: the largest whose bucket is at least lo, the least whose
   // bucket is at most hi; a wave for each, which tries 64 keys at a time
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -458,7 +475,22 @@ __device__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, 
 
 // Puts the values of v0 .. v1 that lie in the ranges into s.list, s.listed of them.
 template <typename X, bool WIDE>
-__device__ void gather(const Row<X, WIDE>& row, int v0, int v1, Shared& s) {
+__device__ void gather(const Row<X, WIDE>& row, const Scale& scale, int v0, int v1, Shared& s) {
+  auto put = [&](int v, float y) {
+    const unsigned at = atomicAdd(&s.listed, 1u);
+    if (at < CAP) s.list[at] = (unsigned long long)key_of(y) << 32 | (uint32_t)~v;
+  };
+  if (row.V <= SHORT) {                           // too few values to look for the ranges' borders first
+    row.each(v0, v1, [&](int v, float x) {
+      const float y = row.divided(x);
+      const int b = scale.bucket(y);
+      bool in = false;
+      for (int i = 0; i < s.ranges; ++i) in |= b >= s.range[i].lo && b <= s.range[i].hi;
+      if (in && x == x) put(v, y);
+    });
+    __syncthreads();
+    return;
+  }
   float least[4], most[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -470,10 +502,7 @@ __device__ void gather(const Row<X, WIDE>& row, int v0, int v1, Shared& s) {
     bool in = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) in |= x >= least[i] && x <= most[i];
-    if (in) {
-      const unsigned at = atomicAdd(&s.listed, 1u);
-      if (at < CAP) s.list[at] = (unsigned long long)key_of(row.divided(x)) << 32 | (uint32_t)~v;
-    }
+    if (in) put(v, row.divided(x));
   });
   __syncthreads();
 }
@@ -757,13 +786,14 @@ __device__ bool finish_early(const Args& a, int r, const Params& q, unsigned lon
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
   const int r = blockIdx.x;
-  const Row<X, WIDE> row(a, r);
+  const Given given(a, r);
+  const Row<X, WIDE> row(a, given, r);
   unsigned long long best;
   int n;
   survey(row, 0, a.V, s, best, n);
-  const Params q(a, r, n);
+  const Params q(given, n);
   if (finish_early(a, r, q, best, n)) return;
   const uint32_t top = key_of(row.divided(value_of((uint32_t)(best >> 32))));
   const Scale scale(value_of(top));
@@ -774,7 +804,7 @@ __global__ __launch_bounds__(NT) void row_kernel(Args a) {
     finish_digits(a, r, row, q, scale, top, n, s);
     return;
   }
-  gather(row, 0, a.V, s);
+  gather(row, scale, 0, a.V, s);
   sort_list(s.total, s);
   finish_list(a, r, q, scale, top, n, s);
 }
@@ -804,9 +834,10 @@ struct RowSpace {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
-  const Row<X, WIDE> row(a, r);
+  const Given given(a, r);
+  const Row<X, WIDE> row(a, given, r);
   const RowSpace w(a, r);
   const int v0 = g * a.slice, v1 = min(v0 + a.slice, a.V);
   unsigned long long best;
@@ -818,7 +849,7 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
     if (g == 0) { *w.listed = 0; *w.arrived = 0; }
   }
   if (n == 0 || !(row.T > 0.f) || scale.wild) return;   // nothing of it is read
-  histogram(row, v0, v1, scale, a.bits, !lists(a, r), s);
+  histogram(row, v0, v1, scale, a.bits, !given.lists(), s);
   for (int i = threadIdx.x; i < NB; i += NT) {
     w.count[(size_t)g * NB + i] = s.count[i];
     w.mass[(size_t)g * NB + i] = s.mass[i];
@@ -828,9 +859,10 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x < PER_BIT) s.roots[threadIdx.x] = power((double)threadIdx.x / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
-  const Row<X, WIDE> row(a, r);
+  const Given given(a, r);
+  const Row<X, WIDE> row(a, given, r);
   const RowSpace w(a, r);
   SliceInfo* info = reinterpret_cast<SliceInfo*>(s.list);   // of all slices, here
   for (int i = threadIdx.x; i < a.slices; i += NT) info[i] = w.info[i];
@@ -841,7 +873,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
     best = info[i].best > best ? info[i].best : best;
     n += info[i].n;
   }
-  const Params q(a, r, n);
+  const Params q(given, n);
   if (n == 0 || q.greedy) {
     if (g == 0) finish_early(a, r, q, best, n);
     return;
@@ -904,7 +936,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   // The list passes between workgroups of one launch, on whatever XCD they run: its stores and loads are of device
   // scope, which pass the L2s by, and done before the arrival is counted.  (Plain stores and a fence write
   // back the whole L2 for every workgroup.)
-  gather(row, alone ? 0 : g * a.slice, alone ? a.V : min((g + 1) * a.slice, a.V), s);
+  gather(row, scale, alone ? 0 : g * a.slice, alone ? a.V : min((g + 1) * a.slice, a.V), s);
   if (threadIdx.x == 0) s.found = (int)atomicAdd(w.listed, s.listed);
   __syncthreads();
   for (int i = threadIdx.x; i < (int)s.listed; i += NT)
