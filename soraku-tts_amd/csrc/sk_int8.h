@@ -256,20 +256,23 @@ struct LinearArgs {
   int mt, nt, gm;                                 // tiles along M and N, tiles along M per group
 };
 
-// g / (1 + e^-g) with the GPU's own powers of two and reciprocals (each within a step of the result): t = -g log2(e)
-// in two parts, 2^t_hi (1 + t_lo ln 2).  Below -87 it is 0.
+// g / (1 + e^-g) with the GPU's own powers of two and reciprocals (each within a step of the result).  For FP32 outputs
+// t = -g log2(e) in two parts, 2^t_hi (1 + t_lo ln 2); below -87 it is 0.  For BF16 ones t alone: its rounding moves e^-g by
+// |g| 2^-24, where the output's is 2^-8 (7,680 x 6144 outputs: 5 of 26 instructions each).
+template <typename X>
 __device__ __forceinline__ float silu(float g) {
   constexpr float L = 1.44269504088896341f, L2 = 1.92596299e-8f, LN2 = 0.693147181f;   // log2(e) = L + L2
+  if constexpr (sizeof(X) == 2) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-g * L));
   const float h = __builtin_amdgcn_fmed3f(g, -150.f, 150.f);   // past those e is 0 or infinite
   const float t = -h * L, lo = fmaf(-h, L2, fmaf(-h, L, -t));
   const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, LN2, 1.f);
   return g * __builtin_amdgcn_rcpf(1.f + e);
 }
 // act of sums of row m (scale s) and column c (scale w, bias b; SwiGLU: and of its up column).
-template <bool SWIGLU>
+template <typename X, bool SWIGLU>
 __device__ __forceinline__ float act_of(int acc, int up, float s, float w, float w2, float b, float b2) {
   const float y = (float)acc * s * w + b;
-  if constexpr (SWIGLU) return silu(y) * ((float)up * s * w2 + b2);
+  if constexpr (SWIGLU) return silu<X>(y) * ((float)up * s * w2 + b2);
   else return y;
 }
 
@@ -471,10 +474,10 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
           }
           const v16i &y = acc[i][j], &u = acc[i][SWIGLU ? j + TN / 2 : j];
           float4 o;
-          o.x = act_of<SWIGLU>(y[4 * g], u[4 * g], sc, w.x, w2.x, b.x, b2.x);
-          o.y = act_of<SWIGLU>(y[4 * g + 1], u[4 * g + 1], sc, w.y, w2.y, b.y, b2.y);
-          o.z = act_of<SWIGLU>(y[4 * g + 2], u[4 * g + 2], sc, w.z, w2.z, b.z, b2.z);
-          o.w = act_of<SWIGLU>(y[4 * g + 3], u[4 * g + 3], sc, w.w, w2.w, b.w, b2.w);
+          o.x = act_of<X, SWIGLU>(y[4 * g], u[4 * g], sc, w.x, w2.x, b.x, b2.x);
+          o.y = act_of<X, SWIGLU>(y[4 * g + 1], u[4 * g + 1], sc, w.y, w2.y, b.y, b2.y);
+          o.z = act_of<X, SWIGLU>(y[4 * g + 2], u[4 * g + 2], sc, w.z, w2.z, b.z, b2.z);
+          o.w = act_of<X, SWIGLU>(y[4 * g + 3], u[4 * g + 3], sc, w.w, w2.w, b.w, b2.w);
           *reinterpret_cast<float4*>(part + i32 * LD + (j - j0) * 32 + g * 8 + hi * 4) = o;
         }
       __builtin_amdgcn_wave_barrier();
@@ -490,10 +493,16 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   }
 }
 
+// This wave's loads into LDS but the last N are in.
+template <int N>
+__device__ __forceinline__ void loads_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
 // Products of few rows: a workgroup has NT tiles of 16 weight rows (SwiGLU: half of them gate,
 // half the same rows of up) and MT tiles of 16 activation rows, and its W waves take every W-th
-// unit of 128 codes; their sums meet in LDS.  The weights' bytes bound it: they go
-// straight to registers as matrix fragments, D units ahead, and are read once for all rows.
+// unit of 128 codes; their sums meet in LDS.  The weights' bytes bound it.  They go to LDS in whole lines,
+// 8 lanes to a row, into a ring of D units that is the wave's own, so that no wave waits for another, and
+// from there to registers as matrix fragments (a load in the order of a fragment's lanes, 16 rows next to each other,
+// takes 3.5 times as long: 2048 x 6144, 128 workgroups, 4.5 us against 2.7 with the launch).
 //
 // FUSED (up to 8 rows, a power of two times K at most 16,384): the workgroup codes the
 // activations' rows itself, each into its own LDS, which saves the launch that writes them;
@@ -502,41 +511,46 @@ template <typename X, bool SWIGLU, bool FUSED, bool WHOLE, int MT, int NT, int W
 __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
   static_assert(!SWIGLU || NT % 2 == 0, "gate and up of the same columns");
   static_assert(!FUSED || (MT == 1 && W == 8), "8 waves code up to 8 rows");
-  constexpr int NC = (SWIGLU ? NT / 2 : NT) * 16;
-  extern __shared__ __attribute__((aligned(16))) char dyn[];   // FUSED: codes, rows Kp + 16 apart; then the waves' sums
+  constexpr int NC = (SWIGLU ? NT / 2 : NT) * 16, AT = FUSED ? 0 : MT, T = NT + AT;   // tiles that a unit loads
+  constexpr int RING = W * D * T * 2048, VECS = MT * NT * 64;   // of four sums: [MT][NT][lane]
+  static_assert(RING >= W * VECS * 16, "the waves' sums lie in the ring");
+  __shared__ __attribute__((aligned(1024))) char ring[RING];
+  __shared__ __attribute__((aligned(16))) char own[FUSED ? 8 * (2048 + 16) : 16];   // codes of rows, Kp + 16 apart
+  __shared__ float row_scale[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane & 15, q4 = lane >> 4;
   const int n0 = blockIdx.x * NC, m0 = blockIdx.y * (MT * 16);
   const int Kp = a.Kp, units = Kp / 128;
   const int mine = units > wave ? (units - wave + W - 1) / W : 0;
 
-  const int8_t* wp[NT];
+  // tile t, half h: 8 rows; the lane of slot c takes piece c ^ (row / 2 % 8) of its row, so that the 16 rows of a
+  // fragment lie in different banks
+  const char* gb[T];
+  unsigned voff[T][2];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const bool is_up = SWIGLU && j >= NT / 2;
-    const int n = min(n0 + (is_up ? j - NT / 2 : j) * 16 + i16, a.N - 1);
-    wp[j] = a.w + ((size_t)(is_up ? a.N : 0) + n) * Kp + wave * 128 + q4 * 16;
+  for (int t = 0; t < T; ++t) {
+    const bool act = t >= NT, is_up = SWIGLU && !act && t >= NT / 2;
+    const int first = act ? m0 + (t - NT) * 16 : n0 + (is_up ? t - NT / 2 : t) * 16, last = act ? a.M - 1 : a.N - 1;
+    const int r0 = min(first, last);
+    gb[t] = reinterpret_cast<const char*>(act ? a.a : a.w) + ((size_t)(is_up ? a.N : 0) + r0) * Kp + wave * 128;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = h * 8 + (lane >> 3);
+      voff[t][h] = (unsigned)((min(first + row, last) - r0) * Kp + ((lane & 7) ^ (row >> 1)) * 16);
+    }
   }
-  v4i b[D][NT][2];
-  auto load_w = [&](int d, int i) {
+  char* mine_at = ring + wave * (D * T * 2048);
+  auto issue = [&](int d, int i) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) b[d][j][h] = *reinterpret_cast<const v4i*>(wp[j] + (size_t)i * (W * 128) + h * 64);
+      for (int h = 0; h < 2; ++h) lds_load16(gb[t] + (size_t)i * (W * 128), voff[t][h], mine_at + (d * T + t) * 2048 + h * 1024);
   };
 #pragma unroll
   for (int d = 0; d < D; ++d)
-    if (d < mine) load_w(d, d);
+    if (d < mine) issue(d, d);
 
-  const int8_t* ap[MT];
-  v4i af[D][MT][2];
-  auto load_a = [&](int d, int i) {
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) af[d][j][h] = *reinterpret_cast<const v4i*>(ap[j] + (size_t)i * (W * 128) + h * 64);
-  };
-  __shared__ float row_scale[8];
+  const int8_t* ap = nullptr;
   if constexpr (FUSED) {
     constexpr int C = 4;
     __shared__ uint32_t tops[8];
@@ -580,19 +594,12 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
         if (c * step < Kp) {
           coder.scale8(t[c]);
           const uint2 v = coder.code8(t[c]);
-          if (k < Kp) *reinterpret_cast<uint2*>(dyn + (size_t)row * (Kp + 16) + k) = v;
+          if (k < Kp) *reinterpret_cast<uint2*>(own + (size_t)row * (Kp + 16) + k) = v;
         }
       }
     }
     __syncthreads();
-    ap[0] = reinterpret_cast<const int8_t*>(dyn) + min(i16, a.M - 1) * (Kp + 16) + wave * 128 + q4 * 16;
-  } else {
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-      ap[j] = a.a + (size_t)min(m0 + j * 16 + i16, a.M - 1) * Kp + wave * 128 + q4 * 16;
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (d < mine) load_a(d, d);
+    ap = reinterpret_cast<const int8_t*>(own) + min(i16, a.M - 1) * (Kp + 16) + wave * 128 + q4 * 16;
   }
 
   v4i acc[MT][NT];
@@ -600,28 +607,40 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  constexpr int L = 2 * T;                        // loads of a unit
+  static_assert(D >= 2 && D <= 4 && 3 * L < 64, "the waits below, and their counter");
   for (int i0 = 0; i0 < mine; i0 += D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      if (i0 + d >= mine) break;
-      if constexpr (FUSED) load_a(d, i0 + d);
+      const int i = i0 + d, behind = min(D - 1, mine - 1 - i);
+      if (behind < 0) break;
+      if (D > 3 && behind == 3) loads_but<(D > 3 ? 3 : 0) * L>();
+      else if (D > 2 && behind == 2) loads_but<(D > 2 ? 2 : 0) * L>();
+      else if (behind == 1) loads_but<L>();
+      else loads_but<0>();
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const char* l = mine_at + d * T * 2048 + i16 * 128 + ((h * 4 + q4) ^ (i16 >> 1)) * 16;
+        v4i bf[NT], af[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) bf[j] = *reinterpret_cast<const v4i*>(l + j * 2048);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          af[m] = FUSED ? *reinterpret_cast<const v4i*>(ap + (size_t)i * (W * 128) + h * 64) : *reinterpret_cast<const v4i*>(l + (NT + m) * 2048);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[d][j][h], af[d][i][h], acc[i][j], 0, 0, 0);
-      if (i0 + d + D < mine) {
-        load_w(d, i0 + d + D);
-        if constexpr (!FUSED) load_a(d, i0 + d + D);
+          for (int m = 0; m < MT; ++m) acc[m][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af[m], acc[m][j], 0, 0, 0);
+      }
+      if (i + D < mine) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the unit's place is read
+        issue(d, i + D);
       }
     }
   }
 
-  constexpr int VECS = MT * NT * 64;              // of four sums: [MT][NT][lane]
-  v4i* sum = reinterpret_cast<v4i*>(dyn);
-  if constexpr (FUSED) __syncthreads();           // the codes are read
+  v4i* sum = reinterpret_cast<v4i*>(ring);
+  __syncthreads();                                // the rings are read
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -645,8 +664,8 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int c = min(n + v, a.N - 1);
-      out[v] = act_of<SWIGLU>(y[v], up[v], sc, a.ws[c], SWIGLU ? a.ws[a.N + c] : 0.f, a.bias ? a.bias[c] : 0.f,
-                              SWIGLU && a.bias ? a.bias[a.N + c] : 0.f);
+      out[v] = act_of<X, SWIGLU>(y[v], up[v], sc, a.ws[c], SWIGLU ? a.ws[a.N + c] : 0.f, a.bias ? a.bias[c] : 0.f,
+                                 SWIGLU && a.bias ? a.bias[a.N + c] : 0.f);
     }
     emit<X, 4>(a, m, n, out);
   }

@@ -57,12 +57,18 @@ void launch_rows(const RowsArgs& a, hipStream_t st) {
   else launch_rows_as<X, NORM>(a, st);
 }
 
-// How a product is computed: by a workgroup per 16 columns and up to 32 rows, which
-// may code the rows itself, or in tiles.
+// How a product is computed: by few_kernel, whose workgroups take few rows and columns and may code the rows
+// themselves, or in tiles.
 struct Plan {
   bool fused, few;
-  int tile, bm, bn;                               // of TILES; rows and columns (SwiGLU: gate and up together) of a workgroup
+  int kind, bm, bn;                               // of FEW or TILES; rows and columns (SwiGLU: gate and up together) of a workgroup
 };
+// Estimated us of few_kernel when a CU has r workgroups, which each load u units of `tiles` tiles of 16 rows: 2.1 + 0.9
+// (r - 1) + 0.0265 r u tiles, a CU's 75 GB/s (16 to 256 rows of six projections: within 15%, but 30 to 40% less than SwiGLU products
+// of 25 MB, which come from HBM).  E.g. 32 rows of 2048 x 6144: 16 rows by 16 columns 4.6 us, 32 by 32 6.8, in tiles
+// of 64 x 64 15.4; 128 rows: 32 by 32 7.1, 64 by 32 9.4, 64 x 64 15.2; 256 rows of 4096 x 2048: 64 by 32 9.6, 64 x 64 7.6.
+struct Few { int mt, nt; };
+constexpr Few FEW[] = {{1, 1}, {2, 1}, {1, 2}, {2, 2}, {4, 2}};   // SwiGLU: from the third on
 // Estimated us of a launch of tiles when a CU has r of them, of u stages: fix + r round + u lat + (r - 1) u thr, fitted
 // to 207 times (33 to 7,680 rows, the trunks' projections and odd ones; rms error 7 to 24%).  The tile chosen is on
 // average within 6% of the fastest (SwiGLU 3%).  E.g. 7,680 rows of 2 x 6144 x 2048: 256 x 256 204 us, 128 x 128 231;
@@ -73,28 +79,34 @@ constexpr Tile TILES[] = {{256, 256, 0.f, 7.19f, 1.10f, 2.28f, 0.f, 8.47f, 1.15f
                           {128, 128, .98f, 4.06f, .56f, .37f, 2.16f, 1.92f, .62f, .49f},
                           {64, 128, 2.07f, 1.73f, .41f, .26f, 2.27f, .75f, .44f, .31f},
                           {64, 64, 1.93f, 1.35f, .26f, .18f, 2.31f, 1.04f, .42f, .19f}};
-// Up to 32 rows the weights' bytes bound a product and tiles of 64 rows would be half empty (32 rows of 2048 x
-// 6144: 10.1 us, in tiles 15.4; 64: 15.6 and 15.4).  Up to 8 the workgroups code the rows themselves where each wave
-// then has at most 2,048 values (2 rows x 4096 x 2048: 6.5 us, with a launch for the codes 8 in two).
+// Up to 8 rows the workgroups code the rows themselves where each wave then has at most 2,048 values (2 rows x 4096 x
+// 2048: 5.6 us, with a launch for the codes 7 in two).
 Plan plan_linear(int M, int N, int K, bool swiglu) {
   const int rows2 = M > 4 ? 8 : M > 2 ? 4 : M;
   Plan p{};
-  p.few = M <= 32;
-  p.fused = M <= 8 && rows2 * K <= 16384;
-  if (p.few) {
-    p.bm = M <= 16 ? 16 : 32;
-    // wide ones read their rows' codes less often (32 rows of 2 x 6144 x 2048: 8.4 us, 9.9 by 16 columns)
-    p.bn = !swiglu ? 16 : !p.fused && N >= 4096 ? 64 : 32;
+  if (M <= 8 && rows2 * K <= 16384) {
+    p.few = p.fused = true;
+    p.bm = 16;
+    p.bn = swiglu ? 32 : 16;
     return p;
   }
+  const float u = (float)(padded(K) / 128);
   float best = 1e30f;
+  auto take = [&](bool few, int kind, int bm, int bn, auto us) {
+    const int nc = swiglu ? bn / 2 : bn;
+    const int64_t groups = (int64_t)((M + bm - 1) / bm) * ((N + nc - 1) / nc);
+    const float t = us((float)((groups + 255) / 256));
+    if (t < best) { best = t; p = Plan{false, few, kind, bm, bn}; }
+  };
+  for (int i = swiglu ? 2 : 0; i < (int)(sizeof(FEW) / sizeof(Few)) && M <= 1024; ++i) {
+    const Few f = FEW[i];
+    take(true, i, f.mt * 16, f.nt * 16, [&](float r) { return 2.1f + .9f * (r - 1) + .0265f * r * u * (f.mt + f.nt); });
+  }
   for (int i = 0; i < (int)(sizeof(TILES) / sizeof(Tile)); ++i) {
     const Tile& t = TILES[i];
-    const int nc = swiglu ? t.bn / 2 : t.bn;
-    const int64_t tiles = (int64_t)((M + t.bm - 1) / t.bm) * ((N + nc - 1) / nc);
-    const float r = (float)((tiles + 255) / 256), u = (float)(padded(K) / 128);
-    const float us = swiglu ? t.fix2 + r * t.round2 + u * (t.lat2 + (r - 1) * t.thr2) : t.fix + r * t.round + u * (t.lat + (r - 1) * t.thr);
-    if (us < best) { best = us; p.tile = i; p.bm = t.bm; p.bn = t.bn; }
+    take(false, i, t.bm, t.bn, [&](float r) {
+      return swiglu ? t.fix2 + r * t.round2 + u * (t.lat2 + (r - 1) * t.thr2) : t.fix + r * t.round + u * (t.lat + (r - 1) * t.thr);
+    });
   }
   return p;
 }
@@ -105,21 +117,19 @@ int64_t space_of(const Plan& p, int M, int K) { return p.fused || M == 0 ? 0 : c
 
 template <typename X, bool SWIGLU>
 void launch_few(const Plan& p, const LinearArgs& a, const RowsArgs& r, hipStream_t st) {
-  auto go = [&](auto kernel, int MT, int NT, bool fused) {
-    const size_t codes = fused ? (size_t)a.M * (a.Kp + 16) : 0;
-    hipLaunchKernelGGL(kernel, dim3(a.nt, a.mt), dim3(512), std::max<size_t>(codes, (size_t)8 * MT * NT * 1024), st, a, r);
-  };
+  auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(a.nt, a.mt), dim3(waves * 64), 0, st, a, r); };
   constexpr int NT = SWIGLU ? 2 : 1;
   if (p.fused) {
-    if (r.K % 8 == 0) go(few_kernel<X, SWIGLU, true, true, 1, NT, 8, 2>, 1, NT, true);
-    else go(few_kernel<X, SWIGLU, true, false, 1, NT, 8, 2>, 1, NT, true);
+    if (r.K % 8 == 0) go(few_kernel<X, SWIGLU, true, true, 1, NT, 8, 3>, 8);
+    else go(few_kernel<X, SWIGLU, true, false, 1, NT, 8, 3>, 8);
+    return;
   }
-  else if (p.bm == 16) {
-    if (p.bn == 64) { if constexpr (SWIGLU) go(few_kernel<X, SWIGLU, false, true, 1, 4, 8, 2>, 1, 4, false); }
-    else go(few_kernel<X, SWIGLU, false, true, 1, NT, 8, 2>, 1, NT, false);
-  } else {
-    if (p.bn == 64) { if constexpr (SWIGLU) go(few_kernel<X, SWIGLU, false, true, 2, 4, 8, 2>, 2, 4, false); }
-    else go(few_kernel<X, SWIGLU, false, true, 2, NT, 8, 2>, 2, NT, false);
+  switch (p.kind) {
+    case 0: if constexpr (!SWIGLU) go(few_kernel<X, SWIGLU, false, true, 1, 1, 8, 2>, 8); break;
+    case 1: if constexpr (!SWIGLU) go(few_kernel<X, SWIGLU, false, true, 2, 1, 8, 2>, 8); break;
+    case 2: go(few_kernel<X, SWIGLU, false, true, 1, 2, 8, 2>, 8); break;
+    case 3: go(few_kernel<X, SWIGLU, false, true, 2, 2, 8, 2>, 8); break;
+    default: go(few_kernel<X, SWIGLU, false, true, 4, 2, 4, 2>, 4); break;
   }
 }
 template <typename X, bool SWIGLU>
@@ -128,7 +138,7 @@ void launch_tiles(const Plan& p, const LinearArgs& a, hipStream_t st) {
     const int64_t tiles = (int64_t)a.mt * a.nt;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(waves * 64), 0, st, a);
   };
-  switch (p.tile) {
+  switch (p.kind) {
     case 0: go(tiles_kernel<X, SWIGLU, 256, 256, 4, 4, 2, 2>, 16); break;
     case 1: go(tiles_kernel<X, SWIGLU, 192, 256, 2, 4, 2, 2>, 8); break;
     case 2: go(tiles_kernel<X, SWIGLU, 128, 128, 2, 2, 2, 2>, 4); break;

@@ -379,8 +379,8 @@ def int8_rows(K: int):
     def kernel(x):
         T = _torch()
         at, rows, xd = _matrix(x, "x", K, T.codes)
-        codes = T.empty((rows, -(-K // 128) * 128), device=x.device, dtype=T.i8)
-        scales = T.empty((rows,), device=x.device, dtype=T.f32)
+        codes = x.new_empty(rows, -(-K // 128) * 128, dtype=T.i8)
+        scales = x.new_empty(rows, dtype=T.f32)
         _call(T, T.lib.sk_op_int8_rows, at, rows, K, xd, x.data_ptr(), codes.data_ptr(), scales.data_ptr())
         return codes, scales
     return kernel
@@ -406,12 +406,12 @@ def int8_linear(N: int, K: int, act: str | None = None, eps: float | None = None
         at, rows, xd = _matrix(x, "x", K, T.codes)
         shape = (rows, N)
         if out is None:
-            out = T.empty(shape, device=x.device, dtype=dt)
+            out = x.new_empty(rows, N)
             op = out.data_ptr()
         else:
             op = _need(out, "out", dt, at, shape)
         size = _linear_workspace(rows, N, K, xd, act)
-        ws = T.empty(size, device=x.device, dtype=T.u8) if size else None
+        ws = x.new_empty(size, dtype=T.u8) if size else None
         _call(T, T.lib.sk_op_int8_linear, at, rows, N, K, xd, act, eps, x.data_ptr(),
               None if gain is None else _need(gain, "gain", f32, at, (K,)), _need(codes, "codes", T.i8, at, (both, kp)),
               _need(scales, "scales", f32, at, (both,)), None if bias is None else _need(bias, "bias", f32, at, (both,)),
@@ -460,7 +460,7 @@ def sample_rows(V: int, cfg: bool = False):
             raise ValueError("cfg_scale comes with cfg")
         n = (rows,)
         if out is None:
-            out = T.empty(n, device=logits.device, dtype=T.i64)
+            out = logits.new_empty(rows, dtype=T.i64)
             op = out.data_ptr()
         else:
             op = _need(out, "out", T.i64, at, n)
@@ -471,7 +471,7 @@ def sample_rows(V: int, cfg: bool = False):
             _need(allowed, "allowed", i32, at, (allowed.shape[0], words))
             apart = words if allowed.shape[0] == rows else 0
         size = _sample_workspace(rows, V, dt)
-        ws = T.empty(size, device=logits.device, dtype=T.u8) if size else None
+        ws = logits.new_empty(size, dtype=T.u8) if size else None
         _call(T, T.lib.sk_op_sample_rows, at, rows, V, dt, logits.data_ptr(), stride, _need(u, "u", T.f64, at, n),
               None if temperature is None else _need(temperature, "temperature", f32, at, n),
               None if top_k is None else _need(top_k, "top_k", i32, at, n),

@@ -29,7 +29,7 @@ def codes(t):
     return out, scale
 
 
-def linear(x, w, ws, gain=None, eps=None, bias=None, residual=None, swiglu=False):
+def linear(x, w, ws, gain=None, eps=None, bias=None, residual=None, swiglu=False, bf16=False):
     """(out, bound): the projection in 64 bits from FP32 values x and codes w, and how far FP32
     arithmetic may be from it before the output's own rounding.
 
@@ -37,8 +37,10 @@ def linear(x, w, ws, gain=None, eps=None, bias=None, residual=None, swiglu=False
     at most K/512 + 14 positive terms one on another (8 in a lane, 6 exchanges, the blocks), so it is
     within (K/512 + 14) EPS32; root and quotient halve that and add two steps, the mean and eps two more
     halves; top / 127, the product with it, the whole sum as FP32 and two products by scales: five
-    more.  silu(g) = g / (1 + e^-g): the exponential within 4 EPS32, sum and quotient 2; an error r of g
-    moves it by at most (1 + |g|) r."""
+    more.  silu(g) = g / (1 + e^-g): the GPU's power of two and its reciprocal are each within a step (2 EPS32) of the
+    result; the power's correction adds 2, the sum, the product and the last product 1 each: 9.  For BF16 outputs the
+    exponent -g log2(e) is rounded (EPS32 of it, and 0.22 for the constant: together 1.25 |g| ln 2 log2(e) EPS32 of
+    the power).  An error r of g moves silu by at most (1 + |g|) r."""
     x = np.asarray(x, np.float32)
     with np.errstate(all="ignore"):
         t = x if gain is None else (x * np.asarray(gain, np.float32)).astype(np.float32)
@@ -64,7 +66,7 @@ def linear(x, w, ws, gain=None, eps=None, bias=None, residual=None, swiglu=False
         # |d silu| <= 1.1, and where silu is tiny its slope is at most (1 + |g|) of its value over |g|
         slope = np.minimum(1.1, np.abs(a) * (1 + np.abs(g)) / np.maximum(np.abs(g), 1e-300))
         slope = np.where(np.abs(g) < 1, 1.1, slope)
-        oa = slope * og * 1.01 + np.abs(a) * 7 * EPS32
+        oa = slope * og * 1.01 + np.abs(a) * (9 + (1.25 * np.abs(g) if bf16 else 0)) * EPS32
         y = a * u
         off = oa * np.abs(u) + np.abs(a) * ou + oa * ou + np.abs(y) * EPS32
     if residual is not None:

@@ -108,7 +108,7 @@ def on(d, dev):
 
 def expected(d, eps, swiglu):
     np_ = {k: None if v is None else (v.numpy() if k in ("codes", "scales") else f32(v)) for k, v in d.items()}
-    return ref.linear(np_["x"], np_["codes"], np_["scales"], np_["gain"], eps, np_["bias"], np_["residual"], swiglu)
+    return ref.linear(np_["x"], np_["codes"], np_["scales"], np_["gain"], eps, np_["bias"], np_["residual"], swiglu, d["x"].dtype == BF16)
 
 
 def check_linear(ops, m, n, k, dtype, dev, eps=None, swiglu=False, **kw):
