@@ -10,8 +10,10 @@ def safe(v):
     """Weights are rounded to whole multiples of 2^-bits of a power of two that is at most twice the largest weight, bits =
     min(46, 62 - log2 v): each is off by at most half of one, at random; 16 sqrt(v) of them is 55 standard deviations of
     their sum (0.29 sqrt(v)), and the whole is at least the largest weight.  The reference's own sums in 64 bits are off by
-    less (at most v 2^-53, as they fall sqrt(v) 2^-53)."""
-    return 16 * 2 * v ** 0.5 * 2.0 ** -min(46, 62 - int(np.ceil(np.log2(max(v, 2)))))
+    less (at most v 2^-53, as they fall sqrt(v) 2^-53).  Past 16,384 values up to 10 workgroups each leave 1,504 sums cut to
+    whole multiples, less than one each."""
+    cut = 10 * 1504 if v > 16384 else 0
+    return 2 * (16 * v ** 0.5 + cut) * 2.0 ** -min(46, 62 - int(np.ceil(np.log2(max(v, 2)))))
 
 
 def merge(logits, scale):

@@ -327,3 +327,17 @@ def test_python_refusals(ops, hip_device):
         g(x.view(2, 2, 100), u[:2])
     with pytest.raises(ValueError):
         g(x, u, cfg_scale=u.float())
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_a_slice_past_4096_below_a_largest_within(ops, hip_device, rows):
+    """Largest values within 4,096 of 0 in one workgroup's part of the row, those of the other parts just past it."""
+    rng = np.random.default_rng(44)
+    V = 20000
+    x = -4101 - 6 * rng.random((rows, V))
+    x[:, 15000] = -4094.5
+    x[:, 15003] = -4095
+    x[-1, 9] = -4096.5
+    p = dict(top_p=torch.full((rows,), 0.97), top_k=torch.tensor([0, 5000, 0][:rows], dtype=torch.int32))
+    for u in (0.01, 0.3, 0.6, 0.95):
+        check(ops, hip_device, torch.from_numpy(x.astype(np.float32)), [u] * rows, least=1.0, **p)
