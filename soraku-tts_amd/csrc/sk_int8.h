@@ -185,7 +185,9 @@ struct RowsArgs {
 
 // Codes of R rows: W waves per row, C chunks of 512 W values held in registers (C = 0:
 // any K, read twice).  Bytes bound it: each value read once (the second read of C = 0
-// comes from cache) and each code written once.
+// comes from cache) and each code written once.  12,288 x 2048 in BF16: 15.4 us, 4.9 TB/s; 5,999 x 6144: 18.6 us,
+// 6.0 TB/s; 16,404 x 2048 in FP32: 34 us, 4.9 TB/s.  A few hundred rows take 3 to 4 us, the time of a launch and
+// of one load and one exchange after the other.
 template <typename X, int W, int C, bool WHOLE, int MODE>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -319,15 +321,21 @@ __device__ __forceinline__ void emit(const LinearArgs& a, int m, int n, float (&
 
 // Products of many rows, in tiles of BM x BN (SwiGLU: BN / 2 gate and the same BN / 2 up
 // columns) by WM x WN waves.  A stage is 128 codes of every row of the tile, loaded straight
-// to LDS: 8 lanes take a row's whole line, and the lane of slot c takes piece c ^ (row % 8),
-// so that the 16 rows of a matrix fragment lie in different banks.  S stages in a ring with one
+// to LDS: 8 lanes take a row's whole line, and the lane of slot c takes piece c ^ (row / 2 % 8),
+// so that the rows of a matrix fragment lie in different banks.  S stages in a ring with one
 // barrier each.  The matrix cores take the weights as their row operand, so a lane ends up
 // with 4 neighbouring columns of one row.  Rows past M or N are clamped on load and not stored.
-template <typename X, bool SWIGLU, int BM, int BN, int WM, int WN, int S, int H>
+//
+// The matrix cores alone reach 3.6 POP/s on random codes (4.9 on zeros: the clock follows the power).  7,680 rows of
+// 2 x 6144 x 2048 (SwiGLU, BF16 out) take 204 us, 1.9 POP/s, of 2048 x 6144 82 us, 1.8 to 2.3 POP/s by what lies in
+// cache: a tile's first stage, its epilogue (26 instructions per SwiGLU output) and its store have no products beside
+// them, since LDS holds one 256 x 256 tile per CU.  Smaller tiles, two to a CU, overlap them, but load twice the
+// bytes per product: 231 us in tiles of 128 x 128.
+template <typename X, bool SWIGLU, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
-  constexpr int W = WM * WN, ROWS = BM + BN, LR = 16 / H, PER = ROWS / LR / W;   // rows per load, loads per wave
+  constexpr int W = WM * WN, ROWS = BM + BN, LR = 8, PER = ROWS / LR / W;   // rows per load, loads per wave
   static_assert(ROWS % (LR * W) == 0 && BM % 16 == 0, "every wave loads alike");
-  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, RB = 64 * H, STAGE = ROWS * RB;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, RB = 128, STAGE = ROWS * RB;
   static_assert(!SWIGLU || TN % 2 == 0, "every wave holds gate and up of its columns");
   __shared__ __attribute__((aligned(1024))) char lds[S * STAGE];
   __shared__ __attribute__((aligned(16))) float row_s[BM], col_s[BN], col_b[BN];
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   const int n0 = gr / gm * NC;
 
   const int Kp = a.Kp, nst = Kp / RB;
-  auto turn = [](int row) { return H == 1 ? row >> 2 & 3 : row >> 1 & 7; };
+  auto turn = [](int row) { return row >> 1 & 7; };
   const char* gb[PER];
   unsigned voff[PER];
 #pragma unroll
@@ -366,8 +374,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
     }
     const int r0 = min(first, last);
     gb[c] = base + (size_t)r0 * Kp;
-    const int lr = lane / (4 * H), row = g * LR + lr;
-    voff[c] = (unsigned)((min(first + lr, last) - r0) * Kp + ((lane & (4 * H - 1)) ^ turn(row)) * 16);
+    const int lr = lane / 8, row = g * LR + lr;
+    voff[c] = (unsigned)((min(first + lr, last) - r0) * Kp + ((lane & 7) ^ turn(row)) * 16);
   }
   auto issue = [&](int s, int c) {
     lds_load16(gb[c] + (size_t)s * RB, voff[c], lds + (s % S) * STAGE + (wave * PER + c) * 1024);
@@ -402,7 +410,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   };
   // Loads are spread over the products too: a wave that issues all of a stage's at once stands in line for
   // the memory pipe, and its matrix core idles.
-  constexpr int P = TM * TN, L0 = (PER + 1) / 2;  // products of a piece; loads in the stage's last piece, the others in the next one's first
+  constexpr int P = TM * TN, L0 = (PER + 1) / 2;  // products of a quarter; loads in the stage's last quarter, the others in the next one's first
   auto multiply = [&](int set, const char* l, int load, int c0, int c1) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -422,13 +430,12 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   };
   // stages in flight behind the one that is waited for: at most S - 1 (first wait), then S - 2
   auto arrive = [&](int behind) {
-    if (S > 4 && behind >= 4) stage_sync<(S > 4 ? 4 : 0) * PER>();
-    else if (S > 3 && behind >= 3) stage_sync<(S > 3 ? 3 : 0) * PER>();
+    if (S > 3 && behind >= 3) stage_sync<(S > 3 ? 3 : 0) * PER>();
     else if (S > 2 && behind >= 2) stage_sync<(S > 2 ? 2 : 0) * PER>();
     else if (behind >= 1) stage_sync<PER>();
     else stage_sync<0>();
   };
-  static_assert(S >= 2 && S <= 5, "arrive() counts up to four stages");
+  static_assert(S >= 2 && S <= 4, "arrive() counts up to three stages");
 #pragma unroll
   for (int s = 0; s < S; ++s)
     if (s < nst) {
@@ -438,7 +445,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   arrive(min(S, nst) - 1);
 #pragma unroll
   for (int f = 0; f < TM + TN; ++f) fetch(piece(0, 0), 0, f);
-  constexpr int Q = 2 * H;                        // pieces of a stage
+  constexpr int Q = 4;                            // quarters of a stage
   for (int s = 0; s < nst; ++s) {
     // stage s - 1 + S goes on into the place of stage s - 1
     multiply(0, piece(s, 1), s && s - 1 + S < nst ? s - 1 + S : -1, L0, PER);
@@ -502,7 +509,9 @@ __device__ __forceinline__ void loads_but() { asm volatile("s_waitcnt vmcnt(%0)"
 // unit of 128 codes; their sums meet in LDS.  The weights' bytes bound it.  They go to LDS in whole lines,
 // 8 lanes to a row, into a ring of D units that is the wave's own, so that no wave waits for another, and
 // from there to registers as matrix fragments (a load in the order of a fragment's lanes, 16 rows next to each other,
-// takes 3.5 times as long: 2048 x 6144, 128 workgroups, 4.5 us against 2.7 with the launch).
+// takes 3.5 times as long: 2048 x 6144, 128 workgroups, 4.5 us against 2.7 with the launch).  In a cold cache 32 rows
+// of 2 x 6144 x 2048 take 8.7 us, 2.9 TB/s of weights, 32 rows of 2048 x 6144 5.1, 2 rows of 4096 x 2048 with their codes 5.5,
+// 1 row of 2051 x 1024 4.6: the launch, the latency of a ring's first units and the sum over the waves, in turn.
 //
 // FUSED (up to 8 rows, a power of two times K at most 16,384): the workgroup codes the
 // activations' rows itself, each into its own LDS, which saves the launch that writes them;

@@ -139,13 +139,13 @@ void launch_tiles(const Plan& p, const LinearArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(waves * 64), 0, st, a);
   };
   switch (p.kind) {
-    case 0: go(tiles_kernel<X, SWIGLU, 256, 256, 4, 4, 2, 2>, 16); break;
-    case 1: go(tiles_kernel<X, SWIGLU, 192, 256, 2, 4, 2, 2>, 8); break;
-    case 2: go(tiles_kernel<X, SWIGLU, 128, 128, 2, 2, 2, 2>, 4); break;
-    case 3: go(tiles_kernel<X, SWIGLU, 64, 128, 2, 2, 2, 2>, 4); break;
+    case 0: go(tiles_kernel<X, SWIGLU, 256, 256, 4, 4, 2>, 16); break;
+    case 1: go(tiles_kernel<X, SWIGLU, 192, 256, 2, 4, 2>, 8); break;
+    case 2: go(tiles_kernel<X, SWIGLU, 128, 128, 2, 2, 2>, 4); break;
+    case 3: go(tiles_kernel<X, SWIGLU, 64, 128, 2, 2, 2>, 4); break;
     default:
-      if constexpr (SWIGLU) go(tiles_kernel<X, SWIGLU, 64, 64, 2, 1, 3, 2>, 2);
-      else go(tiles_kernel<X, SWIGLU, 64, 64, 2, 2, 4, 2>, 4);
+      if constexpr (SWIGLU) go(tiles_kernel<X, SWIGLU, 64, 64, 2, 1, 3>, 2);
+      else go(tiles_kernel<X, SWIGLU, 64, 64, 2, 2, 4>, 4);
       break;
   }
 }
@@ -212,7 +212,7 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
   a.w = codes; a.ws = scales; a.bias = bias; a.res = residual; a.out = out;
   a.M = M; a.N = N; a.Kp = padded(K);
   a.mt = (M + p.bm - 1) / p.bm; a.nt = (N + nc - 1) / nc; a.gm = 8;
-  SK_CHECK((int64_t)a.mt * a.nt < INT32_MAX - 8, SK_EINVAL, "M * N is too large: several calls are needed");
+  SK_CHECK((int64_t)a.mt * a.nt < (1 << 22) - 8, SK_EINVAL, "M * N is too large: several calls are needed");   // 2^32 threads
   const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as)};
   return xdtype == SK_BF16 ? run_linear<uint16_t>((hipStream_t)stream, p, a, r, swiglu)
                            : run_linear<float>((hipStream_t)stream, p, a, r, swiglu);

@@ -57,6 +57,14 @@ def test_linear_asks_for_its_workspace(L):
     assert L.sk_op_int8_linear_workspace(0, 48, 200, 1, 1, C.byref(n)) == 0 and n.value == 0
 
 
+def test_linear_refuses_more_than_a_launch_holds(L):
+    n = C.c_int64(-1)
+    sizes = dict(M=2 ** 24 - 1, N=2 ** 20, K=128)
+    assert L.sk_op_int8_linear_workspace(*sizes.values(), 0, 0, C.byref(n)) == 0
+    assert L.sk_op_int8_linear(*dict(LINEAR, **sizes, ws=P, ws_bytes=n.value).values()) == -1
+    assert "several calls" in L.sk_last_error().decode()
+
+
 def test_python_refusals():
     import torch
 
