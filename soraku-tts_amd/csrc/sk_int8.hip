@@ -73,12 +73,12 @@ constexpr Few FEW[] = {{1, 1}, {2, 1}, {1, 2}, {2, 2}, {4, 2}};   // SwiGLU: fro
 // to 207 times (33 to 7,680 rows, the trunks' projections and odd ones; rms error 7 to 24%).  The tile chosen is on
 // average within 6% of the fastest (SwiGLU 3%).  E.g. 7,680 rows of 2 x 6144 x 2048: 256 x 256 204 us, 128 x 128 231;
 // 774 of 4096 x 1024: 64 x 128 9.2, 128 x 128 10.0, 256 x 256 15.6; 64 of 2048 x 6144: 64 x 64 15.4, 64 x 128 21.6.
-struct Tile { int bm, bn; float fix, round, lat, thr, fix2, round2, lat2, thr2; };   // 2: SwiGLU
-constexpr Tile TILES[] = {{256, 256, 0.f, 7.19f, 1.10f, 2.28f, 0.f, 8.47f, 1.15f, 1.87f},
-                          {192, 256, 0.f, 7.00f, .92f, 1.53f, 0.f, 7.23f, 1.00f, 1.40f},
-                          {128, 128, .98f, 4.06f, .56f, .37f, 2.16f, 1.92f, .62f, .49f},
-                          {64, 128, 2.07f, 1.73f, .41f, .26f, 2.27f, .75f, .44f, .31f},
-                          {64, 64, 1.93f, 1.35f, .26f, .18f, 2.31f, 1.04f, .42f, .19f}};
+struct Tile { int bm, bn, waves; float fix, round, lat, thr, fix2, round2, lat2, thr2; };   // 2: SwiGLU
+constexpr Tile TILES[] = {{256, 256, 16, 0.f, 7.19f, 1.10f, 2.28f, 0.f, 8.47f, 1.15f, 1.87f},
+                          {192, 256, 8, 0.f, 7.00f, .92f, 1.53f, 0.f, 7.23f, 1.00f, 1.40f},
+                          {128, 128, 4, .98f, 4.06f, .56f, .37f, 2.16f, 1.92f, .62f, .49f},
+                          {64, 128, 4, 2.07f, 1.73f, .41f, .26f, 2.27f, .75f, .44f, .31f},
+                          {64, 64, 4, 1.93f, 1.35f, .26f, .18f, 2.31f, 1.04f, .42f, .19f}};
 // Up to 8 rows the workgroups code the rows themselves where each wave then has at most 2,048 values (2 rows x 4096 x
 // 2048: 5.6 us, with a launch for the codes 7 in two).
 Plan plan_linear(int M, int N, int K, bool swiglu) {
@@ -135,8 +135,7 @@ void launch_few(const Plan& p, const LinearArgs& a, const RowsArgs& r, hipStream
 template <typename X, bool SWIGLU>
 void launch_tiles(const Plan& p, const LinearArgs& a, hipStream_t st) {
   auto go = [&](auto kernel, int waves) {
-    const int64_t tiles = (int64_t)a.mt * a.nt;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(waves * 64), 0, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.mt * a.nt + 7) / 8 * 8)), dim3(waves * 64), 0, st, a);
   };
   switch (p.kind) {
     case 0: go(tiles_kernel<X, SWIGLU, 256, 256, 4, 4, 2>, 16); break;
@@ -212,7 +211,8 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
   a.w = codes; a.ws = scales; a.bias = bias; a.res = residual; a.out = out;
   a.M = M; a.N = N; a.Kp = padded(K);
   a.mt = (M + p.bm - 1) / p.bm; a.nt = (N + nc - 1) / nc; a.gm = 8;
-  SK_CHECK((int64_t)a.mt * a.nt < (1 << 22) - 8, SK_EINVAL, "M * N is too large: several calls are needed");   // 2^32 threads
+  SK_CHECK(p.few || ((int64_t)a.mt * a.nt + 7) * TILES[p.kind].waves * 64 < (int64_t)1 << 32, SK_EINVAL,
+           "M * N is too large: several calls are needed");   // a launch has less than 2^32 threads
   const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as)};
   return xdtype == SK_BF16 ? run_linear<uint16_t>((hipStream_t)stream, p, a, r, swiglu)
                            : run_linear<float>((hipStream_t)stream, p, a, r, swiglu);
