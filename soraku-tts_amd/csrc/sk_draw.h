@@ -28,6 +28,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 // Each operation rounds by itself: guidance and quotients are defined so, and a t that enters a bucket
 // and a weight is one number.
 #pragma clang fp contract(off)
@@ -76,7 +78,7 @@ struct Given {
   float T, s, p, m;
   int k;
   double u;
-  __device__ Given(const Args& a, int r) {
+  __device__ __forceinline__ Given(const Args& a, int r) {
     T = a.temperature ? a.temperature[r] : 1.f;
     s = a.cfg ? a.cfg[r] : 0.f;
     p = a.top_p ? a.top_p[r] : 0.f;
@@ -97,15 +99,17 @@ struct Row {
   const uint32_t* allowed;
   float s, T;
   double inv;                                     // 1 / T, or 0: divide
+  bool whole;                                     // T = 1, or greedy: x itself
   int V;
-  __device__ Row(const Args& a, const Given& g, int r) {
+  __device__ __forceinline__ Row(const Args& a, const Given& g, int r) {
     const X* l = static_cast<const X*>(a.logits);
     cond = l + (size_t)(a.cfg ? 2 * (size_t)r : r) * a.stride;
     uncond = a.cfg ? cond + a.stride : nullptr;
     allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride : nullptr;
     s = g.s;
     T = g.T;
-    inv = !(T > 0.f) ? 1.0 : T > 0x1p-20f && T < 0x1p20f ? 1.0 / (double)T : 0.0;   // (greedy: x itself)
+    inv = T > 0x1p-20f && T < 0x1p20f ? 1.0 / (double)T : 0.0;
+    whole = __builtin_amdgcn_readfirstlane(T == 1.f || !(T > 0.f));   // one branch for a wave
     V = a.V;
   }
   // x / T rounded to FP32, held to the finite range.  By the reciprocal in 64 bits that is the same: its product is within
@@ -113,24 +117,29 @@ struct Row {
   // 2^-49 from any (x - T m is a multiple of the last place of a 49-bit product).  Results below the normal range
   // have fewer bits, so those are divided, and so is by temperatures that could make them of ordinary x.
   __device__ __forceinline__ float divided(float x) const {
+    if (whole) return x;
     float y = (float)((double)x * inv);
-    if (fabsf(y) < 0x1p-100f && x != 0.f) y = T > 0.f ? x / T : x;
+    if (fabsf(y) < 0x1p-100f && x != 0.f) y = x / T;
     return __builtin_amdgcn_fmed3f(y, -3.402823466e38f, 3.402823466e38f);
   }
-  // x of cond and uncond; NaN: no candidate
-  __device__ __forceinline__ float x_of(float x, float u, bool on) const {
-    if (uncond) x = u + s * (x - u);
-    return fabsf(x) <= 3.402823466e38f && on ? x : __uint_as_float(0x7fc00000u);
-  }
+  // x of cond and uncond
+  __device__ __forceinline__ float x_of(float x, float u) const { return u + s * (x - u); }
+  static __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
   // the key of y
   __device__ __forceinline__ uint32_t key(int v) const {
-    const float x = x_of(to_f<X>(cond[v]), uncond ? to_f<X>(uncond[v]) : 0.f, !allowed || (allowed[v >> 5] >> (v & 31) & 1u));
-    return x == x ? key_of(divided(x)) : 0u;
+    float x = to_f<X>(cond[v]);
+    if (uncond) x = x_of(x, to_f<X>(uncond[v]));
+    return finite(x) && (!allowed || (allowed[v >> 5] >> (v & 31) & 1u)) ? key_of(divided(x)) : 0u;
   }
-  // f(id, x) of values v0 .. v1 (x NaN: no candidate), 16 values of a thread (8 of them one by one) on their way at a time.  WIDE: v0
-  // and v1 are at whole pieces.
+  // f(id, x, whether it is a candidate) of values v0 .. v1, a thread's in the order of ids, 16 of them (8 of them one by one) on
+  // their way at a time.  WIDE: v0 and v1 are at whole pieces.
   template <typename F>
   __device__ __forceinline__ void each(int v0, int v1, F f) const {
+    if (uncond || allowed) each_as<true>(v0, v1, f);
+    else each_as<false>(v0, v1, f);
+  }
+  template <bool MORE, typename F>
+  __device__ __forceinline__ void each_as(int v0, int v1, F f) const {
     constexpr int P = WIDE ? 16 / (int)sizeof(X) : 1, U = WIDE ? 16 / P : 8;
     auto load = [](const X* p) {
       if constexpr (WIDE) return *reinterpret_cast<const uint4*>(p);
@@ -146,21 +155,31 @@ struct Row {
     };
     using Piece = decltype(load(cond));
     for (int at = v0; at < v1; at += U * P * NT) {
-      Piece c[U], u[U];
-      uint32_t bits[U];
+      Piece c[U], u[MORE ? U : 1];
+      uint32_t bits[MORE ? U : 1];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int l = min(at + (i * NT + (int)threadIdx.x) * P, v1 - P);
         c[i] = load(cond + l);
-        u[i] = uncond ? load(uncond + l) : c[i];
-        bits[i] = allowed ? allowed[l >> 5] >> (l & 31) : ~0u;   // a piece's bits lie in one word
+        if constexpr (MORE) {
+          u[i] = uncond ? load(uncond + l) : c[i];
+          bits[i] = allowed ? allowed[l >> 5] >> (l & 31) : ~0u;   // a piece's bits lie in one word
+        }
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int v = at + (i * NT + (int)threadIdx.x) * P;
         if (v < v1) {
 #pragma unroll
-          for (int j = 0; j < P; ++j) f(v + j, x_of(part(c[i], j), part(u[i], j), bits[i] >> j & 1u));
+          for (int j = 0; j < P; ++j) {
+            float x = part(c[i], j);
+            if constexpr (MORE) {
+              if (uncond) x = x_of(x, part(u[i], j));
+              f(v + j, x, finite(x) && (bits[i] >> j & 1u));
+            } else {
+              f(v + j, x, finite(x));
+            }
+          }
         }
       }
     }
@@ -186,62 +205,71 @@ __device__ __forceinline__ double power(double e) {
   p = fma(p, z, 1.0);
   return ldexp(p, -(int)n);
 }
-// The weight 2^-e of a value b steps below ref, in units of 2^-bits, rounded to nearest: with e = (b + f) / 64, f in 0 .. 1
-// but for the step's rounding, 2^(-b / 64) from a table of 64 and the exponential series in -f ln 2 / 64 (to the 6th: 1e-17).
-__device__ __forceinline__ unsigned long long weight(double e, int b, int bits, const double* roots) {
-  constexpr double C = -LN2 / PER_BIT;
-  const double z = fma(e, (double)PER_BIT, -(double)b) * C;
-  double p = fma(1.0 / 720.0, z, 1.0 / 120.0);
-  p = fma(p, z, 1.0 / 24.0);
+// The weight of a value in units of 2^-bits, rounded to nearest: 2^(-(b + 1/2) / 64) e^z of a value z above the middle of step b
+// below ref.  The first from a table of 64, the second by the exponential series (|z| < 0.006, terms to the 5th: 1e-16).
+__device__ __forceinline__ unsigned long long weight(double z, int b, int bits, const double* roots) {
+  double p = fma(1.0 / 120.0, z, 1.0 / 24.0);
   p = fma(p, z, 1.0 / 6.0);
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
   p = fma(p, z, 1.0) * roots[b & (PER_BIT - 1)];
-  const double x = ldexp(p, bits - b / PER_BIT) + 0x1p52;   // the sum's last bits are the whole number
+  const double x = ldexp(p, bits - (b >> 6)) + 0x1p52;   // the sum's last bits are the whole number
   return (unsigned long long)__double_as_longlong(x) & 0xfffffffffffffull;
 }
+static_assert(PER_BIT == 64 && STEP == 8 && FINE % STEP == 0, "the shifts above and below");
 constexpr int LAST = FINE + (NB - 1 - FINE) * STEP;   // the first step of the last bucket, which has all that is far below
-__device__ __forceinline__ int bucket_of(int b) { return b < FINE ? b : FINE + (b - FINE) / STEP; }
+// b < FINE ? b : FINE + (b - FINE) / STEP, b >= 0
+__device__ __forceinline__ int bucket_of(int b) { return min(b, (FINE - FINE / STEP) + (b >> 3)); }
 // Where a row's values lie below its reference.  Steps of y are the same number for the same value wherever they are asked,
 // larger for larger values, and counted down from 64 ref, ref a whole number, so counts from the refs of two slices are whole
 // numbers apart.  FP32 does for that up to |y| of 4096 (steps within 0.05 of those of 64 bits).  Past it (a temperature of 1 /
 // 1000, values of a mask's making) ref is the largest value itself, and its row is one workgroup's.
 struct Scale {
   double ref, from, off;                          // in powers of two; e = (from - y) log2(e) + off
-  float ref64;                                    // 64 ref
+  double a, b;                                    // a b is minus the y of ref
+  float ref64;                                    // 64 ref - 1
   bool wild;
   static __device__ __forceinline__ float steps(float y) { return floorf(y * (float)(LOG2E * PER_BIT)); }
-  __device__ explicit Scale(float y) {
-    wild = !(fabsf(y) < 4096.f);
+  __device__ __forceinline__ explicit Scale(float of) {           // the workgroup's
+    const uint32_t u = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(of));
+    const float y = __uint_as_float(u);
+    wild = (u & 0x7fffffffu) >= 0x45800000u;      // 4096
     const float whole = floorf(steps(y) * (1.f / PER_BIT)) + 1.f;
-    ref64 = whole * PER_BIT;
+    ref64 = whole * PER_BIT - 1.f;
     ref = wild ? (double)y * LOG2E : (double)whole;
     from = wild ? (double)y : 0.0;
     off = wild ? 0.0 : ref;
+    a = wild ? -(double)y : -(double)whole;
+    b = wild ? 1.0 : LN2;
   }
   // powers of two below ref
   __device__ __forceinline__ double e(float y) const { return fma(from - (double)y, LOG2E, off); }
   // whole steps below ref, at most LAST
-  __device__ __forceinline__ int below(float y) const {
-    if (wild) return (int)fmin(e(y) * PER_BIT, (double)LAST);
-    return (int)__builtin_amdgcn_fmed3f(ref64 - steps(y) - 1.f, 0.f, (float)LAST);
+  __device__ __forceinline__ float belowf(float y) const {
+    if (wild) return (float)(int)fmin(e(y) * PER_BIT, (double)LAST);
+    return __builtin_amdgcn_fmed3f(ref64 - steps(y), 0.f, (float)LAST);
   }
-  __device__ __forceinline__ int bucket(float y) const { return bucket_of(below(y)); }
+  __device__ __forceinline__ int bucket(float y) const { return bucket_of((int)belowf(y)); }
   // The bucket of the least value that min-p keeps, give (-1) or take (1) rounding.
   __device__ __forceinline__ int least(float top, double m, double side) const {
     const double d = e(top) - log2(m) + side * 1e-3;
     return bucket_of((int)fmin(fmax(d * PER_BIT, 0.0), (double)LAST));
   }
+  // The weight of a value that many steps below.
+  __device__ __forceinline__ unsigned long long weight_at(float y, float below, int bits, const double* roots) const {
+    const double z = fma((double)(below + .5f), LN2 / PER_BIT, fma(a, b, (double)y));
+    return draw::weight(z, (int)below, bits, roots);
+  }
   // A value's weight: 0 in the last bucket.
   __device__ __forceinline__ unsigned long long weight(float y, int bits, const double* roots) const {
-    const int b = below(y);
-    return b < LAST ? draw::weight(e(y), b, bits, roots) : 0;
+    const float d = belowf(y);
+    return d < (float)LAST ? weight_at(y, d, bits, roots) : 0;
   }
 };
 
 // The workgroup's shared memory.
 struct Shared {
-  double roots[PER_BIT];                          // 2^(-i / 64)
+  double roots[PER_BIT];                          // 2^(-(i + 1/2) / 64)
   unsigned long long mass[NB + 1];                // of a bucket, then of all before it
   alignas(16) unsigned long long list[2 * CAP];   // then their sums (digit by digit: histograms)
   unsigned count[NB + 1];
@@ -329,30 +357,30 @@ __device__ __forceinline__ void block_scan(unsigned* count, unsigned long long* 
 
 // The largest key of x, the lowest id that has it, and how many candidates values v0 .. v1 hold.
 template <typename X, bool WIDE>
-__device__ void survey(const Row<X, WIDE>& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
-  unsigned long long b = 0;
+__device__ __forceinline__ void survey(const Row<X, WIDE>& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
+  float most = -INFINITY;
+  int id = 0;
   unsigned c = 0;
-  row.each(v0, v1, [&](int v, float x) {
-    const unsigned long long k = x == x ? (unsigned long long)key_of(x) << 32 | (uint32_t)~v : 0ull;
-    c += x == x;
-    b = k > b ? k : b;
+  row.each(v0, v1, [&](int v, float x, bool on) __attribute__((always_inline)) {
+    c += on;
+    if (on && x > most) { most = x; id = v; }     // ids come in order: the first of equal ones stays
   });
-  block_max_sum(b, c, s);
-  best = b;
+  best = c ? (unsigned long long)key_of(most) << 32 | (uint32_t)~id : 0ull;
+  block_max_sum(best, c, s);
   n = (int)c;
 }
 // Counts and (with sums) sums of weights by bucket of values v0 .. v1 in s.count and s.mass.
 template <typename X, bool WIDE>
-__device__ void histogram(const Row<X, WIDE>& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
+__device__ __forceinline__ void histogram(const Row<X, WIDE>& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
   for (int i = threadIdx.x; i < NB; i += NT) { s.count[i] = 0; s.mass[i] = 0; }
   __syncthreads();
-  row.each(v0, v1, [&](int, float x) {
-    const float y = row.divided(x);
-    const int d = at.below(y), b = bucket_of(d);
-    const unsigned long long w = sums ? weight(at.e(y), d, bits, s.roots) : 0;
-    if (x == x) {
+  row.each(v0, v1, [&](int, float x, bool on) __attribute__((always_inline)) {
+    const float y = row.divided(x), d = at.belowf(y);
+    const int b = bucket_of((int)d);
+    const unsigned long long w = sums ? at.weight_at(y, d, bits, s.roots) : 0;
+    if (on) {
       atomicAdd(&s.count[b], 1u);
-      if (sums && d < LAST) atomicAdd(&s.mass[b], w);
+      if (sums && d < (float)LAST) atomicAdd(&s.mass[b], w);
     }
   });
   __syncthreads();
@@ -363,7 +391,7 @@ struct Params {
   double p, m, u;                                 // p in (0, 1) or 0: none; m in (0, 1] or 0: none
   int k;                                          // 0: none
   bool greedy, list;                              // list: all that top-k leaves is listed, and no sums are asked of the histogram
-  __device__ Params(const Given& g, int n) {
+  __device__ __forceinline__ Params(const Given& g, int n) {
     greedy = !(g.T > 0.f);
     list = g.lists();
     k = g.k > 0 && g.k < n ? g.k : 0;
@@ -388,7 +416,7 @@ __device__ __forceinline__ bool heavy(uint32_t key, uint32_t top, double m) {
 // known up to the bucket in which the bound before lies, so theirs may be several.  All threads:
 // each looks at two buckets.
 template <typename X, bool WIDE>
-__device__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, float top, Shared& s) {
+__device__ __forceinline__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, float top, Shared& s) {
   // the buckets b with a[b] <= x < a[b + 1] (sums of all before) for lo and hi
   auto find = [&](const auto* a, auto lo, auto hi, int& lo_b, int& hi_b, int i) {
     for (int b = threadIdx.x; b < NB; b += NT) {
@@ -480,42 +508,47 @@ __device__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, 
 
 // Puts the values of v0 .. v1 that lie in the ranges into s.list, s.listed of them.
 template <typename X, bool WIDE>
-__device__ void gather(const Row<X, WIDE>& row, const Scale& scale, int v0, int v1, Shared& s) {
-  auto put = [&](int v, float y) {
+__device__ __forceinline__ void gather(const Row<X, WIDE>& row, const Scale& scale, int v0, int v1, Shared& s) {
+  auto put = [&](int v, float y) __attribute__((always_inline)) {
     const unsigned at = atomicAdd(&s.listed, 1u);
     if (at < CAP) s.list[at] = (unsigned long long)key_of(y) << 32 | (uint32_t)~v;
   };
   if (row.V <= SHORT) {                           // too few values to look for the ranges' borders first
-    row.each(v0, v1, [&](int v, float x) {
+    row.each(v0, v1, [&](int v, float x, bool on) __attribute__((always_inline)) {
       const float y = row.divided(x);
       const int b = scale.bucket(y);
       bool in = false;
       for (int i = 0; i < s.ranges; ++i) in |= b >= s.range[i].lo && b <= s.range[i].hi;
-      if (in && x == x) put(v, y);
+      if (in && on) put(v, y);
     });
     __syncthreads();
     return;
   }
-  float least[4], most[4];
+  auto pass = [&](auto ranges) __attribute__((always_inline)) {
+    constexpr int N = decltype(ranges)::value;
+    float least[N], most[N];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool is = i < s.ranges;
-    least[i] = is ? value_of(s.range[i].least) : INFINITY;
-    most[i] = is ? value_of(s.range[i].most) : 0.f;
-  }
-  row.each(v0, v1, [&](int v, float x) {
-    bool in = false;
+    for (int i = 0; i < N; ++i) {
+      const bool is = i < s.ranges;
+      least[i] = is ? value_of(s.range[i].least) : INFINITY;
+      most[i] = is ? value_of(s.range[i].most) : 0.f;
+    }
+    row.each(v0, v1, [&](int v, float x, bool on) __attribute__((always_inline)) {
+      bool in = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) in |= x >= least[i] && x <= most[i];
-    if (in) put(v, row.divided(x));
-  });
+      for (int i = 0; i < N; ++i) in |= x >= least[i] && x <= most[i];
+      if (in && on) put(v, row.divided(x));
+    });
+  };
+  if (s.ranges <= 2) pass(std::integral_constant<int, 2>{});   // most rows
+  else pass(std::integral_constant<int, 4>{});
   __syncthreads();
 }
 
 // s.list[0 .. n), largest first; n at most CAP.  Up to NT values each finds its place by counting the
 // larger ones, NT / P threads to a value (181 values: 2,000 clocks, by the network, whose steps are a barrier
 // each, 17,600); more take the network.
-__device__ void sort_list(int n, Shared& s) {
+__device__ __forceinline__ void sort_list(int n, Shared& s) {
   int P = 2;
   while (P < n) P <<= 1;
   if (P <= NT) {
@@ -554,7 +587,7 @@ __device__ void sort_list(int n, Shared& s) {
     }
 }
 
-__device__ void answer(const Args& a, int r, int token, double logprob, int kept) {
+__device__ __forceinline__ void answer(const Args& a, int r, int token, double logprob, int kept) {
   a.token[r] = token;
   if (a.logprob) a.logprob[r] = (float)logprob;
   if (a.kept) a.kept[r] = kept;
@@ -565,7 +598,7 @@ __device__ __forceinline__ double part_log(uint32_t key, const Scale& at, unsign
 }
 
 // The row's answer from the sorted list of its ranges.
-__device__ void finish_list(const Args& a, int r, const Params& q, const Scale& scale, uint32_t top, int n, Shared& s) {
+__device__ __forceinline__ void finish_list(const Args& a, int r, const Params& q, const Scale& scale, uint32_t top, int n, Shared& s) {
   const int total = s.total, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   unsigned long long* sum_at = s.list + CAP;
   // sums up to and with each, `per` neighbours to a thread
@@ -663,7 +696,7 @@ __device__ void finish_list(const Args& a, int r, const Params& q, const Scale& 
 // Digit by digit: the value at which the count of the largest (by_count) or their sum passes T, in
 // s.at: its key, the count and sum of all above it, and its own.
 template <typename X, bool WIDE>
-__device__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bits, bool by_count, unsigned long long T, Shared& s) {
+__device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bits, bool by_count, unsigned long long T, Shared& s) {
   unsigned long long* mass = s.list;              // [DIGITS + 1], then counts
   unsigned* count = reinterpret_cast<unsigned*>(s.list + DIGITS + 1);
   uint32_t prefix = 0, mask = 0;
@@ -721,7 +754,7 @@ __device__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bits, b
 
 // The row's answer where the list does not hold its ranges.
 template <typename X, bool WIDE>
-__device__ void finish_digits(const Args& a, int r, const Row<X, WIDE>& row, const Params& q, const Scale& scale, uint32_t top,
+__device__ __forceinline__ void finish_digits(const Args& a, int r, const Row<X, WIDE>& row, const Params& q, const Scale& scale, uint32_t top,
                               int n, Shared& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   unsigned kept = (unsigned)n;
@@ -781,7 +814,7 @@ __device__ void finish_digits(const Args& a, int r, const Row<X, WIDE>& row, con
 }
 
 // A row that needs no sums: greedy, or without candidates.
-__device__ bool finish_early(const Args& a, int r, const Params& q, unsigned long long best, int n) {
+__device__ __forceinline__ bool finish_early(const Args& a, int r, const Params& q, unsigned long long best, int n) {
   if (n && !q.greedy) return false;
   if (threadIdx.x == 0) answer(a, r, n ? (int)~(uint32_t)best : -1, n ? 0.0 : -INFINITY, n ? 1 : 0);
   return true;
@@ -791,7 +824,7 @@ __device__ bool finish_early(const Args& a, int r, const Params& q, unsigned lon
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
   const int r = blockIdx.x;
   const Given given(a, r);
   const Row<X, WIDE> row(a, given, r);
@@ -825,7 +858,7 @@ struct RowSpace {
   static __host__ __device__ size_t bytes(int slices) {
     return (slices * (sizeof(SliceInfo) + NB * 12) + CAP * 8 + 8 + 255) / 256 * 256;
   }
-  __device__ RowSpace(const Args& a, int r) {
+  __device__ __forceinline__ RowSpace(const Args& a, int r) {
     char* p = a.ws + r * bytes(a.slices);
     info = reinterpret_cast<SliceInfo*>(p); p += a.slices * sizeof(SliceInfo);
     mass = reinterpret_cast<unsigned long long*>(p); p += (size_t)a.slices * NB * 8;
@@ -839,7 +872,7 @@ struct RowSpace {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
   const Given given(a, r);
   const Row<X, WIDE> row(a, given, r);
@@ -864,20 +897,17 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((double)(NT - 1 - threadIdx.x) / PER_BIT);
+  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
   const int r = blockIdx.y, g = blockIdx.x;
   const Given given(a, r);
   const Row<X, WIDE> row(a, given, r);
   const RowSpace w(a, r);
-  SliceInfo* info = reinterpret_cast<SliceInfo*>(s.list);   // of all slices, here
-  for (int i = threadIdx.x; i < a.slices; i += NT) info[i] = w.info[i];
-  __syncthreads();
-  unsigned long long best = 0;
-  int n = 0;
-  for (int i = 0; i < a.slices; ++i) {
-    best = info[i].best > best ? info[i].best : best;
-    n += info[i].n;
-  }
+  // a lane for each slice
+  const int lane = threadIdx.x & 63;
+  SliceInfo info{0.0, 0ull, 0, 0};
+  if (lane < a.slices) info = w.info[lane];
+  const unsigned long long best = wave_all(info.best, Larger{});
+  const int n = (int)wave_all((unsigned)info.n, Plus{});
   const Params q(given, n);
   if (n == 0 || q.greedy) {
     if (g == 0) finish_early(a, r, q, best, n);
@@ -885,18 +915,22 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   }
   const uint32_t top = key_of(row.divided(value_of((uint32_t)(best >> 32))));
   const Scale scale(value_of(top));
-  bool alone = scale.wild;                        // one workgroup does all: of a slice of such values, near the largest, there is no histogram
-  for (int i = 0; i < a.slices; ++i) alone |= info[i].n && info[i].wild && scale.ref - info[i].ref < NEAR;
+  const double up = scale.ref - info.ref;         // a whole number, or of no use
+  const bool near = info.n && up < NEAR;
+  const int lower = near ? (int)up : -1;
+  // One workgroup does all if the row's values, or those of a slice near the largest, are such that there is no histogram.
+  const bool alone = scale.wild || __any(near && info.wild);
   if (alone && g) return;
   if (alone) {
     histogram(row, 0, a.V, scale, a.bits, !q.list, s);
   } else {
-    // A slice's ref is `up` powers of two lower, so its steps lie 64 up further below the row's: a fine bucket has one of
+    // A slice's ref is `by` powers of two lower, so its steps lie 64 by further below the row's: a fine bucket has one of
     // the slice's fine ones, a wide one one of its wide ones or eight of its fine ones.
     constexpr int GROUP = 5;                      // slices whose loads are on their way together
     for (int b = threadIdx.x; b < NB; b += NT) {
       unsigned c = 0;
       unsigned long long m = 0;
+      const int first = b < NB - 1 ? b < FINE ? b : FINE + (b - FINE) * STEP : -1;   // the last bucket has the rest
       for (int i0 = 0; i0 < a.slices; i0 += GROUP) {
         unsigned x[GROUP];
         unsigned long long y[GROUP];
@@ -904,12 +938,9 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
           const int i = min(i0 + j, a.slices - 1);
-          const double up = scale.ref - info[i].ref;   // a whole number, or beyond all buckets
-          const bool near = i0 + j < a.slices && info[i].n && up < NEAR && b < NB - 1;   // the last bucket has the rest
-          by[j] = near ? (int)up : 0;
-          const int d = (b < FINE ? b : FINE + (b - FINE) * STEP) - by[j] * PER_BIT;
-          from[j] = !near || d < 0 ? -1 : d;
-          const size_t at = (size_t)i * NB + max(bucket_of(max(d, 0)), 0);
+          by[j] = i0 + j < a.slices ? __builtin_amdgcn_readlane(lower, i) : -1;
+          from[j] = by[j] < 0 ? -1 : first - by[j] * PER_BIT;
+          const int at = i * NB + bucket_of(max(from[j], 0));
           x[j] = w.count[at];                     // a slice without candidates left none: loaded, not taken
           y[j] = w.mass[at];
         }
@@ -920,7 +951,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
             m += y[j] >> by[j];
             if (b >= FINE && from[j] < FINE)
               for (int k = 1; k < STEP; ++k) {
-                const size_t at = (size_t)(i0 + j) * NB + from[j] + k;
+                const int at = (i0 + j) * NB + from[j] + k;
                 c += w.count[at];
                 m += w.mass[at] >> by[j];
               }

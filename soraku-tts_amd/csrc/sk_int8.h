@@ -186,7 +186,7 @@ struct RowsArgs {
 // Codes of R rows: W waves per row, C chunks of 512 W values held in registers (C = 0:
 // any K, read twice).  Bytes bound it: each value read once (the second read of C = 0
 // comes from cache) and each code written once.  12,288 x 2048 in BF16: 15.4 us, 4.9 TB/s; 5,999 x 6144: 18.6 us,
-// 6.0 TB/s; 16,404 x 2048 in FP32: 34 us, 4.9 TB/s.  A few hundred rows take 3 to 4 us, the time of a launch and
+// 6.0 TB/s; 32,816 x 1024 in FP32: 34 us, 4.9 TB/s.  A few hundred rows take 3 to 4 us, the time of a launch and
 // of one load and one exchange after the other.
 template <typename X, int W, int C, bool WHOLE, int MODE>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
