@@ -41,6 +41,7 @@ constexpr int NT = 1024;                          // threads of a workgroup
 constexpr int PER_BIT = 64, FINE = 20 * PER_BIT;  // buckets per power of two of the weight, for the first 20 of them,
 constexpr int STEP = 8, NB = FINE + 28 * PER_BIT / STEP;   // then an eighth as many, down to 2^-48
 constexpr double NEAR = 48.0;                     // a slice whose ref is further below the row's has nothing but weights of 0
+constexpr int MOST_SLICES = 10;                   // workgroups per row
 constexpr int CAP = 2048;                         // values of the list
 constexpr int SHORT = 4096;                       // values of a row that is read once more rather than searched for borders
 constexpr int DIGITS = 2048;                      // of 11, 11 and 10 bits of a key
@@ -122,6 +123,8 @@ struct Row {
     if (fabsf(y) < 0x1p-100f && x != 0.f) y = x / T;
     return __builtin_amdgcn_fmed3f(y, -3.402823466e38f, 3.402823466e38f);
   }
+  // About the x of a y.
+  __device__ __forceinline__ float near(double y) const { return (float)(whole ? y : y * (double)T); }
   // x of cond and uncond
   __device__ __forceinline__ float x_of(float x, float u) const { return u + s * (x - u); }
   static __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
@@ -220,6 +223,7 @@ static_assert(PER_BIT == 64 && STEP == 8 && FINE % STEP == 0, "the shifts above 
 constexpr int LAST = FINE + (NB - 1 - FINE) * STEP;   // the first step of the last bucket, which has all that is far below
 // b < FINE ? b : FINE + (b - FINE) / STEP, b >= 0
 __device__ __forceinline__ int bucket_of(int b) { return min(b, (FINE - FINE / STEP) + (b >> 3)); }
+__device__ __forceinline__ int first_step(int bucket) { return max(bucket, FINE + (bucket - FINE) * STEP); }
 // Where a row's values lie below its reference.  Steps of y are the same number for the same value wherever they are asked,
 // larger for larger values, and counted down from 64 ref, ref a whole number, so counts from the refs of two slices are whole
 // numbers apart.  FP32 does for that up to |y| of 4096 (steps within 0.05 of those of 64 bits).  Past it (a temperature of 1 /
@@ -250,6 +254,10 @@ struct Scale {
     return __builtin_amdgcn_fmed3f(ref64 - steps(y), 0.f, (float)LAST);
   }
   __device__ __forceinline__ int bucket(float y) const { return bucket_of((int)belowf(y)); }
+  // About the least y that is less than that many steps below.
+  __device__ __forceinline__ double at_step(int step) const {
+    return (double)(ref64 - (float)step + 1.f) * (LN2 / PER_BIT);
+  }
   // The bucket of the least value that min-p keeps, give (-1) or take (1) rounding.
   __device__ __forceinline__ int least(float top, double m, double side) const {
     const double d = e(top) - log2(m) + side * 1e-3;
@@ -486,16 +494,30 @@ __device__ __forceinline__ void plan(const Row<X, WIDE>& row, const Params& q, c
   // bucket is at most hi; a wave for each, which tries 64 keys at a time
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (wave < 2 * s.ranges) {
-    const int i = wave / 2, lo_b = s.range[i].lo, hi_b = s.range[i].hi;
+    const int i = wave / 2, border = __builtin_amdgcn_readfirstlane(wave & 1 ? s.range[i].hi + 1 : s.range[i].lo);
     // keys before `from` are on this side of the border, from `from + size` on they are not (border: the first
-    // key whose bucket is at most hi, or the first whose bucket is below lo)
+    // key whose bucket is before this one)
     uint32_t from = 0x00800000u, size = 0xff800000u - 0x00800000u;   // of the finite numbers
+    auto past = [&](uint32_t key) { return at.bucket(row.divided(value_of(key))) < border; };
+    if (border == 0) {
+      from += size; size = 0;                     // none is
+    } else if (border == NB) {
+      size = 0;                                   // all are
+    } else {
+      // 64 keys where the border should be
+      const float x = row.near(at.at_step(first_step(border)));
+      const uint32_t k = min(max(key_of(x), from + 64), from + size - 64) - 32;
+      const uint64_t is = __ballot(past(k + lane));
+      if (is && !(is & 1)) {
+        from = k + __builtin_ctzll(is);
+        size = 0;
+      }
+    }
     while (size) {
       const uint32_t part = size / 64 + 1, end = from + size;   // lane l asks of key from + (l + 1) part - 1
       const uint64_t key = (uint64_t)from + (lane + 1) * (uint64_t)part - 1;
-      const int b = at.bucket(row.divided(value_of((uint32_t)min(key, (uint64_t)(end - 1)))));
-      const bool past = key >= end || (wave & 1 ? b <= hi_b : b < lo_b);   // 64 parts are more than size: one is past
-      from += __builtin_ctzll(__ballot(past)) * part;
+      const bool is = key >= end || past((uint32_t)key);   // 64 parts are more than size: one is past
+      from += __builtin_ctzll(__ballot(is)) * part;
       size = min(part - 1, end - from);
     }
     if (lane == 0) {
@@ -889,8 +911,8 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
   if (n == 0 || !(row.T > 0.f) || scale.wild) return;   // nothing of it is read
   histogram(row, v0, v1, scale, a.bits, !given.lists(), s);
   for (int i = threadIdx.x; i < NB; i += NT) {
-    w.count[(size_t)g * NB + i] = s.count[i];
-    w.mass[(size_t)g * NB + i] = s.mass[i];
+    w.count[g * NB + i] = s.count[i];
+    w.mass[g * NB + i] = s.mass[i];
   }
 }
 
@@ -925,40 +947,62 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
     histogram(row, 0, a.V, scale, a.bits, !q.list, s);
   } else {
     // A slice's ref is `by` powers of two lower, so its steps lie 64 by further below the row's: a fine bucket has one of
-    // the slice's fine ones, a wide one one of its wide ones or eight of its fine ones.
-    constexpr int GROUP = 5;                      // slices whose loads are on their way together
-    for (int b = threadIdx.x; b < NB; b += NT) {
+    // the slice's fine ones, a wide one has one of its wide ones, or eight of its last fine ones.  All loads
+    // are on their way at once: they come from other XCDs' stores, 1 us away.
+    constexpr int U = (NB + NT - 1) / NT;         // buckets of a thread
+    const bool sums = !q.list;
+    unsigned x[MOST_SLICES][U];
+    unsigned long long y[MOST_SLICES][U];
+#pragma unroll
+    for (int i = 0; i < MOST_SLICES; ++i)
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int b = j * NT + threadIdx.x, by = __builtin_amdgcn_readlane(lower, i);   // -1 past the slices too
+        const int d = b < FINE ? b - by * PER_BIT : b - by * (PER_BIT / STEP);
+        x[i][j] = 0;
+        y[i][j] = 0;
+        if (by >= 0 && b < NB - 1 && d >= (b < FINE ? 0 : FINE)) {   // the row's last bucket has the rest
+          x[i][j] = w.count[i * NB + d];
+          if (sums) y[i][j] = w.mass[i * NB + d];
+        }
+      }
+    // a wave for each slice's last fine ones, the first of them on their way too
+    static_assert(MOST_SLICES <= NT / 64, "a wave for each");
+    constexpr int AHEAD = 3;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), by = __builtin_amdgcn_readlane(lower, wave);
+    const int d0 = max(FINE - by * PER_BIT, 0) + lane;   // none where by is -1 or 0
+    unsigned xf[AHEAD];
+    unsigned long long yf[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int d = d0 + j * 64;
+      xf[j] = d < FINE ? w.count[wave * NB + d] : 0;
+      yf[j] = sums && d < FINE ? w.mass[wave * NB + d] : 0;
+    }
+    for (int i = threadIdx.x; i < NB; i += NT) { s.count[i] = 0; s.mass[i] = 0; }
+    __syncthreads();
+    auto put = [&](int d, unsigned c, unsigned long long m) __attribute__((always_inline)) {
+      const int to = bucket_of(d + by * PER_BIT);
+      if (to < NB - 1 && c) {
+        atomicAdd(&s.count[to], c);
+        if (sums) atomicAdd(&s.mass[to], m >> by);
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) put(d0 + j * 64, xf[j], yf[j]);
+    for (int d = d0 + AHEAD * 64; d < FINE; d += 64) put(d, w.count[wave * NB + d], sums ? w.mass[wave * NB + d] : 0);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int b = j * NT + threadIdx.x;
       unsigned c = 0;
       unsigned long long m = 0;
-      const int first = b < NB - 1 ? b < FINE ? b : FINE + (b - FINE) * STEP : -1;   // the last bucket has the rest
-      for (int i0 = 0; i0 < a.slices; i0 += GROUP) {
-        unsigned x[GROUP];
-        unsigned long long y[GROUP];
-        int from[GROUP], by[GROUP];
 #pragma unroll
-        for (int j = 0; j < GROUP; ++j) {
-          const int i = min(i0 + j, a.slices - 1);
-          by[j] = i0 + j < a.slices ? __builtin_amdgcn_readlane(lower, i) : -1;
-          from[j] = by[j] < 0 ? -1 : first - by[j] * PER_BIT;
-          const int at = i * NB + bucket_of(max(from[j], 0));
-          x[j] = w.count[at];                     // a slice without candidates left none: loaded, not taken
-          y[j] = w.mass[at];
-        }
-#pragma unroll
-        for (int j = 0; j < GROUP; ++j)
-          if (from[j] >= 0) {
-            c += x[j];
-            m += y[j] >> by[j];
-            if (b >= FINE && from[j] < FINE)
-              for (int k = 1; k < STEP; ++k) {
-                const int at = (i0 + j) * NB + from[j] + k;
-                c += w.count[at];
-                m += w.mass[at] >> by[j];
-              }
-          }
+      for (int i = 0; i < MOST_SLICES; ++i) {
+        c += x[i][j];
+        m += y[i][j] >> max(__builtin_amdgcn_readlane(lower, i), 0);
       }
-      s.count[b] = c;
-      s.mass[b] = m;
+      if (b < NB) { s.count[b] += c; s.mass[b] += m; }
     }
     __syncthreads();
   }

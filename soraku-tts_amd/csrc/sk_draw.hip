@@ -25,7 +25,7 @@ int check_sizes(int32_t R, int32_t V, int32_t dtype) {
 // Workgroups per row: one of the GPU's 256 CUs each, as few rows allow, but no more than ten, whose histograms every
 // one of them adds up (a row of 151,936: 69 us in 3, 41 in 10, 43 in 24; 64 rows 61 us in 4, 82 in 8; 256 rows 141
 // us whole, 165 in 2).
-int slices_of(int R, int V) { return V <= 16384 ? 1 : std::max(1, std::min(10, 256 / std::max(R, 1))); }
+int slices_of(int R, int V) { return V <= 16384 ? 1 : std::max(1, std::min(MOST_SLICES, 256 / std::max(R, 1))); }
 // Sums of V weights of up to 2^bits stay below 2^63.
 int bits_of(int V) {
   int b = 0;

@@ -341,3 +341,17 @@ def test_a_slice_past_4096_below_a_largest_within(ops, hip_device, rows):
     p = dict(top_p=torch.full((rows,), 0.97), top_k=torch.tensor([0, 5000, 0][:rows], dtype=torch.int32))
     for u in (0.01, 0.3, 0.6, 0.95):
         check(ops, hip_device, torch.from_numpy(x.astype(np.float32)), [u] * rows, least=1.0, **p)
+
+
+@pytest.mark.parametrize("fall", [3.0, 14.0, 40.0])
+def test_parts_of_a_row_far_apart(ops, hip_device, fall):
+    """Each part's largest value a good deal below the one before, bounds far below the row's largest: sums of parts are
+    counted from refs of their own."""
+    rng = np.random.default_rng(45)
+    V, rows = 40000, 8
+    x = 2.0 * rng.standard_normal((rows, V)) - np.linspace(0, fall, V)
+    x[1::2] = x[1::2, ::-1]
+    p = dict(top_k=torch.tensor([0, 20000, 35000, 3000, 0, 0, 39000, 12000], dtype=torch.int32),
+             min_p=torch.tensor([1e-12, 0, 0, 1e-8, 1e-5, 1e-3, 0, 1e-10]), top_p=torch.tensor([1, 0.999999, 1, 1, 1, 0.9999, 0.99, 1.0]))
+    for u in (0.2, 0.999):
+        check(ops, hip_device, torch.from_numpy(x.astype(np.float32)), [u] * rows, least=0.8, **p)
