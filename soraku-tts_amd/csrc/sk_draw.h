@@ -611,7 +611,7 @@ __device__ __forceinline__ void sort_list(int n, Shared& s) {
 
 __device__ __forceinline__ void answer(const Args& a, int r, int token, double logprob, int kept) {
   a.token[r] = token;
-  if (a.logprob) a.logprob[r] = (float)logprob;
+  if (a.logprob) a.logprob[r] = kept == 1 ? 0.f : (float)logprob;   // the only one is the whole: exactly 0
   if (a.kept) a.kept[r] = kept;
 }
 // ln of the drawn one's part of the kept sum.

@@ -355,3 +355,13 @@ def test_parts_of_a_row_far_apart(ops, hip_device, fall):
              min_p=torch.tensor([1e-12, 0, 0, 1e-8, 1e-5, 1e-3, 0, 1e-10]), top_p=torch.tensor([1, 0.999999, 1, 1, 1, 0.9999, 0.99, 1.0]))
     for u in (0.2, 0.999):
         check(ops, hip_device, torch.from_numpy(x.astype(np.float32)), [u] * rows, least=0.8, **p)
+
+
+@pytest.mark.parametrize("v", [100, 2051, 40000])
+def test_the_only_one_has_logarithm_0(ops, hip_device, v):
+    rng = np.random.default_rng(46)
+    x = 3 * torch.from_numpy(rng.standard_normal((6, v)).astype(np.float32))
+    p = dict(temperature=torch.tensor([0.7, 1.0, 1.3, 0.9, 1.0, 0.0]), top_k=torch.tensor([1, 1, 0, 0, 2000, 0], dtype=torch.int32),
+             top_p=torch.tensor([0, 0.5, 1e-9, 0, 1e-6, 0]), min_p=torch.tensor([0, 0, 0, 1.0, 0, 0]))
+    got, logprob, kept = sample(ops, hip_device, x, [0.7] * 6, **p)
+    assert (got == x.argmax(1).numpy()).all() and (kept == 1).all() and (logprob == 0).all()
