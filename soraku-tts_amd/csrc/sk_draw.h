@@ -21,7 +21,7 @@
 // one per bucket and slice less, 2^-30 of the largest weight in all.
 //
 // A row is small work with many steps that wait for each other, on few CUs: its latency bounds it.  16 rows of 2051 with
-// guidance: 15 us; one row of 151,936: 11 us for the histograms and 19 for the rest; 64 of them in BF16 (19 MB): 23
+// guidance: 12 us; one row of 151,936: 11 us for the histograms and 19 for the rest; 64 of them in BF16 (19 MB): 23
 // (VALU 87% busy, 62 instructions per value) and 29 us.
 #pragma once
 
@@ -43,7 +43,6 @@ constexpr int STEP = 8, NB = FINE + 28 * PER_BIT / STEP;   // then an eighth as 
 constexpr double NEAR = 48.0;                     // a slice whose ref is further below the row's has nothing but weights of 0
 constexpr int MOST_SLICES = 10;                   // workgroups per row
 constexpr int CAP = 2048;                         // values of the list
-constexpr int SHORT = 4096;                       // values of a row that is read once more rather than searched for borders
 constexpr int DIGITS = 2048;                      // of 11, 11 and 10 bits of a key
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
@@ -96,6 +95,7 @@ struct Given {
 // WIDE: rows begin at multiples of 16 bytes and are whole pieces of 16, so that a load takes 4 or 8 values.
 template <typename X, bool WIDE>
 struct Row {
+  static constexpr bool HELD = false;
   const X* cond; const X* uncond;
   const uint32_t* allowed;
   float s, T;
@@ -186,6 +186,43 @@ struct Row {
         }
       }
     }
+  }
+};
+
+// A row of up to 4 NT values, four of them in each thread's registers: read once (16 rows of 2051 with guidance and a mask: 12.4
+// us in place of 15.0; 4,096 values without either 14.5 and 14.6; sixteen per thread 16,384 values 24 us, where reading them three
+// times takes 19).  Its values' buckets are then found faster than the borders of ranges.
+template <typename X>
+struct Held : Row<X, false> {
+  static constexpr bool HELD = true;
+  static constexpr int N = 4;
+  float x[N];                                     // NaN: no candidate
+  __device__ __forceinline__ Held(const Args& a, const Given& g, int r) : Row<X, false>(a, g, r) {
+    float c[N], u[N];
+    uint32_t bits[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      c[i] = u[i] = 0.f;
+      bits[i] = ~0u;
+      if (i * NT < this->V) {                     // the workgroup's
+        const int v = min(i * NT + (int)threadIdx.x, this->V - 1);
+        c[i] = to_f<X>(this->cond[v]);
+        if (this->uncond) u[i] = to_f<X>(this->uncond[v]);
+        if (this->allowed) bits[i] = this->allowed[v >> 5] >> (v & 31);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = this->uncond ? this->x_of(c[i], u[i]) : c[i];
+      const bool on = this->finite(y) && (bits[i] & 1u) && i * NT + (int)threadIdx.x < this->V;
+      x[i] = on ? y : __uint_as_float(0x7fc00000u);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(int, int, F f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * NT < this->V) f(i * NT + (int)threadIdx.x, x[i], x[i] == x[i]);
   }
 };
 
@@ -364,8 +401,8 @@ __device__ __forceinline__ void block_scan(unsigned* count, unsigned long long* 
 }
 
 // The largest key of x, the lowest id that has it, and how many candidates values v0 .. v1 hold.
-template <typename X, bool WIDE>
-__device__ __forceinline__ void survey(const Row<X, WIDE>& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
+template <typename R>
+__device__ __forceinline__ void survey(const R& row, int v0, int v1, Shared& s, unsigned long long& best, int& n) {
   float most = -INFINITY;
   int id = 0;
   unsigned c = 0;
@@ -378,8 +415,8 @@ __device__ __forceinline__ void survey(const Row<X, WIDE>& row, int v0, int v1, 
   n = (int)c;
 }
 // Counts and (with sums) sums of weights by bucket of values v0 .. v1 in s.count and s.mass.
-template <typename X, bool WIDE>
-__device__ __forceinline__ void histogram(const Row<X, WIDE>& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
+template <typename R>
+__device__ __forceinline__ void histogram(const R& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
   for (int i = threadIdx.x; i < NB; i += NT) { s.count[i] = 0; s.mass[i] = 0; }
   __syncthreads();
   row.each(v0, v1, [&](int, float x, bool on) __attribute__((always_inline)) {
@@ -423,8 +460,8 @@ __device__ __forceinline__ bool heavy(uint32_t key, uint32_t top, double m) {
 // that they hold.  The whole that top-p takes its part of, and the kept sum that the draw takes its part of, are
 // known up to the bucket in which the bound before lies, so theirs may be several.  All threads:
 // each looks at two buckets.
-template <typename X, bool WIDE>
-__device__ __forceinline__ void plan(const Row<X, WIDE>& row, const Params& q, const Scale& at, float top, Shared& s) {
+template <typename R>
+__device__ __forceinline__ void plan(const R& row, const Params& q, const Scale& at, float top, Shared& s) {
   // the buckets b with a[b] <= x < a[b + 1] (sums of all before) for lo and hi
   auto find = [&](const auto* a, auto lo, auto hi, int& lo_b, int& hi_b, int i) {
     for (int b = threadIdx.x; b < NB; b += NT) {
@@ -489,7 +526,7 @@ __device__ __forceinline__ void plan(const Row<X, WIDE>& row, const Params& q, c
     s.listed = 0;
   }
   __syncthreads();
-  if (row.V <= SHORT) return;
+  if constexpr (R::HELD) return;                  // gather looks at buckets
   // the keys of x that a range begins and ends with: the largest whose bucket is at least lo, the least whose
   // bucket is at most hi; a wave for each, which tries 64 keys at a time
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -529,13 +566,13 @@ __device__ __forceinline__ void plan(const Row<X, WIDE>& row, const Params& q, c
 }
 
 // Puts the values of v0 .. v1 that lie in the ranges into s.list, s.listed of them.
-template <typename X, bool WIDE>
-__device__ __forceinline__ void gather(const Row<X, WIDE>& row, const Scale& scale, int v0, int v1, Shared& s) {
+template <typename R>
+__device__ __forceinline__ void gather(const R& row, const Scale& scale, int v0, int v1, Shared& s) {
   auto put = [&](int v, float y) __attribute__((always_inline)) {
     const unsigned at = atomicAdd(&s.listed, 1u);
     if (at < CAP) s.list[at] = (unsigned long long)key_of(y) << 32 | (uint32_t)~v;
   };
-  if (row.V <= SHORT) {                           // too few values to look for the ranges' borders first
+  if constexpr (R::HELD) {
     row.each(v0, v1, [&](int v, float x, bool on) __attribute__((always_inline)) {
       const float y = row.divided(x);
       const int b = scale.bucket(y);
@@ -843,13 +880,9 @@ __device__ __forceinline__ bool finish_early(const Args& a, int r, const Params&
 }
 
 // A whole row in one workgroup.
-template <typename X, bool WIDE>
-__global__ __launch_bounds__(NT) void row_kernel(Args a) {
-  __shared__ Shared s;
+template <typename R>
+__device__ __forceinline__ void whole_row(const Args& a, int r, const Given& given, const R& row, Shared& s) {
   if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
-  const int r = blockIdx.x;
-  const Given given(a, r);
-  const Row<X, WIDE> row(a, given, r);
   unsigned long long best;
   int n;
   survey(row, 0, a.V, s, best, n);
@@ -867,6 +900,22 @@ __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   gather(row, scale, 0, a.V, s);
   sort_list(s.total, s);
   finish_list(a, r, q, scale, top, n, s);
+}
+template <typename X>
+__global__ __launch_bounds__(NT) void held_kernel(Args a) {
+  __shared__ Shared s;
+  const int r = blockIdx.x;
+  const Given given(a, r);
+  const Held<X> row(a, given, r);
+  whole_row(a, r, given, row, s);
+}
+template <typename X, bool WIDE>
+__global__ __launch_bounds__(NT) void row_kernel(Args a) {
+  __shared__ Shared s;
+  const int r = blockIdx.x;
+  const Given given(a, r);
+  const Row<X, WIDE> row(a, given, r);
+  whole_row(a, r, given, row, s);
 }
 
 // A row over several workgroups, in two launches.  The first leaves each slice's histogram,

@@ -37,7 +37,8 @@ int bits_of(int V) {
 template <typename X, bool WIDE>
 int run(const Args& a, hipStream_t st) {
   if (a.slices == 1) {
-    hipLaunchKernelGGL((row_kernel<X, WIDE>), dim3(a.R), dim3(NT), 0, st, a);
+    if (a.V <= Held<X>::N * NT) hipLaunchKernelGGL((held_kernel<X>), dim3(a.R), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((row_kernel<X, WIDE>), dim3(a.R), dim3(NT), 0, st, a);
     SK_HIP(hipGetLastError());
     return SK_OK;
   }
