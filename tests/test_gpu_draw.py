@@ -109,12 +109,12 @@ def test_equal_values(ops, hip_device, v):
 
 
 @pytest.mark.parametrize("v", [2051, 20000, 151936])
-def test_close_values(ops, hip_device, v):
+def test_close_values(ops, hip_device, v, least=0.9):
     """Values that differ in their last bits only, thousands to a bucket."""
     rng = np.random.default_rng(v + 1)
     rows = 16
     x = (4.0 + rng.integers(0, 5000, (rows, v)) * 2.0 ** -21).astype(np.float32)
-    check(ops, hip_device, torch.from_numpy(x), rng.random(rows), **params(rng, rows))
+    check(ops, hip_device, torch.from_numpy(x), rng.random(rows), least=least, **params(rng, rows))
 
 
 @pytest.mark.parametrize("v", [64, 2051, 20000, 151936])
@@ -365,3 +365,31 @@ def test_the_only_one_has_logarithm_0(ops, hip_device, v):
              top_p=torch.tensor([0, 0.5, 1e-9, 0, 1e-6, 0]), min_p=torch.tensor([0, 0, 0, 1.0, 0, 0]))
     got, logprob, kept = sample(ops, hip_device, x, [0.7] * 6, **p)
     assert (got == x.argmax(1).numpy()).all() and (kept == 1).all() and (logprob == 0).all()
+
+
+@pytest.mark.parametrize("v", [4095, 4096, 4097, 7001, 12000])
+def test_rows_around_what_threads_hold(ops, hip_device, v):
+    """One workgroup, the row in its threads' registers or read again for each step, by pieces or value by value."""
+    for dtype in (F32, BF16):
+        test_sizes(ops, hip_device, v, dtype)
+        test_guidance_and_allowed(ops, hip_device, v, dtype)
+    test_equal_values(ops, hip_device, v)
+    # of 12,000, two rows' two largest are equal and alone after top-k, with a top_p of 0.5: its bound 0.5 (w + w) is the first
+    # sum w itself, which no rounding decides, so 14 of 16 rows are determined
+    test_close_values(ops, hip_device, v, least=0.875)
+    test_masked_and_infinite_values(ops, hip_device, v)
+    test_temperatures(ops, hip_device, v, 1e-4)
+    test_ends_of_the_draw(ops, hip_device, v)
+
+
+@pytest.mark.parametrize("v", [16500, 16501])
+def test_many_long_rows_are_whole(ops, hip_device, v):
+    """So many rows that each is one workgroup's, longer than those of few are."""
+    rng = np.random.default_rng(v)
+    rows = 300
+    for dtype in (F32, BF16):
+        x = torch.from_numpy(rng.standard_normal((rows, 2, v)).astype(np.float32) * np.float32(2.0)).to(dtype)
+        scale = torch.from_numpy(rng.uniform(0.0, 3.0, rows).astype(np.float32))
+        p = params(rng, rows)
+        check(ops, hip_device, x, rng.random(rows), cfg=True, allowed=rng.random((1, v)) < 0.7, cfg_scale=scale, **p)
+        check(ops, hip_device, x[:, 0].contiguous(), rng.random(rows), **p)
