@@ -396,9 +396,9 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
  * down to the k-th's value (all that equal it); top_p[r] in (0, 1) of these the first ones up to and with the one
  * whose sum of weights e^(x - largest) passes top_p of their whole; min_p[r] in (0, 1] of these the ones with a weight of at
  * least min_p.  Other values of these, and NULL arrays, filter nothing (temperature: 1).  token[r] is
- * the first kept one whose sum passes u[r] of the kept sum; u is in [0, 1) (below it counts as 0, above as the last one).  Sums are of
- * weights rounded to 2^-44 of the largest's power of two or finer (2^-42 past 2^19 values), without further rounding up to V =
- * 16,384; past it a row's sums may differ by 2^-30 of the largest weight with R, and repeat bit for bit for one R.  logprob (may be NULL): the
+ * the first kept one whose sum passes u[r] of the kept sum; u is in [0, 1) (below it counts as 0; 1 or more draws the last one that
+ * adds to the sum).  Sums are within 2^-31 of the largest weight and 2^-42 of themselves (up to 2^16 values 2^-35 and
+ * 2^-46), and a row's results have the same bits in any call.  logprob (may be NULL): the
  * logarithm of the drawn one's part of the kept sum, 0 when greedy or of an only one; kept (may be NULL): how many were kept.  A row without candidates
  * gives -1, -infinity and 0.  R may be 0 and is at most 65535.  No call allocates, waits or copies to the host.  Workspace as for
  * the operators above. */

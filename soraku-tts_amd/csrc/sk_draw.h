@@ -15,10 +15,15 @@
 // * where those buckets hold more values than the list (thousands of equal logits), the bounds are
 //   found digit by digit of the value, three passes over the row for each.
 //
-// Weights are 2^(t - ref), t = y log2(e) in 64 bits, ref the next whole number above the largest t, as
-// whole multiples of 2^-bits: their sums are exact in any order, so results repeat bit for bit.  A row over
-// several workgroups has its slices' sums from the slices' own refs, each bucket's cut to a multiple of the row's: up to
-// one per bucket and slice less, 2^-30 of the largest weight in all.
+// Weights are 2^(t - ref), t = y log2(e) in 64 bits, ref the next whole number above the largest t.  A bucket lies within one
+// power of two, and its values' weights are whole multiples of 2^-bits of that: their sums are exact in any order and in
+// any number of parts.  The sum of all before a place in the order is that of the whole buckets before it, each rounded to the nearest
+// 2^-bits of 2^ref, and that of its own bucket's values before it, rounded alike.  Every step below asks for this one number, wherever it
+// gets the parts from, so bounds and draws agree with each other, and a row has the same bits however many workgroups share
+// it.  Off by half a unit per bucket, 1,600 / 2: 2^-31 of the largest weight at 2^20 values, 2^-35 up to 2^16.  (Weights in
+// units of the row's 2^ref lose a flat tail of light values, all of them rounded the same way, and sums cut to those
+// units between workgroups disagree with sums of values.)  A row of which top-k leaves few is listed whole and its weights
+// rounded to the row's units one by one, half a unit for each of at most 2,048.
 //
 // A row is small work with many steps that wait for each other, on few CUs: its latency bounds it.  16 rows of 2051 with
 // guidance: 12 us; one row of 151,936: 11 us for the histograms and 19 for the rest; 64 of them in BF16 (19 MB): 23
@@ -39,8 +44,8 @@ namespace draw {
 
 constexpr int NT = 1024;                          // threads of a workgroup
 constexpr int PER_BIT = 64, FINE = 20 * PER_BIT;  // buckets per power of two of the weight, for the first 20 of them,
-constexpr int STEP = 8, NB = FINE + 28 * PER_BIT / STEP;   // then an eighth as many, down to 2^-48
-constexpr double NEAR = 48.0;                     // a slice whose ref is further below the row's has nothing but weights of 0
+constexpr int STEP = 8, NB = FINE + 40 * PER_BIT / STEP;   // then an eighth as many, down to 2^-60 (2^20 weights of that are 2^-40)
+constexpr double NEAR = 60.0;                     // a slice whose ref is further below the row's has nothing but weights of 0
 constexpr int MOST_SLICES = 10;                   // workgroups per row
 constexpr int CAP = 2048;                         // values of the list
 constexpr int DIGITS = 2048;                      // of 11, 11 and 10 bits of a key
@@ -245,15 +250,16 @@ __device__ __forceinline__ double power(double e) {
   p = fma(p, z, 1.0);
   return ldexp(p, -(int)n);
 }
-// The weight of a value in units of 2^-bits, rounded to nearest: 2^(-(b + 1/2) / 64) e^z of a value z above the middle of step b
-// below ref.  The first from a table of 64, the second by the exponential series (|z| < 0.006, terms to the 5th: 1e-16).
-__device__ __forceinline__ unsigned long long weight(double z, int b, int bits, const double* roots) {
+// The weight of a value in units of 2^-bits of its step's power of two, rounded to nearest: 2^(-(b + 1/2) / 64) e^z of a value z
+// above the middle of step b below a whole number.  The first from a table of 64, times 2^bits; the second by the exponential
+// series (|z| < 0.006, terms to the 5th: 1e-16).  Below 1.001 2^bits.
+__device__ __forceinline__ unsigned long long weight(double z, int b, const double* roots) {
   double p = fma(1.0 / 120.0, z, 1.0 / 24.0);
   p = fma(p, z, 1.0 / 6.0);
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
-  p = fma(p, z, 1.0) * roots[b & (PER_BIT - 1)];
-  const double x = ldexp(p, bits - (b >> 6)) + 0x1p52;   // the sum's last bits are the whole number
+  p = fma(p, z, 1.0);
+  const double x = fma(p, roots[b & (PER_BIT - 1)], 0x1p52);   // the sum's last bits are the whole number
   return (unsigned long long)__double_as_longlong(x) & 0xfffffffffffffull;
 }
 static_assert(PER_BIT == 64 && STEP == 8 && FINE % STEP == 0, "the shifts above and below");
@@ -261,14 +267,25 @@ constexpr int LAST = FINE + (NB - 1 - FINE) * STEP;   // the first step of the l
 // b < FINE ? b : FINE + (b - FINE) / STEP, b >= 0
 __device__ __forceinline__ int bucket_of(int b) { return min(b, (FINE - FINE / STEP) + (b >> 3)); }
 __device__ __forceinline__ int first_step(int bucket) { return max(bucket, FINE + (bucket - FINE) * STEP); }
+// How many powers of two below the row's a bucket lies: all its steps within one, as 64 are, and 8 | 64.
+__device__ __forceinline__ int powers_below(int bucket) { return first_step(bucket) >> 6; }
+// A sum of a bucket's weights in the row's units, to nearest.
+__device__ __forceinline__ unsigned long long in_row(unsigned long long sum, int bucket) {
+  const int o = powers_below(bucket);
+  return (sum + (1ull << o >> 1)) >> o;
+}
+// The largest sum of a bucket's weights that in_row keeps from passing x, x + 1 being at most in_row of them all.
+__device__ __forceinline__ unsigned long long in_bucket(unsigned long long x, int bucket) {
+  const int o = powers_below(bucket);
+  return ((x + 1) << o) - (1ull << o >> 1) - 1;
+}
 // Where a row's values lie below its reference.  Steps of y are the same number for the same value wherever they are asked,
 // larger for larger values, and counted down from 64 ref, ref a whole number, so counts from the refs of two slices are whole
 // numbers apart.  FP32 does for that up to |y| of 4096 (steps within 0.05 of those of 64 bits).  Past it (a temperature of 1 /
 // 1000, values of a mask's making) ref is the largest value itself, and its row is one workgroup's.
 struct Scale {
   double ref, from, off;                          // in powers of two; e = (from - y) log2(e) + off
-  double a, b;                                    // a b is minus the y of ref
-  float ref64;                                    // 64 ref - 1
+  float ref64, mid;                               // 64 ref - 1; what to take off a step for its middle, counted from `from` up
   bool wild;
   static __device__ __forceinline__ float steps(float y) { return floorf(y * (float)(LOG2E * PER_BIT)); }
   __device__ __forceinline__ explicit Scale(float of) {           // the workgroup's
@@ -280,8 +297,7 @@ struct Scale {
     ref = wild ? (double)y * LOG2E : (double)whole;
     from = wild ? (double)y : 0.0;
     off = wild ? 0.0 : ref;
-    a = wild ? -(double)y : -(double)whole;
-    b = wild ? 1.0 : LN2;
+    mid = wild ? -.5f : ref64 + .5f;
   }
   // powers of two below ref
   __device__ __forceinline__ double e(float y) const { return fma(from - (double)y, LOG2E, off); }
@@ -300,22 +316,24 @@ struct Scale {
     const double d = e(top) - log2(m) + side * 1e-3;
     return bucket_of((int)fmin(fmax(d * PER_BIT, 0.0), (double)LAST));
   }
-  // The weight of a value that many steps below.
-  __device__ __forceinline__ unsigned long long weight_at(float y, float below, int bits, const double* roots) const {
-    const double z = fma((double)(below + .5f), LN2 / PER_BIT, fma(a, b, (double)y));
-    return draw::weight(z, (int)below, bits, roots);
+  // The weight of a value that many steps below, in its bucket's units.  Nothing in it depends on ref (64 of which is what a
+  // step's number and mid have in common): slices of a row give a value one weight.
+  __device__ __forceinline__ unsigned long long weight_at(float y, float below, const double* roots) const {
+    const double z = fma((double)(below - mid), LN2 / PER_BIT, (double)y - from);
+    return draw::weight(z, (int)below, roots);
   }
-  // A value's weight: 0 in the last bucket.
-  __device__ __forceinline__ unsigned long long weight(float y, int bits, const double* roots) const {
+  // A value's bucket, and its weight in the bucket's units: 0 in the last one.
+  __device__ __forceinline__ unsigned long long weight(float y, int& bucket, const double* roots) const {
     const float d = belowf(y);
-    return d < (float)LAST ? weight_at(y, d, bits, roots) : 0;
+    bucket = bucket_of((int)d);
+    return d < (float)LAST ? weight_at(y, d, roots) : 0;
   }
 };
 
 // The workgroup's shared memory.
 struct Shared {
-  double roots[PER_BIT];                          // 2^(-(i + 1/2) / 64)
-  unsigned long long mass[NB + 1];                // of a bucket, then of all before it
+  double roots[PER_BIT];                          // 2^(bits - (i + 1/2) / 64)
+  unsigned long long mass[NB + 1];                // of a bucket in its units, then of all before it in the row's
   alignas(16) unsigned long long list[2 * CAP];   // then their sums (digit by digit: histograms)
   unsigned count[NB + 1];
   unsigned long long wave64[16];
@@ -325,8 +343,12 @@ struct Shared {
   // ranges of buckets: first and last, the keys of x between them, where they begin in the list, what lies before them
   struct { int lo, hi, pos; uint32_t least, most; unsigned cp; unsigned long long mp; } range[4];
   int lo[4], hi[4], ranges, total;
-  // digit by digit
+  // digit by digit, within a bucket
   struct { unsigned prefix; unsigned cp; unsigned long long mp; unsigned cnt; unsigned long long mass; } at;
+  __device__ __forceinline__ void fill_roots(int bits) {
+    const int i = NT - 1 - threadIdx.x;
+    if (i < PER_BIT) roots[i] = ldexp(power((i + 0.5) / PER_BIT), bits);
+  }
 };
 static_assert(CAP * 16 >= (DIGITS + 1) * 12, "digits' histograms lie in the list's place");
 
@@ -378,12 +400,18 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, Sh
   __syncthreads();
   return wave_all(lane < 16 ? s.wave64[lane] : 0, Plus{});
 }
-// Exclusive sums of count[0 .. n) and mass[0 .. n) in place, and the wholes at n; n at most 2 NT.
+// Exclusive sums of count[0 .. n) and mass[0 .. n) in place, and the wholes at n; n at most 2 NT.  BUCKETS: masses are
+// buckets' and become the row's.
+template <bool BUCKETS>
 __device__ __forceinline__ void block_scan(unsigned* count, unsigned long long* mass, int n, Shared& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x * 2;
   const bool on0 = at < n, on1 = at + 1 < n;
   const unsigned c0 = on0 ? count[at] : 0, c1 = on1 ? count[at + 1] : 0;
-  const unsigned long long m0 = on0 ? mass[at] : 0, m1 = on1 ? mass[at + 1] : 0;
+  unsigned long long m0 = on0 ? mass[at] : 0, m1 = on1 ? mass[at + 1] : 0;
+  if constexpr (BUCKETS) {
+    m0 = in_row(m0, on0 ? at : 0);
+    m1 = in_row(m1, on1 ? at + 1 : 0);
+  }
   unsigned c = wave_incl(c0 + c1, Plus{});
   unsigned long long m = wave_incl(m0 + m1, Plus{});
   if (lane == 63) { s.wave32[wave] = c; s.wave64[wave] = m; }
@@ -414,15 +442,15 @@ __device__ __forceinline__ void survey(const R& row, int v0, int v1, Shared& s, 
   block_max_sum(best, c, s);
   n = (int)c;
 }
-// Counts and (with sums) sums of weights by bucket of values v0 .. v1 in s.count and s.mass.
+// Counts and (with sums) sums of weights by bucket, in its units, of values v0 .. v1 in s.count and s.mass.
 template <typename R>
-__device__ __forceinline__ void histogram(const R& row, int v0, int v1, const Scale& at, int bits, bool sums, Shared& s) {
+__device__ __forceinline__ void histogram(const R& row, int v0, int v1, const Scale& at, bool sums, Shared& s) {
   for (int i = threadIdx.x; i < NB; i += NT) { s.count[i] = 0; s.mass[i] = 0; }
   __syncthreads();
   row.each(v0, v1, [&](int, float x, bool on) __attribute__((always_inline)) {
     const float y = row.divided(x), d = at.belowf(y);
     const int b = bucket_of((int)d);
-    const unsigned long long w = sums ? at.weight_at(y, d, bits, s.roots) : 0;
+    const unsigned long long w = sums ? at.weight_at(y, d, s.roots) : 0;
     if (on) {
       atomicAdd(&s.count[b], 1u);
       if (sums && d < (float)LAST) atomicAdd(&s.mass[b], w);
@@ -660,7 +688,8 @@ __device__ __forceinline__ double part_log(uint32_t key, const Scale& at, unsign
 __device__ __forceinline__ void finish_list(const Args& a, int r, const Params& q, const Scale& scale, uint32_t top, int n, Shared& s) {
   const int total = s.total, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   unsigned long long* sum_at = s.list + CAP;
-  // sums up to and with each, `per` neighbours to a thread
+  // sums up to and with each, `per` neighbours to a thread: of the row's units if all that is kept is listed, of each bucket's own
+  // if not (differences within a bucket are all that is taken of them)
   const int per = (total + NT - 1) / NT;
   {
     unsigned long long v[CAP / NT], mine = 0;
@@ -670,7 +699,9 @@ __device__ __forceinline__ void finish_list(const Args& a, int r, const Params& 
       v[i] = 0;
       if (i < per && at < total) {
         const uint32_t key = (uint32_t)(s.list[at] >> 32);
-        v[i] = scale.weight(value_of(key), a.bits, s.roots);
+        int b;
+        v[i] = scale.weight(value_of(key), b, s.roots);
+        if (q.list) v[i] = in_row(v[i], b);
       }
       mine += v[i];
     }
@@ -692,8 +723,10 @@ __device__ __forceinline__ void finish_list(const Args& a, int r, const Params& 
   auto end_of = [&](int i) { return i + 1 < s.ranges ? s.range[i + 1].pos : total; };
   // sum of all up to and with list entry i of range g
   auto upto = [&](int g, int i) {
-    const int p = s.range[g].pos;
-    return s.range[g].mp + sum_at[i] - (p ? sum_at[p - 1] : 0);
+    if (q.list) return sum_at[i];
+    const int b = scale.bucket(value_of((uint32_t)(s.list[i] >> 32)));
+    const int p = s.range[g].pos + (int)(s.count[b] - s.range[g].cp);   // where the bucket begins
+    return s.mass[b] + in_row(sum_at[i] - (p ? sum_at[p - 1] : 0), b);
   };
   // first entry of range g for which `past` holds (it holds from some entry on), or its end; 64 at a time
   auto first = [&](int g, auto past) {
@@ -752,10 +785,10 @@ __device__ __forceinline__ void finish_list(const Args& a, int r, const Params& 
   if (lane == 0) answer(a, r, (int)~(uint32_t)s.list[i], part_log((uint32_t)(s.list[i] >> 32), scale, sum, a.bits), (int)kept);
 }
 
-// Digit by digit: the value at which the count of the largest (by_count) or their sum passes T, in
-// s.at: its key, the count and sum of all above it, and its own.
+// Digit by digit among the values of one bucket: the value at which their count, largest first (by_count), or the sum of their weights
+// in the bucket's units passes T, less than the whole, in s.at: its key, the count and sum of all above it, and its own.
 template <typename X, bool WIDE>
-__device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bits, bool by_count, unsigned long long T, Shared& s) {
+__device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& scale, int bucket, bool by_count, unsigned long long T, Shared& s) {
   unsigned long long* mass = s.list;              // [DIGITS + 1], then counts
   unsigned* count = reinterpret_cast<unsigned*>(s.list + DIGITS + 1);
   uint32_t prefix = 0, mask = 0;
@@ -768,18 +801,17 @@ __device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& sc
     for (int v0 = 0; v0 < row.V; v0 += NT) {      // whole waves
       const int v = v0 + threadIdx.x;
       const uint32_t k = v < row.V ? row.key(v) : 0;
-      const bool on = k && (k & mask) == prefix;
-      const int d = digits - 1 - (int)(k >> shift & (digits - 1));
+      int b = -1;
       unsigned long long w = 0;
-      if (on) {
-        w = scale.weight(value_of(k), bits, s.roots);
-      }
+      if (k && (k & mask) == prefix) w = scale.weight(value_of(k), b, s.roots);
+      const bool on = b == bucket;
+      const int d = digits - 1 - (int)(k >> shift & (digits - 1));
       // where a wave's values all have one digit, as equal logits do, one lane adds for all
       const unsigned long long who = __ballot(on);
       if (!who) continue;
       const int d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(who));
       if (__ballot(on && d == d0) == who) {
-        w = wave_all(w, Plus{});
+        w = wave_all(on ? w : 0ull, Plus{});
         if ((threadIdx.x & 63) == 0) {
           atomicAdd(&count[d0], (unsigned)__popcll(who));
           atomicAdd(&mass[d0], w);
@@ -790,7 +822,7 @@ __device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& sc
       }
     }
     __syncthreads();
-    block_scan(count, mass, digits, s);
+    block_scan<false>(count, mass, digits, s);
     if (threadIdx.x == 0) {
       int lo = 0, hi = digits - 1;
       while (lo < hi) {
@@ -811,47 +843,60 @@ __device__ __forceinline__ void descend(const Row<X, WIDE>& row, const Scale& sc
   }
 }
 
-// The row's answer where the list does not hold its ranges.
+// The row's answer where the list does not hold its ranges: the bucket of each bound from the histogram's sums, then its value.
 template <typename X, bool WIDE>
 __device__ __forceinline__ void finish_digits(const Args& a, int r, const Row<X, WIDE>& row, const Params& q, const Scale& scale, uint32_t top,
                               int n, Shared& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  unsigned kept = (unsigned)n;
-  unsigned long long sum = s.mass[NB];            // (with q.list there is a k: the list holds any row of fewer)
-  if (q.k) {
-    descend(row, scale, a.bits, true, q.k - 1, s);
-    kept = s.at.cp + s.at.cnt;
-    sum = s.at.mp + s.at.mass;
+  if (q.list) {                                   // the histogram has no sums yet
+    histogram(row, 0, a.V, scale, true, s);
+    block_scan<true>(s.count, s.mass, NB, s);
   }
+  // the bucket b with of[b] <= x < of[b + 1], x less than the whole
+  auto bucket = [&](const auto* of, auto x) {
+    int lo = 0, hi = NB - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (of[mid + 1] > x) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  };
+  unsigned kept = (unsigned)n;
+  unsigned long long sum = s.mass[NB];
+  // all down to the value of the c-th of all (from 0) are kept
+  auto keep_to = [&](unsigned c) {
+    const int b = bucket(s.count, c);
+    descend(row, scale, b, true, c - s.count[b], s);
+    kept = s.count[b] + s.at.cp + s.at.cnt;
+    sum = s.mass[b] + in_row(s.at.mp + s.at.mass, b);
+  };
+  // the value at which the sum of all passes T, in s.at, and how many of its equal ones are before the one that does
+  auto pass = [&](unsigned long long T, int& b, unsigned long long& w) {
+    b = bucket(s.mass, T);
+    const unsigned long long most = in_bucket(T - s.mass[b], b);
+    descend(row, scale, b, false, most, s);
+    w = s.at.mass / s.at.cnt;                     // equal values have one weight, and not 0 where sums pass anything
+    return (unsigned)((most - s.at.mp) / w);
+  };
+  int b;
+  unsigned long long w;
+  if (q.k) keep_to(q.k - 1);
   if (q.p > 0.0) {
-    const unsigned long long T = part_of(q.p, sum);
-    __syncthreads();
-    descend(row, scale, a.bits, false, T, s);
-    // of the equal values so many that the sum passes T
-    const unsigned long long w = s.at.cnt ? s.at.mass / s.at.cnt : 0;
-    unsigned c = w ? (unsigned)min((T - s.at.mp) / w + 1, (unsigned long long)s.at.cnt) : s.at.cnt;
-    if (s.at.cp + c < kept) { kept = s.at.cp + c; sum = s.at.mp + c * w; }
+    const unsigned nth = pass(part_of(q.p, sum), b, w), c = s.count[b] + s.at.cp + nth + 1;
+    if (c < kept) { kept = c; sum = s.mass[b] + in_row(s.at.mp + (nth + 1) * w, b); }
   }
   if (q.m > 0.0) {
-    unsigned c = 0;
-    unsigned long long w = 0;
+    unsigned long long c = 0;
     for (int v = tid; v < row.V; v += NT) {
       const uint32_t k = row.key(v);
-      if (k && heavy(k, top, q.m)) {
-        ++c;
-        w += scale.weight(value_of(k), a.bits, s.roots);
-      }
+      c += k && heavy(k, top, q.m);
     }
-    c = (unsigned)block_sum(c, s);
-    w = block_sum(w, s);
-    if (c < kept) { kept = c; sum = w; }
+    c = block_sum(c, s);
+    if (c < kept) keep_to((unsigned)c - 1);       // equal values are alike: these and no others
   }
-  const unsigned long long T = part_of(q.u, sum);
-  __syncthreads();
-  descend(row, scale, a.bits, false, T, s);
+  const unsigned nth = pass(part_of(q.u, sum), b, w);
   const uint32_t key = s.at.prefix;
-  const unsigned long long w = s.at.cnt ? s.at.mass / s.at.cnt : 0;
-  const unsigned long long nth = w ? (T - s.at.mp) / w : 0;   // from 0, among the equal ones by id
   // each wave counts the equal ones of its run of ids, then the one that has it looks again
   const int run = (row.V + NT / 64 - 1) / (NT / 64), v0 = wave * run, v1 = min(v0 + run, row.V);
   unsigned c = 0;
@@ -882,7 +927,7 @@ __device__ __forceinline__ bool finish_early(const Args& a, int r, const Params&
 // A whole row in one workgroup.
 template <typename R>
 __device__ __forceinline__ void whole_row(const Args& a, int r, const Given& given, const R& row, Shared& s) {
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
+  s.fill_roots(a.bits);
   unsigned long long best;
   int n;
   survey(row, 0, a.V, s, best, n);
@@ -890,8 +935,8 @@ __device__ __forceinline__ void whole_row(const Args& a, int r, const Given& giv
   if (finish_early(a, r, q, best, n)) return;
   const uint32_t top = key_of(row.divided(value_of((uint32_t)(best >> 32))));
   const Scale scale(value_of(top));
-  histogram(row, 0, a.V, scale, a.bits, !q.list, s);
-  block_scan(s.count, s.mass, NB, s);
+  histogram(row, 0, a.V, scale, !q.list, s);
+  block_scan<true>(s.count, s.mass, NB, s);
   plan(row, q, scale, value_of(top), s);
   if (s.total > CAP) {
     finish_digits(a, r, row, q, scale, top, n, s);
@@ -943,7 +988,7 @@ struct RowSpace {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
+  s.fill_roots(a.bits);
   const int r = blockIdx.y, g = blockIdx.x;
   const Given given(a, r);
   const Row<X, WIDE> row(a, given, r);
@@ -958,7 +1003,7 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
     if (g == 0) { *w.listed = 0; *w.arrived = 0; }
   }
   if (n == 0 || !(row.T > 0.f) || scale.wild) return;   // nothing of it is read
-  histogram(row, v0, v1, scale, a.bits, !given.lists(), s);
+  histogram(row, v0, v1, scale, !given.lists(), s);
   for (int i = threadIdx.x; i < NB; i += NT) {
     w.count[g * NB + i] = s.count[i];
     w.mass[g * NB + i] = s.mass[i];
@@ -968,7 +1013,7 @@ __global__ __launch_bounds__(NT) void slice_kernel(Args a) {
 template <typename X, bool WIDE>
 __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   __shared__ Shared s;
-  if (threadIdx.x >= NT - PER_BIT) s.roots[NT - 1 - threadIdx.x] = power((NT - 1 - threadIdx.x + 0.5) / PER_BIT);
+  s.fill_roots(a.bits);
   const int r = blockIdx.y, g = blockIdx.x;
   const Given given(a, r);
   const Row<X, WIDE> row(a, given, r);
@@ -993,10 +1038,10 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
   const bool alone = scale.wild || __any(near && info.wild);
   if (alone && g) return;
   if (alone) {
-    histogram(row, 0, a.V, scale, a.bits, !q.list, s);
+    histogram(row, 0, a.V, scale, !q.list, s);
   } else {
     // A slice's ref is `by` powers of two lower, so its steps lie 64 by further below the row's: a fine bucket has one of
-    // the slice's fine ones, a wide one has one of its wide ones, or eight of its last fine ones.  All loads
+    // the slice's fine ones, a wide one has one of its wide ones, or eight of its last fine ones, in the same units.  All loads
     // are on their way at once: they come from other XCDs' stores, 1 us away.
     constexpr int U = (NB + NT - 1) / NT;         // buckets of a thread
     const bool sums = !q.list;
@@ -1034,7 +1079,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
       const int to = bucket_of(d + by * PER_BIT);
       if (to < NB - 1 && c) {
         atomicAdd(&s.count[to], c);
-        if (sums) atomicAdd(&s.mass[to], m >> by);
+        if (sums) atomicAdd(&s.mass[to], m);
       }
     };
 #pragma unroll
@@ -1049,13 +1094,13 @@ __global__ __launch_bounds__(NT) void pick_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < MOST_SLICES; ++i) {
         c += x[i][j];
-        m += y[i][j] >> max(__builtin_amdgcn_readlane(lower, i), 0);
+        m += y[i][j];
       }
       if (b < NB) { s.count[b] += c; s.mass[b] += m; }
     }
     __syncthreads();
   }
-  block_scan(s.count, s.mass, NB, s);
+  block_scan<true>(s.count, s.mass, NB, s);
   if (threadIdx.x == 0) s.count[NB] = n;
   __syncthreads();
   plan(row, q, scale, value_of(top), s);
