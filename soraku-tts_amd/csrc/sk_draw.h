@@ -679,9 +679,9 @@ __device__ __forceinline__ void answer(const Args& a, int r, int token, double l
   if (a.logprob) a.logprob[r] = kept == 1 ? 0.f : (float)logprob;   // the only one is the whole: exactly 0
   if (a.kept) a.kept[r] = kept;
 }
-// ln of the drawn one's part of the kept sum.
+// ln of the drawn one's part of the kept sum, which may be all that the sum holds of it.
 __device__ __forceinline__ double part_log(uint32_t key, const Scale& at, unsigned long long kept, int bits) {
-  return (bits - at.e(value_of(key))) * LN2 - log((double)kept);
+  return fmin((bits - at.e(value_of(key))) * LN2 - log((double)kept), 0.0);
 }
 
 // The row's answer from the sorted list of its ranges.

@@ -148,6 +148,19 @@ def test_a_row_has_the_same_bits_in_any_call(ops, hip_device, v):
             assert (part[1].view(np.int32) == whole[1][s].view(np.int32)).all()
 
 
+@pytest.mark.parametrize("v", [40, 3000, 20000])
+def test_logarithms_are_not_above_0(ops, hip_device, v):
+    """Of several kept ones whose others weigh next to nothing."""
+    rng = np.random.default_rng(v)
+    rows = 100
+    x = np.full((rows, v), -90.0, np.float32)
+    x[np.arange(rows), rng.integers(0, v, rows)] = rng.standard_normal(rows)
+    t = rng.uniform(0.5, 1.5, rows).astype(np.float32)
+    tok, lp, kept = draw(ops, hip_device, torch.from_numpy(x).to(hip_device), rng.random(rows), temperature=torch.from_numpy(t))
+    assert (tok == x.argmax(1)).all() and (kept == v).all()
+    assert (lp <= 0).all() and (lp > -1e-9).all(), lp.max()
+
+
 @pytest.mark.parametrize("v", [300, 5000, 40000])
 def test_close_values_and_light_ones(ops, hip_device, v):
     """Bounds among thousands of close values, with light ones below them, against the row sorted in 64 bits."""
