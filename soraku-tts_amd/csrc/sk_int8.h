@@ -13,7 +13,7 @@
 //
 // A normalised row is coded as t = fp32(x gain) with the norm's factor in its scale: the
 // factor is the whole row's, so it moves no code, and sums of squares in another order
-// change none.
+// change none.  Factor and scale are taken in 64 bits and rounded once.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -97,13 +97,21 @@ __device__ __forceinline__ uint32_t top8(const float (&t)[8], uint32_t top) {
 struct Coder {
   float r, up, top;                               // 127 / (top up), up, top up
   float scale;                                    // top / 127
+  float plain;                                    // top, NaN where it is no number
   __device__ explicit Coder(uint32_t bits) {
     const float t = __uint_as_float(bits);
     const bool bad = bits >= 0x7f800000u;
     up = t < 0x1p-60f ? 0x1p80f : t > 0x1p100f ? 0x1p-20f : 1.f;
     top = t * up;
     r = bad || bits == 0 ? 0.f : 127.f / top;
-    scale = bad ? __uint_as_float(0x7fc00000u) : t / 127.f;
+    plain = bad ? __uint_as_float(0x7fc00000u) : t;
+    scale = plain / 127.f;
+  }
+  // fp32(top / 127 / sqrt(m)), m a mean of squares and eps: the GPU's own reciprocal root, within 2^-24, and one step of Newton's.
+  __device__ __forceinline__ float normed(double m) const {
+    double r = __builtin_amdgcn_rsq(m);
+    r *= fma(-0.5 * m * r, r, 1.5);
+    return (float)((double)plain * (1.0 / 127.0) * r);
   }
   // The nearest whole number of 127 t / top, t multiplied by up, exactly.  With the middle m = floor(t r) + 1/2 (floor
   // of the rounded product may be one off next to a whole number, where the other side of m decides alike), m top
@@ -171,16 +179,29 @@ __device__ __forceinline__ float wave_sum(float v) {
 // hang on the size of the call: 8 values one after the other, the 64 such sums of a block of 512 by
 // wave_sum, the blocks one after the other.
 constexpr int BLOCK = 512;
-__device__ __forceinline__ float norm_of(const float* blocks, int K, float eps) {
+// The mean of a row's squares, in every lane of a whole wave.  Past FP32's range, or so far below it that squares lose bits which
+// eps does not cover (up to 2^17 squares are each off by 2^-150), it is summed again in 64 bits from the row itself.
+template <typename X>
+__device__ __forceinline__ double mean_of(const X* x, const float* blocks, int K, double per, float eps) {
   float s = 0.f;
   for (int b = 0; b * BLOCK < K; ++b) s += blocks[b];
-  return 1.f / sqrtf(s / (float)K + eps);
+  double t = s;
+  if (!(s <= 3.402823466e38f && (s >= 0x1p-100f || eps >= 0x1p-60f))) {
+    t = 0.0;
+    for (int k = threadIdx.x & 63; k < K; k += 64) {
+      const double v = to_f<X>(x[k]);
+      t = fma(v, v, t);
+    }
+    for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
+  }
+  return t * per;
 }
 
 struct RowsArgs {
   const void* x; const float* gain; float eps;    // eps < 0: not normalised
   int R, K, Kp;
   int8_t* codes; float* scales;
+  double per;                                     // 1 / K
 };
 
 // Codes of R rows: W waves per row, C chunks of 512 W values held in registers (C = 0:
@@ -227,7 +248,12 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
   }
   const Coder coder(top);
-  if (wave % W == 0 && lane == 0) a.scales[row] = MODE != PLAIN ? coder.scale * norm_of(mine, a.K, a.eps) : coder.scale;
+  __builtin_amdgcn_wave_barrier();                // W = 1: the sums in `mine` are this wave's own
+  if (wave % W == 0) {
+    float s = coder.scale;
+    if constexpr (MODE != PLAIN) s = coder.normed(mean_of(x, mine, a.K, a.per, a.eps) + (double)a.eps);
+    if (lane == 0) a.scales[row] = s;
+  }
   int8_t* q = a.codes + (size_t)row * a.Kp;
   if constexpr (C > 0) {
 #pragma unroll
@@ -595,8 +621,11 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
     if (row < a.M) {
       for (int w = row * wpr; w < (row + 1) * wpr; ++w) top = max(top, tops[w]);
       const Coder coder(top);
-      if (wave % wpr == 0 && lane == 0)
-        row_scale[row] = norm ? coder.scale * norm_of(blocks + row * wpr * C, r.K, r.eps) : coder.scale;
+      if (wave % wpr == 0) {
+        float s = coder.scale;
+        if (norm) s = coder.normed(mean_of(static_cast<const X*>(r.x) + (size_t)row * r.K, blocks + row * wpr * C, r.K, r.per, r.eps) + (double)r.eps);
+        if (lane == 0) row_scale[row] = s;
+      }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int k = k0 + c * step;

@@ -172,7 +172,7 @@ int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const vo
   if (R == 0) return SK_OK;
   SK_CHECK(x && codes && scales, SK_EINVAL, "NULL operand");
   SK_CHECK(aligned16(x) && aligned16(codes), SK_EINVAL, "operands must be 16-byte aligned");
-  const RowsArgs a{x, nullptr, -1.f, R, K, padded(K), codes, scales};
+  const RowsArgs a{x, nullptr, -1.f, R, K, padded(K), codes, scales, 1.0 / K};
   if (xdtype == SK_BF16) launch_rows<uint16_t>(a, (hipStream_t)stream);
   else launch_rows<float>(a, (hipStream_t)stream);
   SK_HIP(hipGetLastError());
@@ -213,7 +213,7 @@ int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdt
   a.mt = (M + p.bm - 1) / p.bm; a.nt = (N + nc - 1) / nc; a.gm = 8;
   SK_CHECK(p.few || ((int64_t)a.mt * a.nt + 7) * TILES[p.kind].waves * 64 < (int64_t)1 << 32, SK_EINVAL,
            "M * N is too large: several calls are needed");   // a launch has less than 2^32 threads
-  const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as)};
+  const RowsArgs r{x, gain, eps, M, K, padded(K), const_cast<int8_t*>(a.a), const_cast<float*>(a.as), 1.0 / K};
   return xdtype == SK_BF16 ? run_linear<uint16_t>((hipStream_t)stream, p, a, r, swiglu)
                            : run_linear<float>((hipStream_t)stream, p, a, r, swiglu);
 }

@@ -1,0 +1,66 @@
+"""8-bit projections of rows of any finite size: norms whose squares leave FP32's range."""
+
+import numpy as np
+import pytest
+import torch
+
+import int8_ref as ref
+from test_gpu_int8 import BF16, F32, expected, make, on
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(hip_device):
+    from soraku_amd import ops as O
+
+    return O
+
+
+def check(ops, dev, d, n, k, eps, swiglu=False):
+    got = ops.int8_linear(n, k, act="swiglu" if swiglu else None, eps=eps)(**on(d, dev)).double().cpu().numpy()
+    want, off = expected(d, eps, swiglu)
+    assert np.isfinite(want).all()
+    lim = off + (np.abs(want) + off) * ref.HALF_STEP[str(d["x"].dtype)[6:]] + 2.0 ** -133
+    assert (np.abs(got - want) <= lim).all(), (got[:, 0], want[:, 0])
+
+
+# rows of one, a few, some and many, as the kernels divide them; K in registers, read twice, and not of whole pieces
+SHAPES = [(1, 200), (2, 2048), (7, 1001), (7, 2048), (20, 512), (20, 1537), (90, 6144), (5, 8200), (40, 9001), (1100, 384), (1100, 2048)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gain", [True, False])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_norms_of_any_finite_row(ops, hip_device, m, k, gain, dtype):
+    n = 24
+    d = make(m, n, k, dtype, norm=gain, bias=True, residual=True, seed=3)
+    base = (d["x"].float() / d["x"].float().abs().amax(1, keepdim=True)).to(dtype)
+    sizes = [1e20, 1.0, 1e30, 1e38, 1e19, 6e18, 1e-3]
+    for eps, factors in ((1e-6, sizes), (0.0, sizes + [1e-15, 1e-19, 1e-25, 1e-34]), (1e-30, [1e-15, 1e-17, 1e-25, 1e22])):
+        x = base.double()
+        for r in range(m):
+            x[r] *= factors[r % len(factors)] if m > 1 else factors[0]
+        d["x"] = x.to(dtype)
+        check(ops, hip_device, d, n, k, eps)
+    if m == 1:
+        for size in sizes[2:] + [1e-25]:
+            d["x"] = (base.double() * size).to(dtype)
+            check(ops, hip_device, d, n, k, 0.0)
+    # one value whose square alone is past the range
+    x = base.double()
+    x[:, k - 1] = -3e25
+    d["x"] = x.to(dtype)
+    check(ops, hip_device, d, n, k, 1e-6)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_norms_do_not_hang_on_their_call(ops, hip_device, eps):
+    for k in (1024, 1537):
+        d = on(make(1200, 40, k, F32, norm=True, seed=4), hip_device)
+        d["x"][::3] *= 1e22
+        d["x"][1::3] *= 1e-22
+        f = ops.int8_linear(40, k, eps=eps)
+        whole = f(**d)
+        for m in (1, 2, 5, 8, 9, 40, 300):
+            assert torch.equal(f(**dict(d, x=d["x"][:m])), whole[:m])
