@@ -296,11 +296,18 @@ __device__ __forceinline__ float silu(float g) {
   const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, LN2, 1.f);
   return g * __builtin_amdgcn_rcpf(1.f + e);
 }
+// A row's scale as two factors, one of them 1: what sums are multiplied by, and what columns' scales are.  Sums are below 2^31, so
+// products with scales up to 2^96 stay finite; rows of larger ones (values past 1e31) take theirs with the columns' first, which
+// leaves FP32's range only where the output does.
+struct RowScale {
+  float s, t;
+  __device__ __forceinline__ explicit RowScale(float x) : s(x > 0x1p96f ? 1.f : x), t(x > 0x1p96f ? x : 1.f) {}
+};
 // act of sums of row m (scale s) and column c (scale w, bias b; SwiGLU: and of its up column).
 template <typename X, bool SWIGLU>
-__device__ __forceinline__ float act_of(int acc, int up, float s, float w, float w2, float b, float b2) {
-  const float y = (float)acc * s * w + b;
-  if constexpr (SWIGLU) return silu<X>(y) * ((float)up * s * w2 + b2);
+__device__ __forceinline__ float act_of(int acc, int up, RowScale s, float w, float w2, float b, float b2) {
+  const float y = fmaf((float)acc * s.s, s.t * w, b);
+  if constexpr (SWIGLU) return silu<X>(y) * fmaf((float)up * s.s, s.t * w2, b2);
   else return y;
 }
 
@@ -491,7 +498,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int r0 = (wm * TM + i) * 32;
-    const float sc = row_s[r0 + i32];
+    const RowScale sc(row_s[r0 + i32]);
 #pragma unroll
     for (int j0 = 0; j0 < TO; j0 += CJ) {
 #pragma unroll
@@ -698,7 +705,7 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
     const v4i up = SWIGLU ? add_waves((i * NT + j + NT / 2) * 64 + l) : y;
     const int m = m0 + i * 16 + (l & 15), n = n0 + j * 16 + (l >> 4) * 4;
     float out[4];
-    const float sc = a.as[min(m, a.M - 1)];
+    const RowScale sc(a.as[min(m, a.M - 1)]);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int c = min(n + v, a.N - 1);

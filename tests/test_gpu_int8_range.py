@@ -1,4 +1,5 @@
-"""8-bit projections of rows of any finite size: norms whose squares leave FP32's range."""
+"""8-bit projections of rows of any finite size: norms whose squares leave FP32's range, scales that sums of codes
+would carry past it."""
 
 import numpy as np
 import pytest
@@ -64,3 +65,15 @@ def test_norms_do_not_hang_on_their_call(ops, hip_device, eps):
         whole = f(**d)
         for m in (1, 2, 5, 8, 9, 40, 300):
             assert torch.equal(f(**dict(d, x=d["x"][:m])), whole[:m])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,n,k", [(2, 40, 256), (7, 40, 300), (20, 40, 256), (70, 264, 384), (400, 264, 384), (3000, 264, 256)])
+def test_sums_past_the_range_before_their_weights_scale(ops, hip_device, m, n, k, dtype):
+    """Rows of up to 3e38 by weights of a usual size: outputs are finite, sums of codes times the row's scale alone are not."""
+    d = make(m, n, k, dtype, bias=True, residual=True, seed=5)
+    d["scales"] = d["scales"] * 2.0 ** -8
+    top = d["x"].float().abs().amax(1, keepdim=True)
+    size = torch.tensor([3e38, 1.0, 2e37, 1e30, 2.0 ** 103, 2.0 ** 104])[torch.arange(m) % 6][:, None]
+    d["x"] = (d["x"].double() / top.double() * size.double()).to(dtype)
+    check(ops, hip_device, d, n, k, None)
