@@ -373,7 +373,7 @@ int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const vo
  * The rows of x become codes on the way; with eps >= 0 x is normalised first (RMSNorm with gain [K], or NULL for
  * none): then fp32(x gain) is coded and the norm's factor goes into the scale.  Products are summed
  * in whole numbers, exactly, so a row's result does not hang on what else is in the call; scales, bias, act
- * and residual follow in FP32, rounded once at the end.  A row of x with an infinity or NaN gives NaN, and so does one whose
+ * and residual follow in FP32, rounded once at the end (silu of less than -87.3 is 0: it is 1.03e-36 at most there).  A row of x with an infinity or NaN gives NaN, and so does one whose
  * x gain is past FP32's range; any other row is normalised, however large or small its values are.  Codes of W
  * may be any bytes, -128 too, whoever made them (behind K they meet zeros).
  * M may be 0 and is below 2^24; N is at most 2^20.  The workspace holds the bytes that _workspace gives for the same

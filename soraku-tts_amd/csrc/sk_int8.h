@@ -285,7 +285,8 @@ struct LinearArgs {
 };
 
 // g / (1 + e^-g) with the GPU's own powers of two and reciprocals (each within a step of the result).  For FP32 outputs
-// t = -g log2(e) in two parts, 2^t_hi (1 + t_lo ln 2); below -87 it is 0.  For BF16 ones t alone: its rounding moves e^-g by
+// t = -g log2(e) in two parts, 2^t_hi (1 + t_lo ln 2).  Below -87.3, where the reciprocal is denormal, it is 0 (silu is 1.03e-36 at
+// most there; 1 / (1 + e^88.8) in FP32 is 0 as well).  For BF16 ones t alone: its rounding moves e^-g by
 // |g| 2^-24, where the output's is 2^-8 (7,680 x 6144 outputs: 5 of 26 instructions each).
 template <typename X>
 __device__ __forceinline__ float silu(float g) {
