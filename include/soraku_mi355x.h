@@ -376,7 +376,8 @@ int sk_op_int8_rows(void* stream, int32_t R, int32_t K, int32_t xdtype, const vo
  * and residual follow in FP32, rounded once at the end (silu of less than -87.3 is 0: it is 1.03e-36 at most there).  A row of x with an infinity or NaN gives NaN, and so does one whose
  * x gain is past FP32's range; any other row is normalised, however large or small its values are.  Codes of W
  * may be any bytes, -128 too, whoever made them (behind K they meet zeros).
- * M may be 0 and is below 2^24; N is at most 2^20.  The workspace holds the bytes that _workspace gives for the same
+ * M may be 0 and is below 2^24; N is at most 2^20; M N of up to 2^35 is taken, and more may be refused (SK_EINVAL) by the call though
+ * not by _workspace: it then takes several calls.  The workspace holds the bytes that _workspace gives for the same
  * sizes (where that is 0 it may be NULL) and belongs to the call until it has run. */
 int sk_op_int8_linear_workspace(int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act, int64_t* bytes);
 int sk_op_int8_linear(void* stream, int32_t M, int32_t N, int32_t K, int32_t xdtype, int32_t act, float eps,
