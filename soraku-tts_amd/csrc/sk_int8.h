@@ -213,7 +213,8 @@ template <typename X, int W, int C, bool WHOLE, int MODE>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x * (4 / W) + wave / W;
-  if (W < 4 && row >= a.R) return;                // whole waves, and no barrier below for W = 1
+  static_assert(W == 1 || W == 4, "a row is a wave's or the workgroup's");
+  if (W < 4 && row >= a.R) return;                // whole waves, and no barrier below
   const X* x = static_cast<const X*>(a.x) + (size_t)row * a.K;
   const int k0 = (wave % W * 64 + lane) * 8;
   constexpr int STEP = W * BLOCK, R = 4 / W;       // values per step, rows per workgroup
@@ -654,14 +655,13 @@ __global__ __launch_bounds__(W * 64) void few_kernel(LinearArgs a, RowsArgs r) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = v4i{0, 0, 0, 0};
   constexpr int L = 2 * T;                        // loads of a unit
-  static_assert(D >= 2 && D <= 4 && 3 * L < 64, "the waits below, and their counter");
+  static_assert((D == 2 || D == 3) && 2 * L < 64, "the waits below, and their counter");
   for (int i0 = 0; i0 < mine; i0 += D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int i = i0 + d, behind = min(D - 1, mine - 1 - i);
       if (behind < 0) break;
-      if (D > 3 && behind == 3) loads_but<(D > 3 ? 3 : 0) * L>();
-      else if (D > 2 && behind == 2) loads_but<(D > 2 ? 2 : 0) * L>();
+      if (D > 2 && behind == 2) loads_but<(D > 2 ? 2 : 0) * L>();
       else if (behind == 1) loads_but<L>();
       else loads_but<0>();
 #pragma unroll

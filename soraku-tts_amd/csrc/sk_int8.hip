@@ -5,8 +5,6 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <algorithm>
-
 #include "sk_error.h"
 #include "sk_int8.h"
 #include "soraku_mi355x.h"
