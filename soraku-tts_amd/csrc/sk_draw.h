@@ -27,7 +27,7 @@
 //
 // A row is small work with many steps that wait for each other, on few CUs: its latency bounds it.  16 rows of 2051 with
 // guidance: 12 us; one row of 151,936: 11 us for the histograms and 19 for the rest; 64 of them in BF16 (19 MB): 23
-// (VALU 87% busy, 62 instructions per value) and 29 us.
+// (VALU 87% busy, 59 instructions per value) and 30 us.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -23,9 +23,9 @@ int check_sizes(int32_t R, int32_t V, int32_t dtype) {
   return SK_OK;
 }
 // Workgroups per row: one of the GPU's 256 CUs each, as few rows allow, but no more than ten, whose histograms every
-// one of them adds up. A row of 151,936: 77 us whole, 42 in 3, 31 in 8, 29 in 10; 64 of them 55 us in 2, 42 in 4, 59 in 5; 256
-// 86 us whole, 101 in 2. Short rows stay whole, as a second launch costs more: 12,000 values 17 us whole, 22 in 2 to 10; 16,384
-// 19 and 22; 32,000 27 and 23.
+// one of them adds up. Calls one after the other over changing logits, FP32: a row of 151,936 88 us whole, 44 in 3, 29 in 8, 27 in
+// 10; 64 of them 62 us in 2, 48 in 4, 69 in 5 (BF16 60, 42 and 61); 256 114 us whole, 136 in 2. Short rows stay whole, as
+// a second launch costs more: 12,000 values 17.5 us whole, 20 to 21 in 2 to 10; 16,384 19.6 and 20.5 to 22; 32,000 27.5 and 22.
 int slices_of(int R, int V) { return V <= 16384 ? 1 : std::max(1, std::min(MOST_SLICES, 256 / std::max(R, 1))); }
 // Sums of V weights of up to 2^bits stay below 2^63.
 int bits_of(int V) {

@@ -362,10 +362,10 @@ __device__ __forceinline__ void emit(const LinearArgs& a, int m, int n, float (&
 // with 4 neighbouring columns of one row.  Rows past M or N are clamped on load and not stored.
 //
 // The matrix cores alone reach 3.6 POP/s on random codes (4.9 on zeros: the clock follows the power).  7,680 rows of
-// 2 x 6144 x 2048 (SwiGLU, BF16 out) take 204 us, 1.9 POP/s, of 2048 x 6144 82 us, 1.8 to 2.3 POP/s by what lies in
-// cache: a tile's first stage, its epilogue (26 instructions per SwiGLU output) and its store have no products beside
+// 2 x 6144 x 2048 (SwiGLU, BF16 out) take 201 us, 1.9 POP/s, 5,999 of 2048 x 6144 71 us with inputs in cache and 78 without, 2.1 and
+// 1.9 POP/s: a tile's first stage, its epilogue (26 instructions per SwiGLU output) and its store have no products beside
 // them, since LDS holds one 256 x 256 tile per CU.  Smaller tiles, two to a CU, overlap them, but load twice the
-// bytes per product: 231 us in tiles of 128 x 128.
+// bytes per product: 221 to 247 us in tiles of 128 x 128.
 template <typename X, bool SWIGLU, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM * WN * 64) void tiles_kernel(LinearArgs a) {
   constexpr int W = WM * WN, ROWS = BM + BN, LR = 8, PER = ROWS / LR / W;   // rows per load, loads per wave
@@ -544,9 +544,9 @@ __device__ __forceinline__ void loads_but() { asm volatile("s_waitcnt vmcnt(%0)"
 // unit of 128 codes; their sums meet in LDS.  The weights' bytes bound it.  They go to LDS in whole lines,
 // 8 lanes to a row, into a ring of D units that is the wave's own, so that no wave waits for another, and
 // from there to registers as matrix fragments (a load in the order of a fragment's lanes, 16 rows next to each other,
-// takes 3.5 times as long: 2048 x 6144, 128 workgroups, 4.5 us against 2.7 with the launch).  In a cold cache 32 rows
-// of 2 x 6144 x 2048 take 8.7 us, 2.9 TB/s of weights, 32 rows of 2048 x 6144 5.1, 2 rows of 4096 x 2048 with their codes 5.5,
-// 1 row of 2051 x 1024 4.6: the launch, the latency of a ring's first units and the sum over the waves, in turn.
+// takes 3.5 times as long: 2048 x 6144, 128 workgroups, 4.5 us against 2.7 with the launch).  With two sets of inputs in turn 32 rows
+// of 2 x 6144 x 2048 take 8.5 us, 3.0 TB/s of weights (7.2 in cache, 13.4 from memory; LDS holds one workgroup per CU, of 384), 32 rows
+// of 2048 x 6144 5.0, 2 rows of 4096 x 2048 with their codes 5.4, 1 row of 2051 x 1024 4.6: the launch, the latency of a ring's first units and the sum over the waves, in turn.
 //
 // FUSED (up to 8 rows, a power of two times K at most 16,384): the workgroup codes the
 // activations' rows itself, each into its own LDS, which saves the launch that writes them;

@@ -68,9 +68,12 @@ struct Plan {
 struct Few { int mt, nt; };
 constexpr Few FEW[] = {{1, 1}, {2, 1}, {1, 2}, {2, 2}, {4, 2}};   // SwiGLU: from the third on
 // Estimated us of a launch of tiles when a CU has r of them, of u stages: fix + r round + u lat + (r - 1) u thr, fitted
-// to 207 times (33 to 7,680 rows, the trunks' projections and odd ones; rms error 7 to 24%).  The tile chosen is on
-// average within 6% of the fastest (SwiGLU 3%).  E.g. 7,680 rows of 2 x 6144 x 2048: 256 x 256 204 us, 128 x 128 231;
-// 774 of 4096 x 1024: 64 x 128 9.2, 128 x 128 10.0, 256 x 256 15.6; 64 of 2048 x 6144: 64 x 64 15.4, 64 x 128 21.6.
+// to 207 times of launches one after the other with inputs in cache (33 to 7,680 rows, the trunks' projections and odd ones; rms error 7 to
+// 24%, and 28% too little for the long one below).  It is there to choose, and the tile chosen is on average within 6% of the fastest (SwiGLU
+// 3%).  Measured with inputs in cache, then from memory: 7,680 rows of 2 x 6144 x 2048: 256 x 256 199 and 201 us, 128 x 128 221 and
+// 247; 5,999 of 2048 x 6144 (51 estimated): 192 x 256 71 and 78, 256 x 256 77 and 83, 128 x 128 91 and 107; 774 of 4096 x 1024 (128 x
+// 128 taken, 9.5 estimated): 64 x 128 9.1 and 11.4, 128 x 128 10.0 and 12.7, 256 x 256 16.1 and 18.9; 64 of 2048 x 6144: 64 x 64 15.2 and
+// 17.7, 64 x 128 21.5 and 45.
 struct Tile { int bm, bn, waves; float fix, round, lat, thr, fix2, round2, lat2, thr2; };   // 2: SwiGLU
 constexpr Tile TILES[] = {{256, 256, 16, 0.f, 7.19f, 1.10f, 2.28f, 0.f, 8.47f, 1.15f, 1.87f},
                           {192, 256, 8, 0.f, 7.00f, .92f, 1.53f, 0.f, 7.23f, 1.00f, 1.40f},
