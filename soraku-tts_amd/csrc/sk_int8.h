@@ -298,12 +298,11 @@ __device__ __forceinline__ float silu(float g) {
   const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, LN2, 1.f);
   return g * __builtin_amdgcn_rcpf(1.f + e);
 }
-// A row's scale as two factors, one of them 1: what sums are multiplied by, and what columns' scales are.  Sums are below 2^31, so
-// products with scales up to 2^96 stay finite; rows of larger ones (values past 1e31) take theirs with the columns' first, which
-// leaves FP32's range only where the output does.
+// A row's scale as two factors: what sums are multiplied by, and what columns' scales are.  Sums are below 2^31, so their
+// products with 2^96 stay finite; what a larger scale (of values past 1e31) has beyond that, a power of two less, goes to the columns'.
 struct RowScale {
   float s, t;
-  __device__ __forceinline__ explicit RowScale(float x) : s(x > 0x1p96f ? 1.f : x), t(x > 0x1p96f ? x : 1.f) {}
+  __device__ __forceinline__ explicit RowScale(float x) : s(x > 0x1p96f ? 0x1p96f : x), t(x > 0x1p96f ? x * 0x1p-96f : 1.f) {}
 };
 // act of sums of row m (scale s) and column c (scale w, bias b; SwiGLU: and of its up column).
 template <typename X, bool SWIGLU>

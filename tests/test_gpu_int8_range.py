@@ -77,3 +77,15 @@ def test_sums_past_the_range_before_their_weights_scale(ops, hip_device, m, n, k
     size = torch.tensor([3e38, 1.0, 2e37, 1e30, 2.0 ** 103, 2.0 ** 104])[torch.arange(m) % 6][:, None]
     d["x"] = (d["x"].double() / top.double() * size.double()).to(dtype)
     check(ops, hip_device, d, n, k, None)
+
+
+@pytest.mark.parametrize("m", [2, 20, 400])
+def test_sums_of_zero_by_large_scales(ops, hip_device, m):
+    """Sums that are 0 stay 0 where the two scales' product is past the range."""
+    x = torch.full((m, 64), 3e38)
+    x[:, 1::2] = -3e38
+    codes = torch.zeros(70, 128, dtype=torch.int8)
+    codes[:, :64] = 127
+    bias = torch.arange(70.0)
+    got = ops.int8_linear(70, 64)(x.to(hip_device), codes.to(hip_device), torch.full((70,), 1e15, device=hip_device), bias=bias.to(hip_device))
+    assert torch.equal(got.cpu(), bias.expand(m, 70))
